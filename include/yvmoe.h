@@ -29,6 +29,9 @@
  *                           _apply_skip_residual model/moe/layer.py:741-753
  *   yvmoe_forward        -> YvDeepSeekMoELayer.forward / YvDynamicMoELayer.forward
  *                           model/moe/layer.py:1283-1396 / :867-963 (inference)
+ *   yvmoe_forward_few, yvmoe_experts_few
+ *                        -> yvmoe_forward and yvmoe_dispatch (with the shared experts) for up
+ *                           to 16 tokens
  *   yvmoe_moegate_logits -> YvMoEGate.forward in eval mode up to the top-k (steps 2-8 and the
  *                           loss of step 13), model/moe/gate.py:310-393, :433-444; the top-k
  *                           and its softmax (gate.py:414-416) are yvmoe_route in fixed mode
@@ -267,6 +270,40 @@ int32_t yvmoe_forward_static(const void* x, int32_t act_dtype, int32_t n_tokens,
                              const yvmoe_router* router, const yvmoe_expert_weights* experts,
                              const float* mix, const void* skip, void* out, void* shared_out,
                              yvmoe_routing* routing, void* stream);
+
+/*
+ * The layer for a few tokens (0 <= N <= YVMOE_FEW_TOKENS) in two kernels, for decoding one or a few
+ * sequences. Routing, formats, shapes, results and limits are yvmoe_forward's, with fewer roundings: quantized
+ * weights enter the products exactly (yvmoe_forward rounds bf16(q * s)), gate and up stay fp32, h is
+ * rounded to bf16 once, expert outputs and their weighted sum stay fp32, and out and shared_out are each
+ * rounded once. Router logits are fp32 sums in an order of their own (a tie within the last bits may
+ * fall the other way). Equal calls give equal bits.
+ *
+ * yvmoe_forward_few: the whole layer with YvStableMoEGate's routing.
+ * yvmoe_experts_few: the routed and shared experts, the weighted sum and the skip residual for a
+ * routing that another router computed: routing_weights [N][k] (weight_dtype fp32 or bf16),
+ * expert_indices [N][k] int64, k = slots_per_token <= YVMOE_MAX_TOPK; a token may name an expert more
+ * than once; a slot whose index lies outside [0, E) is not computed and adds nothing, and *invalid
+ * (int32 device scalar, may be NULL) receives their number. With num_shared == 0 and skip NULL this
+ * is yvmoe_dispatch.
+ *   mix, skip, shared_out: as for yvmoe_combine.
+ * workspace: yvmoe_few_workspace_bytes() bytes, which nothing need initialise; calls that overlap in
+ * time need workspaces of their own. (Overlapping calls on one workspace end, but out is undefined.)
+ */
+#define YVMOE_FEW_TOKENS 16
+size_t yvmoe_few_workspace_bytes(int32_t n_tokens, int32_t act_dtype, int32_t slots_per_token,
+                                 const yvmoe_expert_weights* experts);
+int32_t yvmoe_forward_few(const void* x, int32_t act_dtype, int32_t n_tokens,
+                          const yvmoe_router* router, const yvmoe_expert_weights* experts,
+                          const float* mix, const void* skip, void* out, void* shared_out,
+                          yvmoe_routing* routing, void* workspace, size_t workspace_bytes,
+                          void* stream);
+int32_t yvmoe_experts_few(const void* x, int32_t act_dtype, int32_t n_tokens,
+                          const void* routing_weights, int32_t weight_dtype,
+                          const int64_t* expert_indices, int32_t slots_per_token,
+                          const yvmoe_expert_weights* experts, const float* mix, const void* skip,
+                          void* out, void* shared_out, int32_t* invalid, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 /*
  * YvMoEGate (model/moe/gate.py:140-451), the router the reference's MoE layers build

@@ -35,6 +35,7 @@ MAX_EXPERTS = 256
 MAX_TOPK = 16
 MAX_SHARED = 8
 PREDICTOR_DIM = 64
+FEW_TOKENS = 16
 STATIC_SCRATCH_BYTES = 64 << 20
 
 EXPORTED_SYMBOLS = (
@@ -57,6 +58,9 @@ EXPORTED_SYMBOLS = (
     "yvmoe_forward_moegate_workspace_bytes",
     "yvmoe_forward_moegate",
     "yvmoe_rmsnorm",
+    "yvmoe_few_workspace_bytes",
+    "yvmoe_forward_few",
+    "yvmoe_experts_few",
 )
 
 # YvMoEGate auxiliary heads (YVMOE_HEAD_*)
@@ -203,6 +207,14 @@ def _declare(l: ctypes.CDLL) -> None:
     l.yvmoe_forward_static.argtypes = [vp, i32, i32, ctypes.POINTER(Router),
                                        ctypes.POINTER(ExpertWeights), vp, vp, vp, vp,
                                        ctypes.POINTER(Routing), vp]
+    l.yvmoe_few_workspace_bytes.restype = sz
+    l.yvmoe_few_workspace_bytes.argtypes = [i32, i32, i32, ctypes.POINTER(ExpertWeights)]
+    l.yvmoe_forward_few.restype = i32
+    l.yvmoe_forward_few.argtypes = [vp, i32, i32, ctypes.POINTER(Router), ctypes.POINTER(ExpertWeights),
+                                    vp, vp, vp, vp, ctypes.POINTER(Routing), vp, sz, vp]
+    l.yvmoe_experts_few.restype = i32
+    l.yvmoe_experts_few.argtypes = [vp, i32, i32, vp, i32, vp, i32, ctypes.POINTER(ExpertWeights),
+                                    vp, vp, vp, vp, vp, vp, sz, vp]
     l.yvmoe_forward.restype = i32
     l.yvmoe_forward.argtypes = [vp, i32, i32, ctypes.POINTER(Router), ctypes.POINTER(ExpertWeights),
                                 vp, vp, vp, vp, ctypes.POINTER(Routing), vp, sz, vp]

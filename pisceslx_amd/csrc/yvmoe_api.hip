@@ -403,6 +403,80 @@ int32_t yvmoe_forward_static(const void* x, int32_t act_dtype, int32_t n_tokens,
                        (size_t)YVMOE_STATIC_SCRATCH_BYTES, stream, true);
 }
 
+size_t yvmoe_few_workspace_bytes(int32_t n_tokens, int32_t act_dtype, int32_t slots_per_token,
+                                 const yvmoe_expert_weights* experts) {
+    if (n_tokens < 0 || n_tokens > kFewTokens || check_experts(experts, act_dtype) != YVMOE_OK) return 0;
+    if (slots_per_token < 1 || slots_per_token > YVMOE_MAX_TOPK) return 0;
+    return few_ws(n_tokens, slots_per_token, experts->num_routed, experts->num_shared, experts->hidden,
+                  experts->ffn, act_dtype).bytes;
+}
+
+// Checks that both few-token entries share.
+static int check_few(const void* x, int act, int N, int k, const yvmoe_expert_weights* w, const float* mix,
+                     const void* out, const void* workspace, size_t workspace_bytes) {
+    YV_REQUIRE(act == YVMOE_ACT_F32 || act == YVMOE_ACT_BF16, YVMOE_ERR_DTYPE,
+               "unknown activation dtype %d", act);
+    int rc = check_experts(w, act);
+    if (rc) return rc;
+    YV_REQUIRE(N >= 0, YVMOE_ERR_ARG, "n_tokens=%d < 0", N);
+    YV_REQUIRE(N <= kFewTokens, YVMOE_ERR_SHAPE, "n_tokens=%d: the few-token layer takes up to %d", N, kFewTokens);
+    YV_REQUIRE(w->w_gate && w->w_up && w->w_down, YVMOE_ERR_ARG, "expert weights are NULL");
+    YV_REQUIRE(((uintptr_t)w->w_gate | (uintptr_t)w->w_up | (uintptr_t)w->w_down) % 16 == 0 &&
+                   ((uintptr_t)w->s_gate | (uintptr_t)w->s_up | (uintptr_t)w->s_down) % 8 == 0,
+               YVMOE_ERR_ARG, "expert weights must be 16-byte and scales 8-byte aligned");
+    const size_t need = few_ws(N, k, w->num_routed, w->num_shared, w->hidden, w->ffn, act).bytes;
+    YV_REQUIRE(workspace != nullptr && workspace_bytes >= need, YVMOE_ERR_WORKSPACE,
+               "workspace %zu bytes, need %zu", workspace_bytes, need);
+    YV_REQUIRE(N == 0 || (x && out), YVMOE_ERR_ARG, "NULL pointer");
+    YV_REQUIRE(((uintptr_t)x | (uintptr_t)out | (uintptr_t)workspace) % 16 == 0, YVMOE_ERR_ARG,
+               "x, out and workspace must be 16-byte aligned");
+    YV_REQUIRE(w->num_shared == 0 || mix != nullptr, YVMOE_ERR_ARG, "shared experts need mix weights");
+    return YVMOE_OK;
+}
+
+int32_t yvmoe_forward_few(const void* x, int32_t act_dtype, int32_t n_tokens,
+                          const yvmoe_router* router, const yvmoe_expert_weights* experts,
+                          const float* mix, const void* skip, void* out, void* shared_out,
+                          yvmoe_routing* routing, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+    clear_error();
+    int rc = check_router(router, act_dtype);
+    if (rc) return rc;
+    rc = check_few(x, act_dtype, n_tokens, router->top_k, experts, mix, out, workspace, workspace_bytes);
+    if (rc) return rc;
+    rc = check_routing(routing, n_tokens);
+    if (rc) return rc;
+    YV_REQUIRE(router->num_experts == experts->num_routed && router->hidden == experts->hidden,
+               YVMOE_ERR_SHAPE, "router (E=%d, H=%d) and experts (E=%d, H=%d) disagree",
+               router->num_experts, router->hidden, experts->num_routed, experts->hidden);
+    YV_REQUIRE(router->w_router && (uintptr_t)router->w_router % 16 == 0, YVMOE_ERR_ARG,
+               "w_router is NULL or not 16-byte aligned");
+    if (!router->fixed_shape_mode && router->dynamic_capacity)
+        YV_REQUIRE(router->b1 && router->w2 && router->b2, YVMOE_ERR_ARG,
+                   "dynamic capacity needs the predictor's weights");
+    return few_launch(x, act_dtype, n_tokens, router->top_k, router, nullptr, 0, nullptr, experts, mix, skip, out,
+                      shared_out, routing, nullptr, (char*)workspace, (hipStream_t)stream);
+}
+
+int32_t yvmoe_experts_few(const void* x, int32_t act_dtype, int32_t n_tokens,
+                          const void* routing_weights, int32_t weight_dtype,
+                          const int64_t* expert_indices, int32_t slots_per_token,
+                          const yvmoe_expert_weights* experts, const float* mix, const void* skip,
+                          void* out, void* shared_out, int32_t* invalid, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+    clear_error();
+    YV_REQUIRE(slots_per_token >= 1 && slots_per_token <= YVMOE_MAX_TOPK, YVMOE_ERR_SHAPE,
+               "slots_per_token=%d outside [1, %d]", slots_per_token, YVMOE_MAX_TOPK);
+    YV_REQUIRE(weight_dtype == YVMOE_ACT_F32 || weight_dtype == YVMOE_ACT_BF16, YVMOE_ERR_DTYPE,
+               "routing weights must be fp32 or bf16 (got dtype %d)", weight_dtype);
+    const int rc = check_few(x, act_dtype, n_tokens, slots_per_token, experts, mix, out, workspace, workspace_bytes);
+    if (rc) return rc;
+    YV_REQUIRE(n_tokens == 0 || (routing_weights && expert_indices), YVMOE_ERR_ARG, "NULL pointer");
+    return few_launch(x, act_dtype, n_tokens, slots_per_token, nullptr, routing_weights,
+                      weight_dtype == YVMOE_ACT_BF16, expert_indices, experts, mix, skip, out, shared_out, nullptr,
+                      invalid, (char*)workspace, (hipStream_t)stream);
+}
+
 static int check_moegate(const yvmoe_moegate* g, int act) {
     YV_REQUIRE(g != nullptr, YVMOE_ERR_ARG, "gate is NULL");
     YV_REQUIRE(act == YVMOE_ACT_F32 || act == YVMOE_ACT_BF16, YVMOE_ERR_DTYPE,

@@ -251,6 +251,22 @@ inline DispatchWs dispatch_ws(int N, int k, int E, int H, int F, int act) {
     return w;
 }
 
+// The few-token layer (yvmoe_few.hip): counters, the router's logits in up to four K splits, h.
+constexpr int kFewTokens = YVMOE_FEW_TOKENS;
+inline int few_splits(int H) { return H >= 4096 ? 4 : H >= 1024 ? H / 1024 : 1; }
+struct FewWs {
+    size_t counters, logits, h, bytes;
+};
+inline FewWs few_ws(int N, int k, int E, int S, int H, int F, int act) {
+    FewWs w{};
+    size_t o = 0;
+    w.counters = o; o = align_up(o + 9 * 128, 256);
+    w.logits = o;   o = align_up(o + (size_t)few_splits(H) * N * router_ld(E, act) * 4, 256);
+    w.h = o;        o = align_up(o + (size_t)N * (k + S) * F * (act == YVMOE_ACT_BF16 ? 2 : 4), 256);
+    w.bytes = o;
+    return w;
+}
+
 // ---------------------------------------------------------------- launchers
 // Tile table of the expert GEMMs (segments = E routed experts, then S shared experts of N
 // rows each; every segment cut into tile_rows-row tiles), in the FFN workspace region. With
@@ -432,5 +448,11 @@ int rmsnorm_launch(const void* x, int act, int N, int H, const NormChain& nc, in
 int combine_launch(const void* y, int act, int N, int H, int k, int S,
                    const yvmoe_routing* routing, const float* mix, const void* skip,
                    void* out, void* shared_out, hipStream_t st);
+// The layer for up to kFewTokens tokens (yvmoe_few.hip): with r its own routing, written to routing;
+// without, the given weights (fp32 or bf16) and indices, *invalid (may be NULL) the slots whose index is
+// outside [0, E).
+int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, const void* rweights, int rweights_bf16,
+               const int64_t* rindices, const yvmoe_expert_weights* w, const float* mix, const void* skip, void* out,
+               void* shared_out, const yvmoe_routing* routing, int* invalid, char* ws, hipStream_t st);
 
 }  // namespace yvmoe

@@ -26,29 +26,6 @@
 namespace yvmoe {
 namespace {
 
-// complexity_predictor of one token by its 16 lanes: sigmoid(w2 . relu(W1 x + b1) + b2)
-// (gate.py:930-936); hidden unit c of W1 x is the sum of pred_terms columns q * 64 + c.
-// The result is valid on lane 0.
-template <typename PredFn>
-__device__ __forceinline__ float predictor_token(PredFn predcol, int pred_terms, const float* __restrict__ b1,
-                                                 const float* __restrict__ w2, const float* __restrict__ b2,
-                                                 int l) {
-    float acc = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPredDim / kLanes; ++i) {
-        const int c = l + kLanes * i;
-        float hsum = 0.0f;
-        for (int q = 0; q < pred_terms; ++q) hsum = hsum + predcol(q * kPredDim + c);
-        hsum = hsum + b1[c];
-        hsum = hsum > 0.0f ? hsum : 0.0f;
-        acc = acc + w2[c] * hsum;
-    }
-#define YV_SUMSTEP(O) acc = acc + rot16<O>(acc)
-    YV_BFLY16(YV_SUMSTEP);
-#undef YV_SUMSTEP
-    return 1.0f / (1.0f + expf(-(acc + b2[0])));
-}
-
 // One block = 64 tokens, 16 lanes per token, all 64 tokens in one pass (1024 threads).
 template <int NV>
 __global__ __launch_bounds__(1024) void route_topk_kernel(

@@ -5,10 +5,13 @@
 // specification: Cody-Waite exp with the Cephes ln2 split and a degree-7 Taylor polynomial,
 // 16-lane butterfly sums, an IEEE divide, top-k by (p desc, index asc). No multiply-add is
 // fused in these functions whatever the including file's flags (the pragmas below), and the
-// including file is built with the correctly rounded fp32 divide.
+// including file is built with the correctly rounded fp32 divide. Also the complexity predictor of
+// one token (predictor_token), on the same 16 lanes.
 #pragma once
 
 #include <hip/hip_runtime.h>
+
+#include "yvmoe_internal.h"
 
 namespace yvmoe {
 namespace {
@@ -143,6 +146,30 @@ __device__ __forceinline__ void topk_token(LogitFn logit, const float* __restric
         }
     }
     my_w0 = e0 / tot;
+}
+
+// complexity_predictor of one token by its 16 lanes: sigmoid(w2 . relu(W1 x + b1) + b2)
+// (gate.py:930-936); hidden unit c of W1 x is the sum of pred_terms columns q * 64 + c.
+// The result is valid on lane 0.
+template <typename PredFn>
+__device__ __forceinline__ float predictor_token(PredFn predcol, int pred_terms, const float* __restrict__ b1,
+                                                 const float* __restrict__ w2, const float* __restrict__ b2,
+                                                 int l) {
+#pragma clang fp contract(off)
+    float acc = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPredDim / kLanes; ++i) {
+        const int c = l + kLanes * i;
+        float hsum = 0.0f;
+        for (int q = 0; q < pred_terms; ++q) hsum = hsum + predcol(q * kPredDim + c);
+        hsum = hsum + b1[c];
+        hsum = hsum > 0.0f ? hsum : 0.0f;
+        acc = acc + w2[c] * hsum;
+    }
+#define YV_SUMSTEP(O) acc = acc + rot16<O>(acc)
+    YV_BFLY16(YV_SUMSTEP);
+#undef YV_SUMSTEP
+    return 1.0f / (1.0f + expf(-(acc + b2[0])));
 }
 
 }  // namespace

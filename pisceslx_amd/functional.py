@@ -295,6 +295,82 @@ def moe_forward_static(x2d: torch.Tensor, router: RouterState, experts: PackedEx
     return out, (shared_out if S > 0 else None), routing
 
 
+def few_workspace_bytes(n_tokens: int, act: int, top_k: int, experts: PackedExperts) -> int:
+    """Workspace of moe_forward_few and experts_few (0 for sizes they do not take)."""
+    e = experts.struct()
+    return int(_lib.lib().yvmoe_few_workspace_bytes(n_tokens, act, top_k, ctypes.byref(e)))
+
+
+def _few_args(x2d, top_k, experts, mix, skip, workspace, dev):
+    """Checks that the few-token calls share; returns (act, shared_out or None, workspace)."""
+    act = _act(x2d.dtype)
+    if x2d.dim() != 2 or x2d.shape[1] != experts.hidden:
+        raise ValueError(f"x must be [N, {experts.hidden}], got {tuple(x2d.shape)}")
+    N = x2d.shape[0]
+    if N > _lib.FEW_TOKENS:
+        raise ValueError(f"{N} tokens: the few-token layer takes up to {_lib.FEW_TOKENS} "
+                         "(moe_forward and dispatch take any number)")
+    if skip is not None and (skip.shape != x2d.shape or skip.dtype != x2d.dtype):
+        raise ValueError("skip buffer must match x")
+    if mix is not None and (mix.dtype != torch.float32 or mix.numel() != experts.num_shared):
+        raise ValueError("mix must be fp32 [S]")
+    if mix is None and experts.num_shared > 0:
+        raise ValueError("shared experts need mix weights")
+    need = few_workspace_bytes(N, act, top_k, experts)
+    if workspace is None or workspace.numel() < need or workspace.device != dev:
+        workspace = _workspace(need, dev)
+    return act, (torch.empty_like(x2d) if experts.num_shared > 0 else None), workspace
+
+
+def moe_forward_few(x2d: torch.Tensor, router: RouterState, experts: PackedExperts,
+                    mix: Optional[torch.Tensor], skip: Optional[torch.Tensor],
+                    workspace: Optional[torch.Tensor] = None):
+    """moe_forward for up to 16 tokens in two kernels (yvmoe_forward_few), with fewer roundings:
+    weights enter exactly, h and the outputs are rounded once. ``workspace`` is scratch of
+    few_workspace_bytes (allocated here when None or too small); calls that overlap in time need
+    one each. Returns (out [N,H], shared_out [N,H] or None, Routing)."""
+    dev = _require_cuda(x2d, router.w_router, mix, skip, *experts.tensors())
+    if router.hidden != experts.hidden or router.num_experts != experts.num_routed:
+        raise ValueError("router and experts disagree")
+    act, shared_out, workspace = _few_args(x2d, router.top_k, experts, mix, skip, workspace, dev)
+    N = x2d.shape[0]
+    routing = Routing.empty(N, router.num_experts, router.top_k, dev)
+    out = torch.empty_like(x2d)
+    r, e, o = router.struct(), experts.struct(), routing.struct()
+    _lib.check(_lib.lib().yvmoe_forward_few(
+        x2d.data_ptr(), act, N, ctypes.byref(r), ctypes.byref(e), _ptr(mix), _ptr(skip), out.data_ptr(),
+        _ptr(shared_out), ctypes.byref(o), workspace.data_ptr(), workspace.numel(), _stream(dev)),
+        "yvmoe_forward_few")
+    return out, shared_out, routing
+
+
+def experts_few(x2d: torch.Tensor, routing_weights: torch.Tensor, expert_indices: torch.Tensor,
+                experts: PackedExperts, mix: Optional[torch.Tensor] = None,
+                skip: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
+    """Routed and shared experts, weighted sum and skip residual of up to 16 tokens on a routing
+    from any router (yvmoe_experts_few): ``routing_weights`` [N, k] fp32 or bf16,
+    ``expert_indices`` [N, k] int64. Nothing synchronizes with the host. Returns (out [N,H],
+    shared_out [N,H] or None, invalid [1] int32 = slots whose index lies outside [0, E), which
+    add nothing)."""
+    dev = _require_cuda(x2d, routing_weights, expert_indices, mix, skip, *experts.tensors())
+    if expert_indices.dtype != torch.int64 or expert_indices.dim() != 2 or \
+            expert_indices.shape[0] != x2d.shape[0]:
+        raise ValueError("expert_indices must be int64 [N, k]")
+    if routing_weights.shape != expert_indices.shape:
+        raise ValueError(f"routing_weights must be {tuple(expert_indices.shape)}")
+    k = expert_indices.shape[1]
+    wdt = _act(routing_weights.dtype)
+    act, shared_out, workspace = _few_args(x2d, k, experts, mix, skip, workspace, dev)
+    out = torch.empty_like(x2d)
+    invalid = torch.empty(1, dtype=torch.int32, device=dev)
+    e = experts.struct()
+    _lib.check(_lib.lib().yvmoe_experts_few(
+        x2d.data_ptr(), act, x2d.shape[0], routing_weights.data_ptr(), wdt, expert_indices.data_ptr(), k,
+        ctypes.byref(e), _ptr(mix), _ptr(skip), out.data_ptr(), _ptr(shared_out), invalid.data_ptr(),
+        workspace.data_ptr(), workspace.numel(), _stream(dev)), "yvmoe_experts_few")
+    return out, shared_out, invalid
+
+
 @dataclass
 class MoEGateState:
     """Device tensors and constants of one YvMoEGate, regrouped for yvmoe_moegate_logits."""
