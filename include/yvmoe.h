@@ -38,6 +38,8 @@
  *   yvmoe_moegate_forward-> YvMoEGate.forward in eval mode (logits, loss and routing)
  *   yvmoe_forward_moegate-> YvDynamicMoELayer.forward with its YvMoEGate router
  *                           model/moe/layer.py:867-963 (inference)
+ *   yvmoe_int4_linear    -> _YvQuantizedLinear.forward model/utils/quantization.py:486-496 with
+ *                           the codes of quantize_to_int4_blockwise opss/quantize/engine.py:889-941
  *   yvmoe_rmsnorm        -> YvRMSNorm.forward model/core/norms.py:206-208 via
  *                           fused_rms_norm opss/kernels/fused_rms_norm.py:42; two in a
  *                           row = YvHybridBlock's norm_fusion then norm_mlp
@@ -408,6 +410,29 @@ typedef struct yvmoe_rmsnorm_params {
  */
 int32_t yvmoe_rmsnorm(const void* x, int32_t act_dtype, int32_t n_tokens, int32_t hidden,
                       const yvmoe_rmsnorm_params* norms, int32_t n_norms, void* out, void* stream);
+
+/*
+ * Linear layer with 4-bit weights (int4, group 128 along in, zero point 8):
+ *   out[n][o] = sum_i x[n][i] * (q[o][i] - 8) * s[o][i / 128] + bias[o], in fp32 sums of exact
+ *   products, rounded once to the activation dtype.
+ * x [N][in], bias [out] or NULL and out [N][out] in the activation dtype, row-major, at any address
+ * that suits their elements; any in_features, out_features >= 1 and n_rows >= 0. out may not overlap x.
+ *   codes [ceil(out/16)][ceil(in/128)] blocks of 1 KB, each 16 rows x 128 columns: byte
+ *         16 (16 g + r) starts row r's columns 32 g .. 32 g + 31 (g = 0..3), eight of them in each
+ *         of four dwords, columns 0, 2, 4, 6, 1, 3, 5, 7 of the eight from the lowest nibble up;
+ *         codes of columns past in_features are 8 (rows past out_features: any)
+ *   scales [ceil(out/16)][ceil(in/128)][16] bf16
+ *   pisceslx_amd/quant.py pack_linear() writes this order. codes are 16-byte, scales 8-byte aligned.
+ */
+typedef struct {
+    int32_t in_features;
+    int32_t out_features;
+    const void* codes;
+    const void* scales;
+} yvmoe_int4_matrix;
+
+int32_t yvmoe_int4_linear(const void* x, int32_t act_dtype, int32_t n_rows,
+                          const yvmoe_int4_matrix* weight, const void* bias, void* out, void* stream);
 
 /*
  * The whole layer with YvMoEGate as its router, as YvDynamicMoELayer builds it

@@ -61,6 +61,7 @@ EXPORTED_SYMBOLS = (
     "yvmoe_few_workspace_bytes",
     "yvmoe_forward_few",
     "yvmoe_experts_few",
+    "yvmoe_int4_linear",
 )
 
 # YvMoEGate auxiliary heads (YVMOE_HEAD_*)
@@ -122,6 +123,16 @@ class RMSNormParams(ctypes.Structure):
         ("bias", ctypes.c_void_p),
         ("eps", ctypes.c_float),
         ("reserved", ctypes.c_int32),
+    ]
+
+
+class Int4Matrix(ctypes.Structure):
+    """yvmoe_int4_matrix (include/yvmoe.h)."""
+    _fields_ = [
+        ("in_features", ctypes.c_int32),
+        ("out_features", ctypes.c_int32),
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
     ]
 
 
@@ -207,6 +218,8 @@ def _declare(l: ctypes.CDLL) -> None:
     l.yvmoe_forward_static.argtypes = [vp, i32, i32, ctypes.POINTER(Router),
                                        ctypes.POINTER(ExpertWeights), vp, vp, vp, vp,
                                        ctypes.POINTER(Routing), vp]
+    l.yvmoe_int4_linear.restype = i32
+    l.yvmoe_int4_linear.argtypes = [vp, i32, i32, ctypes.POINTER(Int4Matrix), vp, vp, vp]
     l.yvmoe_few_workspace_bytes.restype = sz
     l.yvmoe_few_workspace_bytes.argtypes = [i32, i32, i32, ctypes.POINTER(ExpertWeights)]
     l.yvmoe_forward_few.restype = i32

@@ -694,4 +694,24 @@ int32_t yvmoe_rmsnorm(const void* x, int32_t act_dtype, int32_t n_tokens, int32_
     return rmsnorm_launch(x, act_dtype, n_tokens, hidden, nc, n_norms, out, (hipStream_t)stream);
 }
 
+int32_t yvmoe_int4_linear(const void* x, int32_t act_dtype, int32_t n_rows,
+                          const yvmoe_int4_matrix* weight, const void* bias, void* out, void* stream) {
+    clear_error();
+    YV_REQUIRE(act_dtype == YVMOE_ACT_F32 || act_dtype == YVMOE_ACT_BF16, YVMOE_ERR_DTYPE,
+               "unknown activation dtype %d", act_dtype);
+    YV_REQUIRE(weight != nullptr, YVMOE_ERR_ARG, "weight is NULL");
+    YV_REQUIRE(n_rows >= 0, YVMOE_ERR_ARG, "n_rows=%d < 0", n_rows);
+    YV_REQUIRE(weight->in_features >= 1 && weight->out_features >= 1 && weight->in_features <= (1 << 24) &&
+                   weight->out_features <= (1 << 24),
+               YVMOE_ERR_SHAPE, "in_features=%d, out_features=%d outside [1, 2^24]", weight->in_features,
+               weight->out_features);
+    if (n_rows == 0) return YVMOE_OK;
+    YV_REQUIRE(weight->codes && weight->scales && x && out, YVMOE_ERR_ARG, "NULL pointer");
+    YV_REQUIRE((uintptr_t)weight->codes % 16 == 0 && (uintptr_t)weight->scales % 8 == 0, YVMOE_ERR_ARG,
+               "codes must be 16-byte and scales 8-byte aligned");
+    YV_REQUIRE(((uintptr_t)x | (uintptr_t)bias | (uintptr_t)out) % (act_dtype == YVMOE_ACT_F32 ? 4 : 2) == 0,
+               YVMOE_ERR_ARG, "x, bias and out must be aligned to their elements");
+    return int4_linear_launch(x, act_dtype, n_rows, weight, bias, out, (hipStream_t)stream);
+}
+
 }  // extern "C"

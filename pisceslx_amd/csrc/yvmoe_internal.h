@@ -454,5 +454,8 @@ int combine_launch(const void* y, int act, int N, int H, int k, int S,
 int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, const void* rweights, int rweights_bf16,
                const int64_t* rindices, const yvmoe_expert_weights* w, const float* mix, const void* skip, void* out,
                void* shared_out, const yvmoe_routing* routing, int* invalid, char* ws, hipStream_t st);
+// Linear layer with 4-bit weights (yvmoe_linear.hip).
+int int4_linear_launch(const void* x, int act, int N, const yvmoe_int4_matrix* w, const void* bias, void* out,
+                       hipStream_t st);
 
 }  // namespace yvmoe

@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .quant import PackedExperts
+from .quant import PackedExperts, PackedLinear
 
 
 def _act(dtype: torch.dtype) -> int:
@@ -562,4 +562,30 @@ def rms_norm(x: torch.Tensor, norms, out: Optional[torch.Tensor] = None) -> torc
                                   out.data_ptr() if N > 0 else None, _stream(dev))
     if rc:
         _lib.check(rc, "yvmoe_rmsnorm")
+    return out
+
+
+def int4_linear(x: torch.Tensor, weight: PackedLinear, bias: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [..., in] · Wᵀ (+ bias [out]) with a 4-bit weight (quant.pack_linear), in fp32 sums of exact
+    products rounded once to x's dtype (bf16 or fp32), which bias and ``out`` share. Any number of
+    rows; ``out`` [..., out] must not overlap x."""
+    K, O = weight.in_features, weight.out_features
+    shape, dt = x.shape, x.dtype
+    if x.dim() == 0 or shape[-1] != K:
+        raise ValueError(f"x must be [..., {K}], got {tuple(shape)}")
+    dev = _require_cuda(x, weight.codes, weight.scales, bias, out)
+    act = _act(dt)
+    if bias is not None and (bias.dtype != dt or bias.numel() != O):
+        raise ValueError(f"bias must be {dt} [{O}]")
+    want = (*shape[:-1], O)
+    if out is None:
+        out = torch.empty(want, dtype=dt, device=x.device)
+    elif out.shape != want or out.dtype != dt:
+        raise ValueError(f"out must be {dt} {tuple(want)}")
+    w = weight.struct()
+    rc = _lib.lib().yvmoe_int4_linear(x.data_ptr(), act, x.numel() // K, ctypes.byref(w), _ptr(bias),
+                                      out.data_ptr(), _stream(dev))
+    if rc:
+        _lib.check(rc, "yvmoe_int4_linear")
     return out

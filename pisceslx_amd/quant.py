@@ -298,6 +298,70 @@ def pack_experts(weights: Sequence[Tuple[torch.Tensor, torch.Tensor, torch.Tenso
     return pk.packed
 
 
+# ------------------------------------------------------------------ linear layers, int4 g128
+@dataclass
+class PackedLinear:
+    """A linear layer's weight in int4 with a scale per 128 columns, in the order yvmoe_int4_linear
+    reads (include/yvmoe.h): codes [out/16][in/128] blocks of 1 KB, scales [out/16][in/128][16] bf16,
+    both counts rounded up. Any in_features and out_features."""
+
+    in_features: int
+    out_features: int
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def to(self, device) -> "PackedLinear":
+        return PackedLinear(self.in_features, self.out_features, self.codes.to(device),
+                            self.scales.to(device))
+
+    def struct(self) -> _lib.Int4Matrix:
+        return _lib.Int4Matrix(self.in_features, self.out_features, self.codes.data_ptr(),
+                               self.scales.data_ptr())
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """The dense [out][in] weight (for checkers)."""
+        ob, groups = self.codes.shape[:2]
+        w = self.codes.view(torch.int32).view(ob, groups, 4, 16, 4, 1)     # [g][r][dword]
+        shift = torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], dtype=torch.int32, device=w.device)
+        q = ((w >> shift) & 15).permute(0, 3, 1, 2, 4, 5).reshape(ob * 16, groups, 128)
+        s = self.scales.permute(0, 2, 1).reshape(ob * 16, groups, 1)
+        return ((q.float() - 8.0) * s.float()).view(ob * 16, -1)[:self.out_features, :self.in_features].to(dtype)
+
+
+def pack_linear_codes(codes: torch.Tensor, scales: torch.Tensor, in_features: int) -> PackedLinear:
+    """A PackedLinear of codes in the int4 format (:func:`quantize_int4`): codes [out][groups*64] uint8,
+    two a byte, low nibble = even column, and scales [out][groups] bf16, groups = in_features / 128
+    rounded up. Codes of columns past in_features are taken as 8 (zero), whatever they hold."""
+    out = codes.shape[0]
+    groups = -(-in_features // 128)
+    if in_features < 1 or out < 1:
+        raise ValueError(f"a linear layer needs features, got in {in_features}, out {out}")
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] != groups * 64:
+        raise ValueError(f"codes must be uint8 [out, {groups * 64}], got {codes.dtype} {tuple(codes.shape)}")
+    if scales.dtype != torch.bfloat16 or tuple(scales.shape) != (out, groups):
+        raise ValueError(f"scales must be bfloat16 [{out}, {groups}], got {scales.dtype} {tuple(scales.shape)}")
+    ob = -(-out // 16)
+    q = torch.stack([codes & 15, codes >> 4], dim=-1).view(out, groups * 128)
+    q[:, in_features:] = 8
+    q = torch.nn.functional.pad(q, (0, 0, 0, ob * 16 - out), value=8)
+    s = torch.nn.functional.pad(scales, (0, 0, 0, ob * 16 - out))
+    # dword nibbles from the lowest: columns 0, 2, 4, 6, 1, 3, 5, 7; bytes hold two of them
+    q = q.view(ob, 16, groups, 4, 4, 8)[..., [0, 2, 4, 6, 1, 3, 5, 7]]     # [r][group][g][dword]
+    b = (q[..., 0::2] | (q[..., 1::2] << 4)).permute(0, 2, 3, 1, 4, 5)     # [group][g][r][dword][4]
+    return PackedLinear(in_features, out, b.reshape(ob, groups, 1024).contiguous(),
+                        s.view(ob, 16, groups).permute(0, 2, 1).contiguous())
+
+
+def pack_linear(w: torch.Tensor) -> PackedLinear:
+    """Quantize a [out][in] weight (nn.Linear.weight) to int4 with group-128 scales and pack it."""
+    if w.dim() != 2:
+        raise ValueError(f"a linear weight is [out, in], got {tuple(w.shape)}")
+    inn = w.shape[1]
+    pad = -inn % 128
+    q, s = quantize_int4(torch.nn.functional.pad(w.float(), (0, pad)) if pad else w)
+    return pack_linear_codes(q, s, inn)
+
+
 # ------------------------------------------------------------------ router
 def split_bf16x3(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """fp32 w -> (hi, mid, lo) bf16 with hi + mid + lo == w to within one fp32 ulp."""
