@@ -408,7 +408,7 @@ size_t yvmoe_few_workspace_bytes(int32_t n_tokens, int32_t act_dtype, int32_t sl
     if (n_tokens < 0 || n_tokens > kFewTokens || check_experts(experts, act_dtype) != YVMOE_OK) return 0;
     if (slots_per_token < 1 || slots_per_token > YVMOE_MAX_TOPK) return 0;
     return few_ws(n_tokens, slots_per_token, experts->num_routed, experts->num_shared, experts->hidden,
-                  experts->ffn, act_dtype).bytes;
+                  experts->ffn, experts->format, act_dtype).bytes;
 }
 
 // Checks that both few-token entries share.
@@ -420,11 +420,13 @@ static int check_few(const void* x, int act, int N, int k, const yvmoe_expert_we
     if (rc) return rc;
     YV_REQUIRE(N >= 0, YVMOE_ERR_ARG, "n_tokens=%d < 0", N);
     YV_REQUIRE(N <= kFewTokens, YVMOE_ERR_SHAPE, "n_tokens=%d: the few-token layer takes up to %d", N, kFewTokens);
+    YV_REQUIRE((long long)N * (k + w->num_shared) * w->ffn < (1ll << 28) && (long long)N * w->hidden < (1ll << 28),
+               YVMOE_ERR_SHAPE, "problem too large");  // activations' byte offsets below 2^31
     YV_REQUIRE(w->w_gate && w->w_up && w->w_down, YVMOE_ERR_ARG, "expert weights are NULL");
     YV_REQUIRE(((uintptr_t)w->w_gate | (uintptr_t)w->w_up | (uintptr_t)w->w_down) % 16 == 0 &&
                    ((uintptr_t)w->s_gate | (uintptr_t)w->s_up | (uintptr_t)w->s_down) % 8 == 0,
                YVMOE_ERR_ARG, "expert weights must be 16-byte and scales 8-byte aligned");
-    const size_t need = few_ws(N, k, w->num_routed, w->num_shared, w->hidden, w->ffn, act).bytes;
+    const size_t need = few_ws(N, k, w->num_routed, w->num_shared, w->hidden, w->ffn, w->format, act).bytes;
     YV_REQUIRE(workspace != nullptr && workspace_bytes >= need, YVMOE_ERR_WORKSPACE,
                "workspace %zu bytes, need %zu", workspace_bytes, need);
     YV_REQUIRE(N == 0 || (x && out), YVMOE_ERR_ARG, "NULL pointer");

@@ -12,16 +12,20 @@
 // 1. few_front_kernel: everything that needs no routing. The router's logits, as K-split partial
 //    sums, and the gate/up products of the shared experts; it also clears the counters of 2.
 // 2. few_experts_kernel: every work-group computes the routing from the logits by itself (N·k <= 256
-//    slots in LDS; cheaper than another launch), then the gate/up products of the routed experts
-//    are dealt out as (16-row tile, 16 columns of F) items, and once all of them are there each
-//    work-group takes 16 columns of H of *all* tiles, so that the weighted sum, the shared mixture
-//    and the skip residual end in its LDS: no expert output leaves the chip.
+//    slots in LDS; cheaper than another launch), then the gate/up products of the routed experts as
+//    (16-row tile, 16 columns of F) items, and once all of them are there each work-group takes 16
+//    columns of H of *all* tiles, so that the weighted sum, the shared mixture and the skip residual
+//    end in its LDS: no expert output leaves the chip. Where H gives too few work-groups, up to eight
+//    share 16 columns, and the last one to finish adds up their sums, in their order.
 //
-// Between the two halves of 2 work-groups wait for each other. The gate/up items are taken from
-// counters and never assigned to a work-group beforehand, so every item that a wait is for is held
-// by a work-group that runs and that waits for nothing: the wait ends whichever part of the grid is
-// resident, also beside other kernels. (Should two calls be given one workspace at the same time,
-// which is an error, the wait is left after kSpinLimit looks and out becomes NaN.)
+// Between the two halves of 2 work-groups wait for each other's h. A work-group's first five items are
+// its own, and it marks them when they are done; the rest are handed out by a counter, which evens out
+// the work-groups, and those done are counted. Items of the second kind are held by work-groups that
+// run and wait for nothing; those of the first kind are computed by a work-group that has waited long
+// for their mark (the same bits, so doing them twice is harmless). So the wait ends whichever part of
+// the grid is resident, also beside other kernels that wait. What work-groups hand to each other is
+// written through and read past the caches (sc1): an acquire would invalidate every L2, 30 us for
+// the 4,096 wavefronts of a launch.
 //
 // Rounding: weights enter exactly (codes as bf16, scales on the fp32 sums), h is rounded once to
 // bf16 for the second product's MFMAs, the outputs once at the end.
@@ -31,16 +35,56 @@
 #include "yvmoe_internal.h"
 #include "yvmoe_topk.h"
 
+#ifndef YV_B
+#define YV_B 1, 3, 2, 3, 2, 3, 4, 3
+#endif
+#ifndef YV_I
+#define YV_I 2, 2, 4, 2, 2, 3, 4, 3
+#endif
+#ifndef YV_P
+#define YV_P 2, 2, 4, 2, 2, 3, 4, 3
+#endif
+#ifndef YV_Q
+#define YV_Q 2, 3, 4, 4, 4, 3, 8, 3
+#endif
+#ifndef YV_F
+#define YV_F 1, 2, 1, 3, 1, 3, 2, 3
+#endif
+
 namespace yvmoe {
 namespace {
 
+// k-steps per chunk and chunks held for two matrices and for one, without and with activations in LDS.
+struct Depth {
+    int u2, r2, u1, r1, lu2, lr2, lu1, lr1;
+    constexpr int unit(int nm, bool lds) const { return nm == 2 ? (lds ? lu2 : u2) : (lds ? lu1 : u1); }
+    constexpr int ring(int nm, bool lds) const { return nm == 2 ? (lds ? lr2 : r2) : (lds ? lr1 : r1); }
+};
+
 constexpr int kFewSlots = kFewTokens * YVMOE_MAX_TOPK;
 constexpr int kFewTiles = kFewSlots + YVMOE_MAX_SHARED;
-constexpr int kWaves = 8, kThreads = 64 * kWaves;
+// Wavefronts that stream weights; one more sums their products, stores h, takes items and waits, so that
+// the streams never wait for a store or an atomic (which answer after microseconds, and in the order
+// of the loads round them).
+constexpr int kWaves = 8, kThreads = 64 * kWaves, kAllThreads = kThreads + 64;
 constexpr int kYRows = 512;            // rows of partial expert outputs that a work-group holds
-constexpr int kRanges = 8;             // ranges of gate/up items, one per XCD
-constexpr int kCounterStride = 32;     // ints between counters (a cache line each)
-constexpr int kSpinLimit = 1 << 21;    // looks at the counter, about a microsecond each
+constexpr int kGrid = kFewGrid;  // most work-groups of the second kernel: one per CU
+constexpr int kPatience = 4096;  // looks at a signal, about half a microsecond each, before helping
+
+constexpr int kOwnItems = 5;  // gate/up items that a work-group takes without asking (GateUpItems)
+constexpr int kMarkWords = kGrid / 32, kGoLines = 32;
+// Words that work-groups signal with, each on a line of its own: an address serves some 50 accesses a
+// microsecond, and all work-groups come at about the same time.
+enum Signal {
+    SIG_MARKS = 0,               // kMarkWords words of 32 bits: the work-group's own items are done
+    SIG_FINISHED = kMarkWords,   // items handed out that are done
+    SIG_ROOT,                    // of the above, how many are complete
+    SIG_TICKET,                  // items handed out
+    SIG_GO,                      // kGoLines words: all is done
+    SIG_COUNT = SIG_GO + kGoLines
+};
+constexpr int kSignalBytes = SIG_COUNT * 128;
+static_assert(kSignalBytes <= kFewSignalBytes, "workspace layout");
 
 struct FewArgs {
     const void* x;
@@ -63,27 +107,45 @@ struct FewArgs {
     const void* skip;
     void* out;
     void* shared_out;
+    const void* xo; // x, for int4 in its order of columns
     void* h;        // [N k + S N][F], routed rows by expert, then the shared experts' tokens
-    int* counters;  // [kRanges + 1] x kCounterStride: items taken per range, work-groups' items done
+    unsigned* signals;  // Signal words, 32 apart
+    int hparts;       // work-groups per 16 columns of H
+    int* hcount;      // [H / 16]: those of them that are done
+    float* hsum;      // [hparts][2][N][H]: their sums of the routed and of the shared experts
 };
 
 // ---------------------------------------------------------------- weights and activations
-// A wavefront multiplies 16 rows of a weight matrix (the first MFMA operand) with 16 activation
-// rows over 64-wide k-steps. Lane l = 16 g + r holds columns 16 g .. 16 g + 15 of weight row r and of
-// activation row r; the accumulator holds weight rows 4 g + i of activation row r.
+// A wavefront multiplies 16 activation rows (the first MFMA operand) with 16 rows of a weight matrix
+// over 64-wide k-steps. Lane l = 16 g + r holds columns 16 g .. 16 g + 15 of activation row r and of
+// weight row r; the accumulator holds activation rows 4 g + i of weight row r, so that a row's scale
+// stays in the lanes that hold its codes.
 //
-// Raw: a k-step's weights as stored. Act: a k-step's activations. UNIT: k-steps per chunk.
+// Raw: a k-step's weights as stored. Act: a k-step's activations. DEPTH: k-steps per chunk, and
+// chunks that the registers hold, all but one of them in flight.
 // GROUPED: the scale belongs to a row (int4) or 128 rows (fp8) and 128 columns, that is two k-steps.
 template <int WF>
 struct Wt;
 
+// 16 bytes at an offset (none, and nothing read, past the buffer's end). FRESH: read past the caches (h,
+// which other work-groups of the launch have written).
+template <bool FRESH>
+__device__ __forceinline__ uint4 act_load16(__amdgpu_buffer_rsrc_t b, unsigned offset) {
+    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, FRESH ? 16 : 0);
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+
 struct ActB16 {
     Frag16 f;
-    static constexpr int BYTES = 2;
-    __device__ __forceinline__ void load(const char* row, int ks) {
-        const uint4* p = (const uint4*)(row + (size_t)ks * 128);
-        f.u[0] = p[0];
-        f.u[1] = p[1];
+    static constexpr int BYTES = 2, LANE = 16;  // of an element; columns between lane groups
+    template <bool FRESH>
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t b, unsigned row, int ks) {
+        f.u[0] = act_load16<FRESH>(b, row + ks * 128);
+        f.u[1] = act_load16<FRESH>(b, row + ks * 128 + 16);
+    }
+    __device__ __forceinline__ void read(const char* row, int ks) {
+        f.u[0] = *(const uint4*)(row + ks * 128);
+        f.u[1] = *(const uint4*)(row + ks * 128 + 16);
     }
 };
 
@@ -102,7 +164,7 @@ template <>
 struct Wt<YVMOE_W_BF16> {
     typedef Frag16 Raw;
     typedef ActB16 Act;
-    static constexpr int UNIT = 2;
+    static constexpr Depth DEPTH = {YV_B};
     static constexpr bool GROUPED = false;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return block_ptr(b, e * 2, n0, K, 2048, 16, lane);
@@ -112,8 +174,8 @@ struct Wt<YVMOE_W_BF16> {
         r.u[1] = nt_load16(p + (size_t)ks * 2048 + 1024);
     }
     static __device__ __forceinline__ void mma(const Raw& w, const Act& a, f32x4& acc) {
-        acc = mfma16(w.v[0], a.f.v[0], acc);
-        acc = mfma16(w.v[1], a.f.v[1], acc);
+        acc = mfma16(a.f.v[0], w.v[0], acc);
+        acc = mfma16(a.f.v[1], w.v[1], acc);
     }
 };
 
@@ -121,7 +183,7 @@ template <>
 struct Wt<YVMOE_W_INT8> {
     typedef uint4 Raw;
     typedef ActB16 Act;
-    static constexpr int UNIT = 2;
+    static constexpr Depth DEPTH = {YV_I};
     static constexpr bool GROUPED = false;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return block_ptr(b, e, n0, K, 1024, 16, lane);
@@ -144,8 +206,8 @@ struct Wt<YVMOE_W_INT8> {
         Frag16 f;
         f.u[0] = make_uint4(o[0], o[1], o[2], o[3]);
         f.u[1] = make_uint4(o[4], o[5], o[6], o[7]);
-        acc = mfma16(f.v[0], a.f.v[0], acc);
-        acc = mfma16(f.v[1], a.f.v[1], acc);
+        acc = mfma16(a.f.v[0], f.v[0], acc);
+        acc = mfma16(a.f.v[1], f.v[1], acc);
     }
 };
 
@@ -153,7 +215,7 @@ template <>
 struct Wt<YVMOE_W_FP8> {
     typedef uint4 Raw;
     typedef ActB16 Act;
-    static constexpr int UNIT = 2;
+    static constexpr Depth DEPTH = {YV_P};
     static constexpr bool GROUPED = true;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return block_ptr(b, e, n0, K, 1024, 16, lane);
@@ -172,31 +234,20 @@ struct Wt<YVMOE_W_FP8> {
         Frag16 f;
         f.u[0] = make_uint4(o[0], o[1], o[2], o[3]);
         f.u[1] = make_uint4(o[4], o[5], o[6], o[7]);
-        acc = mfma16(f.v[0], a.f.v[0], acc);
-        acc = mfma16(f.v[1], a.f.v[1], acc);
+        acc = mfma16(a.f.v[0], f.v[0], acc);
+        acc = mfma16(a.f.v[1], f.v[1], acc);
     }
 };
 
-// int4: a nibble q at bits 3-6 of 0x4180 is the bf16 number 16 + q, so two codes cost one shift and
-// one and-or; the products' sum is Σ x (16 + q), and one more MFMA with a constant operand gives
-// -24 Σ x for the group, which makes it Σ x (q - 8). Both are fp32 sums of exact products. Dword
-// j of an operand then holds columns j and j + 4 of eight, and the activations are put in that order.
+// int4: a byte of value q < 16 is the e4m3 number q / 512, so two codes cost a conversion to bf16 and a
+// share of the masks; the products' sum is Σ x q / 512, and one more MFMA with a constant operand gives
+// -8 / 512 Σ x for the group, which makes it Σ x (q - 8) / 512. All are fp32 sums of exact products. The
+// operand's columns then are 0, 2, 4, 6, 1, 3, 5, 7 of eight, and activations are kept in that order.
 template <>
 struct Wt<YVMOE_W_INT4> {
     typedef uint2 Raw;
-    struct Act : ActB16 {
-        __device__ __forceinline__ void order() {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint4 v = f.u[h];
-                f.u[h] = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u),
-                                    __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-                                    __builtin_amdgcn_perm(v.w, v.y, 0x05040100u),
-                                    __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
-            }
-        }
-    };
-    static constexpr int UNIT = 2;
+    typedef ActB16 Act;
+    static constexpr Depth DEPTH = {YV_Q};
     static constexpr bool GROUPED = true;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return block_ptr(b, e / 2, n0, K, 512, 8, lane);
@@ -205,68 +256,98 @@ struct Wt<YVMOE_W_INT4> {
         r = nt_load8(p + (size_t)ks * 512);
     }
     static __device__ __forceinline__ uint4 codes(unsigned w) {
-        return make_uint4(((w << 3) & 0x00780078u) | 0x41804180u, ((w >> 1) & 0x00780078u) | 0x41804180u,
-                          ((w >> 5) & 0x00780078u) | 0x41804180u, ((w >> 9) & 0x00780078u) | 0x41804180u);
+        const int lo = (int)(w & 0x0F0F0F0Fu), hi = (int)(w >> 4 & 0x0F0F0F0Fu);
+        return make_uint4(__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
+                          __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
+                          __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
+                          __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true)));
     }
     static __device__ __forceinline__ void offset(const Act& a, f32x4& corr) {
         Frag16 c;
-        c.u[0] = make_uint4(0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u);  // -24
-        corr = mfma16(c.v[0], a.f.v[0], corr);
-        corr = mfma16(c.v[0], a.f.v[1], corr);
+        c.u[0] = make_uint4(0xBC80BC80u, 0xBC80BC80u, 0xBC80BC80u, 0xBC80BC80u);  // -8 / 512
+        corr = mfma16(a.f.v[0], c.v[0], corr);
+        corr = mfma16(a.f.v[1], c.v[0], corr);
     }
     static __device__ __forceinline__ void mma(const Raw& r, const Act& a, f32x4& acc) {
         Frag16 f;
         f.u[0] = codes(r.x);
         f.u[1] = codes(r.y);
-        acc = mfma16(f.v[0], a.f.v[0], acc);
-        acc = mfma16(f.v[1], a.f.v[1], acc);
+        acc = mfma16(a.f.v[0], f.v[0], acc);
+        acc = mfma16(a.f.v[1], f.v[1], acc);
     }
 };
+// Eight columns of bf16 activations in int4's order; its inverse place of a column is int4_place.
+__device__ __forceinline__ uint4 int4_order(const uint4& v) {
+    return make_uint4(__builtin_amdgcn_perm(v.y, v.x, 0x05040100u), __builtin_amdgcn_perm(v.w, v.z, 0x05040100u),
+                      __builtin_amdgcn_perm(v.y, v.x, 0x07060302u), __builtin_amdgcn_perm(v.w, v.z, 0x07060302u));
+}
+__device__ __forceinline__ int int4_place(int col) { return (col & ~7) | (col & 7) >> 1 | (col & 1) << 2; }
 
-// fp32: rows as they are, 64 bytes per lane and k-step, on the fp32 MFMAs.
+// fp32: rows as they are, on the fp32 MFMAs. Lane group g holds columns 16 i + 4 g .. 16 i + 4 g + 3 for
+// i = 0..3, so that a load of 16 bytes takes 64 of a row.
 template <>
 struct Wt<YVMOE_W_F32> {
     struct Raw {
-        float4 v[4];
+        uint4 v[4];
     };
     struct Act {
-        float4 v[4];
-        static constexpr int BYTES = 4;
-        __device__ __forceinline__ void load(const char* row, int ks) {
-            const float4* p = (const float4*)(row + (size_t)ks * 256);
+        uint4 v[4];
+        static constexpr int BYTES = 4, LANE = 4;
+        template <bool FRESH>
+        __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t b, unsigned row, int ks) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = p[i];
+            for (int i = 0; i < 4; ++i) v[i] = act_load16<FRESH>(b, row + ks * 256 + 64 * i);
+        }
+        __device__ __forceinline__ void read(const char* row, int ks) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = *(const uint4*)(row + ks * 256 + 64 * i);
         }
     };
-    static constexpr int UNIT = 1;
+    static constexpr Depth DEPTH = {YV_F};
     static constexpr bool GROUPED = false;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
-        return (const char*)b + (e + (long long)(n0 + (lane & 15)) * K + 16 * (lane >> 4)) * 4;
+        return (const char*)b + (e + (long long)(n0 + (lane & 15)) * K + 4 * (lane >> 4)) * 4;
     }
     static __device__ __forceinline__ void load(Raw& r, const char* p, int ks) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint4 u = nt_load16(p + (size_t)ks * 256 + 16 * i);
-            r.v[i] = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
-        }
+        for (int i = 0; i < 4; ++i) r.v[i] = nt_load16(p + (size_t)ks * 256 + 64 * i);
     }
     static __device__ __forceinline__ void mma(const Raw& w, const Act& a, f32x4& acc) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w.v[i].x, a.v[i].x, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w.v[i].y, a.v[i].y, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w.v[i].z, a.v[i].z, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w.v[i].w, a.v[i].w, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.v[i].x), __uint_as_float(w.v[i].x), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.v[i].y), __uint_as_float(w.v[i].y), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.v[i].z), __uint_as_float(w.v[i].z), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.v[i].w), __uint_as_float(w.v[i].w), acc, 0, 0, 0);
         }
     }
 };
 
+// Activation rows that fit are kept in LDS, padded so that 16 rows' pieces fall on different banks.
+constexpr int kActBytes = 84 << 10, kRowPad = 16;
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef const __attribute__((address_space(1))) void* gbl_ptr_t;
+
+// Loads nrows rows of bytes (a multiple of 128) straight into LDS; done when the loads are. FRESH as above.
+template <bool FRESH>
+__device__ __forceinline__ void stage_rows(const void* src, int nrows, int bytes, char* lds, int wave, int lane) {
+    const int pieces = (bytes + 1023) / 1024;  // of a row, 16 bytes per lane
+    for (int i = wave; i < nrows * pieces; i += kWaves + 1) {
+        const int row = i / pieces, at = (i - row * pieces) * 1024;
+        if (at + 16 * lane < bytes)
+            __builtin_amdgcn_global_load_lds((gbl_ptr_t)((const char*)src + (long long)row * bytes + at + 16 * lane),
+                                             (lds_ptr_t)(lds + row * (bytes + kRowPad) + at), 16, 0, FRESH ? 16 : 0);
+    }
+}
+
 // NM matrices' 16 rows from n0 against one set of activation rows.
 template <int WF, int NM>
 struct Operands {
+    typedef typename Wt<WF>::Act Act;
     const char* w[NM];
-    const void* s[NM];  // GROUPED: the scales of these rows (int4: of the lane's row)
-    const char* act;    // the lane's activation row at its columns
+    const void* s[NM];  // the scales: int8, int4 of the lane's row, fp8 of these rows
+    __amdgpu_buffer_rsrc_t buf;  // the activations, and the lane's row in them at its columns
+    unsigned off;
 
     __device__ __forceinline__ void set(int m, const void* base, const void* scales, long long e, int out, int K,
                                         int n0, int lane) {
@@ -275,23 +356,40 @@ struct Operands {
             s[m] = (const unsigned short*)scales + (e * out + n0 + (lane & 15)) * (K / 128);
         else if constexpr (WF == YVMOE_W_FP8)
             s[m] = (const float*)scales + (e * (out / 128) + n0 / 128) * (K / 128);
+        else if constexpr (WF == YVMOE_W_INT8)
+            s[m] = (const unsigned short*)scales + e * out + n0 + (lane & 15);
         else s[m] = nullptr;
     }
-    __device__ __forceinline__ void rows(const void* base, long long row, int K, int lane) {
-        act = (const char*)base + (row * K + 16 * (lane >> 4)) * Wt<WF>::Act::BYTES;
+    // row < 0: a lane without a row, whose loads give zero and read nothing. LDS: where stage_rows puts
+    // the rows (such a lane then reads some row; its products are not used).
+    template <bool LDS>
+    __device__ __forceinline__ void rows(const void* base, int nrows, int row, int K, int lane) {
+        if constexpr (LDS) {
+            off = (unsigned)((row < 0 ? 0 : row) * (K * Act::BYTES + kRowPad) + Act::LANE * (lane >> 4) * Act::BYTES);
+            return;
+        }
+        buf = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, nrows * K * Act::BYTES, 0x00027000);
+        off = row < 0 ? 0x80000000u : (unsigned)(row * K + Act::LANE * (lane >> 4)) * Act::BYTES;
     }
 };
 
-template <int WF, int NM>
+// A chunk in flight: its weights with their scales, and where its activations are.
+template <int WF, int NM, bool LDS>
 struct Chunk {
     typedef Wt<WF> W;
-    static constexpr int U = W::UNIT;
+    static constexpr int U = W::DEPTH.unit(NM, LDS);
     typename W::Raw w[U][NM];
-    typename W::Act a[U];
     float s[W::GROUPED ? U / 2 : 1][NM];
+    float rs[NM];  // int8: the row's scale
+    int c;
+    unsigned act;
 
-    // k-steps past the end: the last one again, not used
-    __device__ __forceinline__ void load_weights(const Operands<WF, NM>& o, int c, int nks) {
+    // k-steps past the end: the last one again, not used. int8's scales with every chunk: loads on one
+    // path only would make the compiler wait for them at once.
+    template <class Ops>
+    __device__ __forceinline__ void load_weights(const Ops& o, int chunk, int nks) {
+        c = chunk;
+        act = o.off;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int ks = min(c * U + u, nks - 1);
@@ -300,95 +398,135 @@ struct Chunk {
                 W::load(w[u][m], o.w[m], ks);
                 if constexpr (W::GROUPED)
                     if (u % 2 == 0)
-                        s[u / 2][m] = WF == YVMOE_W_INT4 ? bf16_to_f32(((const unsigned short*)o.s[m])[ks / 2])
+                        s[u / 2][m] = WF == YVMOE_W_INT4 ? 512.0f * bf16_to_f32(((const unsigned short*)o.s[m])[ks / 2])
                                                          : ((const float*)o.s[m])[ks / 2];
             }
         }
+        if constexpr (WF == YVMOE_W_INT8)
+#pragma unroll
+            for (int m = 0; m < NM; ++m) rs[m] = bf16_to_f32(*(const unsigned short*)o.s[m]);
     }
-    __device__ __forceinline__ void load_acts(const Operands<WF, NM>& o, int c, int nks) {
+};
+template <int WF, int NM, bool LDS>
+struct Acts {
+    static constexpr int U = Wt<WF>::DEPTH.unit(NM, LDS);
+    typename Wt<WF>::Act a[U];
+    template <bool FRESH>
+    __device__ __forceinline__ void load(const Chunk<WF, NM, LDS>& q, __amdgpu_buffer_rsrc_t buf, int nks) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) a[u].load(o.act, min(c * U + u, nks - 1));
+        for (int u = 0; u < U; ++u) a[u].template load<FRESH>(buf, q.act, min(q.c * U + u, nks - 1));
     }
-    __device__ __forceinline__ void mma(int c, int nks, f32x4 (&acc)[NM]) {
-        if constexpr (!W::GROUPED) {
+    __device__ __forceinline__ void read(const Chunk<WF, NM, LDS>& q, const char* lds, int nks) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (c * U + u < nks)
+        for (int u = 0; u < U; ++u) a[u].read(lds + q.act, min(q.c * U + u, nks - 1));
+    }
+};
+
+// ORDER: the activations are as the caller has them, not in int4's order yet.
+template <int WF, int NM, bool LDS, bool ORDER>
+__device__ __forceinline__ void mma(const Chunk<WF, NM, LDS>& q, Acts<WF, NM, LDS>& x, int nks, f32x4 (&acc)[NM]) {
+    typedef Wt<WF> W;
+    const int c = q.c;
+    constexpr int U = W::DEPTH.unit(NM, LDS);
+    if constexpr (!W::GROUPED) {
 #pragma unroll
-                    for (int m = 0; m < NM; ++m) W::mma(w[u][m], a[u], acc[m]);
-        } else {
+        for (int u = 0; u < U; ++u)
+            if (c * U + u < nks)
 #pragma unroll
-            for (int p = 0; p < U; p += 2) {
-                if (c * U + p >= nks) break;
-                f32x4 part[NM], corr = {0.f, 0.f, 0.f, 0.f};
+                for (int m = 0; m < NM; ++m) W::mma(q.w[u][m], x.a[u], acc[m]);
+    } else {
 #pragma unroll
-                for (int m = 0; m < NM; ++m) part[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < U; p += 2) {
+            if (c * U + p >= nks) break;
+            f32x4 part[NM], corr = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int u = p; u < p + 2; ++u) {
-                    if constexpr (WF == YVMOE_W_INT4) {
-                        a[u].order();
-                        W::offset(a[u], corr);
-                    }
+            for (int m = 0; m < NM; ++m) part[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int m = 0; m < NM; ++m) W::mma(w[u][m], a[u], part[m]);
+            for (int u = p; u < p + 2; ++u) {
+                if constexpr (WF == YVMOE_W_INT4) {
+                    if constexpr (ORDER)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) x.a[u].f.u[h] = int4_order(x.a[u].f.u[h]);
+                    W::offset(x.a[u], corr);
                 }
 #pragma unroll
-                for (int m = 0; m < NM; ++m)
+                for (int m = 0; m < NM; ++m) W::mma(q.w[u][m], x.a[u], part[m]);
+            }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (WF == YVMOE_W_INT4) {
-                            // the scale of weight row 4 g + i, from the lane that loaded it
-                            const float si = __int_as_float(__builtin_amdgcn_ds_bpermute(
-                                4 * (4 * ((threadIdx.x & 63) >> 4) + i), __float_as_int(s[p / 2][m])));
-                            acc[m][i] = __builtin_fmaf(si, part[m][i] + corr[i], acc[m][i]);
-                        } else {
-                            acc[m][i] = __builtin_fmaf(s[p / 2][m], part[m][i], acc[m][i]);
-                        }
-                    }
+            for (int m = 0; m < NM; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    acc[m][i] = __builtin_fmaf(q.s[p / 2][m], WF == YVMOE_W_INT4 ? part[m][i] + corr[i] : part[m][i],
+                                               acc[m][i]);
+        }
+    }
+}
+
+template <int WF, int NM, bool LDS>
+__device__ __forceinline__ int chunks(int K) {
+    constexpr int U = Wt<WF>::DEPTH.unit(NM, LDS);
+    return (K / 64 + U - 1) / U;
+}
+
+// A wavefront's products along a walk. The walk stands at a chunk (o, c; c past the end: nothing) with
+// its place(): whether the products up to it end there (ends) and whether they are all (all); next()
+// moves it one on, after the end to lines that everyone reads. While a chunk is multiplied, the weights
+// of the next ones and (without LDS) the activations of the next are in flight, across items too. The
+// start is apart, so that the weights' part of it can come before a wait.
+template <int WF, int NM, class Walk, bool LDS, bool FRESH = false, bool ORDER = false>
+struct Ring {
+    static constexpr int kRing = Wt<WF>::DEPTH.ring(NM, LDS);
+    static_assert(kRing <= kOwnItems - 1, "what the streams look ahead");
+    Chunk<WF, NM, LDS> q[kRing];
+    Acts<WF, NM, LDS> x[LDS ? 1 : 2];
+    typename Walk::Place place[kRing];
+
+    __device__ __forceinline__ void start_weights(Walk& w, int nks) {
+#pragma unroll
+        for (int i = 0; i < kRing - 1; ++i) {
+            q[i].load_weights(w.o, w.c, nks);
+            place[i] = w.place();
+            w.next();
+        }
+    }
+    __device__ __forceinline__ void start_acts(Walk& w, int nks) {
+        if constexpr (!LDS) x[0].template load<FRESH>(q[0], w.o.buf, nks);
+    }
+
+    template <class End>
+    __device__ __forceinline__ void run(Walk& w, const char* lds, int nks, End end) {
+        constexpr int STEPS = LDS || kRing % 2 == 0 ? kRing : 2 * kRing;
+        f32x4 acc[NM];
+#pragma unroll
+        for (int m = 0; m < NM; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+        while (true) {
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                constexpr int AHEAD = kRing - 1;
+                Chunk<WF, NM, LDS>&p = q[i % kRing], &n = q[(i + AHEAD) % kRing];
+                if constexpr (!LDS && kRing > 2) x[(i + 1) % 2].template load<FRESH>(q[(i + 1) % kRing], w.o.buf, nks);
+                n.load_weights(w.o, w.c, nks);
+                if constexpr (!LDS && kRing == 2) x[(i + 1) % 2].template load<FRESH>(n, w.o.buf, nks);
+                place[(i + AHEAD) % kRing] = w.place();
+                w.next();
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (LDS) x[0].read(p, lds, nks);
+                mma<WF, NM, LDS, ORDER>(p, x[LDS ? 0 : i % 2], nks, acc);
+                if (place[i % kRing].ends) {
+                    if constexpr (WF == YVMOE_W_INT8)
+#pragma unroll
+                        for (int m = 0; m < NM; ++m)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[m][r] = acc[m][r] * p.rs[m];
+                    end(place[i % kRing], acc);
+#pragma unroll
+                    for (int m = 0; m < NM; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (place[i % kRing].all) return;
+                }
             }
         }
     }
 };
-
-// acc += the products over chunks c0, c0 + step, ... below c1, the next chunk's loads in flight
-// during the current one's MFMAs.
-template <int WF, int NM>
-__device__ __forceinline__ void stream(const Operands<WF, NM>& o, int nks, int c0, int c1, int step,
-                                       f32x4 (&acc)[NM]) {
-    Chunk<WF, NM> q0, q1;
-    auto load = [&](Chunk<WF, NM>& q, int c) {
-        q.load_weights(o, c, nks);
-        q.load_acts(o, c, nks);
-    };
-    int c = c0;
-    if (c < c1) load(q0, c);
-    for (; c + step < c1; c += 2 * step) {
-        load(q1, c + step);
-        __builtin_amdgcn_sched_barrier(0);
-        q0.mma(c, nks, acc);
-        if (c + 2 * step < c1) load(q0, c + 2 * step);
-        __builtin_amdgcn_sched_barrier(0);
-        q1.mma(c + step, nks, acc);
-    }
-    if (c < c1) q0.mma(c, nks, acc);
-}
-
-template <int WF>
-__device__ __forceinline__ int chunks(int K) {
-    return (K / 64 + Wt<WF>::UNIT - 1) / Wt<WF>::UNIT;
-}
-
-// int8: the scales of weight rows n0 + 4 g .. n0 + 4 g + 3 on an accumulator; other formats' are in it.
-template <int WF>
-__device__ __forceinline__ void row_scale(f32x4& acc, const void* scales, long long row, int lane) {
-    if constexpr (WF == YVMOE_W_INT8) {
-        const ushort4 s = *(const ushort4*)((const unsigned short*)scales + row + 4 * (lane >> 4));
-        acc[0] = acc[0] * bf16_to_f32(s.x);
-        acc[1] = acc[1] * bf16_to_f32(s.y);
-        acc[2] = acc[2] * bf16_to_f32(s.z);
-        acc[3] = acc[3] * bf16_to_f32(s.w);
-    }
-}
 
 // Sum of the wavefronts' accumulators, in wavefront order.
 template <int NM>
@@ -405,90 +543,207 @@ __device__ __forceinline__ void sum_waves(const f32x4 (&red)[kWaves][2][64], int
     }
 }
 
-// h of the lane's activation row and four columns from col, rounded once. PUBLISH: written through to
-// where every XCD reads it.
+// h of four activation rows from row and one column, below row + n, rounded once (int4: in its order of
+// columns). PUBLISH: written through to where every XCD reads it.
 template <int WF, bool PUBLISH>
-__device__ __forceinline__ void store_h(void* h, long long row, int F, int col, const f32x4& g, const f32x4& u) {
-    float v[4];
+__device__ __forceinline__ void store_h(void* h, long long row, int n, int F, int col, const f32x4& g, const f32x4& u) {
+    const int at = WF == YVMOE_W_INT4 ? int4_place(col) : col;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = silu(g[i]) * u[i];
-    unsigned long long w[2];
-    char* p;
-    constexpr int NW = WF == YVMOE_W_F32 ? 2 : 1;
-    if constexpr (WF == YVMOE_W_F32) {
-        p = (char*)h + (row * F + col) * 4;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            w[i] = (unsigned long long)__float_as_uint(v[2 * i]) | (unsigned long long)__float_as_uint(v[2 * i + 1]) << 32;
-    } else {
-        p = (char*)h + (row * F + col) * 2;
-        w[0] = (unsigned long long)pack_bf16(v[0], v[1]) | (unsigned long long)pack_bf16(v[2], v[3]) << 32;
-    }
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-        if constexpr (PUBLISH)
-            __hip_atomic_store((unsigned long long*)p + i, w[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        else
-            ((unsigned long long*)p)[i] = w[i];
+    for (int i = 0; i < 4; ++i) {
+        if (i >= n) break;
+        const float f = silu(g[i]) * u[i];
+        if constexpr (WF == YVMOE_W_F32) {
+            float* p = (float*)h + (row + i) * F + at;
+            if constexpr (PUBLISH) __hip_atomic_store(p, f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            else *p = f;
+        } else {
+            unsigned short* p = (unsigned short*)h + (row + i) * F + at;
+            if constexpr (PUBLISH) __hip_atomic_store(p, f32_to_bf16_rne(f), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            else *p = f32_to_bf16_rne(f);
+        }
     }
 }
 
-// One gate/up item: 16 columns of F from n0 of expert e for n rows, the lane's activation row in
-// token. The wavefronts deal out K; the wavefront that ends it writes h rows from row0.
-template <int WF, bool PUBLISH>
-__device__ __forceinline__ void gate_up_item(const FewArgs& a, int e, int n0, int token, int n, long long row0,
-                                             f32x4 (&red)[kWaves][2][64], int wave, int lane, int closer) {
+// A work-group's gate/up items: 16 columns of F of a tile each. at(item) sets e, n0, row0, n and the
+// lane's token (-1: none). The items are first, first + own, ... (kOwnItems, below nitems), then, where
+// ahead is given, those that stand in ahead[it & 7] for the it-th.
+// A stream that has passed item i - 1's barrier may load item i + RING - 1 and, to know whether that is
+// its last, looks at the item after it: i + 4 at most. That one is there before item i - 1's barrier.
+struct GateUpItems {
+    int item, nitems, own;
+    const int* ahead;
+    int it;
+    __device__ __forceinline__ bool advance() {
+        ++it;
+        item = it < kOwnItems ? item + own
+               : ahead != nullptr ? __builtin_amdgcn_readfirstlane(ahead[it & 7])
+                                  : nitems;
+        return item < nitems;
+    }
+};
+
+// A streaming wavefront's way along them: the wavefronts deal out the chunks of K.
+template <int WF, bool LDS, class At>
+struct GateUpWalk {
+    struct Place {
+        bool ends, all;
+    };
+    const FewArgs& a;
+    const void* x;
+    At at;
+    GateUpItems items;
+    int nch, wave, lane;
     Operands<WF, 2> o;
-    o.set(0, a.w_gate, a.s_gate, e, a.F, a.H, n0, lane);
-    o.set(1, a.w_up, a.s_up, e, a.F, a.H, n0, lane);
-    o.rows(a.x, token, a.H, lane);
-    f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-    stream<WF, 2>(o, a.H / 64, wave, chunks<WF>(a.H), kWaves, acc);
-    red[wave][0][lane] = acc[0];
-    red[wave][1][lane] = acc[1];
-    __syncthreads();
-    if (wave != closer) return;
-    f32x4 sum[2];
-    sum_waves<2>(red, lane, sum);
-    row_scale<WF>(sum[0], a.s_gate, (long long)e * a.F + n0, lane);
-    row_scale<WF>(sum[1], a.s_up, (long long)e * a.F + n0, lane);
-    const int r = lane & 15;
-    if (r < n) store_h<WF, PUBLISH>(a.h, row0 + r, a.F, n0 + 4 * (lane >> 4), sum[0], sum[1]);
+    int c, s;
+    bool stop, final;
+
+    __device__ __forceinline__ GateUpWalk(const FewArgs& args, const void* acts, At f, const GateUpItems& list, int wv,
+                                          int ln)
+        : a(args), x(acts), at(f), items(list), nch(chunks<WF, 2, LDS>(args.H)), wave(wv), lane(ln), stop(false) {
+        enter();
+    }
+    __device__ __forceinline__ void enter() {
+        int e, n0, row0, n, token;
+        at(items.item, e, n0, row0, n, token);
+        o.set(0, a.w_gate, a.s_gate, e, a.F, a.H, n0, lane);
+        o.set(1, a.w_up, a.s_up, e, a.F, a.H, n0, lane);
+        o.template rows<LDS>(x, a.N, token, a.H, lane);
+        s = 0;
+        c = wave;
+    }
+    // every wavefront takes as many steps, chunks past the end among them, so that all end alike
+    __device__ __forceinline__ Place place() {
+        const bool last = (s + 1) * kWaves >= nch && !stop;
+        if (last) final = !items.advance();
+        return {last, last && final};
+    }
+    __device__ __forceinline__ void next() {
+        if ((s + 1) * kWaves < nch || stop) {
+            ++s;
+            c += stop ? 0 : kWaves;
+        } else if (!final) {
+            enter();
+        } else {
+            o.set(0, a.w_gate, a.s_gate, 0, a.F, a.H, 0, lane);
+            o.set(1, a.w_up, a.s_up, 0, a.F, a.H, 0, lane);
+            c = 0;
+            stop = true;
+        }
+    }
+};
+
+// Runs a list of items to their h rows; returns their number on the last wavefront. PUBLISH: h is read in
+// this launch, and x is xo (the second kernel; the first makes xo). One barrier an
+// item (red alternates between two sets): the last wavefront sums an item while the others stream the
+// next. Items past the list's own are taken from the counter (ticket), kOwnItems ahead of their turn.
+template <int WF, bool PUBLISH, bool LDS, class At>
+__device__ __forceinline__ int gate_up(const FewArgs& a, At at, GateUpItems items, f32x4 (&red)[2][kWaves][2][64],
+                                       int* ahead, unsigned* ticket, const char* lds, int wave, int lane) {
+    if (wave < kWaves) {
+        typedef GateUpWalk<WF, LDS, At> Walk;
+        Walk w(a, PUBLISH ? a.xo : a.x, at, items, wave, lane);
+        Ring<WF, 2, Walk, LDS, false, !PUBLISH> ring;
+        ring.start_weights(w, a.H / 64);
+        ring.start_acts(w, a.H / 64);
+        int it = 0;
+        ring.run(w, lds, a.H / 64, [&](const typename Walk::Place&, const f32x4 (&acc)[2]) {
+            red[it & 1][wave][0][lane] = acc[0];
+            red[it & 1][wave][1][lane] = acc[1];
+            __syncthreads();
+            ++it;
+        });
+        return 0;
+    }
+    const int limit = kOwnItems * items.own;
+    bool more;
+    do {
+        int e, n0, row0, n, token;
+        at(items.item, e, n0, row0, n, token);
+        const int it = items.it;
+        if (items.ahead != nullptr && lane == 0)
+            ahead[(it + kOwnItems) & 7] =
+                limit + (int)__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        f32x4 sum[2];
+        sum_waves<2>(red[it & 1], lane, sum);
+        const int g = lane >> 4;
+        store_h<WF, PUBLISH>(a.h, row0 + 4 * g, n - 4 * g, a.F, n0 + (lane & 15), sum[0], sum[1]);
+        more = items.advance();
+    } while (more);
+    return items.it;
 }
 
 // ---------------------------------------------------------------- first kernel
+// The router's products: 16 columns, K's chunks [c, end) dealt out to the wavefronts.
+template <int RF>
+struct RouterWalk {
+    struct Place {
+        bool ends, all;
+    };
+    Operands<RF, 1> o;
+    int c, end;
+    __device__ __forceinline__ Place place() const { return {c < end && c + kWaves >= end, c < end && c + kWaves >= end}; }
+    __device__ __forceinline__ void next() { c += kWaves; }
+};
+
 // Work-groups: the router's (16 columns, K split) items, then the shared experts' gate/up items.
 template <int WF>
-__global__ __launch_bounds__(kThreads, 4) void few_front_kernel(FewArgs a) {
+__global__ __launch_bounds__(kAllThreads, 3) void few_front_kernel(FewArgs a) {
     constexpr int RF = WF == YVMOE_W_F32 ? YVMOE_W_F32 : YVMOE_W_BF16;
-    __shared__ f32x4 red[kWaves][2][64];
+    __shared__ f32x4 red[2][kWaves][2][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15;
     int b = blockIdx.x;
-    if (b == 0 && threadIdx.x <= kRanges) a.counters[threadIdx.x * kCounterStride] = 0;
+    if (b == 0) {
+        for (int i = threadIdx.x; i < SIG_COUNT; i += kAllThreads) a.signals[32 * i] = 0;
+        if (a.hparts > 1)
+            for (int i = threadIdx.x; i < a.H / 16; i += kAllThreads) a.hcount[i] = 0;
+    }
+    if constexpr (WF == YVMOE_W_INT4)
+        for (long long i = (long long)b * kAllThreads + threadIdx.x; i < (long long)a.N * a.H / 8;
+             i += (long long)gridDim.x * kAllThreads)
+            ((uint4*)a.xo)[i] = int4_order(((const uint4*)a.x)[i]);
     const int nrouter = a.self ? a.ncols / 16 * a.nsplit : 0;
     if (b < nrouter) {
-        const int n0 = b / a.nsplit * 16, z = b % a.nsplit, nch = chunks<RF>(a.H);
-        Operands<RF, 1> o;
-        o.set(0, a.w_router, nullptr, 0, a.ld, a.H, n0, lane);
-        o.rows(a.x, min(r, a.N - 1), a.H, lane);
-        f32x4 acc[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
-        stream<RF, 1>(o, a.H / 64, z * nch / a.nsplit + wave, (z + 1) * nch / a.nsplit, kWaves, acc);
-        red[wave][0][lane] = acc[0];
+        const int n0 = b / a.nsplit * 16, z = b % a.nsplit, nch = chunks<RF, 1, false>(a.H), nks = a.H / 64;
+        RouterWalk<RF> w;
+        w.o.set(0, a.w_router, nullptr, 0, a.ld, a.H, n0, lane);
+        w.o.template rows<false>(a.x, a.N, r < a.N ? r : -1, a.H, lane);
+        w.c = z * nch / a.nsplit + wave;
+        w.end = (z + 1) * nch / a.nsplit;
+        if (wave < kWaves) red[0][wave][0][lane] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (wave < kWaves && w.c < w.end) {
+            Ring<RF, 1, RouterWalk<RF>, false> ring;
+            ring.start_weights(w, nks);
+            ring.start_acts(w, nks);
+            ring.run(w, nullptr, nks, [&](const typename RouterWalk<RF>::Place&, const f32x4 (&acc)[1]) {
+                red[0][wave][0][lane] = acc[0];
+            });
+        }
         __syncthreads();
-        if (wave != 0 || r >= a.N) return;
+        if (wave != kWaves) return;
         f32x4 sum[1];
-        sum_waves<1>(red, lane, sum);
-        *(f32x4*)(a.logits + ((long long)z * a.N + r) * a.ld + n0 + 4 * (lane >> 4)) = sum[0];
+        sum_waves<1>(red[0], lane, sum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int tok = 4 * (lane >> 4) + i;
+            if (tok < a.N) a.logits[((long long)z * a.N + tok) * a.ld + n0 + r] = sum[0][i];
+        }
         return;
     }
     b -= nrouter;
-    const int nfb = a.F / 16;
-    if (b >= a.S * nfb) return;
-    const int s = b / nfb;
-    gate_up_item<WF, false>(a, a.E + s, b % nfb * 16, min(r, a.N - 1), a.N, (long long)a.N * (a.k + s), red, wave,
-                            lane, 0);
+    const int nfb = a.F / 16, nitems = a.S * nfb;
+    if (b >= nitems) return;
+    auto at = [&](int item, int& e, int& n0, int& row0, int& n, int& token) {
+        const int s = item / nfb;
+        e = a.E + s;
+        n0 = item % nfb * 16;
+        row0 = a.N * (a.k + s);
+        n = a.N;
+        token = r < a.N ? r : -1;
+    };
+    gate_up<WF, false, false>(a, at, GateUpItems{b, b + 1, 1, nullptr, 0}, red, nullptr, nullptr, nullptr, wave, lane);
 }
 
 // ---------------------------------------------------------------- second kernel
@@ -496,67 +751,180 @@ struct FewTables {
     short expert[kFewSlots];  // of each slot, -1: none
     float p[kFewSlots];       // its probability
     float w[kFewSlots];       // its weight
+    int place[kFewSlots];     // slots of lower experts, earlier ones of its own, better ones of its own
     short pos[kFewSlots];     // its row, -1: none
     short slot[kFewSlots];    // slot of each routed row
     short first[kFewSlots];   // a routed row's place among its expert's
+    short tile[kFewSlots];    // tile of each routed row
     short tile_e[kFewTiles], tile_row0[kFewTiles], tile_n[kFewTiles];
     float score[kFewTokens];
     int counts[YVMOE_MAX_EXPERTS];
     int wave_starts[4];
-    int nrows, ntiles, cap, item[2];
+    int nrows, ntiles, cap, help;
+    int ahead[8];
 };
+
+// Logits and predictor terms of the tokens, summed over the splits, and the predictor's constants.
+struct FewLogits {
+    float z[kFewTokens][YVMOE_MAX_EXPERTS];
+    float pred[kFewTokens][3 * kPredDim];
+    float b1[kPredDim], w2[kPredDim], b2[1], bias[YVMOE_MAX_EXPERTS];
+};
+
+// Largest of the wavefront's numbers, on every lane: rows of 16 by rotation, then row to row.
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+#define YV_STEP(CTRL, ROWS) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false))
+    YV_STEP(0x128, 0xf);  // row_ror 8, 4, 2, 1
+    YV_STEP(0x124, 0xf);
+    YV_STEP(0x122, 0xf);
+    YV_STEP(0x121, 0xf);
+    YV_STEP(0x142, 0xa);  // row_bcast 15, 31
+    YV_STEP(0x143, 0xc);
+#undef YV_STEP
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// topk_token by a whole wavefront (lane l holds experts l, l + 64, ...): the same arithmetic, its 16
+// partial sums included, so the same bits. A candidate's key is its probability's bits plus one; taken
+// and NaN entries hold 0.
+template <int NV>
+__device__ __forceinline__ void topk_wave(const float* lg, const float* bias, int lane, int E, int k, int& my_id,
+                                          float& my_ts, float& my_w0) {
+#pragma clang fp contract(off)
+    float z[NV];
+    float m = -__builtin_huge_valf();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = lane + 64 * i;
+        z[i] = e < E ? (bias != nullptr ? lg[e] + bias[e] : lg[e]) : -__builtin_huge_valf();
+        if (z[i] > m) m = z[i];
+    }
+    const unsigned mb = __float_as_uint(m);  // floats' order as unsigned numbers'
+    const unsigned mo = wave_max(mb & 0x80000000u ? ~mb : mb | 0x80000000u);
+    m = __uint_as_float(mo & 0x80000000u ? mo & 0x7fffffffu : ~mo);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) z[i] = lane + 64 * i < E ? yv_expf(z[i] - m) : 0.0f;
+    // partial l: experts l, l + 16, ... in order
+    float part = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float v = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (16 * q + (lane & 15)), __float_as_int(z[i])));
+            if (64 * i + 16 * q + (lane & 15) < E) part = part + v;
+        }
+#define YV_SUMSTEP(O) part = part + rot16<O>(part)
+    YV_BFLY16(YV_SUMSTEP);
+#undef YV_SUMSTEP
+    unsigned key[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const float p = z[i] / part;
+        key[i] = (lane + 64 * i < E && p == p) ? __float_as_uint(p) + 1u : 0u;
+    }
+    my_ts = 0.0f;
+    my_id = 0;
+    for (int j = 0; j < k; ++j) {
+        unsigned b = key[0];
+#pragma unroll
+        for (int i = 1; i < NV; ++i) b = max(b, key[i]);
+        b = wave_max(b);
+        int id = 0x7fffffff;  // the lowest expert with that key
+#pragma unroll
+        for (int i = NV - 1; i >= 0; --i) {
+            const unsigned long long who = __ballot(key[i] == b);
+            if (who != 0) id = 64 * i + __ffsll(who) - 1;
+        }
+        if (b == 0) id = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] = lane + 64 * i == id ? 0u : key[i];
+        if (lane == j) {
+            my_ts = b != 0 ? __uint_as_float(b - 1u) : -1.0f;
+            my_id = id;
+        }
+    }
+    const float ts0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_ts), 0));
+    const float ej = yv_expf(my_ts - ts0);
+    float tot = 0.0f;
+    for (int j = 0; j < k; ++j) tot = tot + __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ej), j));
+    my_w0 = ej / tot;
+}
 
 // The routing of up to 16 tokens, from the logits or as given, and the tiles: up to 16 rows of one
 // expert each. Every work-group computes it; the first one also writes it out.
-__device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, bool writer) {
+__device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, FewLogits& lg, bool writer) {
 #pragma clang fp contract(off)
     const int tid = threadIdx.x, N = a.N, E = a.E, k = a.k, ns = N * k;
     if (tid == 0) {
         t.nrows = 0;
         t.cap = -1;
     }
-    for (int e = tid; e < YVMOE_MAX_EXPERTS; e += kThreads) t.counts[e] = 0;
+    if (tid < YVMOE_MAX_EXPERTS) t.counts[tid] = 0;
+    if (tid < kFewSlots) t.place[tid] = 0;
     if (a.self) {
+        const bool scores = a.cap_mode == 2;
+        const int Ep = (E + 15) / 16 * 16, terms = (a.ld - Ep) / kPredDim;
+        const int ncols = scores ? a.ld : E;
         const long long sstride = (long long)N * a.ld;
-        if (tid < 16 * N) {  // 16 lanes a token
-            const int tok = tid / kLanes, l = tid % kLanes;
-            const float* lg = a.logits + (long long)tok * a.ld;
-            auto logit = [&](int e) {
-                float v = lg[e];
-                for (int z = 1; z < a.nsplit; ++z) v = v + lg[z * sstride + e];
-                return v;
-            };
-            int id;
-            float p, w;
-            if (E <= 64) topk_token<4>(logit, a.bias, l, E, k, id, p, w);
-            else topk_token<16>(logit, a.bias, l, E, k, id, p, w);
-            if (l < k) {
-                t.expert[tok * k + l] = id < E ? (short)id : -1;
-                t.p[tok * k + l] = p;
-                t.w[tok * k + l] = w;
-                if (writer) a.out_routing.indices[tok * k + l] = id;
+        const int total = N * ncols;
+        for (int base = 0; base < total; base += 4 * kAllThreads) {
+            float part[4][4];  // unconditional loads, so that all are in flight together
+            int tok[4], col[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = min(base + j * kAllThreads + tid, total - 1);
+                tok[j] = i / ncols;
+                col[j] = i - tok[j] * ncols;
+                const float* p = a.logits + (long long)tok[j] * a.ld + col[j];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) part[j][z] = p[min(z, a.nsplit - 1) * sstride];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (base + j * kAllThreads + tid >= total) break;
+                float v = part[j][0];
+#pragma unroll
+                for (int z = 1; z < 4; ++z) v = z < a.nsplit ? v + part[j][z] : v;
+                if (col[j] < E) lg.z[tok[j]][col[j]] = v;
+                else if (col[j] >= Ep) lg.pred[tok[j]][col[j] - Ep] = v;
             }
         }
-        const int pt = tid - 256;
-        if (a.cap_mode == 2 && pt >= 0 && pt < 16 * N) {
-            const int tok = pt / kLanes;
-            const float* pr = a.logits + (long long)tok * a.ld + (E + 15) / 16 * 16;
-            const int terms = (a.ld - (E + 15) / 16 * 16) / kPredDim;
-            const float sc = predictor_token([&](int c) {
-                float v = pr[c];
-                for (int z = 1; z < a.nsplit; ++z) v = v + pr[z * sstride + c];
-                return v;
-            }, terms, a.b1, a.w2, a.b2, pt % kLanes);
-            if (pt % kLanes == 0) t.score[tok] = sc;
+        if (tid < E) lg.bias[tid] = a.bias != nullptr ? a.bias[tid] : 0.0f;
+        if (scores && tid < kPredDim) {
+            lg.b1[tid] = a.b1[tid];
+            lg.w2[tid] = a.w2[tid];
+            if (tid == 0) lg.b2[0] = a.b2[0];
+        }
+        __syncthreads();
+        const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        for (int job = wave < kWaves ? wave : 2 * N; job < (scores ? 2 * N : N); job += kWaves) {
+            if (job < N) {
+                int id;
+                float p, w;
+                const float* bias = a.bias != nullptr ? lg.bias : nullptr;
+                if (E <= 64) topk_wave<1>(lg.z[job], bias, lane, E, k, id, p, w);
+                else if (E <= 128) topk_wave<2>(lg.z[job], bias, lane, E, k, id, p, w);
+                else topk_wave<4>(lg.z[job], bias, lane, E, k, id, p, w);
+                if (lane < k) {
+                    t.expert[job * k + lane] = id < E ? (short)id : (short)-1;
+                    t.p[job * k + lane] = p;
+                    t.w[job * k + lane] = w;
+                    if (writer) a.out_routing.indices[job * k + lane] = id;
+                }
+            } else {
+                const float sc = predictor_token([&](int c) { return lg.pred[job - N][c]; }, terms, lg.b1, lg.w2,
+                                                 lg.b2, lane & 15);
+                if (lane == 0) t.score[job - N] = sc;
+            }
         }
     } else if (tid < ns) {
         const int64_t id = a.rindices[tid];
-        t.expert[tid] = id >= 0 && id < E ? (short)id : -1;
+        t.expert[tid] = id >= 0 && id < E ? (short)id : (short)-1;
         t.w[tid] = a.rweights_bf16 ? bf16_to_f32(((const unsigned short*)a.rweights)[tid])
                                    : ((const float*)a.rweights)[tid];
     }
     __syncthreads();
-    if (tid == 0 && a.self && a.cap_mode != 0) {
+    if (tid == kThreads - 1 && a.self && a.cap_mode != 0) {
         // capacity (gate.py:1096-1120) in double, the scores' mean in fp32 in token order
         double cf = a.cap_factor;
         if (a.cap_mode == 2 && N > 0) {
@@ -568,25 +936,48 @@ __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, bool
         const int cap = (int)((double)N * cf / (double)E);
         t.cap = cap < a.min_cap || N == 0 ? a.min_cap : cap;
     }
-    // a slot's row: after all slots of lower experts and the earlier ones of its own
+    // a slot's row: after all slots of lower experts and the earlier ones of its own; its rank among its
+    // expert's by probability. Several threads a slot, each over a part of the slots.
+    {
+        int threads = kThreads, pad = 1;  // slots rounded up to a power of two: pad threads a part
+        while (pad < ns) pad *= 2;
+        const int nparts = threads / pad, i = tid & (pad - 1), q = tid / pad;
+        const int len = (ns + nparts - 1) / nparts, s1 = min(ns, (q + 1) * len);
+        const int e = i < ns ? t.expert[i] : -1;
+        const float p = i < ns && a.self ? t.p[i] : 0.0f;
+        int lower = 0, before = 0, better = 0;
+        if (e >= 0) {
+            for (int s = q * len; s < s1; s += 4) {
+                int es[4];
+                float ps[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    es[j] = t.expert[min(s + j, kFewSlots - 1)];
+                    ps[j] = t.p[min(s + j, kFewSlots - 1)];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool in = s + j < s1, same = in && es[j] == e, earlier = s + j < i;
+                    lower += in && es[j] >= 0 && es[j] < e ? 1 : 0;
+                    before += same && earlier ? 1 : 0;
+                    better += same && (ps[j] > p || (ps[j] == p && earlier)) ? 1 : 0;
+                }
+            }
+            atomicAdd(&t.place[i], lower | before << 10 | better << 20);
+            if (q == 0) atomicAdd(&t.counts[e], 1);
+        }
+    }
+    __syncthreads();
     int mine = -1, before = 0, better = 0;
     if (tid < ns) {
         mine = t.expert[tid];
-        const float p = a.self ? t.p[tid] : 0.0f;
-        int pos = 0;
+        const int v = t.place[tid];
+        before = v >> 10 & 1023;
+        better = v >> 20;
+        const int pos = (v & 1023) + before;
         if (mine >= 0) {
-            for (int s = 0; s < ns; ++s) {
-                const int e = t.expert[s];
-                pos += e >= 0 && e < mine ? 1 : 0;
-                if (e == mine) {
-                    before += s < tid ? 1 : 0;
-                    if (a.self) better += t.p[s] > p || (t.p[s] == p && s < tid) ? 1 : 0;
-                }
-            }
-            pos += before;
             t.slot[pos] = (short)tid;
             t.first[pos] = (short)before;
-            atomicAdd(&t.counts[mine], 1);
             atomicAdd(&t.nrows, 1);
         }
         t.pos[tid] = mine >= 0 ? (short)pos : (short)-1;
@@ -618,13 +1009,18 @@ __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, bool
         t.tile_row0[i] = (short)tid;
         t.tile_n[i] = (short)min(16, t.counts[e] - t.first[tid]);
     }
-    if (tid < a.S) {
-        const int i = t.wave_starts[0] + t.wave_starts[1] + t.wave_starts[2] + t.wave_starts[3] + tid;
-        t.tile_e[i] = (short)(E + tid);
-        t.tile_row0[i] = (short)(ns + tid * N);
-        t.tile_n[i] = (short)N;
+    if (tid < nrows) {  // the tile that starts here, or the last one that started before
+        int i = below + (start ? 1 : 0) - 1;
+        for (int w = 0; w < (tid >> 6); ++w) i += t.wave_starts[w];
+        t.tile[tid] = (short)i;
     }
-    if (tid == 0) t.ntiles = t.wave_starts[0] + t.wave_starts[1] + t.wave_starts[2] + t.wave_starts[3];
+    const int ntiles = t.wave_starts[0] + t.wave_starts[1] + t.wave_starts[2] + t.wave_starts[3];
+    if (tid < a.S) {
+        t.tile_e[ntiles + tid] = (short)(E + tid);
+        t.tile_row0[ntiles + tid] = (short)(ns + tid * N);
+        t.tile_n[ntiles + tid] = (short)N;
+    }
+    if (tid == 0) t.ntiles = ntiles;
     __syncthreads();
     if (!writer) return;
     if (!a.self) {
@@ -647,13 +1043,15 @@ __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, bool
     if (tid == 0) *o.capacity = t.cap;
 }
 
-// How many parts of K each tile's down product is cut into, so that the wavefronts end together:
-// the fewest with the least work of the busiest wavefront.
-__device__ __forceinline__ int down_parts(int tiles, int rows, int nch) {
-    int best = 1, cost = (tiles + kWaves - 1) / kWaves * 840;  // 840: a multiple of 1 .. 8
-    for (int q = 2; q <= 8; ++q) {
-        const int c = (tiles * q + kWaves - 1) / kWaves * (840 / q);
-        if (c < cost && q * rows <= kYRows && q <= nch) {
+// How many parts of K each tile's down product is cut into, so that the wavefronts of the shares
+// work-groups that deal out the units end together: the fewest with the least work of the busiest.
+__device__ __forceinline__ int down_parts(int tiles, int rows, int nch, int shares) {
+    int best = 1;
+    float cost = 1e30f;
+    for (int q = 1; q <= 32 && q <= nch && q * rows <= kYRows; ++q) {
+        const int units = (tiles * q + shares - 1) / shares;
+        const float c = (float)((units + kWaves - 1) / kWaves) / (float)q;
+        if (c < 0.97f * cost) {
             best = q;
             cost = c;
         }
@@ -661,110 +1059,299 @@ __device__ __forceinline__ int down_parts(int tiles, int rows, int nch) {
     return best;
 }
 
+// A share's own items are done, and so are extra items that were handed out: called by one wavefront
+// when their h has been written. Whoever completes the last of the words says so to everyone.
+__device__ __forceinline__ void signal_done(const FewArgs& a, int share, int used, int extra, int handed, int lane) {
+    auto word = [&](int i) { return a.signals + 32 * i; };
+    unsigned complete = 0;
+    if (lane == 0) {
+        const unsigned bit = 1u << (share % 32), full = used - share / 32 * 32 >= 32 ? ~0u : (1u << (used % 32)) - 1u;
+        const unsigned old =
+            __hip_atomic_fetch_or(word(SIG_MARKS + share / 32), bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (old != full && (old | bit) == full) ++complete;
+        if (extra > 0 && __hip_atomic_fetch_add(word(SIG_FINISHED), (unsigned)extra, __ATOMIC_RELAXED,
+                                                __HIP_MEMORY_SCOPE_AGENT) + extra == (unsigned)handed)
+            ++complete;
+        const unsigned all = (used + 31) / 32 + (handed > 0 ? 1 : 0);
+        if (complete > 0)
+            complete = __hip_atomic_fetch_add(word(SIG_ROOT), complete, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) +
+                               complete == all;
+    }
+    if (__builtin_amdgcn_readfirstlane(complete) != 0 && lane < kGoLines)
+        __hip_atomic_store(word(SIG_GO + lane), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Waits until all is done (-1), or kPatience looks: then a share whose mark is missing, if there is one.
+// Called by one wavefront.
+__device__ __forceinline__ int wait_done(const FewArgs& a, int used, int lane) {
+    unsigned* go = a.signals + 32 * (SIG_GO + blockIdx.x % kGoLines);
+    for (int round = 0;; ++round) {
+        for (int i = 0; i < kPatience; ++i) {
+            if (__builtin_amdgcn_readfirstlane(
+                    __hip_atomic_load(go, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) != 0)
+                return -1;
+            __builtin_amdgcn_s_sleep(8);
+        }
+        unsigned m = ~0u;
+        if (lane * 32 < used) {
+            m = __hip_atomic_load(a.signals + 32 * (SIG_MARKS + lane), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (used - lane * 32 < 32) m |= ~0u << (used - lane * 32);
+        }
+        const unsigned long long open = __ballot(m != ~0u);
+        if (open != 0) {
+            // work-groups start to help at different places
+            const unsigned long long turned = open & ~((1ull << (blockIdx.x & 7)) - 1ull);
+            const int l = __ffsll(turned != 0 ? turned : open) - 1;
+            return __builtin_amdgcn_readlane(32 * lane + __ffs(~m) - 1, l);
+        }
+        if (round >= 1 << 9) return -1;  // only if another call has cleared the words
+    }
+}
+
+// Down products: an item is 16 columns of H and a share of the units (tile, part of K), which the
+// wavefronts deal out; the work-group's items are first, first + step, ...
+struct DownItems {
+    int item, step, nitems;
+    int hparts, units;
+    __device__ __forceinline__ int n0() const { return item / hparts * 16; }
+    __device__ __forceinline__ int share() const { return item % hparts; }
+    __device__ __forceinline__ int lo() const { return share() * units / hparts; }
+    __device__ __forceinline__ int hi() const { return (share() + 1) * units / hparts; }
+};
+
+template <int WF, bool LDS>
+struct DownWalk {
+    struct Place {
+        bool ends, item_ends, all, unit;  // unit: there is one, and these are its rows
+        int row, n;
+    };
+    const FewArgs& a;
+    const FewTables& t;
+    DownItems items;
+    int wave, parts, nch, nrows, lane;
+    Operands<WF, 1> o;
+    int unit, hi, c, c1, row, n;
+    bool stop;
+
+    __device__ __forceinline__ DownWalk(const FewArgs& args, const FewTables& tab, const DownItems& list, int p, int rows,
+                                        int wv, int ln)
+        : a(args), t(tab), items(list), wave(wv), parts(p), nch(chunks<WF, 1, LDS>(args.F)), nrows(rows), lane(ln), stop(false) {
+        enter_item();
+    }
+    __device__ __forceinline__ void enter_item() {
+        unit = items.lo() + wave;
+        hi = items.hi();
+        if (unit < hi) {
+            enter_unit();
+        } else {
+            nothing();
+        }
+    }
+    __device__ __forceinline__ void enter_unit() {
+        const int tile = unit / parts, part = unit - tile * parts, e = __builtin_amdgcn_readfirstlane(t.tile_e[tile]);
+        const int row0 = __builtin_amdgcn_readfirstlane(t.tile_row0[tile]);
+        n = __builtin_amdgcn_readfirstlane(t.tile_n[tile]);
+        row = part * nrows + row0;
+        o.set(0, a.w_down, a.s_down, e, a.H, a.F, items.n0(), lane);
+        o.template rows<LDS>(a.h, nrows, (lane & 15) < n ? row0 + (lane & 15) : -1, a.F, lane);
+        c = part * nch / parts;
+        c1 = (part + 1) * nch / parts;
+    }
+    // no unit: a chunk past the end, from lines that everyone reads
+    __device__ __forceinline__ void nothing() {
+        o.set(0, a.w_down, a.s_down, 0, a.H, a.F, 0, lane);
+        o.template rows<LDS>(a.h, nrows, -1, a.F, lane);
+        c = nch;
+        c1 = nch + 1;
+        row = 0;
+        n = 0;
+    }
+    __device__ __forceinline__ Place place() const {
+        const bool ends = c + 1 >= c1 && !stop, item_ends = ends && unit + kWaves >= hi;
+        return {ends, item_ends, item_ends && items.item + items.step >= items.nitems, unit < hi, row, n};
+    }
+    __device__ __forceinline__ void next() {
+        if (stop) return;
+        if (c + 1 < c1) {
+            ++c;
+        } else if (unit + kWaves < hi) {
+            unit += kWaves;
+            enter_unit();
+        } else if (items.item + items.step < items.nitems) {
+            items.item += items.step;
+            enter_item();
+        } else {
+            nothing();
+            stop = true;
+        }
+    }
+};
+
+// The last wavefront's part of a down item: the weighted sum, the shared mixture and the skip residual
+// of 16 columns for every token, from the partial outputs y; shared between work-groups, the sum of
+// their sums by the last of them.
 template <int WF>
-__global__ __launch_bounds__(kThreads, 4) void few_experts_kernel(FewArgs a) {
+__device__ __forceinline__ void combine(const FewArgs& a, const FewTables& t, const DownItems& d, int parts, int nrows,
+                                        const float (&y)[kYRows][16], int lane) {
     constexpr bool F32 = WF == YVMOE_W_F32;
+    const int c = lane & 15, ns = a.N * a.k, lo = d.lo(), hi = d.hi(), n0 = d.n0();
+    const long long stride = (long long)a.N * a.H;
+    const bool alone = d.hparts == 1;
+    auto row = [&](int i, int tile) {  // the parts that this work-group has computed
+        float v = 0.0f;
+        for (int q = 0; q < parts; ++q) {
+            const int u = tile * parts + q;
+            if (alone || (u >= lo && u < hi)) v = v + y[q * nrows + i][c];
+        }
+        return v;
+    };
+    auto write = [&](int tok, float v, float sh) {
+        const long long at = (long long)tok * a.H + n0 + c;
+        v = v + sh;
+        if (a.skip != nullptr)
+            v = v + 0.1f * (F32 ? ((const float*)a.skip)[at] : bf16_to_f32(((const unsigned short*)a.skip)[at]));
+        if constexpr (F32) {
+            ((float*)a.out)[at] = v;
+            if (a.shared_out != nullptr) ((float*)a.shared_out)[at] = sh;
+        } else {
+            ((unsigned short*)a.out)[at] = f32_to_bf16_rne(v);
+            if (a.shared_out != nullptr) ((unsigned short*)a.shared_out)[at] = f32_to_bf16_rne(sh);
+        }
+    };
+    for (int tok = lane >> 4; tok < a.N; tok += 4) {
+        float v = 0.0f, sh = 0.0f;
+        for (int j = 0; j < a.k; ++j) {
+            const int p = t.pos[tok * a.k + j];
+            if (p >= 0) v = v + t.w[tok * a.k + j] * row(p, t.tile[p]);
+            else if (a.self) v = __builtin_nanf("");  // logits that are not numbers choose nothing
+        }
+        for (int s = 0; s < a.S; ++s) sh = sh + a.mix[s] * row(ns + s * a.N + tok, t.ntiles + s);
+        if (alone) {
+            write(tok, v, sh);
+        } else {
+            float* p = a.hsum + 2 * d.share() * stride + (long long)tok * a.H + n0 + c;
+            __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(p + stride, sh, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    if (alone) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    int before = 0;
+    if (lane == 0)
+        before = __hip_atomic_fetch_add(a.hcount + n0 / 16, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__builtin_amdgcn_readfirstlane(before) != d.hparts - 1) return;
+    for (int tok = lane >> 4; tok < a.N; tok += 4) {
+        float pv[kFewParts], ps[kFewParts];
+#pragma unroll
+        for (int i = 0; i < kFewParts; ++i) {
+            float* q = a.hsum + 2 * min(i, d.hparts - 1) * stride + (long long)tok * a.H + n0 + c;
+            pv[i] = __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            ps[i] = __hip_atomic_load(q + stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        float v = pv[0], sh = ps[0];
+#pragma unroll
+        for (int i = 1; i < kFewParts; ++i) {
+            v = i < d.hparts ? v + pv[i] : v;
+            sh = i < d.hparts ? sh + ps[i] : sh;
+        }
+        write(tok, v, sh);
+    }
+}
+
+template <int WF, bool LDS>
+__global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) {
+    constexpr int BYTES = WF == YVMOE_W_F32 ? 4 : 2;
     __shared__ FewTables t;
+    __shared__ __align__(16) char acts[LDS ? kActBytes : 16];
     __shared__ union {
+        FewLogits lg;
         f32x4 red[2][kWaves][2][64];
-        float y[kYRows][16];
+        float y[2][kYRows][16];
     } u;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 15;
-    few_routing(a, t, blockIdx.x == 0);
+    const int r = lane & 15, grid = gridDim.x;
+    if constexpr (LDS) stage_rows<false>(a.xo, a.N, a.H * BYTES, acts, wave, lane);
+    few_routing(a, t, u.lg, blockIdx.x == 0);
     if (a.N == 0) return;
+    if constexpr (LDS) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
     const int ns = a.N * a.k;
 
-    // gate/up: the items' ranges, one per XCD, taken by its work-groups first
+    // gate/up: this work-group's items, then, if it waits long, the missing ones of others
     const int nfb = a.F / 16, nitems = t.ntiles * nfb;
-    int range = blockIdx.x % kRanges, done = 0;
-    auto range_start = [&](int i) { return (int)((long long)nitems * i / kRanges); };
-    auto take = [&]() {  // thread 0: the next item, -1: none left
-        for (int i = 0; i < kRanges; ++i) {
-            const int n = range_start(range + 1) - range_start(range);
-            const int got = __hip_atomic_fetch_add(a.counters + range * kCounterStride, 1, __ATOMIC_RELAXED,
-                                                   __HIP_MEMORY_SCOPE_AGENT);
-            if (got < n) return range_start(range) + got;
-            range = (range + 1) % kRanges;
-        }
-        return -1;
+    auto at = [&](int item, int& e, int& n0, int& row0, int& n, int& token) {
+        const int tile = item / nfb;
+        n0 = (item - tile * nfb) * 16;
+        e = __builtin_amdgcn_readfirstlane(t.tile_e[tile]);
+        row0 = __builtin_amdgcn_readfirstlane(t.tile_row0[tile]);
+        n = __builtin_amdgcn_readfirstlane(t.tile_n[tile]);
+        token = r < n ? t.slot[row0 + r] / a.k : -1;
     };
-    if (tid == 0) t.item[0] = take();
-    __syncthreads();
-    for (int it = 0;; ++it) {
-        const int item = __builtin_amdgcn_readfirstlane(t.item[it & 1]);
-        if (item < 0) break;
-        if (tid == 0) t.item[(it + 1) & 1] = take();
-        const int tile = item / nfb, n0 = item % nfb * 16;
-        const int e = t.tile_e[tile], row0 = t.tile_row0[tile], n = t.tile_n[tile];
-        const int token = t.slot[row0 + min(r, n - 1)] / a.k;
-        gate_up_item<WF, true>(a, e, n0, token, n, row0, u.red[it & 1], wave, lane, it & (kWaves - 1));
-        ++done;
-    }
-    // h is written through; once this work-group's stores are there, say so
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    int* flag = a.counters + kRanges * kCounterStride;
-    if (tid == 0) {
-        if (done > 0) __hip_atomic_fetch_add(flag, done, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        int ok = 0;
-        for (int i = 0; i < kSpinLimit && !ok; ++i) {
-            ok = __hip_atomic_load(flag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nitems;
-            if (!ok) __builtin_amdgcn_s_sleep(2);
+    // Work-groups with items: all, or so many that a few rounds come out even.
+    const int rounds = (nitems + grid - 1) / grid;
+    const int used = nitems > kOwnItems * grid ? grid : rounds > 0 ? (nitems + rounds - 1) / rounds : 0;
+    const int handed = max(0, nitems - kOwnItems * used), hitems = a.H / 16 * a.hparts;
+    if ((int)blockIdx.x >= used && (int)blockIdx.x >= hitems) return;
+    const int ntiles = t.ntiles + a.S, nrows = ns + a.S * a.N;
+    const int parts = down_parts(ntiles, nrows, chunks<WF, 1, LDS>(a.F), a.hparts);
+    const DownItems down{(int)blockIdx.x, grid, hitems, a.hparts, ntiles * parts};
+    auto stage_h = [&]() {
+        if constexpr (LDS) {
+            stage_rows<true>(a.h, nrows, a.F * BYTES, acts, wave, lane);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
         }
-        t.item[0] = ok;
-    }
-    __syncthreads();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    const bool ok = t.item[0] != 0;
-
-    // down: 16 columns of H of every tile, the units (tile, part of K) dealt out to the wavefronts
-    const int ntiles = t.ntiles + a.S, nrows = ns + a.S * a.N, nch = chunks<WF>(a.F);
-    const int parts = down_parts(ntiles, nrows, nch);
-    for (int hb = blockIdx.x; hb < a.H / 16; hb += gridDim.x) {
-        const int n0 = hb * 16;
-        for (int unit = wave; unit < ntiles * parts; unit += kWaves) {
-            const int tile = unit / parts, q = unit % parts;
-            const int e = t.tile_e[tile], row0 = t.tile_row0[tile], n = t.tile_n[tile];
-            Operands<WF, 1> o;
-            o.set(0, a.w_down, a.s_down, e, a.H, a.F, n0, lane);
-            o.rows(a.h, row0 + min(r, n - 1), a.F, lane);
-            f32x4 acc[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
-            stream<WF, 1>(o, a.F / 64, q * nch / parts, (q + 1) * nch / parts, 1, acc);
-            row_scale<WF>(acc[0], a.s_down, (long long)e * a.H + n0, lane);
-            if (r < n) *(f32x4*)&u.y[q * nrows + row0 + r][4 * (lane >> 4)] = acc[0];
-        }
-        __syncthreads();
-        if (tid < 16 * a.N) {
-            const int tok = tid / 16, c = tid % 16;
-            auto row = [&](int i) {
-                float v = u.y[i][c];
-                for (int q = 1; q < parts; ++q) v = v + u.y[q * nrows + i][c];
-                return v;
-            };
-            float v = 0.0f;
-            for (int j = 0; j < a.k; ++j) {
-                const int p = t.pos[tok * a.k + j];
-                if (p >= 0) v = v + t.w[tok * a.k + j] * row(p);
-                else if (a.self) v = __builtin_nanf("");  // logits that are not numbers choose nothing
-            }
-            const long long at = (long long)tok * a.H + n0 + c;
-            float sh = 0.0f;
-            for (int s = 0; s < a.S; ++s) sh = sh + a.mix[s] * row(ns + s * a.N + tok);
-            v = v + sh;
-            if (a.skip != nullptr)
-                v = v + 0.1f * (F32 ? ((const float*)a.skip)[at] : bf16_to_f32(((const unsigned short*)a.skip)[at]));
-            if (!ok) v = __builtin_nanf("");
-            if constexpr (F32) {
-                ((float*)a.out)[at] = v;
-                if (a.shared_out != nullptr) ((float*)a.shared_out)[at] = sh;
-            } else {
-                ((unsigned short*)a.out)[at] = f32_to_bf16_rne(v);
-                if (a.shared_out != nullptr) ((unsigned short*)a.shared_out)[at] = f32_to_bf16_rne(sh);
+    };
+    for (int share = blockIdx.x, own = 1;; own = 0) {
+        if (share < used) {
+            int* ahead = own && handed > 0 ? t.ahead : nullptr;
+            const int done = gate_up<WF, true, LDS>(a, at, GateUpItems{share, nitems, used, ahead, 0}, u.red, ahead,
+                                                    a.signals + 32 * SIG_TICKET, acts, wave, lane);
+            if (wave == kWaves) {
+                // h is written through: once the stores are there, it may be said
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                signal_done(a, share, used, max(0, done - kOwnItems), handed, lane);
             }
         }
+        if ((int)blockIdx.x >= hitems) return;
+        if (wave < kWaves) {
+            typedef DownWalk<WF, LDS> Walk;
+            Walk w(a, t, down, parts, nrows, wave, lane);
+            Ring<WF, 1, Walk, LDS, true> ring;
+            ring.start_weights(w, a.F / 64);  // no h is needed for these
+            __syncthreads();
+            share = __builtin_amdgcn_readfirstlane(t.help);
+            if (share >= 0) continue;
+            stage_h();
+            ring.start_acts(w, a.F / 64);
+            int it = 0;
+            ring.run(w, acts, a.F / 64, [&](const typename Walk::Place& p, const f32x4 (&acc)[1]) {
+                if (p.unit)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (4 * (lane >> 4) + i < p.n) u.y[it & 1][p.row + 4 * (lane >> 4) + i][r] = acc[0][i];
+                if (p.item_ends) {
+                    __syncthreads();
+                    ++it;
+                }
+            });
+            return;
+        }
+        const int m = nitems > 0 ? wait_done(a, used, lane) : -1;
+        if (lane == 0) t.help = m;
         __syncthreads();
+        share = m;
+        if (share >= 0) continue;
+        stage_h();
+        DownItems d = down;
+        for (int it = 0; d.item < hitems; ++it, d.item += grid) {
+            __syncthreads();
+            combine<WF>(a, t, d, parts, nrows, u.y[it & 1], lane);
+        }
+        return;
     }
 }
 
@@ -774,7 +1361,7 @@ int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, cons
                const int64_t* rindices, const yvmoe_expert_weights* w, const float* mix, const void* skip, void* out,
                void* shared_out, const yvmoe_routing* routing, int* invalid, char* ws, hipStream_t st) {
     const int E = w->num_routed, S = w->num_shared, H = w->hidden, F = w->ffn;
-    const FewWs L = few_ws(N, k, E, S, H, F, act);
+    const FewWs L = few_ws(N, k, E, S, H, F, w->format, act);
     FewArgs a{};
     a.x = x;
     a.N = N, a.H = H, a.F = F, a.E = E, a.S = S, a.k = k;
@@ -797,19 +1384,28 @@ int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, cons
     a.invalid = invalid;
     a.mix = mix, a.skip = skip, a.out = out, a.shared_out = shared_out;
     a.h = ws + L.h;
-    a.counters = (int*)(ws + L.counters);
-    const int front = (a.self ? a.ncols / 16 * a.nsplit : 0) + S * (F / 16);
+    a.xo = w->format == YVMOE_W_INT4 ? (const void*)(ws + L.xo) : x;
+    a.signals = (unsigned*)(ws + L.signals);
+    a.hparts = few_hparts(N, k, E, S, H, F, w->format);
+    a.hcount = (int*)(ws + L.hcount);
+    a.hsum = (float*)(ws + L.hsum);
+    int front = (a.self ? a.ncols / 16 * a.nsplit : 0) + S * (F / 16);
+    if (w->format == YVMOE_W_INT4) front = std::max(front, ceil_div(N * (H / 8), kAllThreads));
     // two work-groups per CU, fewer where neither half has work for them
-    const int items = std::max(std::min(N * k, E) * (F / 16), H / 16);
-    const int grid = N == 0 ? 1 : std::min(512, items);
-#define YV_FEW(WFV)                                                                          \
-    do {                                                                                     \
-        if (N > 0) {                                                                         \
-            few_front_kernel<WFV><<<std::max(front, 1), kThreads, 0, st>>>(a);               \
-            YV_LAUNCH_CHECK("few_front");                                                    \
-        }                                                                                    \
-        few_experts_kernel<WFV><<<grid, kThreads, 0, st>>>(a);                               \
-        YV_LAUNCH_CHECK("few_experts");                                                      \
+    const int items = std::max(std::min(N * k, E) * (F / 16), H / 16 * a.hparts);
+    const int grid = N == 0 ? 1 : std::min(kGrid, items);
+    const int esz = act == YVMOE_ACT_BF16 ? 2 : 4;
+    const bool lds = (long long)N * (H * esz + kRowPad) <= kActBytes &&
+                     (long long)N * (k + S) * (F * esz + kRowPad) <= kActBytes;
+#define YV_FEW(WFV)                                                                             \
+    do {                                                                                        \
+        if (N > 0) {                                                                            \
+            few_front_kernel<WFV><<<std::max(front, 1), kAllThreads, 0, st>>>(a);               \
+            YV_LAUNCH_CHECK("few_front");                                                       \
+        }                                                                                       \
+        if (lds) few_experts_kernel<WFV, true><<<grid, kAllThreads, 0, st>>>(a);                \
+        else few_experts_kernel<WFV, false><<<grid, kAllThreads, 0, st>>>(a);                   \
+        YV_LAUNCH_CHECK("few_experts");                                                         \
     } while (0)
     switch (w->format) {
         case YVMOE_W_F32: YV_FEW(YVMOE_W_F32); break;

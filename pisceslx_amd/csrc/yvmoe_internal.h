@@ -5,6 +5,9 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "../../include/yvmoe.h"
 
 namespace yvmoe {
@@ -251,17 +254,41 @@ inline DispatchWs dispatch_ws(int N, int k, int E, int H, int F, int act) {
     return w;
 }
 
-// The few-token layer (yvmoe_few.hip): counters, the router's logits in up to four K splits, h.
-constexpr int kFewTokens = YVMOE_FEW_TOKENS;
+// The few-token layer (yvmoe_few.hip): signals and partial sums of work-groups, the
+// router's logits in up to four K splits, h.
+constexpr int kFewTokens = YVMOE_FEW_TOKENS, kFewSignalBytes = 48 * 128;
 inline int few_splits(int H) { return H >= 4096 ? 4 : H >= 1024 ? H / 1024 : 1; }
+// Work-groups that share 16 columns of H of the down product, by the time of the rounds of kFewGrid
+// work-groups: a column group's weights (of the experts that N tokens touch) at a CU's 25 GB/s, and
+// some 3 us around each item. (H 5120: 320 groups are two rounds alone, or five of quarters.)
+constexpr int kFewParts = 8, kFewGrid = 256;
+inline int few_hparts(int N, int k, int E, int S, int H, int F, int wf) {
+    const double each = wf == YVMOE_W_F32 ? 4 : wf == YVMOE_W_BF16 ? 2 : wf == YVMOE_W_INT4 ? 0.5 : 1;
+    const double tiles = std::min((double)N * k, E * (1.0 - std::pow(std::max(0.0, 1.0 - (double)k / E), N)) + 0.5) + S;
+    const double us = tiles * 16 * F * each / 25e3;
+    int best = 1;
+    double cost = 1e30;
+    for (int p = 1; p <= kFewParts; ++p) {
+        const double c = ceil_div(H / 16 * p, kFewGrid) * (us / p + 3.0) + (p > 1 ? 2.0 : 0.0);
+        if (c < 0.97 * cost) {
+            best = p;
+            cost = c;
+        }
+    }
+    return best;
+}
 struct FewWs {
-    size_t counters, logits, h, bytes;
+    size_t signals, hcount, hsum, logits, xo, h, bytes;
 };
-inline FewWs few_ws(int N, int k, int E, int S, int H, int F, int act) {
+inline FewWs few_ws(int N, int k, int E, int S, int H, int F, int wf, int act) {
     FewWs w{};
     size_t o = 0;
-    w.counters = o; o = align_up(o + 9 * 128, 256);
+    w.signals = o;  o = align_up(o + kFewSignalBytes, 256);
+    w.hcount = o;   o = align_up(o + (size_t)H / 16 * 4, 256);
+    const int parts = few_hparts(N, k, E, S, H, F, wf);
+    w.hsum = o;     o = align_up(o + (parts > 1 ? (size_t)parts * 2 * N * H * 4 : 0), 256);
     w.logits = o;   o = align_up(o + (size_t)few_splits(H) * N * router_ld(E, act) * 4, 256);
+    w.xo = o;       o = align_up(o + (wf == YVMOE_W_INT4 ? (size_t)N * H * 2 : 0), 256);
     w.h = o;        o = align_up(o + (size_t)N * (k + S) * F * (act == YVMOE_ACT_BF16 ? 2 : 4), 256);
     w.bytes = o;
     return w;
