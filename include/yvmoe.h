@@ -419,7 +419,7 @@ int32_t yvmoe_rmsnorm(const void* x, int32_t act_dtype, int32_t n_tokens, int32_
  * that suits their elements; any in_features, out_features >= 1 and n_rows >= 0. out may not overlap x.
  *   codes [ceil(out/16)][ceil(in/128)] blocks of 1 KB, each 16 rows x 128 columns: byte
  *         16 (16 g + r) starts row r's columns 32 g .. 32 g + 31 (g = 0..3), eight of them in each
- *         of four dwords, columns 0, 2, 4, 6, 1, 3, 5, 7 of the eight from the lowest nibble up;
+ *         of four dwords, columns 0 .. 3 of the eight in its bytes' lower nibbles, 4 .. 7 in the upper;
  *         codes of columns past in_features are 8 (rows past out_features: any)
  *   scales [ceil(out/16)][ceil(in/128)][16] bf16
  *   pisceslx_amd/quant.py pack_linear() writes this order. codes are 16-byte, scales 8-byte aligned.

@@ -322,7 +322,7 @@ class PackedLinear:
         """The dense [out][in] weight (for checkers)."""
         ob, groups = self.codes.shape[:2]
         w = self.codes.view(torch.int32).view(ob, groups, 4, 16, 4, 1)     # [g][r][dword]
-        shift = torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], dtype=torch.int32, device=w.device)
+        shift = torch.tensor([0, 8, 16, 24, 4, 12, 20, 28], dtype=torch.int32, device=w.device)
         q = ((w >> shift) & 15).permute(0, 3, 1, 2, 4, 5).reshape(ob * 16, groups, 128)
         s = self.scales.permute(0, 2, 1).reshape(ob * 16, groups, 1)
         return ((q.float() - 8.0) * s.float()).view(ob * 16, -1)[:self.out_features, :self.in_features].to(dtype)
@@ -345,9 +345,9 @@ def pack_linear_codes(codes: torch.Tensor, scales: torch.Tensor, in_features: in
     q[:, in_features:] = 8
     q = torch.nn.functional.pad(q, (0, 0, 0, ob * 16 - out), value=8)
     s = torch.nn.functional.pad(scales, (0, 0, 0, ob * 16 - out))
-    # dword nibbles from the lowest: columns 0, 2, 4, 6, 1, 3, 5, 7; bytes hold two of them
-    q = q.view(ob, 16, groups, 4, 4, 8)[..., [0, 2, 4, 6, 1, 3, 5, 7]]     # [r][group][g][dword]
-    b = (q[..., 0::2] | (q[..., 1::2] << 4)).permute(0, 2, 3, 1, 4, 5)     # [group][g][r][dword][4]
+    # a dword's bytes: columns 0 .. 3 of eight in the lower nibbles, 4 .. 7 in the upper
+    q = q.view(ob, 16, groups, 4, 4, 8)                                    # [r][group][g][dword]
+    b = (q[..., :4] | (q[..., 4:] << 4)).permute(0, 2, 3, 1, 4, 5)         # [group][g][r][dword][4]
     return PackedLinear(in_features, out, b.reshape(ob, groups, 1024).contiguous(),
                         s.view(ob, 16, groups).permute(0, 2, 1).contiguous())
 

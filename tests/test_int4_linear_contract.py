@@ -21,13 +21,12 @@ def test_order_of_codes(K, O):
     scales = torch.rand(O, groups, generator=g).to(torch.bfloat16)
     pk = pack_linear_codes(codes, scales, K)
     q = unpack_int4(codes)
-    place = [0, 4, 1, 5, 2, 6, 3, 7]  # nibble of each of a dword's columns
     for o in range(O):
         for i in range(groups * 128):
             r, c = o % 16, i % 128
-            byte = 16 * (16 * (c // 32) + r) + c % 32 // 8 * 4 + place[c % 8] // 2
+            byte = 16 * (16 * (c // 32) + r) + c % 32 // 8 * 4 + c % 4
             b = int(pk.codes[o // 16, i // 128, byte])
-            got = b >> 4 if place[c % 8] % 2 else b & 15
+            got = b >> 4 if c % 8 >= 4 else b & 15
             assert got == (int(q[o, i]) if i < K else 8), (o, i)
         for j in range(groups):
             assert pk.scales[o // 16, j, o % 16] == scales[o, j]
