@@ -18,6 +18,8 @@
 //
 // Forms. Up to 64 rows of x: int4_few_kernel, bound by the stream of codes (out·in / 2 bytes) and at small
 // sizes by one trip to memory. More: int4_rows_kernel, bound by the MFMAs.
+#include <algorithm>
+
 #include "yvmoe_frag.h"
 #include "yvmoe_internal.h"
 
@@ -69,24 +71,37 @@ __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Eight columns of a row of x from column c, zero past the row's end.
+// Eight elements of x. The load is free of branches, so that it can stay in flight: callers let it start 8
+// before the end of x at the latest, and it may run into the next row; fix() then moves the elements to their
+// places and clears those from `valid` on. load_tiny: for an x of fewer than eight elements.
+__device__ __forceinline__ unsigned pick(bool c, unsigned a, unsigned b) { return c ? a : b; }
 template <bool F32>
 struct X8;
 template <>
 struct X8<false> {
     static constexpr int TERMS = 1;
     uint4 v;
-    __device__ __forceinline__ void load(const void* row, int c, int K) {
-        const unsigned short* p = (const unsigned short*)row + c;
-        if (c + 8 <= K) {
-            v = load_any16(p);
-        } else {
-            unsigned d[4];
+    __device__ __forceinline__ void load(const void* x, size_t at) { v = load_any16((const unsigned short*)x + at); }
+    __device__ __forceinline__ void load_tiny(const void* x, int at, int total) {
+        const unsigned short* p = (const unsigned short*)x;
+        unsigned d[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                d[i] = (c + 2 * i < K ? p[2 * i] : 0) | (unsigned)(c + 2 * i + 1 < K ? p[2 * i + 1] : 0) << 16;
-            v = make_uint4(d[0], d[1], d[2], d[3]);
-        }
+        for (int i = 0; i < 4; ++i)
+            d[i] = (at + 2 * i < total ? p[at + 2 * i] : 0) |
+                   (unsigned)(at + 2 * i + 1 < total ? p[at + 2 * i + 1] : 0) << 16;
+        v = make_uint4(d[0], d[1], d[2], d[3]);
+    }
+    __device__ __forceinline__ void fix(int shift, int valid) {
+        unsigned d[5] = {v.x, v.y, v.z, v.w, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = pick(shift & 1, d[i] >> 16 | d[i + 1] << 16, d[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = pick(shift & 2, d[i + 1], d[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = pick(shift & 4, i < 2 ? d[i + 2] : 0u, d[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = pick(valid >= 2 * i + 2, d[i], pick(valid == 2 * i + 1, d[i] & 0xffffu, 0u));
+        v = make_uint4(d[0], d[1], d[2], d[3]);
     }
     __device__ __forceinline__ void terms(bf16x8 (&t)[1]) const {
         Frag8 f;
@@ -98,18 +113,28 @@ template <>
 struct X8<true> {
     static constexpr int TERMS = 3;
     uint4 v[2];
-    __device__ __forceinline__ void load(const void* row, int c, int K) {
-        const unsigned* p = (const unsigned*)row + c;
-        if (c + 8 <= K) {
-            v[0] = load_any16(p);
-            v[1] = load_any16(p + 4);
-        } else {
-            unsigned d[8];
+    __device__ __forceinline__ void load(const void* x, size_t at) {
+        v[0] = load_any16((const unsigned*)x + at);
+        v[1] = load_any16((const unsigned*)x + at + 4);
+    }
+    __device__ __forceinline__ void load_tiny(const void* x, int at, int total) {
+        const unsigned* p = (const unsigned*)x;
+        unsigned d[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = c + i < K ? p[i] : 0u;
-            v[0] = make_uint4(d[0], d[1], d[2], d[3]);
-            v[1] = make_uint4(d[4], d[5], d[6], d[7]);
-        }
+        for (int i = 0; i < 8; ++i) d[i] = at + i < total ? p[at + i] : 0u;
+        v[0] = make_uint4(d[0], d[1], d[2], d[3]);
+        v[1] = make_uint4(d[4], d[5], d[6], d[7]);
+    }
+    __device__ __forceinline__ void fix(int shift, int valid) {
+        unsigned d[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+        for (int bit = 1; bit < 8; bit *= 2)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = pick(shift & bit, i + bit < 8 ? d[i + bit] : 0u, d[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = pick(i < valid, d[i], 0u);
+        v[0] = make_uint4(d[0], d[1], d[2], d[3]);
+        v[1] = make_uint4(d[4], d[5], d[6], d[7]);
     }
     // Three bf16 terms, each the rest's rounding: their sum has 24 bits, as x has.
     __device__ __forceinline__ void terms(bf16x8 (&t)[3]) const {
@@ -145,133 +170,175 @@ __device__ __forceinline__ void put(const LinArgs& a, int n, int o, float v) {
     }
 }
 
-// ---------------------------------------------------------------- up to 64 rows
-// A work-group computes 16 RB outputs of 16 TB rows; its eight wavefronts deal out the groups of K, each
-// with the next group's codes and the next half group's rows in flight, and add up in LDS at the end.
-template <bool F32, int TB, int RB>
-__global__ __launch_bounds__(512, 2) void int4_few_kernel(LinArgs a) {
+// ---------------------------------------------------------------- rows that fit into LDS
+// A work-group keeps all rows of x in LDS (as bf16 terms) beside each group's -8 / 512 Σ x, and computes 16 RB
+// outputs at a time; its eight wavefronts deal out the groups of K. A wavefront's stream of codes runs on
+// over the ends of outputs, D - 1 groups ahead.
+//   LDS: x [T][N][stride] | corrections [groups][16] fp32 | sums [2][7][RB][64 x 16 B]
+struct FewLds {
+    int stride, corr, sums, bytes;
+};
+__host__ __device__ inline FewLds few_lds(int N, int groups, int terms, int rb) {
+    FewLds l;
+    l.stride = groups * kGroup * 2 + 16;  // the 16 rows of an operand fall on different banks
+    l.corr = terms * N * l.stride;
+    l.sums = l.corr + groups * 64;
+    l.bytes = l.sums + 2 * 7 * rb * 1024;
+    return l;
+}
+
+template <bool F32, int RB, int D, bool TINY>
+__global__ __launch_bounds__(512, 4) void int4_few_kernel(LinArgs a) {
     constexpr int T = X8<F32>::TERMS;
-    __shared__ f32x4 red[8][RB * TB][64];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    extern __shared__ __align__(16) char lds[];
+    const FewLds l = few_lds(a.N, a.groups, T, RB);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r = lane & 15;
-    const int n0 = blockIdx.y * 16 * TB, b0 = blockIdx.x * RB;
-    const char* xrow[TB];
-#pragma unroll
-    for (int t = 0; t < TB; ++t)
-        xrow[t] = (const char*)a.x + (long long)min(n0 + 16 * t + r, a.N - 1) * a.K * (F32 ? 4 : 2);
-    const char* codes[RB];
-    const unsigned short* scales[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        const long long at = (long long)min(b0 + b, a.blocks - 1) * a.groups;
-        codes[b] = a.codes + at * 1024 + lane * 16;
-        scales[b] = a.scales + at * 16 + r;
-    }
+    const int sets = (a.blocks + RB - 1) / RB;
+    const int items = (sets - 1 - (int)blockIdx.x) / (int)gridDim.x + 1;
     struct W {
         uint4 w[RB];
         unsigned short s[RB];
     };
-    struct X {
-        X8<F32> x[2][TB];
-    };
-    auto load_w = [&](W& q, int kg) {  // groups past the end: the last one again, not used
-        kg = min(kg, a.groups - 1);
+    int ahead_item = 0, ahead_kg = min(wave, a.groups - 1);
+    auto load_w = [&](W& q) {  // after the last group: that one again, not used
+        const int set = (int)blockIdx.x + ahead_item * (int)gridDim.x;
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            q.w[b] = nt_load16(codes[b] + (long long)kg * 1024);
-            q.s[b] = scales[b][(long long)kg * 16];
+            const long long at = (long long)min(set * RB + b, a.blocks - 1) * a.groups + ahead_kg;
+            q.w[b] = nt_load16(a.codes + at * 1024 + lane * 16);
+            q.s[b] = a.scales[at * 16 + r];
         }
+        if (ahead_kg + 8 < a.groups) ahead_kg += 8;
+        else if (ahead_item + 1 < items) ahead_item += 1, ahead_kg = wave;
     };
-    auto load_x = [&](X& x, int kg, int half) {
-        kg = min(kg, a.groups - 1);
+    W q[D];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int t = 0; t < TB; ++t) x.x[j][t].load(xrow[t], kg * kGroup + 32 * g + 16 * half + 8 * j, a.K);
+    for (int d = 0; d + 1 < D; ++d) load_w(q[d]);
+    const char* xr = lds + min(r, a.N - 1) * l.stride + 64 * g;
+    float* corrs = (float*)(lds + l.corr);
+    auto operand = [&](int k, int kg, int j) {
+        Frag8 f;
+        f.u = *(const uint4*)&xr[k * a.N * l.stride + kg * 256 + 16 * j];
+        return f.v;
     };
-    f32x4 acc[RB][TB];
+    {
+        constexpr int BATCH = 4;
+        const int per_row = a.groups * 16, pieces = a.N * per_row;
+        const int total = a.N * a.K;  // fits LDS
+        for (int p0 = tid; p0 < pieces; p0 += 512 * BATCH) {
+            X8<F32> px[BATCH];
+            int row[BATCH], c[BATCH];
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int t = 0; t < TB; ++t) acc[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto group = [&](W& q, W& qn, X& x0, X& x1, int kg) {
-        f32x4 part[RB][TB], corr[TB];
-#pragma unroll
-        for (int t = 0; t < TB; ++t) {
-            corr[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int b = 0; b < RB; ++b) part[b][t] = corr[t];
-        }
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            X& x = half ? x1 : x0;
-            if (half) {
-                load_w(qn, kg + 8);
-                load_x(x0, kg + 8, 0);
-            } else {
-                load_x(x1, kg, 1);
+            for (int i = 0; i < BATCH; ++i) {
+                const int p = min(p0 + 512 * i, pieces - 1);
+                row[i] = p / per_row, c[i] = p % per_row * 8;
+                const int at = row[i] * a.K + c[i];
+                if constexpr (TINY) px[i].load_tiny(a.x, at, total);
+                else px[i].load(a.x, min(at, total - 8));
             }
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                bf16x8 c[RB];
-#pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                    const unsigned d[4] = {q.w[b].x, q.w[b].y, q.w[b].z, q.w[b].w};
-                    c[b] = codes8(d[2 * half + j]);
+            for (int i = 0; i < BATCH; ++i) {
+                if (p0 + 512 * i >= pieces) continue;
+                if (c[i] + 8 > a.K) {
+                    const int at = row[i] * a.K + c[i];
+                    px[i].fix(TINY ? 0 : min(at - min(at, total - 8), 7), a.K - c[i]);
                 }
+                bf16x8 t[T];
+                px[i].terms(t);
 #pragma unroll
-                for (int t = 0; t < TB; ++t) {
-                    bf16x8 v[T];
-                    x.x[j][t].terms(v);
-#pragma unroll
-                    for (int i = 0; i < T; ++i) {
-                        corr[t] = mfma16(v[i], minus8(), corr[t]);
-#pragma unroll
-                        for (int b = 0; b < RB; ++b) part[b][t] = mfma16(v[i], c[b], part[b][t]);
-                    }
+                for (int k = 0; k < T; ++k) {
+                    Frag8 f;
+                    f.v = t[k];
+                    *(uint4*)&lds[(k * a.N + row[i]) * l.stride + c[i] * 2] = f.u;
                 }
             }
         }
+    }
+    __syncthreads();
+    for (int kg = wave; kg < a.groups; kg += 8) {  // each wavefront the groups that it will use
+        f32x4 corr = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int k = 0; k < T; ++k) corr = mfma16(operand(k, kg, j), minus8(), corr);
+        if (r == 0) *(f32x4*)&corrs[kg * 16 + 4 * g] = corr;
+    }
+    f32x4 acc[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto group = [&](const W& q, W& qn, int kg) {
+        load_w(qn);
+        f32x4 part[RB];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) part[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            bf16x8 v[T];
+#pragma unroll
+            for (int k = 0; k < T; ++k) v[k] = operand(k, kg, j);
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                const unsigned d[4] = {q.w[b].x, q.w[b].y, q.w[b].z, q.w[b].w};
+                const bf16x8 c = codes8(d[j]);
+#pragma unroll
+                for (int k = 0; k < T; ++k) part[b] = mfma16(v[k], c, part[b]);
+            }
+        }
+        const f32x4 corr = *(const f32x4*)&corrs[kg * 16 + 4 * g];
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
             const float s = scale512(q.s[b]);
 #pragma unroll
-            for (int t = 0; t < TB; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[b][t][i] = __builtin_fmaf(s, part[b][t][i] + corr[t][i], acc[b][t][i]);
+            for (int i = 0; i < 4; ++i) acc[b][i] = __builtin_fmaf(s, part[b][i] + corr[i], acc[b][i]);
         }
     };
-    if (wave < a.groups) {
-        W q0, q1;
-        X x0, x1;
-        load_w(q0, wave);
-        load_x(x0, wave, 0);
-        int kg = wave;
-        for (; kg + 8 < a.groups; kg += 16) {
-            group(q0, q1, x0, x1, kg);
-            group(q1, q0, x0, x1, kg + 8);
+    // The end of an item: the wavefronts take turns in adding up the eight sums. They lie in one of two
+    // places in turn, so that one barrier parts the writes of an item from the reads, and these from the
+    // writes two items on.
+    auto finish = [&](int item) {
+        f32x4* place = (f32x4*)(lds + l.sums) + (item & 1) * 7 * RB * 64 + lane;
+        const int owner = item & 7, slot = (wave - owner - 1) & 7;
+        if (slot < 7)
+#pragma unroll
+            for (int b = 0; b < RB; ++b) place[(slot * RB + b) * 64] = acc[b];
+        __syncthreads();
+        if (slot == 7) {
+            const int set = (int)blockIdx.x + item * (int)gridDim.x;
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                f32x4 sum = acc[b];
+#pragma unroll
+                for (int w = 0; w < 7; ++w) {
+                    const f32x4 v = place[(w * RB + b) * 64];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] = sum[e] + v[e];
+                }
+                const int o = (set * RB + b) * 16 + r;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (o < a.O && 4 * g + e < a.N) put<F32>(a, 4 * g + e, o, sum[e]);
+            }
         }
-        if (kg < a.groups) group(q0, q1, x0, x1, kg);
+#pragma unroll
+        for (int b = 0; b < RB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    if (wave >= a.groups) {
+        for (int item = 0; item < items; ++item) finish(item);
+        return;
     }
+    for (int item = 0, kg = wave;;) {
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int t = 0; t < TB; ++t) red[wave][b * TB + t][lane] = acc[b][t];
-    __syncthreads();
-    for (int i = wave; i < RB * TB; i += 8) {
-        f32x4 sum = red[0][i][lane];
-#pragma unroll
-        for (int w = 1; w < 8; ++w) {
-            const f32x4 v = red[w][i][lane];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] = sum[e] + v[e];
+        for (int d = 0; d < D; ++d) {
+            group(q[d], q[(d + D - 1) % D], kg);
+            kg += 8;
+            if (kg >= a.groups) {
+                kg = wave;
+                finish(item);
+                if (++item == items) return;
+            }
         }
-        const int o = (b0 + i / TB) * 16 + r, n = n0 + i % TB * 16 + 4 * g;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (o < a.O && n + e < a.N) put<F32>(a, n + e, o, sum[e]);
     }
 }
 
@@ -280,18 +347,19 @@ __global__ __launch_bounds__(512, 2) void int4_few_kernel(LinArgs a) {
 // 16 TB rows. Each group's 128 columns of the rows go through LDS (as bf16 terms, two stages, rows padded by
 // 16 bytes, so that the 16 rows of an operand fall on different banks), loaded a group ahead; the codes
 // go straight to the wavefront that converts them, each once for its TB MFMAs of every term.
-template <bool F32, int TB, int RB>
+template <bool F32, int TB, int RB, int WO, int WT, int D>
 __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
-    constexpr int T = X8<F32>::TERMS, ROWS = 32 * TB, STRIDE = kGroup * 2 + 16;
-    constexpr int PER = ROWS * 16 / 512;  // pieces of 8 columns that a thread brings
-    __shared__ __align__(16) char xs[2][T][ROWS * STRIDE];
+    constexpr int WK = 8 / WO / WT;
+    constexpr int T = X8<F32>::TERMS, ROWS = 16 * TB * WT, STRIDE = kGroup * 2 + 16;
+    constexpr int PER = ROWS * WK * 16 / 512;  // pieces of 8 columns that a thread brings
+    __shared__ __align__(16) char xs[2][T][WK * ROWS * STRIDE];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r = lane & 15;
-    const int wr = wave & 3, wt = wave >> 2;
+    const int wr = wave % WO, wt = wave / WO % WT, wk = wave / (WO * WT);
     // blocks of rows fastest: work-groups that run together share their codes
     const int nrt = (a.N + ROWS - 1) / ROWS;
-    const int n0 = (int)(blockIdx.x % nrt) * ROWS, b0 = ((int)(blockIdx.x / nrt) * 4 + wr) * RB;
+    const int n0 = (int)(blockIdx.x % nrt) * ROWS, b0 = ((int)(blockIdx.x / nrt) * WO + wr) * RB;
     const char* codes[RB];
     const unsigned short* scales[RB];
 #pragma unroll
@@ -304,34 +372,49 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
         uint4 w[RB];
         unsigned short s[RB];
     };
-    auto load_w = [&](W& q, int kg) {
-        kg = min(kg, a.groups - 1);
+    auto load_w = [&](W& q, int step) {  // groups past the end: the last one's, not used
+        const int kg = min(step * WK + wk, a.groups - 1);
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
             q.w[b] = *(const uint4*)(codes[b] + (long long)kg * 1024);
             q.s[b] = scales[b][(long long)kg * 16];
         }
     };
+    // x from an element near the tile's first one on, so that 32 bits hold the rest of an address
+    const long long total = (long long)a.N * a.K, first = (long long)n0 * a.K;
+    const long long base = first < total - 8 ? first : total - 8;
+    const unsigned last = (unsigned)min(total - 8 - base, 0xFFFFFFFFLL);
+    const char* xb = (const char*)a.x + base * (F32 ? 4 : 2);
+    unsigned at[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int piece = tid + 512 * i, row = piece / (16 * WK), c = piece % (16 * WK);
+        at[i] = (unsigned)(first - base) + (unsigned)min(row, a.N - 1 - n0) * a.K + 8 * c;
+    }
     X8<F32> px[PER];
-    auto load_x = [&](int kg) {
-        kg = min(kg, a.groups - 1);
+    auto load_x = [&](int step) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int piece = tid + 512 * i, row = piece / 16, c = piece % 16;
-            px[i].load((const char*)a.x + (long long)min(n0 + row, a.N - 1) * a.K * (F32 ? 4 : 2), kg * kGroup + 8 * c, a.K);
-        }
+        for (int i = 0; i < PER; ++i) px[i].load(xb, min(at[i] + step * (WK * kGroup), last));
     };
-    auto store_x = [&](int stage) {
+    auto store_x = [&](int step) {
+        if ((step + 1) * (WK * kGroup) > a.K) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const unsigned from = at[i] + step * (WK * kGroup);
+                const int c = (tid + 512 * i) % (16 * WK) * 8 + step * (WK * kGroup);
+                px[i].fix((int)min(from - min(from, last), 7u), a.K - c);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int piece = tid + 512 * i, row = piece / 16, c = piece % 16;
+            const int piece = tid + 512 * i, row = piece / (16 * WK), c = piece % (16 * WK);
             bf16x8 t[T];
             px[i].terms(t);
 #pragma unroll
             for (int q = 0; q < T; ++q) {
                 Frag8 f;
                 f.v = t[q];
-                *(uint4*)&xs[stage][q][row * STRIDE + 16 * c] = f.u;
+                *(uint4*)&xs[step & 1][q][(c / 16 * ROWS + row) * STRIDE + 16 * (c % 16)] = f.u;
             }
         }
     };
@@ -340,9 +423,9 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
     for (int b = 0; b < RB; ++b)
 #pragma unroll
         for (int t = 0; t < TB; ++t) acc[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto group = [&](const W& q, W& qn, int kg) {
-        load_x(kg + 1);
-        load_w(qn, kg + 1);
+    auto group = [&](const W& q, W& qn, int step) {
+        load_x(step + 1);
+        load_w(qn, step + D - 1);
         bf16x8 c[RB][4];
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
@@ -360,7 +443,7 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
 #pragma unroll
                 for (int i = 0; i < T; ++i) {
                     Frag8 f;
-                    f.u = *(const uint4*)&xs[kg & 1][i][((wt * TB + t) * 16 + r) * STRIDE + 64 * g + 16 * j];
+                    f.u = *(const uint4*)&xs[step & 1][i][(wk * ROWS + (wt * TB + t) * 16 + r) * STRIDE + 64 * g + 16 * j];
                     corr = mfma16(f.v, minus8(), corr);
 #pragma unroll
                     for (int b = 0; b < RB; ++b) part[b] = mfma16(f.v, c[b][j], part[b]);
@@ -372,20 +455,45 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
                 for (int i = 0; i < 4; ++i) acc[b][t][i] = __builtin_fmaf(s, part[b][i] + corr[i], acc[b][t][i]);
             }
         }
-        store_x((kg + 1) & 1);
+        store_x(step + 1);
         __syncthreads();
     };
-    W q0, q1;
+    const int steps = (a.groups + WK - 1) / WK;
+    W q[D];
     load_x(0);
-    load_w(q0, 0);
+#pragma unroll
+    for (int d = 0; d + 1 < D; ++d) load_w(q[d], d);
     store_x(0);
     __syncthreads();
-    int kg = 0;
-    for (; kg + 1 < a.groups; kg += 2) {
-        group(q0, q1, kg);
-        group(q1, q0, kg + 1);
+    for (int step = 0;;) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            group(q[d], q[(d + D - 1) % D], step);
+            if (++step == steps) break;
+        }
+        if (step == steps) break;
     }
-    if (kg < a.groups) group(q0, q1, kg);
+    // the last step's barrier is behind: xs is free
+    if constexpr (WK > 1) {
+        f32x4* red = (f32x4*)&xs[0][0][0] + lane;
+#pragma unroll
+        for (int k = WK / 2; k >= 1; k /= 2) {
+            const int at = (wr + WO * (wt + WT * (wk % k))) * RB * TB * 64;
+            if (wk >= k && wk < 2 * k)
+#pragma unroll
+                for (int i = 0; i < RB * TB; ++i) red[at + 64 * i] = acc[i / TB][i % TB];
+            __syncthreads();
+            if (wk < k)
+#pragma unroll
+                for (int i = 0; i < RB * TB; ++i) {
+                    const f32x4 v = red[at + 64 * i];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i / TB][i % TB][e] = acc[i / TB][i % TB][e] + v[e];
+                }
+            __syncthreads();
+        }
+        if (wk > 0) return;
+    }
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
         const int o = (b0 + b) * 16 + r;
@@ -399,26 +507,36 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
     }
 }
 
-template <bool F32, int TB>
-void few_launch_rb(const LinArgs& a, hipStream_t st) {
-    // 16, 32 or 64 outputs per work-group: as many as leave four work-groups per CU
-    const int y = ceil_div(a.N, 16 * TB);
-    const long long wgs = (long long)a.blocks * y;
-    constexpr int MOST = F32 || TB > 2 ? 2 : 4;
-    if (MOST >= 4 && wgs >= 4096) int4_few_kernel<F32, TB, MOST><<<dim3(ceil_div(a.blocks, MOST), y), 512, 0, st>>>(a);
-    else if (wgs >= 1024) int4_few_kernel<F32, TB, 2><<<dim3(ceil_div(a.blocks, 2), y), 512, 0, st>>>(a);
-    else int4_few_kernel<F32, TB, 1><<<dim3(a.blocks, y), 512, 0, st>>>(a);
+constexpr int kLds = 163840;
+
+// Whether the rows fit into LDS beside the sums of RB outputs, and the launch if they do.
+template <bool F32, int RB, int D, bool TINY>
+bool few_launch(const LinArgs& a, int least, hipStream_t st) {
+    if (a.blocks < least || a.groups > kLds / (kGroup * 2)) return false;
+    const FewLds l = few_lds(a.N, a.groups, X8<F32>::TERMS, RB);
+    if (l.bytes > kLds) return false;
+    const int grid = std::min(ceil_div(a.blocks, RB), l.bytes <= kLds / 2 ? 512 : 256);
+    int4_few_kernel<F32, RB, D, TINY><<<grid, 512, l.bytes, st>>>(a);
+    return true;
+}
+template <bool F32>
+bool few_launch(const LinArgs& a, hipStream_t st) {
+    if ((long long)a.N * a.K < 8) return few_launch<F32, 2, 3, true>(a, 0, st);
+    return few_launch<F32, 4, 2, false>(a, 1536, st) || few_launch<F32, 2, 3, false>(a, 512, st) ||
+           few_launch<F32, 1, 3, false>(a, 0, st);
 }
 
-template <bool F32>
-void rows_launch(const LinArgs& a, hipStream_t st) {
-    constexpr int TB = F32 ? 2 : 4;
-    const int nrt = ceil_div(a.N, 32 * TB);
-    if ((long long)nrt * ceil_div(a.blocks, 16) >= 256)
-        int4_rows_kernel<F32, TB, 4><<<nrt * ceil_div(a.blocks, 16), 512, 0, st>>>(a);
-    else if ((long long)nrt * ceil_div(a.blocks, 8) >= 128)
-        int4_rows_kernel<F32, TB, 2><<<nrt * ceil_div(a.blocks, 8), 512, 0, st>>>(a);
-    else int4_rows_kernel<F32, TB, 1><<<nrt * ceil_div(a.blocks, 4), 512, 0, st>>>(a);
+template <bool F32, int TB, int RB, int WO, int WT, int D>
+bool rows_launch(const LinArgs& a, long long least, hipStream_t st) {
+    const long long wgs = (long long)ceil_div(a.N, 16 * TB * WT) * ceil_div(a.blocks, WO * RB);
+    if (wgs < least) return false;
+    int4_rows_kernel<F32, TB, RB, WO, WT, D><<<(unsigned)wgs, 512, 0, st>>>(a);
+    return true;
+}
+
+template <bool F32, int TB, int WO>
+void mid_launch(const LinArgs& a, hipStream_t st) {
+    if (!rows_launch<F32, TB, 2, WO, 1, 3>(a, 512, st)) rows_launch<F32, TB, 1, WO, 1, 3>(a, 0, st);
 }
 
 }  // namespace
@@ -434,15 +552,18 @@ int int4_linear_launch(const void* x, int act, int N, const yvmoe_int4_matrix* w
     a.scales = (const unsigned short*)w->scales;
     a.bias = bias, a.out = out;
     if (act == YVMOE_ACT_F32) {
-        if (N <= 16) few_launch_rb<true, 1>(a, st);
-        else if (N <= 32) few_launch_rb<true, 2>(a, st);
-        else rows_launch<true>(a, st);
+        if (N <= 16) few_launch<true>(a, st) || (mid_launch<true, 1, 2>(a, st), true);
+        else if (N <= 32) mid_launch<true, 2, 4>(a, st);
+        else if (!rows_launch<true, 2, 4, 4, 2, 2>(a, 256, st) && !rows_launch<true, 2, 2, 4, 2, 2>(a, 256, st))
+            rows_launch<true, 2, 1, 4, 2, 2>(a, 0, st);
     } else {
-        if (N <= 16) few_launch_rb<false, 1>(a, st);
-        else if (N <= 32) few_launch_rb<false, 2>(a, st);
-        else if (N <= 48) few_launch_rb<false, 3>(a, st);
-        else if (N <= 64) few_launch_rb<false, 4>(a, st);
-        else rows_launch<false>(a, st);
+        if (N <= 16) few_launch<false>(a, st) || (mid_launch<false, 1, 2>(a, st), true);
+        else if (N <= 32) mid_launch<false, 2, 2>(a, st);
+        else if (N <= 48) mid_launch<false, 3, 2>(a, st);
+        else if (N <= 64) mid_launch<false, 4, 2>(a, st);
+        else if (!rows_launch<false, 4, 4, 4, 2, 2>(a, 256, st) && !rows_launch<false, 4, 2, 4, 2, 2>(a, 256, st) &&
+                 !rows_launch<false, 4, 1, 4, 2, 2>(a, 256, st))
+            rows_launch<false, 4, 1, 2, 2, 2>(a, 0, st);
     }
     YV_LAUNCH_CHECK("int4_linear");
     return YVMOE_OK;
