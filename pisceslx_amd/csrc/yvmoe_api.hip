@@ -702,11 +702,14 @@ int32_t yvmoe_int4_linear(const void* x, int32_t act_dtype, int32_t n_rows,
     YV_REQUIRE(act_dtype == YVMOE_ACT_F32 || act_dtype == YVMOE_ACT_BF16, YVMOE_ERR_DTYPE,
                "unknown activation dtype %d", act_dtype);
     YV_REQUIRE(weight != nullptr, YVMOE_ERR_ARG, "weight is NULL");
-    YV_REQUIRE(n_rows >= 0, YVMOE_ERR_ARG, "n_rows=%d < 0", n_rows);
+    YV_REQUIRE(n_rows >= 0 && n_rows <= (1 << 30), YVMOE_ERR_ARG, "n_rows=%d outside [0, 2^30]", n_rows);
     YV_REQUIRE(weight->in_features >= 1 && weight->out_features >= 1 && weight->in_features <= (1 << 24) &&
                    weight->out_features <= (1 << 24),
                YVMOE_ERR_SHAPE, "in_features=%d, out_features=%d outside [1, 2^24]", weight->in_features,
                weight->out_features);
+    // tiles of at least 64 x 256 outputs, 2^23 work-groups of 512 threads to a launch
+    YV_REQUIRE((long long)ceil_div(n_rows, 64) * ceil_div(weight->out_features, 256) < (1 << 23), YVMOE_ERR_SHAPE,
+               "n_rows=%d x out_features=%d is too much for one call", n_rows, weight->out_features);
     if (n_rows == 0) return YVMOE_OK;
     YV_REQUIRE(weight->codes && weight->scales && x && out, YVMOE_ERR_ARG, "NULL pointer");
     YV_REQUIRE((uintptr_t)weight->codes % 16 == 0 && (uintptr_t)weight->scales % 8 == 0, YVMOE_ERR_ARG,

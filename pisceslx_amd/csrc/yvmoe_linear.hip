@@ -16,8 +16,10 @@
 // 32 g .. 32 g + 31 of row r, a dword eight of them, its bytes' lower nibbles columns 0 .. 3, their upper
 // nibbles columns 4 .. 7, which gives an operand's pairs in order.
 //
-// Forms. Up to 64 rows of x: int4_few_kernel, bound by the stream of codes (out·in / 2 bytes) and at small
-// sizes by one trip to memory. More: int4_rows_kernel, bound by the MFMAs.
+// Forms. Rows that fit into LDS, up to 16: int4_few_kernel, bound by the stream of codes (out·in / 2 bytes: 1 x
+// 4096 x 100003 in 38 us, 5.6 TB/s) and at small sizes by one trip to memory. Else int4_rows_kernel, bound by
+// what a CU gets from L2 while rows are few (each work-group reads them all: 48 x 5120 x 8192 in 16 us), then
+// by the instructions that make operands of codes (4096 x 8192 x 8192: 927 TFLOP/s).
 #include <algorithm>
 
 #include "yvmoe_frag.h"
@@ -343,16 +345,25 @@ __global__ __launch_bounds__(512, 4) void int4_few_kernel(LinArgs a) {
 }
 
 // ---------------------------------------------------------------- more rows
-// A work-group of 4 x 2 wavefronts computes 64 RB outputs of 32 TB rows; a wavefront 16 RB outputs of
-// 16 TB rows. Each group's 128 columns of the rows go through LDS (as bf16 terms, two stages, rows padded by
-// 16 bytes, so that the 16 rows of an operand fall on different banks), loaded a group ahead; the codes
-// go straight to the wavefront that converts them, each once for its TB MFMAs of every term.
+// A work-group of WO x WT x WK wavefronts computes 16 RB WO outputs of 16 TB WT rows, WK groups of K at a time.
+// The rows' columns go through LDS (as bf16 terms, two stages, padded by 16 bytes so that the 16 rows of an
+// operand fall on different banks), loaded a step ahead; the codes go straight to the wavefront that converts
+// them, D - 1 steps ahead, once for the TB MFMAs of every term. The sums of the WK wavefronts meet in LDS.
+//
+// FOLD: with 64 x 64 products per wavefront the MFMAs of -8 / 512 Σ x would be a fifth of all. There the
+// wavefronts that share rows share them, and every 32 groups Σ_groups s (-8 Σ x) is one more product, with
+// the scales (bf16 already) as one operand and the sums in three bf16 terms (24 bits) as the other. That takes
+// the additions out of the group's end as well: 8192 x 8192 at 4096 rows 672 -> 593 us (927 TFLOP/s), and
+// slower where a wavefront has 64 x 16 (100 x 4096 x 28672: 59 -> 68 us).
 template <bool F32, int TB, int RB, int WO, int WT, int D>
 __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
     constexpr int WK = 8 / WO / WT;
     constexpr int T = X8<F32>::TERMS, ROWS = 16 * TB * WT, STRIDE = kGroup * 2 + 16;
     constexpr int PER = ROWS * WK * 16 / 512;  // pieces of 8 columns that a thread brings
     __shared__ __align__(16) char xs[2][T][WK * ROWS * STRIDE];
+    constexpr bool FOLD = !F32 && WK == 1 && TB == WO && RB == 4;
+    constexpr int SUMS = 32, SUMLD = SUMS + 4;
+    __shared__ __align__(16) float sums[FOLD ? ROWS * SUMLD : 4];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r = lane & 15;
@@ -423,40 +434,114 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
     for (int b = 0; b < RB; ++b)
 #pragma unroll
         for (int t = 0; t < TB; ++t) acc[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto group = [&](const W& q, W& qn, int step) {
-        load_x(step + 1);
-        load_w(qn, step + D - 1);
-        bf16x8 c[RB][4];
+    // acc += s (-8 Σ x) over n groups
+    auto fold = [&](int g0, int n) {
+        bf16x8 sc[RB];
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            const unsigned d[4] = {q.w[b].x, q.w[b].y, q.w[b].z, q.w[b].w};
+            unsigned short e[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c[b][j] = codes8(d[j]);
+            for (int i = 0; i < 8; ++i) e[i] = scales[b][(long long)min(g0 + 8 * g + i, a.groups - 1) * 16];
+            Frag8 f;
+            f.u = make_uint4(e[0] | (unsigned)e[1] << 16, e[2] | (unsigned)e[3] << 16, e[4] | (unsigned)e[5] << 16,
+                             e[6] | (unsigned)e[7] << 16);
+            sc[b] = f.v;
         }
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
-            f32x4 part[RB], corr = {0.f, 0.f, 0.f, 0.f};
+            const float* p = &sums[((wt * TB + t) * 16 + r) * SUMLD + 8 * g];
+            X8<true> x;
+            x.v[0] = *(const uint4*)p, x.v[1] = *(const uint4*)(p + 4);
+            x.fix(0, n - 8 * g);
+            bf16x8 v[3];
+            x.terms(v);
 #pragma unroll
-            for (int b = 0; b < RB; ++b) part[b] = corr;
+            for (int b = 0; b < RB; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+                for (int k = 0; k < 3; ++k) acc[b][t] = mfma16(v[k], sc[b], acc[b][t]);
+        }
+    };
+    auto group = [&](const W& q, W& qn, int step) {
+        load_x(step + 1);
+        load_w(qn, step + D - 1);
+        if constexpr (FOLD) {
+            auto operand = [&](int t, int j) {
+                Frag8 f;
+                f.u = *(const uint4*)&xs[step & 1][0][((wt * TB + t) * 16 + r) * STRIDE + 64 * g + 16 * j];
+                return f.v;
+            };
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};  // wavefront wr's share of the rows
 #pragma unroll
-                for (int i = 0; i < T; ++i) {
-                    Frag8 f;
-                    f.u = *(const uint4*)&xs[step & 1][i][(wk * ROWS + (wt * TB + t) * 16 + r) * STRIDE + 64 * g + 16 * j];
-                    corr = mfma16(f.v, minus8(), corr);
+            for (int j = 0; j < 4; ++j) sum = mfma16(operand(wr, j), minus8(), sum);
+            f32x4 part[RB][TB];
 #pragma unroll
-                    for (int b = 0; b < RB; ++b) part[b] = mfma16(f.v, c[b][j], part[b]);
+            for (int j = 0; j < 4; ++j) {
+                bf16x8 c[RB], v[TB];
+#pragma unroll
+                for (int t = 0; t < TB; ++t) v[t] = operand(t, j);
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    const unsigned d[4] = {q.w[b].x, q.w[b].y, q.w[b].z, q.w[b].w};
+                    c[b] = codes8(d[j]);
                 }
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int t = 0; t < TB; ++t)
+                        part[b][t] = mfma16(v[t], c[b], j == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : part[b][t]);
+            }
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
                 const float s = scale512(q.s[b]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[b][t][i] = __builtin_fmaf(s, part[b][i] + corr[i], acc[b][t][i]);
+                for (int t = 0; t < TB; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[b][t][i] = __builtin_fmaf(s, part[b][t][i], acc[b][t][i]);
+            }
+            if (r == 0)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    sums[((wt * TB + wr) * 16 + 4 * g + i) * SUMLD + step % SUMS] = 512.0f * sum[i];
+        } else {
+            bf16x8 c[RB][4];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                const unsigned d[4] = {q.w[b].x, q.w[b].y, q.w[b].z, q.w[b].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[b][j] = codes8(d[j]);
+            }
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
+                f32x4 part[RB], corr = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int b = 0; b < RB; ++b) part[b] = corr;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < T; ++i) {
+                        Frag8 f;
+                        const int row = wk * ROWS + (wt * TB + t) * 16 + r;
+                        f.u = *(const uint4*)&xs[step & 1][i][row * STRIDE + 64 * g + 16 * j];
+                        corr = mfma16(f.v, minus8(), corr);
+#pragma unroll
+                        for (int b = 0; b < RB; ++b) part[b] = mfma16(f.v, c[b][j], part[b]);
+                    }
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    const float s = scale512(q.s[b]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[b][t][i] = __builtin_fmaf(s, part[b][i] + corr[i], acc[b][t][i]);
+                }
             }
         }
         store_x(step + 1);
         __syncthreads();
+        if constexpr (FOLD) {
+            if (step % SUMS == SUMS - 1 || step == a.groups - 1) {
+                fold(step - step % SUMS, step % SUMS + 1);
+                __syncthreads();
+            }
+        }
     };
     const int steps = (a.groups + WK - 1) / WK;
     W q[D];

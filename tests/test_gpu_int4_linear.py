@@ -80,6 +80,23 @@ def test_a_wide_layer(cuda, rows):
     check(x, pk, None, yvf.int4_linear(x, pk), f"{rows} x 9000 x 3000")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,K,O", [
+    (1, 2000, 33000), (16, 1024, 25000), (16, 4096, 9000), (3, 1021, 8300),   # rows in LDS, several rounds of outputs
+    (16, 5001, 700), (16, 14337, 4100), (9, 9999, 9000),                      # rows that do not fit
+    (24, 2050, 9000), (48, 1537, 17000), (61, 777, 8500),                     # two halves of a step, one past the end
+    (128, 5000, 2100), (300, 4224, 8300), (513, 4111, 4400), (1100, 8200, 4400),  # sums of 32 groups and the rest
+])
+def test_forms(cuda, dtype, rows, K, O):
+    print(f"int4_linear {dtype} {rows} x {K} x {O}", flush=True)
+    pk = pack_linear(randn(21, O, K, dtype=F32) * K ** -0.5)
+    x, bias = randn(22, rows, K, dtype=dtype) + 0.5, randn(23, O, dtype=dtype)
+    y = yvf.int4_linear(x, pk, bias)
+    check(x, pk, bias, y, "form")
+    # the last row alone, in the form of one row
+    check(x[-1:], pk, bias, yvf.int4_linear(x[-1:].contiguous(), pk, bias), "last row alone")
+
+
 def test_offsets_past_32_bits(cuda):
     """Codes, inputs and outputs of more than 4 GiB: the last block of outputs, the last rows."""
     K, O = 65536, 139264  # 4.25 GiB of codes

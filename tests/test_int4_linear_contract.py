@@ -67,7 +67,8 @@ def test_refusals():
         (dict(scales=None), _lib.YVMOE_ERR_ARG), (dict(codes=P + 8), _lib.YVMOE_ERR_ARG),
         (dict(scales=P + 4), _lib.YVMOE_ERR_ARG), (dict(x=None), _lib.YVMOE_ERR_ARG), (dict(out=None), _lib.YVMOE_ERR_ARG),
         (dict(x=P + 1), _lib.YVMOE_ERR_ARG), (dict(out=P + 1), _lib.YVMOE_ERR_ARG), (dict(bias=P + 1), _lib.YVMOE_ERR_ARG),
-        (dict(x=P + 2, act=_lib.ACT_F32), _lib.YVMOE_ERR_ARG),
+        (dict(x=P + 2, act=_lib.ACT_F32), _lib.YVMOE_ERR_ARG), (dict(n=(1 << 30) + 1), _lib.YVMOE_ERR_ARG),
+        (dict(n=1 << 30, O=256), _lib.YVMOE_ERR_SHAPE), (dict(n=1 << 16, O=1 << 24), _lib.YVMOE_ERR_SHAPE),
     ]:
         assert call(**kw) == code, kw
         assert _lib.lib().yvmoe_last_error()
