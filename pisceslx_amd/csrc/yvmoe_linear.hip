@@ -355,10 +355,10 @@ __global__ __launch_bounds__(512, 4) void int4_few_kernel(LinArgs a) {
 // the scales (bf16 already) as one operand and the sums in three bf16 terms (24 bits) as the other. That takes
 // the additions out of the group's end as well: 8192 x 8192 at 4096 rows 672 -> 593 us (927 TFLOP/s), and
 // slower where a wavefront has 64 x 16 (100 x 4096 x 28672: 59 -> 68 us).
-template <bool F32, int TB, int RB, int WO, int WT, int D>
+template <bool F32, int TB, int RB, int WO, int WT, int D, int ROWS>
 __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
     constexpr int WK = 8 / WO / WT;
-    constexpr int T = X8<F32>::TERMS, ROWS = 16 * TB * WT, STRIDE = kGroup * 2 + 16;
+    constexpr int T = X8<F32>::TERMS, STRIDE = kGroup * 2 + 16;
     constexpr int PER = ROWS * WK * 16 / 512;  // pieces of 8 columns that a thread brings
     __shared__ __align__(16) char xs[2][T][WK * ROWS * STRIDE];
     constexpr bool FOLD = !F32 && WK == 1 && TB == WO && RB == 4;
@@ -520,7 +520,7 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
 #pragma unroll
                     for (int i = 0; i < T; ++i) {
                         Frag8 f;
-                        const int row = wk * ROWS + (wt * TB + t) * 16 + r;
+                        const int row = wk * ROWS + ((wt * TB + t) * 16 + r) % ROWS;
                         f.u = *(const uint4*)&xs[step & 1][i][row * STRIDE + 64 * g + 16 * j];
                         corr = mfma16(f.v, minus8(), corr);
 #pragma unroll
@@ -594,7 +594,8 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
 
 constexpr int kLds = 163840;
 
-// Whether the rows fit into LDS beside the sums of RB outputs, and the launch if they do.
+// Whether the rows fit into LDS beside the sums of RB outputs, and the launch if they do. Two work-groups per
+// CU if both fit: more of them (768, 1024 in all) cost 1 x 4096 x 100003 a fifth.
 template <bool F32, int RB, int D, bool TINY>
 bool few_launch(const LinArgs& a, int least, hipStream_t st) {
     if (a.blocks < least || a.groups > kLds / (kGroup * 2)) return false;
@@ -604,6 +605,9 @@ bool few_launch(const LinArgs& a, int least, hipStream_t st) {
     int4_few_kernel<F32, RB, D, TINY><<<grid, 512, l.bytes, st>>>(a);
     return true;
 }
+// More outputs at a time make fewer reads of x from LDS, fewer keep more CUs at work: 1 x 4096 x 16384 takes
+// 9.9 us with two blocks and 11.2 with three, 16 x 1024 x 65536 13.4 with four and 14.0 with three. Where
+// four do not fit beside the rows (16 x 4096) two do.
 template <bool F32>
 bool few_launch(const LinArgs& a, hipStream_t st) {
     if ((long long)a.N * a.K < 8) return few_launch<F32, 2, 3, true>(a, 0, st);
@@ -611,17 +615,43 @@ bool few_launch(const LinArgs& a, hipStream_t st) {
            few_launch<F32, 1, 3, false>(a, 0, st);
 }
 
-template <bool F32, int TB, int RB, int WO, int WT, int D>
+template <bool F32, int TB, int RB, int WO, int WT, int D, int ROWS = 16 * TB * WT>
 bool rows_launch(const LinArgs& a, long long least, hipStream_t st) {
-    const long long wgs = (long long)ceil_div(a.N, 16 * TB * WT) * ceil_div(a.blocks, WO * RB);
+    const long long wgs = (long long)ceil_div(a.N, ROWS) * ceil_div(a.blocks, WO * RB);
     if (wgs < least) return false;
-    int4_rows_kernel<F32, TB, RB, WO, WT, D><<<(unsigned)wgs, 512, 0, st>>>(a);
+    int4_rows_kernel<F32, TB, RB, WO, WT, D, ROWS><<<(unsigned)wgs, 512, 0, st>>>(a);
     return true;
 }
-
 template <bool F32, int TB, int WO>
-void mid_launch(const LinArgs& a, hipStream_t st) {
+void rows_launch(const LinArgs& a, hipStream_t st) {
     if (!rows_launch<F32, TB, 2, WO, 1, 3>(a, 512, st)) rows_launch<F32, TB, 1, WO, 1, 3>(a, 0, st);
+}
+
+// The more wavefronts deal out K, the fewer steps there are and the smaller the work-groups' outputs; LDS has
+// room for eight groups of 8 rows in fp32 (7 x 5000 x 3001: 10.3 us, 15.0 with four groups of 16 rows) and of
+// 16 or 32 rows in bf16 (16 x 14336 x 4096: 14.8 us with eight, 19.0 with four; 32 x 14336 x 4096: 20.4 and
+// 26.5, but 32 x 5120 x 8192, with outputs for all CUs, 18.9 and 13.2).
+template <bool F32>
+void launch(const LinArgs& a, hipStream_t st) {
+    const int N = a.N;
+    if (N <= 16 && few_launch<F32>(a, st)) return;
+    if (N <= 8) {
+        if (!rows_launch<F32, 1, 2, 1, 1, 3, 8>(a, 256, st)) rows_launch<F32, 1, 1, 1, 1, 3, 8>(a, 0, st);
+    } else if constexpr (F32) {
+        if (N <= 16) rows_launch<F32, 1, 2>(a, st);
+        else if (N <= 32) rows_launch<F32, 2, 4>(a, st);
+        else if (!rows_launch<F32, 2, 4, 4, 2, 2>(a, 256, st) && !rows_launch<F32, 2, 2, 4, 2, 2>(a, 256, st))
+            rows_launch<F32, 2, 1, 4, 2, 2>(a, 0, st);
+    } else {
+        if (N <= 16) rows_launch<F32, 1, 1>(a, st);
+        else if (N <= 32 && a.blocks <= 256) rows_launch<F32, 2, 1, 1, 1, 3>(a, 0, st);
+        else if (N <= 32) rows_launch<F32, 2, 2>(a, st);
+        else if (N <= 48) rows_launch<F32, 3, 2>(a, st);
+        else if (N <= 64) rows_launch<F32, 4, 2>(a, st);
+        else if (!rows_launch<F32, 4, 4, 4, 2, 2>(a, 256, st) && !rows_launch<F32, 4, 2, 4, 2, 2>(a, 256, st) &&
+                 !rows_launch<F32, 4, 1, 4, 2, 2>(a, 256, st))
+            rows_launch<F32, 4, 1, 2, 2, 2>(a, 0, st);
+    }
 }
 
 }  // namespace
@@ -636,20 +666,8 @@ int int4_linear_launch(const void* x, int act, int N, const yvmoe_int4_matrix* w
     a.codes = (const char*)w->codes;
     a.scales = (const unsigned short*)w->scales;
     a.bias = bias, a.out = out;
-    if (act == YVMOE_ACT_F32) {
-        if (N <= 16) few_launch<true>(a, st) || (mid_launch<true, 1, 2>(a, st), true);
-        else if (N <= 32) mid_launch<true, 2, 4>(a, st);
-        else if (!rows_launch<true, 2, 4, 4, 2, 2>(a, 256, st) && !rows_launch<true, 2, 2, 4, 2, 2>(a, 256, st))
-            rows_launch<true, 2, 1, 4, 2, 2>(a, 0, st);
-    } else {
-        if (N <= 16) few_launch<false>(a, st) || (mid_launch<false, 1, 2>(a, st), true);
-        else if (N <= 32) mid_launch<false, 2, 2>(a, st);
-        else if (N <= 48) mid_launch<false, 3, 2>(a, st);
-        else if (N <= 64) mid_launch<false, 4, 2>(a, st);
-        else if (!rows_launch<false, 4, 4, 4, 2, 2>(a, 256, st) && !rows_launch<false, 4, 2, 4, 2, 2>(a, 256, st) &&
-                 !rows_launch<false, 4, 1, 4, 2, 2>(a, 256, st))
-            rows_launch<false, 4, 1, 2, 2, 2>(a, 0, st);
-    }
+    if (act == YVMOE_ACT_F32) launch<true>(a, st);
+    else launch<false>(a, st);
     YV_LAUNCH_CHECK("int4_linear");
     return YVMOE_OK;
 }
