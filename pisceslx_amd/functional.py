@@ -6,6 +6,7 @@ of them has a CPU or PyTorch fallback — a call on CPU tensors raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional
 
@@ -94,10 +95,41 @@ class Routing:
                        torch.empty(N * k, **i32), torch.empty(N * k, **i32),
                        torch.empty(1, **i32))
 
+    @staticmethod
+    def lazy(N: int, E: int, k: int, device) -> "Routing":
+        """:meth:`empty` with the five int32 tensors in one allocation, made when they are read."""
+        return _LazyRouting(N, E, k, device)
+
     def struct(self) -> _lib.Routing:
         return _lib.Routing(self.weights.data_ptr(), self.indices.data_ptr(), self.counts.data_ptr(),
                             self.offsets.data_ptr(), self.perm.data_ptr(), self.pos.data_ptr(),
                             self.capacity.data_ptr())
+
+
+class _LazyRouting(Routing):
+    _PARTS = ("counts", "offsets", "perm", "pos", "capacity")
+
+    def __init__(self, N: int, E: int, k: int, device):
+        self.weights = torch.empty(N, k, dtype=torch.float32, device=device)
+        self.indices = torch.empty(N, k, dtype=torch.int64, device=device)
+        self._lengths = (E, E + 1, N * k, N * k, 1)
+        at, self._starts = 0, []
+        for n in self._lengths:
+            self._starts.append(at)
+            at += (n + 63) // 64 * 64
+        self._rest = torch.empty(at, dtype=torch.int32, device=device)
+
+    def __getattr__(self, name):  # called for what is not set yet
+        if name not in self._PARTS:
+            raise AttributeError(name)
+        i = self._PARTS.index(name)
+        t = self._rest[self._starts[i]:self._starts[i] + self._lengths[i]]
+        setattr(self, name, t)
+        return t
+
+    def struct(self) -> _lib.Routing:
+        p = self._rest.data_ptr()
+        return _lib.Routing(self.weights.data_ptr(), self.indices.data_ptr(), *(p + 4 * s for s in self._starts))
 
 
 def workspace_bytes(n_tokens: int, act: int, router: RouterState,
@@ -297,7 +329,14 @@ def moe_forward_static(x2d: torch.Tensor, router: RouterState, experts: PackedEx
 
 def few_workspace_bytes(n_tokens: int, act: int, top_k: int, experts: PackedExperts) -> int:
     """Workspace of moe_forward_few and experts_few (0 for sizes they do not take)."""
-    e = experts.struct()
+    return _few_workspace_bytes(n_tokens, act, top_k, experts.format, experts.num_routed, experts.num_shared,
+                                experts.hidden, experts.ffn, experts.s_gate is not None)
+
+
+@functools.lru_cache(maxsize=1024)
+def _few_workspace_bytes(n_tokens, act, top_k, fmt, E, S, H, F, scales) -> int:
+    p, s = 16, 16 if scales else None  # whether there are pointers, not which, goes into the size
+    e = _lib.ExpertWeights(fmt, E, S, H, F, p, p, p, s, s, s)
     return int(_lib.lib().yvmoe_few_workspace_bytes(n_tokens, act, top_k, ctypes.byref(e)))
 
 
@@ -334,7 +373,7 @@ def moe_forward_few(x2d: torch.Tensor, router: RouterState, experts: PackedExper
         raise ValueError("router and experts disagree")
     act, shared_out, workspace = _few_args(x2d, router.top_k, experts, mix, skip, workspace, dev)
     N = x2d.shape[0]
-    routing = Routing.empty(N, router.num_experts, router.top_k, dev)
+    routing = Routing.lazy(N, router.num_experts, router.top_k, dev)
     out = torch.empty_like(x2d)
     r, e, o = router.struct(), experts.struct(), routing.struct()
     _lib.check(_lib.lib().yvmoe_forward_few(

@@ -17,6 +17,11 @@ routed experts first, then the shared experts; ``load_reference_state_dict`` acc
 reference keys ``experts.{e}.{gate,up,down}_proj.weight``,
 ``shared_experts.{s}.expert.{gate,up,down}_proj.weight``, ``shared_expert_weight`` and
 ``router.*``. The whole forward is one libyvmoe call on the current stream.
+
+``few_tokens`` (or ``cfg.moe_few_tokens``, 0 to 16, default 0): calls of up to that many tokens take
+the few-token form (``functional.moe_forward_few``; after YvMoEGate's own call, ``experts_few``),
+which reads each expert's weights once and rounds less often, so its results differ from the general
+form's in the last bits. Longer calls are as without it.
 """
 from __future__ import annotations
 
@@ -47,7 +52,7 @@ class YvDynamicMoELayer(nn.Module):
     def __init__(self, cfg: Any, device=None, dtype=None, num_shared_experts: int = 1,
                  use_fine_grained: bool = False, num_sub_experts: int = 1,
                  compute_mode: str = "default", weight_format: Optional[str] = None,
-                 router: Optional[str] = None):
+                 router: Optional[str] = None, few_tokens: Optional[int] = None):
         super().__init__()
         if compute_mode != "default":
             raise NotImplementedError("compute_split experts (layer.py:646-676) are not supported")
@@ -67,6 +72,11 @@ class YvDynamicMoELayer(nn.Module):
         if weight_format is None:
             weight_format = "bf16" if self.dtype == torch.bfloat16 else "f32"
         self.weight_format = FORMAT_BY_NAME[weight_format]
+        if few_tokens is None:
+            few_tokens = getattr(cfg, "moe_few_tokens", 0) or 0
+        if not 0 <= few_tokens <= _lib.FEW_TOKENS:
+            raise ValueError(f"few_tokens={few_tokens}: 0 to {_lib.FEW_TOKENS}")
+        self.few_tokens = few_tokens
         H = self.hidden_size
         if router is None:
             router = getattr(cfg, "moe_router", "moegate")
@@ -199,7 +209,9 @@ class YvDynamicMoELayer(nn.Module):
             buf = self._apply_skip_residual_buffer((B, Sq, H))
             skip = None if buf is None else buf.reshape(-1, H)
         ws = self._workspace if self._workspace is not None and self._workspace.device == x.device else None
-        if self._router_kind == "moegate":
+        if 0 < x2d.shape[0] <= self.few_tokens:
+            out, shared_out, routing, loss, ws = self._forward_few(x, x2d, act, skip, modal_id, ws)
+        elif self._router_kind == "moegate":
             g = self.router
             st = g.gate_state(act, Sq)
             mid = None if modal_id is None else g._modal_ids(modal_id, B, Sq, x.device)
@@ -225,6 +237,30 @@ class YvDynamicMoELayer(nn.Module):
         return out.view(B, Sq, H), loss
 
 
+    def _forward_few(self, x, x2d, act, skip, modal_id, ws):
+        """The forward on the two kernels of the few-token layer; with a YvMoEGate they follow its gate."""
+        N, k = x2d.shape[0], min(self.top_k, self.num_experts)
+        need = yvf.few_workspace_bytes(N, act, k, self.experts_packed)
+        if ws is None or ws.numel() < need:
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        if self._router_kind == "stable":
+            out, shared_out, routing = yvf.moe_forward_few(
+                x2d, self.router.router_state(act), self.experts_packed, self._mix(), skip, workspace=ws)
+            return out, shared_out, routing, torch.zeros((), device=x.device, dtype=x.dtype), ws
+        g = self.router
+        mid = None if modal_id is None else g._modal_ids(modal_id, x.shape[0], x.shape[1], x.device)
+        cached = g.path_moe_begin(N)
+        logits, loss, routing, ws = yvf.moegate_forward(x2d, g.gate_state(act, x.shape[1]), k, modal_id=mid,
+                                                        workspace=ws)
+        if cached is not None:
+            routing = cached[1]
+        out, shared_out, _ = yvf.experts_few(x2d, routing.weights, routing.indices, self.experts_packed,
+                                             self._mix(), skip, workspace=ws)
+        g.path_moe_end(None if cached is not None else (logits, routing))
+        g.last_routing, g.last_logits, g._last_loss_f32 = routing, logits, loss
+        return out, shared_out, routing, loss.reshape(()).to(x.dtype), ws
+
+
 class YvDeepSeekMoELayer(YvDynamicMoELayer):
     """YvDeepSeekMoELayer (layer.py:967): DeepSeek defaults read from cfg (layer.py:1040-1047).
 
@@ -234,11 +270,11 @@ class YvDeepSeekMoELayer(YvDynamicMoELayer):
     """
 
     def __init__(self, cfg: Any, device=None, dtype=None, weight_format: Optional[str] = None,
-                 router: Optional[str] = None):
+                 router: Optional[str] = None, few_tokens: Optional[int] = None):
         super().__init__(cfg, device=device, dtype=dtype,
                          num_shared_experts=getattr(cfg, "moe_shared_experts", 1),
                          use_fine_grained=getattr(cfg, "moe_fine_grained", True),
                          num_sub_experts=getattr(cfg, "moe_num_sub_experts", 4),
                          compute_mode=getattr(cfg, "moe_compute_mode", "default"),
-                         weight_format=weight_format, router=router)
+                         weight_format=weight_format, router=router, few_tokens=few_tokens)
         self.diversity_weight = getattr(cfg, "diversity_weight", 0.01)

@@ -69,12 +69,12 @@ class YvHybridBlockMLP(nn.Module):
     """
 
     def __init__(self, cfg: Any, device=None, dtype=None, weight_format: Optional[str] = None,
-                 router: Optional[str] = None):
+                 router: Optional[str] = None, few_tokens: Optional[int] = None):
         super().__init__()
         H = cfg.hidden_size
         self.norm_fusion = YvRMSNorm(H, device=device, dtype=dtype)
         self.mlp = YvDeepSeekMoELayer(cfg, device=device, dtype=dtype, weight_format=weight_format,
-                                      router=router)
+                                      router=router, few_tokens=few_tokens)
         self.norm_mlp = YvRMSNorm(H, device=device, dtype=dtype)
         self.residual_scale_mlp = nn.Parameter(
             torch.ones(1, device=device, dtype=dtype) * (2.0 * cfg.n_layer) ** -0.5)

@@ -94,3 +94,33 @@ def test_cpu_tensors_are_refused():
     x = torch.zeros(1, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="GPU"):
         yvf.experts_few(x, torch.ones(1, 1), torch.zeros(1, 1, dtype=torch.int64), ex)
+
+
+def test_layer_argument():
+    from pisceslx_amd import YvDeepSeekMoELayer
+
+    class Cfg:
+        hidden_size = 64
+        intermediate_size = 64
+        moe_num_experts = 4
+        moe_top_k = 2
+    assert YvDeepSeekMoELayer(Cfg(), router="stable").few_tokens == 0
+    assert YvDeepSeekMoELayer(Cfg(), router="stable", few_tokens=16).few_tokens == 16
+    Cfg.moe_few_tokens = 5
+    assert YvDeepSeekMoELayer(Cfg(), router="stable").few_tokens == 5
+    assert YvDeepSeekMoELayer(Cfg(), router="stable", few_tokens=0).few_tokens == 0
+    for bad in (-1, 17):
+        with pytest.raises(ValueError):
+            YvDeepSeekMoELayer(Cfg(), router="stable", few_tokens=bad)
+
+
+def test_lazy_routing():
+    r, e = yvf.Routing.lazy(3, 100, 4, "cpu"), yvf.Routing.empty(3, 100, 4, "cpu")
+    o = r.struct()
+    for name in ("weights", "indices", "counts", "offsets", "perm", "pos", "capacity"):
+        a, b = getattr(r, name), getattr(e, name)
+        assert a.shape == b.shape and a.dtype == b.dtype and a.is_contiguous()
+        assert a.data_ptr() == getattr(o, name) and getattr(r, name) is a
+    assert isinstance(r, yvf.Routing)
+    with pytest.raises(AttributeError):
+        r.other

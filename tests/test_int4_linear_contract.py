@@ -4,6 +4,7 @@ import ctypes
 import pytest
 import torch
 
+from pisceslx_amd import YvInt4Linear
 from pisceslx_amd import _lib
 from pisceslx_amd import functional as yvf
 from pisceslx_amd.quant import dequantize_int4, pack_linear, pack_linear_codes, quantize_int4, unpack_int4
@@ -82,3 +83,37 @@ def test_refused_tensors():
                 lambda: yvf.int4_linear(torch.zeros((), dtype=torch.bfloat16), pk)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_module():
+    dense = torch.nn.Linear(200, 33)
+    m = YvInt4Linear.from_linear(dense)
+    pk = pack_linear(dense.weight.detach())
+    assert torch.equal(m.packed.dequantize(), pk.dequantize()) and torch.equal(m.bias, dense.bias)
+    other = YvInt4Linear(200, 33).to(torch.bfloat16)  # a change of dtype: the bias alone
+    assert other.bias.dtype == torch.bfloat16 and other.packed.scales.dtype == torch.bfloat16
+    other.load_state_dict(m.state_dict())
+    assert torch.equal(other.packed.dequantize(), pk.dequantize())
+    assert torch.equal(other.bias, dense.bias.detach().to(torch.bfloat16))
+    with pytest.raises(NotImplementedError):
+        other.train()(torch.zeros(1, 200))
+    with pytest.raises(ValueError):
+        m(torch.zeros(1, 200))  # no CPU form
+    with pytest.raises(ValueError):
+        m.set_weight(pack_linear(torch.zeros(33, 201)))
+    with pytest.raises(ValueError):
+        YvInt4Linear(0, 33)
+    assert float(YvInt4Linear(130, 17).packed.dequantize().abs().max()) == 0
+
+
+def test_module_from_a_reference_state():
+    w, b = torch.randn(40, 256), torch.randn(40)
+    q = (w / (w.abs().amax(dim=0, keepdim=True) / 127)).round().to(torch.int8)
+    scale, zero = w.abs().amax(dim=0, keepdim=True) / 127, torch.zeros(1, 256)
+    m = YvInt4Linear(256, 40)
+    m.load_reference_state_dict({"a.proj.weight": w, "a.proj.bias": b}, "a.proj")
+    assert torch.equal(m.packed.codes, pack_linear(w).codes) and torch.equal(m.bias.detach(), b)
+    m.load_reference_state_dict({"p.q_weight": q, "p.scale": scale, "p.zero_point": zero, "p.bias": b}, "p")
+    assert torch.equal(m.packed.codes, pack_linear(q.float() * scale).codes)
+    with pytest.raises(KeyError):
+        m.load_reference_state_dict({"p.weight": w}, "p")
