@@ -30,31 +30,20 @@
 // Rounding: weights enter exactly (codes as bf16, scales on the fp32 sums), h is rounded once to
 // bf16 for the second product's MFMAs, the outputs once at the end.
 #include <algorithm>
+#include <type_traits>
 
 #include "yvmoe_frag.h"
 #include "yvmoe_internal.h"
 #include "yvmoe_topk.h"
 
-#ifndef YV_B
-#define YV_B 1, 3, 2, 3, 2, 3, 4, 3
-#endif
-#ifndef YV_I
-#define YV_I 2, 2, 4, 2, 2, 3, 4, 3
-#endif
-#ifndef YV_P
-#define YV_P 2, 2, 4, 2, 2, 3, 4, 3
-#endif
-#ifndef YV_Q
-#define YV_Q 2, 3, 4, 4, 4, 3, 8, 3
-#endif
-#ifndef YV_F
-#define YV_F 1, 2, 1, 3, 1, 3, 2, 3
-#endif
-
 namespace yvmoe {
 namespace {
 
-// k-steps per chunk and chunks held for two matrices and for one, without and with activations in LDS.
+// k-steps per chunk and chunks held for two matrices and for one, without and with activations in LDS. As
+// many bytes in flight as the 168 registers of nine wavefronts hold without spilling (a spill in a loop
+// cost bf16 a half); longer chunks make the last one of a short K emptier (fp32 with two k-steps: 56 -> 70 us
+// at one token, 1024 -> 2816). More and thinner wavefronts do not help: with 11 one int8 token takes 48 us,
+// with 15 61, with 8 44.
 struct Depth {
     int u2, r2, u1, r1, lu2, lr2, lu1, lr1;
     constexpr int unit(int nm, bool lds) const { return nm == 2 ? (lds ? lu2 : u2) : (lds ? lu1 : u1); }
@@ -164,7 +153,7 @@ template <>
 struct Wt<YVMOE_W_BF16> {
     typedef Frag16 Raw;
     typedef ActB16 Act;
-    static constexpr Depth DEPTH = {YV_B};
+    static constexpr Depth DEPTH = {1, 3, 2, 3, 2, 3, 4, 3};
     static constexpr bool GROUPED = false;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return block_ptr(b, e * 2, n0, K, 2048, 16, lane);
@@ -183,7 +172,7 @@ template <>
 struct Wt<YVMOE_W_INT8> {
     typedef uint4 Raw;
     typedef ActB16 Act;
-    static constexpr Depth DEPTH = {YV_I};
+    static constexpr Depth DEPTH = {2, 2, 4, 2, 2, 3, 4, 3};
     static constexpr bool GROUPED = false;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return block_ptr(b, e, n0, K, 1024, 16, lane);
@@ -215,7 +204,7 @@ template <>
 struct Wt<YVMOE_W_FP8> {
     typedef uint4 Raw;
     typedef ActB16 Act;
-    static constexpr Depth DEPTH = {YV_P};
+    static constexpr Depth DEPTH = {2, 2, 4, 2, 2, 3, 4, 3};
     static constexpr bool GROUPED = true;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return block_ptr(b, e, n0, K, 1024, 16, lane);
@@ -247,7 +236,7 @@ template <>
 struct Wt<YVMOE_W_INT4> {
     typedef uint2 Raw;
     typedef ActB16 Act;
-    static constexpr Depth DEPTH = {YV_Q};
+    static constexpr Depth DEPTH = {2, 3, 4, 4, 4, 3, 8, 3};
     static constexpr bool GROUPED = true;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return block_ptr(b, e / 2, n0, K, 512, 8, lane);
@@ -303,7 +292,7 @@ struct Wt<YVMOE_W_F32> {
             for (int i = 0; i < 4; ++i) v[i] = *(const uint4*)(row + ks * 256 + 64 * i);
         }
     };
-    static constexpr Depth DEPTH = {YV_F};
+    static constexpr Depth DEPTH = {1, 2, 1, 3, 1, 3, 2, 3};
     static constexpr bool GROUPED = false;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return (const char*)b + (e + (long long)(n0 + (lane & 15)) * K + 4 * (lane >> 4)) * 4;
@@ -323,7 +312,9 @@ struct Wt<YVMOE_W_F32> {
     }
 };
 
-// Activation rows that fit are kept in LDS, padded so that 16 rows' pieces fall on different banks.
+// Activation rows that fit are kept in LDS, x and h each by itself, padded so that 16 rows' pieces fall on
+// different banks. (int4 reads two bytes of activations for one of weights: with x in LDS 4 tokens of
+// 5120 -> 1536 take 122 us, not 140.)
 constexpr int kActBytes = 84 << 10, kRowPad = 16;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* gbl_ptr_t;
@@ -346,14 +337,18 @@ struct Operands {
     typedef typename Wt<WF>::Act Act;
     const char* w[NM];
     const void* s[NM];  // the scales: int8, int4 of the lane's row, fp8 of these rows
+    int left[NM];       // int4: scales from there to the end of all
     __amdgpu_buffer_rsrc_t buf;  // the activations, and the lane's row in them at its columns
     unsigned off;
 
-    __device__ __forceinline__ void set(int m, const void* base, const void* scales, long long e, int out, int K,
-                                        int n0, int lane) {
+    __device__ __forceinline__ void set(int m, const void* base, const void* scales, long long e, int total, int out,
+                                        int K, int n0, int lane) {
         w[m] = Wt<WF>::ptr(base, e * out * K, n0, K, lane);
-        if constexpr (WF == YVMOE_W_INT4)
-            s[m] = (const unsigned short*)scales + (e * out + n0 + (lane & 15)) * (K / 128);
+        if constexpr (WF == YVMOE_W_INT4) {
+            const long long at = (e * out + n0 + (lane & 15)) * (K / 128);
+            s[m] = (const unsigned short*)scales + at;
+            left[m] = (int)min(total * out * (K / 128) - at, 1ll << 20);
+        }
         else if constexpr (WF == YVMOE_W_FP8)
             s[m] = (const float*)scales + (e * (out / 128) + n0 / 128) * (K / 128);
         else if constexpr (WF == YVMOE_W_INT8)
@@ -379,10 +374,22 @@ struct Chunk {
     typedef Wt<WF> W;
     static constexpr int U = W::DEPTH.unit(NM, LDS);
     typename W::Raw w[U][NM];
-    float s[W::GROUPED ? U / 2 : 1][NM];
+    struct __attribute__((packed, aligned(2))) Scales {
+        typename std::conditional<(U > 4), unsigned long long,
+                                  typename std::conditional<(U > 2), unsigned, unsigned short>::type>::type v;
+    };
+    float s[WF == YVMOE_W_FP8 ? U / 2 : 1][NM];
+    Scales sraw[NM];  // int4
+    int sshift[NM];
     float rs[NM];  // int8: the row's scale
     int c;
     unsigned act;
+
+    __device__ __forceinline__ float scale(int group, int m) const {
+        if constexpr (WF == YVMOE_W_INT4)
+            return 512.0f * bf16_to_f32((unsigned short)(sraw[m].v >> (sshift[m] + 16 * group)));
+        return s[WF == YVMOE_W_FP8 ? group : 0][m];
+    }
 
     // k-steps past the end: the last one again, not used. int8's scales with every chunk: loads on one
     // path only would make the compiler wait for them at once.
@@ -396,10 +403,19 @@ struct Chunk {
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
                 W::load(w[u][m], o.w[m], ks);
-                if constexpr (W::GROUPED)
-                    if (u % 2 == 0)
-                        s[u / 2][m] = WF == YVMOE_W_INT4 ? 512.0f * bf16_to_f32(((const unsigned short*)o.s[m])[ks / 2])
-                                                         : ((const float*)o.s[m])[ks / 2];
+                if constexpr (WF == YVMOE_W_FP8)
+                    if (u % 2 == 0) s[u / 2][m] = ((const float*)o.s[m])[ks / 2];
+            }
+        }
+        if constexpr (WF == YVMOE_W_INT4) {
+            // a row's scales of the chunk in one load (each touches 16 rows' lines, whatever its width: 2 tokens of
+            // 5120 -> 1536 take 79.9 us, 82.3 with a load a group), which starts early enough to end with the array
+            const int start = min(c * (U / 2), (nks - 1) / 2);
+#pragma unroll
+            for (int m = 0; m < NM; ++m) {
+                const int from = min(start, o.left[m] - U / 2);
+                sraw[m] = *(const Scales*)((const unsigned short*)o.s[m] + from);
+                sshift[m] = 16 * (start - from);
             }
         }
         if constexpr (WF == YVMOE_W_INT8)
@@ -453,11 +469,12 @@ __device__ __forceinline__ void mma(const Chunk<WF, NM, LDS>& q, Acts<WF, NM, LD
                 for (int m = 0; m < NM; ++m) W::mma(q.w[u][m], x.a[u], part[m]);
             }
 #pragma unroll
-            for (int m = 0; m < NM; ++m)
+            for (int m = 0; m < NM; ++m) {
+                const float s = q.scale(p / 2, m);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    acc[m][i] = __builtin_fmaf(q.s[p / 2][m], WF == YVMOE_W_INT4 ? part[m][i] + corr[i] : part[m][i],
-                                               acc[m][i]);
+                    acc[m][i] = __builtin_fmaf(s, WF == YVMOE_W_INT4 ? part[m][i] + corr[i] : part[m][i], acc[m][i]);
+            }
         }
     }
 }
@@ -605,8 +622,8 @@ struct GateUpWalk {
     __device__ __forceinline__ void enter() {
         int e, n0, row0, n, token;
         at(items.item, e, n0, row0, n, token);
-        o.set(0, a.w_gate, a.s_gate, e, a.F, a.H, n0, lane);
-        o.set(1, a.w_up, a.s_up, e, a.F, a.H, n0, lane);
+        o.set(0, a.w_gate, a.s_gate, e, a.E + a.S, a.F, a.H, n0, lane);
+        o.set(1, a.w_up, a.s_up, e, a.E + a.S, a.F, a.H, n0, lane);
         o.template rows<LDS>(x, a.N, token, a.H, lane);
         s = 0;
         c = wave;
@@ -624,8 +641,8 @@ struct GateUpWalk {
         } else if (!final) {
             enter();
         } else {
-            o.set(0, a.w_gate, a.s_gate, 0, a.F, a.H, 0, lane);
-            o.set(1, a.w_up, a.s_up, 0, a.F, a.H, 0, lane);
+            o.set(0, a.w_gate, a.s_gate, 0, a.E + a.S, a.F, a.H, 0, lane);
+            o.set(1, a.w_up, a.s_up, 0, a.E + a.S, a.F, a.H, 0, lane);
             c = 0;
             stop = true;
         }
@@ -708,7 +725,7 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_front_kernel(FewArgs a) {
     if (b < nrouter) {
         const int n0 = b / a.nsplit * 16, z = b % a.nsplit, nch = chunks<RF, 1, false>(a.H), nks = a.H / 64;
         RouterWalk<RF> w;
-        w.o.set(0, a.w_router, nullptr, 0, a.ld, a.H, n0, lane);
+        w.o.set(0, a.w_router, nullptr, 0, 1, a.ld, a.H, n0, lane);
         w.o.template rows<false>(a.x, a.N, r < a.N ? r : -1, a.H, lane);
         w.c = z * nch / a.nsplit + wave;
         w.end = (z + 1) * nch / a.nsplit;
@@ -897,7 +914,9 @@ __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, FewL
         }
         __syncthreads();
         const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        for (int job = wave < kWaves ? wave : 2 * N; job < (scores ? 2 * N : N); job += kWaves) {
+        // a token's choice by a wavefront, the scores of four tokens by another
+        const int njobs = N + (scores ? (N + 3) / 4 : 0);
+        for (int job = wave; job < njobs; job += kWaves + 1) {
             if (job < N) {
                 int id;
                 float p, w;
@@ -912,9 +931,10 @@ __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, FewL
                     if (writer) a.out_routing.indices[job * k + lane] = id;
                 }
             } else {
-                const float sc = predictor_token([&](int c) { return lg.pred[job - N][c]; }, terms, lg.b1, lg.w2,
-                                                 lg.b2, lane & 15);
-                if (lane == 0) t.score[job - N] = sc;
+                const int tok = 4 * (job - N) + (lane >> 4), in = min(tok, N - 1);
+                const float sc = predictor_token([&](int c) { return lg.pred[in][c]; }, terms, lg.b1, lg.w2, lg.b2,
+                                                 lane & 15);
+                if ((lane & 15) == 0 && tok < N) t.score[tok] = sc;
             }
         }
     } else if (tid < ns) {
@@ -1152,14 +1172,14 @@ struct DownWalk {
         const int row0 = __builtin_amdgcn_readfirstlane(t.tile_row0[tile]);
         n = __builtin_amdgcn_readfirstlane(t.tile_n[tile]);
         row = part * nrows + row0;
-        o.set(0, a.w_down, a.s_down, e, a.H, a.F, items.n0(), lane);
+        o.set(0, a.w_down, a.s_down, e, a.E + a.S, a.H, a.F, items.n0(), lane);
         o.template rows<LDS>(a.h, nrows, (lane & 15) < n ? row0 + (lane & 15) : -1, a.F, lane);
         c = part * nch / parts;
         c1 = (part + 1) * nch / parts;
     }
     // no unit: a chunk past the end, from lines that everyone reads
     __device__ __forceinline__ void nothing() {
-        o.set(0, a.w_down, a.s_down, 0, a.H, a.F, 0, lane);
+        o.set(0, a.w_down, a.s_down, 0, a.E + a.S, a.H, a.F, 0, lane);
         o.template rows<LDS>(a.h, nrows, -1, a.F, lane);
         c = nch;
         c1 = nch + 1;
@@ -1258,11 +1278,11 @@ __device__ __forceinline__ void combine(const FewArgs& a, const FewTables& t, co
     }
 }
 
-template <int WF, bool LDS>
+template <int WF, bool LDSX, bool LDSH>
 __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) {
     constexpr int BYTES = WF == YVMOE_W_F32 ? 4 : 2;
     __shared__ FewTables t;
-    __shared__ __align__(16) char acts[LDS ? kActBytes : 16];
+    __shared__ __align__(16) char acts[LDSX || LDSH ? kActBytes : 16];
     __shared__ union {
         FewLogits lg;
         f32x4 red[2][kWaves][2][64];
@@ -1271,10 +1291,10 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, grid = gridDim.x;
-    if constexpr (LDS) stage_rows<false>(a.xo, a.N, a.H * BYTES, acts, wave, lane);
+    if constexpr (LDSX) stage_rows<false>(a.xo, a.N, a.H * BYTES, acts, wave, lane);
     few_routing(a, t, u.lg, blockIdx.x == 0);
     if (a.N == 0) return;
-    if constexpr (LDS) {
+    if constexpr (LDSX) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     }
@@ -1296,10 +1316,10 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
     const int handed = max(0, nitems - kOwnItems * used), hitems = a.H / 16 * a.hparts;
     if ((int)blockIdx.x >= used && (int)blockIdx.x >= hitems) return;
     const int ntiles = t.ntiles + a.S, nrows = ns + a.S * a.N;
-    const int parts = down_parts(ntiles, nrows, chunks<WF, 1, LDS>(a.F), a.hparts);
+    const int parts = down_parts(ntiles, nrows, chunks<WF, 1, LDSH>(a.F), a.hparts);
     const DownItems down{(int)blockIdx.x, grid, hitems, a.hparts, ntiles * parts};
     auto stage_h = [&]() {
-        if constexpr (LDS) {
+        if constexpr (LDSH) {
             stage_rows<true>(a.h, nrows, a.F * BYTES, acts, wave, lane);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
@@ -1308,7 +1328,7 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
     for (int share = blockIdx.x, own = 1;; own = 0) {
         if (share < used) {
             int* ahead = own && handed > 0 ? t.ahead : nullptr;
-            const int done = gate_up<WF, true, LDS>(a, at, GateUpItems{share, nitems, used, ahead, 0}, u.red, ahead,
+            const int done = gate_up<WF, true, LDSX>(a, at, GateUpItems{share, nitems, used, ahead, 0}, u.red, ahead,
                                                     a.signals + 32 * SIG_TICKET, acts, wave, lane);
             if (wave == kWaves) {
                 // h is written through: once the stores are there, it may be said
@@ -1318,9 +1338,9 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
         }
         if ((int)blockIdx.x >= hitems) return;
         if (wave < kWaves) {
-            typedef DownWalk<WF, LDS> Walk;
+            typedef DownWalk<WF, LDSH> Walk;
             Walk w(a, t, down, parts, nrows, wave, lane);
-            Ring<WF, 1, Walk, LDS, true> ring;
+            Ring<WF, 1, Walk, LDSH, true> ring;
             ring.start_weights(w, a.F / 64);  // no h is needed for these
             __syncthreads();
             share = __builtin_amdgcn_readfirstlane(t.help);
@@ -1395,16 +1415,17 @@ int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, cons
     const int items = std::max(std::min(N * k, E) * (F / 16), H / 16 * a.hparts);
     const int grid = N == 0 ? 1 : std::min(kGrid, items);
     const int esz = act == YVMOE_ACT_BF16 ? 2 : 4;
-    const bool lds = (long long)N * (H * esz + kRowPad) <= kActBytes &&
-                     (long long)N * (k + S) * (F * esz + kRowPad) <= kActBytes;
+    const bool ldsx = (long long)N * (H * esz + kRowPad) <= kActBytes;
+    const bool ldsh = ldsx && (long long)N * (k + S) * (F * esz + kRowPad) <= kActBytes;
 #define YV_FEW(WFV)                                                                             \
     do {                                                                                        \
         if (N > 0) {                                                                            \
             few_front_kernel<WFV><<<std::max(front, 1), kAllThreads, 0, st>>>(a);               \
             YV_LAUNCH_CHECK("few_front");                                                       \
         }                                                                                       \
-        if (lds) few_experts_kernel<WFV, true><<<grid, kAllThreads, 0, st>>>(a);                \
-        else few_experts_kernel<WFV, false><<<grid, kAllThreads, 0, st>>>(a);                   \
+        if (ldsh) few_experts_kernel<WFV, true, true><<<grid, kAllThreads, 0, st>>>(a);         \
+        else if (ldsx) few_experts_kernel<WFV, true, false><<<grid, kAllThreads, 0, st>>>(a);   \
+        else few_experts_kernel<WFV, false, false><<<grid, kAllThreads, 0, st>>>(a);            \
         YV_LAUNCH_CHECK("few_experts");                                                         \
     } while (0)
     switch (w->format) {
