@@ -593,6 +593,7 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
 }
 
 constexpr int kLds = 163840;
+constexpr long long kAny = 1ll << 62;
 
 // Whether the rows fit into LDS beside the sums of RB outputs, and the launch if they do. Two work-groups per
 // CU if both fit: more of them (768, 1024 in all) cost 1 x 4096 x 100003 a fifth.
@@ -615,42 +616,52 @@ bool few_launch(const LinArgs& a, hipStream_t st) {
            few_launch<F32, 1, 3, false>(a, 0, st);
 }
 
+// int4_rows_kernel, and whether it is launched: if that takes from least to most work-groups.
 template <bool F32, int TB, int RB, int WO, int WT, int D, int ROWS = 16 * TB * WT>
-bool rows_launch(const LinArgs& a, long long least, hipStream_t st) {
+bool rows_launch(const LinArgs& a, long long least, long long most, hipStream_t st) {
     const long long wgs = (long long)ceil_div(a.N, ROWS) * ceil_div(a.blocks, WO * RB);
-    if (wgs < least) return false;
+    if (wgs < least || wgs > most) return false;
     int4_rows_kernel<F32, TB, RB, WO, WT, D, ROWS><<<(unsigned)wgs, 512, 0, st>>>(a);
     return true;
 }
 template <bool F32, int TB, int WO>
 void rows_launch(const LinArgs& a, hipStream_t st) {
-    if (!rows_launch<F32, TB, 2, WO, 1, 3>(a, 512, st)) rows_launch<F32, TB, 1, WO, 1, 3>(a, 0, st);
+    if (!rows_launch<F32, TB, 2, WO, 1, 3>(a, 512, kAny, st)) rows_launch<F32, TB, 1, WO, 1, 3>(a, 0, kAny, st);
 }
 
 // The more wavefronts deal out K, the fewer steps there are and the smaller the work-groups' outputs; LDS has
 // room for eight groups of 8 rows in fp32 (7 x 5000 x 3001: 10.3 us, 15.0 with four groups of 16 rows) and of
 // 16 or 32 rows in bf16 (16 x 14336 x 4096: 14.8 us with eight, 19.0 with four; 32 x 14336 x 4096: 20.4 and
-// 26.5, but 32 x 5120 x 8192, with outputs for all CUs, 18.9 and 13.2).
+// 26.5, but 32 x 5120 x 8192, with outputs for all CUs, 18.9 and 13.2). With more rows, the smallest tiles that
+// all run at once: bf16 100 x 2048 x 1024 7.2 us in 32 rows x 32 outputs, 10.2 in 64 x 32, 14.6 in 128 x 32
+// (4096 x 4096, 200 rows: 27, 30, 26); fp32 64 x 14336 x 1024 33 us in 16 x 32, 105 in 32 x 64, 171 in 64 x 64,
+// 100 x 5120 x 8192 90, 67, 69 and 47 in 32 x 128. Then the largest that give every CU one.
 template <bool F32>
 void launch(const LinArgs& a, hipStream_t st) {
     const int N = a.N;
     if (N <= 16 && few_launch<F32>(a, st)) return;
     if (N <= 8) {
-        if (!rows_launch<F32, 1, 2, 1, 1, 3, 8>(a, 256, st)) rows_launch<F32, 1, 1, 1, 1, 3, 8>(a, 0, st);
+        if (!rows_launch<F32, 1, 2, 1, 1, 3, 8>(a, 256, kAny, st)) rows_launch<F32, 1, 1, 1, 1, 3, 8>(a, 0, kAny, st);
     } else if constexpr (F32) {
         if (N <= 16) rows_launch<F32, 1, 2>(a, st);
         else if (N <= 32) rows_launch<F32, 2, 4>(a, st);
-        else if (!rows_launch<F32, 2, 4, 4, 2, 2>(a, 256, st) && !rows_launch<F32, 2, 2, 4, 2, 2>(a, 256, st))
-            rows_launch<F32, 2, 1, 4, 2, 2>(a, 0, st);
+        else if (!rows_launch<F32, 1, 1, 2, 1, 3>(a, 0, 512, st) && !rows_launch<F32, 2, 1, 4, 1, 3>(a, 0, 256, st) &&
+                 !rows_launch<F32, 2, 2, 4, 1, 3>(a, 0, 256, st) &&
+                 !rows_launch<F32, 2, 4, 4, 2, 2>(a, 256, kAny, st) &&
+                 !rows_launch<F32, 2, 2, 4, 2, 2>(a, 256, kAny, st))
+            rows_launch<F32, 2, 1, 4, 2, 2>(a, 0, kAny, st);
     } else {
         if (N <= 16) rows_launch<F32, 1, 1>(a, st);
-        else if (N <= 32 && a.blocks <= 256) rows_launch<F32, 2, 1, 1, 1, 3>(a, 0, st);
+        else if (N <= 32 && a.blocks <= 256) rows_launch<F32, 2, 1, 1, 1, 3>(a, 0, kAny, st);
         else if (N <= 32) rows_launch<F32, 2, 2>(a, st);
+        else if (rows_launch<F32, 2, 1, 2, 1, 3>(a, 0, 256, st)) return;
         else if (N <= 48) rows_launch<F32, 3, 2>(a, st);
         else if (N <= 64) rows_launch<F32, 4, 2>(a, st);
-        else if (!rows_launch<F32, 4, 4, 4, 2, 2>(a, 256, st) && !rows_launch<F32, 4, 2, 4, 2, 2>(a, 256, st) &&
-                 !rows_launch<F32, 4, 1, 4, 2, 2>(a, 256, st))
-            rows_launch<F32, 4, 1, 2, 2, 2>(a, 0, st);
+        else if (!rows_launch<F32, 4, 1, 2, 1, 3>(a, 0, 256, st) &&
+                 !rows_launch<F32, 4, 4, 4, 2, 2>(a, 256, kAny, st) &&
+                 !rows_launch<F32, 4, 2, 4, 2, 2>(a, 256, kAny, st) &&
+                 !rows_launch<F32, 4, 1, 4, 2, 2>(a, 256, kAny, st))
+            rows_launch<F32, 4, 1, 2, 2, 2>(a, 0, kAny, st);
     }
 }
 

@@ -85,6 +85,7 @@ def test_a_wide_layer(cuda, rows):
     (1, 2000, 33000), (16, 1024, 25000), (16, 4096, 9000), (3, 1021, 8300),   # rows in LDS, several rounds of outputs
     (16, 5001, 700), (16, 14337, 4100), (9, 9999, 9000), (8, 14400, 2000), (2, 40001, 9000),  # rows that do not fit
     (24, 2050, 9000), (32, 5001, 1000), (48, 1537, 17000), (61, 777, 8500),  # two halves of a step, one past the end
+    (50, 1300, 300), (100, 1300, 2100), (100, 640, 4200), (200, 777, 8300),  # tiles of 32, 64 and 128 rows
     (128, 5000, 2100), (300, 4224, 8300), (513, 4111, 4400), (1100, 8200, 4400),  # sums of 32 groups and the rest
 ])
 def test_forms(cuda, dtype, rows, K, O):
