@@ -166,3 +166,19 @@ def test_graph_and_stream(cuda, rows):
         got = y.clone()
         assert torch.equal(got, yvf.int4_linear(x, pk, bias)), rep
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,K,O", [(1, 300, 40), (16, 5001, 700), (48, 777, 300), (300, 1300, 4400), (1100, 4200, 4400)])
+def test_rows_that_are_not_numbers(cuda, dtype, rows, K, O):
+    """An infinity or NaN makes its row NaN and leaves the others as they are."""
+    pk = pack_linear(randn(31, O, K, dtype=F32))
+    x = randn(32, rows, K, dtype=dtype)
+    y = yvf.int4_linear(x, pk)
+    bad = sorted({0, rows // 2, rows - 1})
+    for i, v in zip(bad, (float("inf"), float("nan"), float("-inf"))):
+        x[i, (i * 37 + 5) % K] = v
+    z = yvf.int4_linear(x, pk)
+    assert bool(torch.isnan(z[bad]).all())
+    good = [i for i in range(rows) if i not in bad]
+    assert torch.equal(z[good], y[good])
