@@ -716,6 +716,9 @@ int32_t yvmoe_int4_linear(const void* x, int32_t act_dtype, int32_t n_rows,
                "codes must be 16-byte and scales 8-byte aligned");
     YV_REQUIRE(((uintptr_t)x | (uintptr_t)bias | (uintptr_t)out) % (act_dtype == YVMOE_ACT_F32 ? 4 : 2) == 0,
                YVMOE_ERR_ARG, "x, bias and out must be aligned to their elements");
+    const uintptr_t esz = act_dtype == YVMOE_ACT_F32 ? 4 : 2, xa = (uintptr_t)x, oa = (uintptr_t)out;
+    YV_REQUIRE(oa + esz * n_rows * weight->out_features <= xa || xa + esz * n_rows * weight->in_features <= oa,
+               YVMOE_ERR_ARG, "out overlaps x");
     return int4_linear_launch(x, act_dtype, n_rows, weight, bias, out, (hipStream_t)stream);
 }
 

@@ -347,7 +347,7 @@ struct Operands {
         if constexpr (WF == YVMOE_W_INT4) {
             const long long at = (e * out + n0 + (lane & 15)) * (K / 128);
             s[m] = (const unsigned short*)scales + at;
-            left[m] = (int)min(total * out * (K / 128) - at, 1ll << 20);
+            left[m] = (int)min((long long)total * out * (K / 128) - at, 1ll << 20);
         }
         else if constexpr (WF == YVMOE_W_FP8)
             s[m] = (const float*)scales + (e * (out / 128) + n0 / 128) * (K / 128);

@@ -74,6 +74,9 @@ def test_refusals():
         assert call(**kw) == code, kw
         assert _lib.lib().yvmoe_last_error()
     assert call(n=0, x=None, out=None) == _lib.YVMOE_OK
+    for out in (P, P + 3 * 128 * 2 - 2, P - 3 * 64 * 2 + 2):  # over x, its last element, its first
+        assert call(x=P, out=out) == _lib.YVMOE_ERR_ARG
+        assert b"overlaps" in _lib.lib().yvmoe_last_error()
 
 
 def test_refused_tensors():
