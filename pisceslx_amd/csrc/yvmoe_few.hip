@@ -315,7 +315,7 @@ struct Wt<YVMOE_W_F32> {
 // Activation rows that fit are kept in LDS, x and h each by itself, padded so that 16 rows' pieces fall on
 // different banks. (int4 reads two bytes of activations for one of weights: with x in LDS 4 tokens of
 // 5120 -> 1536 take 122 us, not 140.)
-constexpr int kActBytes = 84 << 10, kRowPad = 16;
+constexpr int kActBytes = 83 << 10, kRowPad = 16;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* gbl_ptr_t;
 
@@ -1064,19 +1064,48 @@ __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, FewL
 }
 
 // How many parts of K each tile's down product is cut into, so that the wavefronts of the shares
-// work-groups that deal out the units end together: the fewest with the least work of the busiest.
-__device__ __forceinline__ int down_parts(int tiles, int rows, int nch, int shares) {
-    int best = 1;
-    float cost = 1e30f;
-    for (int q = 1; q <= 32 && q <= nch && q * rows <= kYRows; ++q) {
-        const int units = (tiles * q + shares - 1) / shares;
-        const float c = (float)((units + kWaves - 1) / kWaves) / (float)q;
-        if (c < 0.97f * cost) {
-            best = q;
-            cost = c;
+// work-groups that deal out the units end together: the fewest within 3 % of the least work of the busiest, a
+// lane a candidate.
+__device__ __forceinline__ int down_parts(int tiles, int rows, int nch, int shares, int lane) {
+    const int q = lane + 1, units = (tiles * q + shares - 1) / shares;
+    const bool can = q == 1 || (q <= 32 && q <= nch && q * rows <= kYRows);
+    const float cost = can ? (float)((units + kWaves - 1) / kWaves) / (float)q : 1e30f;
+    const float least = __uint_as_float(~wave_max(~__float_as_uint(cost)));
+    return __builtin_amdgcn_readfirstlane(__ffsll(__ballot(cost <= 1.03f * least)));
+}
+
+// One term of a token's sum: weight, row of the partial outputs (9 bits) and, above 16 bits, the unit that makes it,
+// which may be another work-group's; kNoTerm: none, kNanTerm: a NaN.
+struct Term {
+    float w;
+    unsigned at;
+};
+constexpr unsigned kNoTerm = 0xffffu, kNanTerm = 0xfffeu;
+
+// The terms of all sums, in order: parts of slots 0 .. N k, then of the shared experts of each token. By the last
+// wavefront, which reads them and has time for it before it waits.
+__device__ __forceinline__ void list_terms(const FewArgs& a, const FewTables& t, Term* list, int parts, int nrows,
+                                           int lane) {
+    const int ns = a.N * a.k;
+    for (int i = lane; i < nrows * parts; i += 64) {
+        const int s = i / parts, q = i - s * parts;
+        int row, tile;
+        float w;
+        if (s < ns) {
+            row = t.pos[s];
+            tile = t.tile[max(row, 0)];
+            w = t.w[s];
+        } else {
+            const int tok = (s - ns) / a.S, e = s - ns - tok * a.S;
+            row = ns + e * a.N + tok;
+            tile = t.ntiles + e;
+            w = a.mix[e];
         }
+        // logits that are not numbers choose nothing: the token's output is none either
+        list[i] = row >= 0            ? Term{w, (unsigned)(q * nrows + row) | (unsigned)(tile * parts + q) << 16}
+                  : a.self && q == 0 ? Term{__builtin_nanf(""), kNanTerm << 16}
+                                     : Term{0.0f, kNoTerm << 16};
     }
-    return best;
 }
 
 // A share's own items are done, and so are extra items that were handed out: called by one wavefront
@@ -1211,17 +1240,28 @@ struct DownWalk {
 // of 16 columns for every token, from the partial outputs y; shared between work-groups, the sum of
 // their sums by the last of them.
 template <int WF>
-__device__ __forceinline__ void combine(const FewArgs& a, const FewTables& t, const DownItems& d, int parts, int nrows,
+__device__ __forceinline__ void combine(const FewArgs& a, const Term* list, const DownItems& d, int parts,
                                         const float (&y)[kYRows][16], int lane) {
     constexpr bool F32 = WF == YVMOE_W_F32;
-    const int c = lane & 15, ns = a.N * a.k, lo = d.lo(), hi = d.hi(), n0 = d.n0();
+    const int c = lane & 15, ns = a.N * a.k, n0 = d.n0();
+    const unsigned lo = d.lo(), hi = d.hi();
     const long long stride = (long long)a.N * a.H;
     const bool alone = d.hparts == 1;
-    auto row = [&](int i, int tile) {  // the parts that this work-group has computed
+    auto sum = [&](int first, int len) {  // the terms that this work-group has computed, eight under way
         float v = 0.0f;
-        for (int q = 0; q < parts; ++q) {
-            const int u = tile * parts + q;
-            if (alone || (u >= lo && u < hi)) v = v + y[q * nrows + i][c];
+#pragma unroll 1
+        for (int i = 0; i < len; i += 8) {
+            Term e[8];
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = list[first + min(i + j, len - 1)];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = y[e[j].at & (kYRows - 1)][c];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const unsigned u = e[j].at >> 16;
+                v = i + j < len && ((u >= lo && u < hi) || u == kNanTerm) ? __builtin_fmaf(e[j].w, p[j], v) : v;
+            }
         }
         return v;
     };
@@ -1238,14 +1278,9 @@ __device__ __forceinline__ void combine(const FewArgs& a, const FewTables& t, co
             if (a.shared_out != nullptr) ((unsigned short*)a.shared_out)[at] = f32_to_bf16_rne(sh);
         }
     };
+#pragma unroll 1
     for (int tok = lane >> 4; tok < a.N; tok += 4) {
-        float v = 0.0f, sh = 0.0f;
-        for (int j = 0; j < a.k; ++j) {
-            const int p = t.pos[tok * a.k + j];
-            if (p >= 0) v = v + t.w[tok * a.k + j] * row(p, t.tile[p]);
-            else if (a.self) v = __builtin_nanf("");  // logits that are not numbers choose nothing
-        }
-        for (int s = 0; s < a.S; ++s) sh = sh + a.mix[s] * row(ns + s * a.N + tok, t.ntiles + s);
+        const float v = sum(tok * a.k * parts, a.k * parts), sh = sum((ns + tok * a.S) * parts, a.S * parts);
         if (alone) {
             write(tok, v, sh);
         } else {
@@ -1283,6 +1318,7 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
     constexpr int BYTES = WF == YVMOE_W_F32 ? 4 : 2;
     __shared__ FewTables t;
     __shared__ __align__(16) char acts[LDSX || LDSH ? kActBytes : 16];
+    __shared__ Term terms[kYRows];
     __shared__ union {
         FewLogits lg;
         f32x4 red[2][kWaves][2][64];
@@ -1316,7 +1352,7 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
     const int handed = max(0, nitems - kOwnItems * used), hitems = a.H / 16 * a.hparts;
     if ((int)blockIdx.x >= used && (int)blockIdx.x >= hitems) return;
     const int ntiles = t.ntiles + a.S, nrows = ns + a.S * a.N;
-    const int parts = down_parts(ntiles, nrows, chunks<WF, 1, LDSH>(a.F), a.hparts);
+    const int parts = down_parts(ntiles, nrows, chunks<WF, 1, LDSH>(a.F), a.hparts, lane);
     const DownItems down{(int)blockIdx.x, grid, hitems, a.hparts, ntiles * parts};
     auto stage_h = [&]() {
         if constexpr (LDSH) {
@@ -1360,6 +1396,7 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
             });
             return;
         }
+        list_terms(a, t, terms, parts, nrows, lane);
         const int m = nitems > 0 ? wait_done(a, used, lane) : -1;
         if (lane == 0) t.help = m;
         __syncthreads();
@@ -1369,7 +1406,7 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
         DownItems d = down;
         for (int it = 0; d.item < hitems; ++it, d.item += grid) {
             __syncthreads();
-            combine<WF>(a, t, d, parts, nrows, u.y[it & 1], lane);
+            combine<WF>(a, terms, d, parts, u.y[it & 1], lane);
         }
         return;
     }
