@@ -27,8 +27,10 @@
 // written through and read past the caches (sc1): an acquire would invalidate every L2, 30 us for
 // the 4,096 wavefronts of a launch.
 //
-// Rounding: weights enter exactly (codes as bf16, scales on the fp32 sums), h is rounded once to
-// bf16 for the second product's MFMAs, the outputs once at the end.
+// Rounding: weights enter exactly (codes as bf16, scales on the fp32 sums), h as two bf16 terms (16 bits) where
+// they fit into LDS, else rounded once to bf16 (each WG reads all of h past the caches: with two terms from there 2
+// tokens of fp8 took 150 us, not 130); the outputs are rounded once at the end. One term's rounding is as large as
+// the outputs' own: errors against 64 bits 1.4 times those of two.
 #include <algorithm>
 #include <type_traits>
 
@@ -97,9 +99,11 @@ struct FewArgs {
     void* out;
     void* shared_out;
     const void* xo; // x, for int4 in its order of columns
-    void* h;        // [N k + S N][F], routed rows by expert, then the shared experts' tokens
+    void* h;        // [terms][N k + S N][F], routed rows by expert, then the shared experts' tokens
     unsigned* signals;  // Signal words, 32 apart
+    int hterms;       // terms of an h
     int hparts;       // work-groups per 16 columns of H
+    int parts;        // parts of a work-group's share of K
     int* hcount;      // [H / 16]: those of them that are done
     float* hsum;      // [hparts][2][N][H]: their sums of the routed and of the shared experts
 };
@@ -153,7 +157,7 @@ template <>
 struct Wt<YVMOE_W_BF16> {
     typedef Frag16 Raw;
     typedef ActB16 Act;
-    static constexpr Depth DEPTH = {1, 3, 2, 3, 2, 3, 4, 3};
+    static constexpr Depth DEPTH = {1, 3, 2, 3, 2, 3, 2, 4};
     static constexpr bool GROUPED = false;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return block_ptr(b, e * 2, n0, K, 2048, 16, lane);
@@ -162,10 +166,7 @@ struct Wt<YVMOE_W_BF16> {
         r.u[0] = nt_load16(p + (size_t)ks * 2048);
         r.u[1] = nt_load16(p + (size_t)ks * 2048 + 1024);
     }
-    static __device__ __forceinline__ void mma(const Raw& w, const Act& a, f32x4& acc) {
-        acc = mfma16(a.f.v[0], w.v[0], acc);
-        acc = mfma16(a.f.v[1], w.v[1], acc);
-    }
+    static __device__ __forceinline__ const Frag16& frag(const Raw& w) { return w; }
 };
 
 template <>
@@ -180,7 +181,7 @@ struct Wt<YVMOE_W_INT8> {
     static __device__ __forceinline__ void load(Raw& r, const char* p, int ks) {
         r = nt_load16(p + (size_t)ks * 1024);
     }
-    static __device__ __forceinline__ void mma(const Raw& r, const Act& a, f32x4& acc) {
+    static __device__ __forceinline__ Frag16 frag(const Raw& r) {
         const unsigned w[4] = {r.x, r.y, r.z, r.w};
         unsigned o[8];
 #pragma unroll
@@ -195,8 +196,7 @@ struct Wt<YVMOE_W_INT8> {
         Frag16 f;
         f.u[0] = make_uint4(o[0], o[1], o[2], o[3]);
         f.u[1] = make_uint4(o[4], o[5], o[6], o[7]);
-        acc = mfma16(a.f.v[0], f.v[0], acc);
-        acc = mfma16(a.f.v[1], f.v[1], acc);
+        return f;
     }
 };
 
@@ -212,7 +212,7 @@ struct Wt<YVMOE_W_FP8> {
     static __device__ __forceinline__ void load(Raw& r, const char* p, int ks) {
         r = nt_load16(p + (size_t)ks * 1024);
     }
-    static __device__ __forceinline__ void mma(const Raw& r, const Act& a, f32x4& acc) {
+    static __device__ __forceinline__ Frag16 frag(const Raw& r) {
         const unsigned w[4] = {r.x, r.y, r.z, r.w};
         unsigned o[8];
 #pragma unroll
@@ -223,8 +223,7 @@ struct Wt<YVMOE_W_FP8> {
         Frag16 f;
         f.u[0] = make_uint4(o[0], o[1], o[2], o[3]);
         f.u[1] = make_uint4(o[4], o[5], o[6], o[7]);
-        acc = mfma16(a.f.v[0], f.v[0], acc);
-        acc = mfma16(a.f.v[1], f.v[1], acc);
+        return f;
     }
 };
 
@@ -257,12 +256,11 @@ struct Wt<YVMOE_W_INT4> {
         corr = mfma16(a.f.v[0], c.v[0], corr);
         corr = mfma16(a.f.v[1], c.v[0], corr);
     }
-    static __device__ __forceinline__ void mma(const Raw& r, const Act& a, f32x4& acc) {
+    static __device__ __forceinline__ Frag16 frag(const Raw& r) {
         Frag16 f;
         f.u[0] = codes(r.x);
         f.u[1] = codes(r.y);
-        acc = mfma16(a.f.v[0], f.v[0], acc);
-        acc = mfma16(a.f.v[1], f.v[1], acc);
+        return f;
     }
 };
 // Eight columns of bf16 activations in int4's order; its inverse place of a column is int4_place.
@@ -312,10 +310,11 @@ struct Wt<YVMOE_W_F32> {
     }
 };
 
-// Activation rows that fit are kept in LDS, x and h each by itself, padded so that 16 rows' pieces fall on
-// different banks. (int4 reads two bytes of activations for one of weights: with x in LDS 4 tokens of
-// 5120 -> 1536 take 122 us, not 140.)
-constexpr int kActBytes = 83 << 10, kRowPad = 16;
+// Activation rows that fit are kept in LDS, padded so that 16 rows' pieces fall on different banks. (int4 reads
+// two bytes of activations for one of weights: with x in LDS 4 tokens of 5120 -> 1536 take 122 us, not 140.) One
+// room for all: x from its start and the router's logits, then the wavefronts' sums at its end; for the down
+// product h from its start, then the partial outputs.
+constexpr int kPoolBytes = 151296, kEndBytes = 32768, kRowPad = 16;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* gbl_ptr_t;
 
@@ -423,24 +422,45 @@ struct Chunk {
             for (int m = 0; m < NM; ++m) rs[m] = bf16_to_f32(*(const unsigned short*)o.s[m]);
     }
 };
-template <int WF, int NM, bool LDS>
+// T terms of each number, the later ones `plane` bytes further on.
+template <int WF, int NM, bool LDS, int T>
 struct Acts {
     static constexpr int U = Wt<WF>::DEPTH.unit(NM, LDS);
-    typename Wt<WF>::Act a[U];
+    typename Wt<WF>::Act a[U][T];
     template <bool FRESH>
-    __device__ __forceinline__ void load(const Chunk<WF, NM, LDS>& q, __amdgpu_buffer_rsrc_t buf, int nks) {
+    __device__ __forceinline__ void load(const Chunk<WF, NM, LDS>& q, __amdgpu_buffer_rsrc_t buf, int plane, int nks) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) a[u].template load<FRESH>(buf, q.act, min(q.c * U + u, nks - 1));
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+                a[u][t].template load<FRESH>(buf, q.act + t * plane, min(q.c * U + u, nks - 1));
     }
-    __device__ __forceinline__ void read(const Chunk<WF, NM, LDS>& q, const char* lds, int nks) {
+    __device__ __forceinline__ void read(const Chunk<WF, NM, LDS>& q, const char* lds, int plane, int nks) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) a[u].read(lds + q.act, min(q.c * U + u, nks - 1));
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < T; ++t) a[u][t].read(lds + q.act + t * plane, min(q.c * U + u, nks - 1));
     }
 };
 
+// A k-step's products of a matrix, its weights converted once for all terms.
+template <int WF, int T>
+__device__ __forceinline__ void products(const typename Wt<WF>::Raw& w, const typename Wt<WF>::Act (&a)[T], f32x4& acc) {
+    if constexpr (WF == YVMOE_W_F32) {
+        Wt<WF>::mma(w, a[0], acc);
+    } else {
+        const Frag16 f = Wt<WF>::frag(w);
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            acc = mfma16(a[t].f.v[0], f.v[0], acc);
+            acc = mfma16(a[t].f.v[1], f.v[1], acc);
+        }
+    }
+}
+
 // ORDER: the activations are as the caller has them, not in int4's order yet.
-template <int WF, int NM, bool LDS, bool ORDER>
-__device__ __forceinline__ void mma(const Chunk<WF, NM, LDS>& q, Acts<WF, NM, LDS>& x, int nks, f32x4 (&acc)[NM]) {
+template <int WF, int NM, bool LDS, bool ORDER, int T>
+__device__ __forceinline__ void mma(const Chunk<WF, NM, LDS>& q, Acts<WF, NM, LDS, T>& x, int nks, f32x4 (&acc)[NM]) {
     typedef Wt<WF> W;
     const int c = q.c;
     constexpr int U = W::DEPTH.unit(NM, LDS);
@@ -449,7 +469,7 @@ __device__ __forceinline__ void mma(const Chunk<WF, NM, LDS>& q, Acts<WF, NM, LD
         for (int u = 0; u < U; ++u)
             if (c * U + u < nks)
 #pragma unroll
-                for (int m = 0; m < NM; ++m) W::mma(q.w[u][m], x.a[u], acc[m]);
+                for (int m = 0; m < NM; ++m) products<WF, T>(q.w[u][m], x.a[u], acc[m]);
     } else {
 #pragma unroll
         for (int p = 0; p < U; p += 2) {
@@ -462,11 +482,12 @@ __device__ __forceinline__ void mma(const Chunk<WF, NM, LDS>& q, Acts<WF, NM, LD
                 if constexpr (WF == YVMOE_W_INT4) {
                     if constexpr (ORDER)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) x.a[u].f.u[h] = int4_order(x.a[u].f.u[h]);
-                    W::offset(x.a[u], corr);
+                        for (int h = 0; h < 2; ++h) x.a[u][0].f.u[h] = int4_order(x.a[u][0].f.u[h]);
+#pragma unroll
+                    for (int t = 0; t < T; ++t) W::offset(x.a[u][t], corr);
                 }
 #pragma unroll
-                for (int m = 0; m < NM; ++m) W::mma(q.w[u][m], x.a[u], part[m]);
+                for (int m = 0; m < NM; ++m) products<WF, T>(q.w[u][m], x.a[u], part[m]);
             }
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
@@ -490,12 +511,12 @@ __device__ __forceinline__ int chunks(int K) {
 // moves it one on, after the end to lines that everyone reads. While a chunk is multiplied, the weights
 // of the next ones and (without LDS) the activations of the next are in flight, across items too. The
 // start is apart, so that the weights' part of it can come before a wait.
-template <int WF, int NM, class Walk, bool LDS, bool FRESH = false, bool ORDER = false>
+template <int WF, int NM, class Walk, bool LDS, int T = 1, bool FRESH = false, bool ORDER = false>
 struct Ring {
     static constexpr int kRing = Wt<WF>::DEPTH.ring(NM, LDS);
     static_assert(kRing <= kOwnItems - 1, "what the streams look ahead");
     Chunk<WF, NM, LDS> q[kRing];
-    Acts<WF, NM, LDS> x[LDS ? 1 : 2];
+    Acts<WF, NM, LDS, T> x[LDS ? 1 : 2];
     typename Walk::Place place[kRing];
 
     __device__ __forceinline__ void start_weights(Walk& w, int nks) {
@@ -506,12 +527,12 @@ struct Ring {
             w.next();
         }
     }
-    __device__ __forceinline__ void start_acts(Walk& w, int nks) {
-        if constexpr (!LDS) x[0].template load<FRESH>(q[0], w.o.buf, nks);
+    __device__ __forceinline__ void start_acts(Walk& w, int plane, int nks) {
+        if constexpr (!LDS) x[0].template load<FRESH>(q[0], w.o.buf, plane, nks);
     }
 
     template <class End>
-    __device__ __forceinline__ void run(Walk& w, const char* lds, int nks, End end) {
+    __device__ __forceinline__ void run(Walk& w, const char* lds, int plane, int nks, End end) {
         constexpr int STEPS = LDS || kRing % 2 == 0 ? kRing : 2 * kRing;
         f32x4 acc[NM];
 #pragma unroll
@@ -521,14 +542,14 @@ struct Ring {
             for (int i = 0; i < STEPS; ++i) {
                 constexpr int AHEAD = kRing - 1;
                 Chunk<WF, NM, LDS>&p = q[i % kRing], &n = q[(i + AHEAD) % kRing];
-                if constexpr (!LDS && kRing > 2) x[(i + 1) % 2].template load<FRESH>(q[(i + 1) % kRing], w.o.buf, nks);
+                if constexpr (!LDS && kRing > 2) x[(i + 1) % 2].template load<FRESH>(q[(i + 1) % kRing], w.o.buf, plane, nks);
                 n.load_weights(w.o, w.c, nks);
-                if constexpr (!LDS && kRing == 2) x[(i + 1) % 2].template load<FRESH>(n, w.o.buf, nks);
+                if constexpr (!LDS && kRing == 2) x[(i + 1) % 2].template load<FRESH>(n, w.o.buf, plane, nks);
                 place[(i + AHEAD) % kRing] = w.place();
                 w.next();
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (LDS) x[0].read(p, lds, nks);
-                mma<WF, NM, LDS, ORDER>(p, x[LDS ? 0 : i % 2], nks, acc);
+                if constexpr (LDS) x[0].read(p, lds, plane, nks);
+                mma<WF, NM, LDS, ORDER, T>(p, x[LDS ? 0 : i % 2], nks, acc);
                 if (place[i % kRing].ends) {
                     if constexpr (WF == YVMOE_W_INT8)
 #pragma unroll
@@ -560,23 +581,30 @@ __device__ __forceinline__ void sum_waves(const f32x4 (&red)[kWaves][2][64], int
     }
 }
 
-// h of four activation rows from row and one column, below row + n, rounded once (int4: in its order of
-// columns). PUBLISH: written through to where every XCD reads it.
+// h of four activation rows from row and one column, below row + n (int4: in its order of columns); with bf16
+// activations as one or two bf16 terms, the second nrows rows further on. PUBLISH: written through to where
+// every XCD reads it.
 template <int WF, bool PUBLISH>
-__device__ __forceinline__ void store_h(void* h, long long row, int n, int F, int col, const f32x4& g, const f32x4& u) {
+__device__ __forceinline__ void store_h(void* h, long long row, int n, int nrows, int terms, int F, int col,
+                                        const f32x4& g, const f32x4& u) {
     const int at = WF == YVMOE_W_INT4 ? int4_place(col) : col;
+    auto put = [&](auto* p, auto v) {
+        if constexpr (PUBLISH) __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        else *p = v;
+    };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (i >= n) break;
         const float f = silu(g[i]) * u[i];
         if constexpr (WF == YVMOE_W_F32) {
-            float* p = (float*)h + (row + i) * F + at;
-            if constexpr (PUBLISH) __hip_atomic_store(p, f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            else *p = f;
+            put((float*)h + (row + i) * F + at, f);
         } else {
             unsigned short* p = (unsigned short*)h + (row + i) * F + at;
-            if constexpr (PUBLISH) __hip_atomic_store(p, f32_to_bf16_rne(f), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            else *p = f32_to_bf16_rne(f);
+            const unsigned short hi = f32_to_bf16_rne(f);
+            const bool finite = (hi & 0x7f80u) != 0x7f80u;
+            put(p, hi);
+            if (terms > 1)
+                put(p + (long long)nrows * F, finite ? f32_to_bf16_rne(f - bf16_to_f32(hi)) : (unsigned short)0);
         }
     }
 }
@@ -659,11 +687,11 @@ __device__ __forceinline__ int gate_up(const FewArgs& a, At at, GateUpItems item
     if (wave < kWaves) {
         typedef GateUpWalk<WF, LDS, At> Walk;
         Walk w(a, PUBLISH ? a.xo : a.x, at, items, wave, lane);
-        Ring<WF, 2, Walk, LDS, false, !PUBLISH> ring;
+        Ring<WF, 2, Walk, LDS, 1, false, !PUBLISH> ring;
         ring.start_weights(w, a.H / 64);
-        ring.start_acts(w, a.H / 64);
+        ring.start_acts(w, 0, a.H / 64);
         int it = 0;
-        ring.run(w, lds, a.H / 64, [&](const typename Walk::Place&, const f32x4 (&acc)[2]) {
+        ring.run(w, lds, 0, a.H / 64, [&](const typename Walk::Place&, const f32x4 (&acc)[2]) {
             red[it & 1][wave][0][lane] = acc[0];
             red[it & 1][wave][1][lane] = acc[1];
             __syncthreads();
@@ -684,7 +712,7 @@ __device__ __forceinline__ int gate_up(const FewArgs& a, At at, GateUpItems item
         f32x4 sum[2];
         sum_waves<2>(red[it & 1], lane, sum);
         const int g = lane >> 4;
-        store_h<WF, PUBLISH>(a.h, row0 + 4 * g, n - 4 * g, a.F, n0 + (lane & 15), sum[0], sum[1]);
+        store_h<WF, PUBLISH>(a.h, row0 + 4 * g, n - 4 * g, a.N * (a.k + a.S), a.hterms, a.F, n0 + (lane & 15), sum[0], sum[1]);
         more = items.advance();
     } while (more);
     return items.it;
@@ -733,8 +761,8 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_front_kernel(FewArgs a) {
         if (wave < kWaves && w.c < w.end) {
             Ring<RF, 1, RouterWalk<RF>, false> ring;
             ring.start_weights(w, nks);
-            ring.start_acts(w, nks);
-            ring.run(w, nullptr, nks, [&](const typename RouterWalk<RF>::Place&, const f32x4 (&acc)[1]) {
+            ring.start_acts(w, 0, nks);
+            ring.run(w, nullptr, 0, nks, [&](const typename RouterWalk<RF>::Place&, const f32x4 (&acc)[1]) {
                 red[0][wave][0][lane] = acc[0];
             });
         }
@@ -1063,48 +1091,30 @@ __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, FewL
     if (tid == 0) *o.capacity = t.cap;
 }
 
-// How many parts of K each tile's down product is cut into, so that the wavefronts of the shares
-// work-groups that deal out the units end together: the fewest within 3 % of the least work of the busiest, a
-// lane a candidate.
-__device__ __forceinline__ int down_parts(int tiles, int rows, int nch, int shares, int lane) {
-    const int q = lane + 1, units = (tiles * q + shares - 1) / shares;
-    const bool can = q == 1 || (q <= 32 && q <= nch && q * rows <= kYRows);
-    const float cost = can ? (float)((units + kWaves - 1) / kWaves) / (float)q : 1e30f;
-    const float least = __uint_as_float(~wave_max(~__float_as_uint(cost)));
-    return __builtin_amdgcn_readfirstlane(__ffsll(__ballot(cost <= 1.03f * least)));
-}
-
-// One term of a token's sum: weight, row of the partial outputs (9 bits) and, above 16 bits, the unit that makes it,
-// which may be another work-group's; kNoTerm: none, kNanTerm: a NaN.
+// One term of a token's sum: weight, and row of the partial outputs, or none.
 struct Term {
     float w;
-    unsigned at;
+    int row;
 };
-constexpr unsigned kNoTerm = 0xffffu, kNanTerm = 0xfffeu;
 
 // The terms of all sums, in order: parts of slots 0 .. N k, then of the shared experts of each token. By the last
 // wavefront, which reads them and has time for it before it waits.
-__device__ __forceinline__ void list_terms(const FewArgs& a, const FewTables& t, Term* list, int parts, int nrows,
-                                           int lane) {
+__device__ __forceinline__ void list_terms(const FewArgs& a, const FewTables& t, Term* list, int nrows, int lane) {
     const int ns = a.N * a.k;
-    for (int i = lane; i < nrows * parts; i += 64) {
-        const int s = i / parts, q = i - s * parts;
-        int row, tile;
+    for (int i = lane; i < nrows * a.parts; i += 64) {
+        const int s = i / a.parts, q = i - s * a.parts;
+        int row;
         float w;
         if (s < ns) {
             row = t.pos[s];
-            tile = t.tile[max(row, 0)];
             w = t.w[s];
         } else {
             const int tok = (s - ns) / a.S, e = s - ns - tok * a.S;
             row = ns + e * a.N + tok;
-            tile = t.ntiles + e;
             w = a.mix[e];
         }
         // logits that are not numbers choose nothing: the token's output is none either
-        list[i] = row >= 0            ? Term{w, (unsigned)(q * nrows + row) | (unsigned)(tile * parts + q) << 16}
-                  : a.self && q == 0 ? Term{__builtin_nanf(""), kNanTerm << 16}
-                                     : Term{0.0f, kNoTerm << 16};
+        list[i] = row >= 0 ? Term{w, q * nrows + row} : a.self ? Term{__builtin_nanf(""), 0} : Term{0.0f, -1};
     }
 }
 
@@ -1157,15 +1167,14 @@ __device__ __forceinline__ int wait_done(const FewArgs& a, int used, int lane) {
     }
 }
 
-// Down products: an item is 16 columns of H and a share of the units (tile, part of K), which the
-// wavefronts deal out; the work-group's items are first, first + step, ...
+// Down products: an item is 16 columns of H and one of hparts shares of K, cut into parts; the wavefronts deal
+// out the units (tile, part). The work-group's items are first, first + step, ... How K is cut goes by sizes
+// alone, so that a token's bits do not go by what the others choose.
 struct DownItems {
     int item, step, nitems;
-    int hparts, units;
+    int hparts;
     __device__ __forceinline__ int n0() const { return item / hparts * 16; }
     __device__ __forceinline__ int share() const { return item % hparts; }
-    __device__ __forceinline__ int lo() const { return share() * units / hparts; }
-    __device__ __forceinline__ int hi() const { return (share() + 1) * units / hparts; }
 };
 
 template <int WF, bool LDS>
@@ -1177,20 +1186,20 @@ struct DownWalk {
     const FewArgs& a;
     const FewTables& t;
     DownItems items;
-    int wave, parts, nch, nrows, lane;
+    int wave, parts, nch, nrows, units, lane;
     Operands<WF, 1> o;
-    int unit, hi, c, c1, row, n;
+    int unit, c, c1, row, n;
     bool stop;
 
-    __device__ __forceinline__ DownWalk(const FewArgs& args, const FewTables& tab, const DownItems& list, int p, int rows,
+    __device__ __forceinline__ DownWalk(const FewArgs& args, const FewTables& tab, const DownItems& list, int rows, int tiles,
                                         int wv, int ln)
-        : a(args), t(tab), items(list), wave(wv), parts(p), nch(chunks<WF, 1, LDS>(args.F)), nrows(rows), lane(ln), stop(false) {
+        : a(args), t(tab), items(list), wave(wv), parts(args.parts), nch(chunks<WF, 1, LDS>(args.F)), nrows(rows),
+          units(tiles * args.parts), lane(ln), stop(false) {
         enter_item();
     }
     __device__ __forceinline__ void enter_item() {
-        unit = items.lo() + wave;
-        hi = items.hi();
-        if (unit < hi) {
+        unit = wave;
+        if (unit < units) {
             enter_unit();
         } else {
             nothing();
@@ -1203,8 +1212,9 @@ struct DownWalk {
         row = part * nrows + row0;
         o.set(0, a.w_down, a.s_down, e, a.E + a.S, a.H, a.F, items.n0(), lane);
         o.template rows<LDS>(a.h, nrows, (lane & 15) < n ? row0 + (lane & 15) : -1, a.F, lane);
-        c = part * nch / parts;
-        c1 = (part + 1) * nch / parts;
+        const int cut = items.share() * parts + part, cuts = items.hparts * parts;
+        c = cut * nch / cuts;
+        c1 = (cut + 1) * nch / cuts;
     }
     // no unit: a chunk past the end, from lines that everyone reads
     __device__ __forceinline__ void nothing() {
@@ -1216,14 +1226,14 @@ struct DownWalk {
         n = 0;
     }
     __device__ __forceinline__ Place place() const {
-        const bool ends = c + 1 >= c1 && !stop, item_ends = ends && unit + kWaves >= hi;
-        return {ends, item_ends, item_ends && items.item + items.step >= items.nitems, unit < hi, row, n};
+        const bool ends = c + 1 >= c1 && !stop, item_ends = ends && unit + kWaves >= units;
+        return {ends, item_ends, item_ends && items.item + items.step >= items.nitems, unit < units, row, n};
     }
     __device__ __forceinline__ void next() {
         if (stop) return;
         if (c + 1 < c1) {
             ++c;
-        } else if (unit + kWaves < hi) {
+        } else if (unit + kWaves < units) {
             unit += kWaves;
             enter_unit();
         } else if (items.item + items.step < items.nitems) {
@@ -1240,14 +1250,12 @@ struct DownWalk {
 // of 16 columns for every token, from the partial outputs y; shared between work-groups, the sum of
 // their sums by the last of them.
 template <int WF>
-__device__ __forceinline__ void combine(const FewArgs& a, const Term* list, const DownItems& d, int parts,
-                                        const float (&y)[kYRows][16], int lane) {
+__device__ __forceinline__ void combine(const FewArgs& a, const Term* list, const DownItems& d, const float* y, int lane) {
     constexpr bool F32 = WF == YVMOE_W_F32;
-    const int c = lane & 15, ns = a.N * a.k, n0 = d.n0();
-    const unsigned lo = d.lo(), hi = d.hi();
+    const int c = lane & 15, ns = a.N * a.k, n0 = d.n0(), parts = a.parts;
     const long long stride = (long long)a.N * a.H;
     const bool alone = d.hparts == 1;
-    auto sum = [&](int first, int len) {  // the terms that this work-group has computed, eight under way
+    auto sum = [&](int first, int len) {  // eight terms under way
         float v = 0.0f;
 #pragma unroll 1
         for (int i = 0; i < len; i += 8) {
@@ -1256,12 +1264,9 @@ __device__ __forceinline__ void combine(const FewArgs& a, const Term* list, cons
 #pragma unroll
             for (int j = 0; j < 8; ++j) e[j] = list[first + min(i + j, len - 1)];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = y[e[j].at & (kYRows - 1)][c];
+            for (int j = 0; j < 8; ++j) p[j] = y[max(e[j].row, 0) * 16 + c];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const unsigned u = e[j].at >> 16;
-                v = i + j < len && ((u >= lo && u < hi) || u == kNanTerm) ? __builtin_fmaf(e[j].w, p[j], v) : v;
-            }
+            for (int j = 0; j < 8; ++j) v = i + j < len && e[j].row >= 0 ? __builtin_fmaf(e[j].w, p[j], v) : v;
         }
         return v;
     };
@@ -1313,22 +1318,25 @@ __device__ __forceinline__ void combine(const FewArgs& a, const Term* list, cons
     }
 }
 
-template <int WF, bool LDSX, bool LDSH>
+// LDS that h takes for the down product.
+__host__ __device__ inline int h_bytes(int terms, int nrows, int bytes) {
+    return (terms * nrows * (bytes + kRowPad) + 127) / 128 * 128;
+}
+
+template <int WF, bool LDSX, bool LDSH, int T>
 __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) {
     constexpr int BYTES = WF == YVMOE_W_F32 ? 4 : 2;
     __shared__ FewTables t;
-    __shared__ __align__(16) char acts[LDSX || LDSH ? kActBytes : 16];
     __shared__ Term terms[kYRows];
-    __shared__ union {
-        FewLogits lg;
-        f32x4 red[2][kWaves][2][64];
-        float y[2][kYRows][16];
-    } u;
+    __shared__ __align__(128) char pool[kPoolBytes];
+    static_assert(sizeof(FewLogits) <= kEndBytes && sizeof(f32x4[2][kWaves][2][64]) <= kEndBytes, "the end's room");
+    FewLogits& lg = *(FewLogits*)(pool + kPoolBytes - kEndBytes);
+    auto& red = *(f32x4(*)[2][kWaves][2][64])(pool + kPoolBytes - kEndBytes);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, grid = gridDim.x;
-    if constexpr (LDSX) stage_rows<false>(a.xo, a.N, a.H * BYTES, acts, wave, lane);
-    few_routing(a, t, u.lg, blockIdx.x == 0);
+    if constexpr (LDSX) stage_rows<false>(a.xo, a.N, a.H * BYTES, pool, wave, lane);
+    few_routing(a, t, lg, blockIdx.x == 0);
     if (a.N == 0) return;
     if constexpr (LDSX) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1352,11 +1360,12 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
     const int handed = max(0, nitems - kOwnItems * used), hitems = a.H / 16 * a.hparts;
     if ((int)blockIdx.x >= used && (int)blockIdx.x >= hitems) return;
     const int ntiles = t.ntiles + a.S, nrows = ns + a.S * a.N;
-    const int parts = down_parts(ntiles, nrows, chunks<WF, 1, LDSH>(a.F), a.hparts, lane);
-    const DownItems down{(int)blockIdx.x, grid, hitems, a.hparts, ntiles * parts};
+    const DownItems down{(int)blockIdx.x, grid, hitems, a.hparts};
+    const int yrows = nrows * a.parts;
+    float* y = (float*)(pool + (LDSH ? h_bytes(T, nrows, a.F * BYTES) : 0));
     auto stage_h = [&]() {
         if constexpr (LDSH) {
-            stage_rows<true>(a.h, nrows, a.F * BYTES, acts, wave, lane);
+            stage_rows<true>(a.h, T * nrows, a.F * BYTES, pool, wave, lane);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
         }
@@ -1364,8 +1373,8 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
     for (int share = blockIdx.x, own = 1;; own = 0) {
         if (share < used) {
             int* ahead = own && handed > 0 ? t.ahead : nullptr;
-            const int done = gate_up<WF, true, LDSX>(a, at, GateUpItems{share, nitems, used, ahead, 0}, u.red, ahead,
-                                                    a.signals + 32 * SIG_TICKET, acts, wave, lane);
+            const int done = gate_up<WF, true, LDSX>(a, at, GateUpItems{share, nitems, used, ahead, 0}, red, ahead,
+                                                    a.signals + 32 * SIG_TICKET, pool, wave, lane);
             if (wave == kWaves) {
                 // h is written through: once the stores are there, it may be said
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1375,20 +1384,21 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
         if ((int)blockIdx.x >= hitems) return;
         if (wave < kWaves) {
             typedef DownWalk<WF, LDSH> Walk;
-            Walk w(a, t, down, parts, nrows, wave, lane);
-            Ring<WF, 1, Walk, LDSH, true> ring;
+            Walk w(a, t, down, nrows, ntiles, wave, lane);
+            Ring<WF, 1, Walk, LDSH, T, true> ring;
             ring.start_weights(w, a.F / 64);  // no h is needed for these
             __syncthreads();
             share = __builtin_amdgcn_readfirstlane(t.help);
             if (share >= 0) continue;
             stage_h();
-            ring.start_acts(w, a.F / 64);
+            const int plane = nrows * (a.F * BYTES + kRowPad);
+            ring.start_acts(w, plane, a.F / 64);
             int it = 0;
-            ring.run(w, acts, a.F / 64, [&](const typename Walk::Place& p, const f32x4 (&acc)[1]) {
+            ring.run(w, pool, plane, a.F / 64, [&](const typename Walk::Place& p, const f32x4 (&acc)[1]) {
                 if (p.unit)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (4 * (lane >> 4) + i < p.n) u.y[it & 1][p.row + 4 * (lane >> 4) + i][r] = acc[0][i];
+                        if (4 * (lane >> 4) + i < p.n) y[((it & 1) * yrows + p.row + 4 * (lane >> 4) + i) * 16 + r] = acc[0][i];
                 if (p.item_ends) {
                     __syncthreads();
                     ++it;
@@ -1396,7 +1406,7 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
             });
             return;
         }
-        list_terms(a, t, terms, parts, nrows, lane);
+        list_terms(a, t, terms, nrows, lane);
         const int m = nitems > 0 ? wait_done(a, used, lane) : -1;
         if (lane == 0) t.help = m;
         __syncthreads();
@@ -1406,10 +1416,25 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
         DownItems d = down;
         for (int it = 0; d.item < hitems; ++it, d.item += grid) {
             __syncthreads();
-            combine<WF>(a, terms, d, parts, u.y[it & 1], lane);
+            combine<WF>(a, terms, d, y + (it & 1) * yrows * 16, lane);
         }
         return;
     }
+}
+
+// Parts of a share of K for each tile, so that the wavefronts that deal out the units end together: the fewest
+// within 3 % of the least work of the busiest.
+int few_parts(int tiles, int rows, int nch, int shares, int room) {
+    int best = 1;
+    double cost = 1e30;
+    for (int q = 1; q == 1 || (q <= 32 && q * shares <= nch && q * rows <= room); ++q) {
+        const double c = (double)ceil_div(tiles * q, kWaves) / q;
+        if (c < 0.97 * cost) {
+            best = q;
+            cost = c;
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -1452,18 +1477,28 @@ int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, cons
     const int items = std::max(std::min(N * k, E) * (F / 16), H / 16 * a.hparts);
     const int grid = N == 0 ? 1 : std::min(kGrid, items);
     const int esz = act == YVMOE_ACT_BF16 ? 2 : 4;
-    const bool ldsx = (long long)N * (H * esz + kRowPad) <= kActBytes;
-    const bool ldsh = ldsx && (long long)N * (k + S) * (F * esz + kRowPad) <= kActBytes;
-#define YV_FEW(WFV)                                                                             \
-    do {                                                                                        \
-        if (N > 0) {                                                                            \
-            few_front_kernel<WFV><<<std::max(front, 1), kAllThreads, 0, st>>>(a);               \
-            YV_LAUNCH_CHECK("few_front");                                                       \
-        }                                                                                       \
-        if (ldsh) few_experts_kernel<WFV, true, true><<<grid, kAllThreads, 0, st>>>(a);         \
-        else if (ldsx) few_experts_kernel<WFV, true, false><<<grid, kAllThreads, 0, st>>>(a);   \
-        else few_experts_kernel<WFV, false, false><<<grid, kAllThreads, 0, st>>>(a);            \
-        YV_LAUNCH_CHECK("few_experts");                                                         \
+    const int nrows = N * (k + S);
+    const bool ldsx = (long long)N * (H * esz + kRowPad) <= kPoolBytes - kEndBytes;
+    auto fits = [&](int terms) {  // h and two sets of partial outputs
+        return ldsx && (long long)terms * nrows * (F * esz + kRowPad) + 128 <= kPoolBytes - 128 * nrows;
+    };
+    const bool two = act == YVMOE_ACT_BF16 && fits(2), one = fits(1);
+    a.hterms = two ? 2 : 1;
+    const int room = std::min(kYRows, two || one ? (kPoolBytes - h_bytes(a.hterms, nrows, F * esz)) / 128 : kYRows);
+    const int tiles = (int)few_tiles(N, k, E, S);
+#define YV_FEW(WFV)                                                                                              \
+    do {                                                                                                         \
+        constexpr int TWO = WFV == YVMOE_W_F32 ? 1 : 2;                                                          \
+        a.parts = few_parts(tiles, nrows, ceil_div(F / 64, Wt<WFV>::DEPTH.unit(1, two || one)), a.hparts, room); \
+        if (N > 0) {                                                                                             \
+            few_front_kernel<WFV><<<std::max(front, 1), kAllThreads, 0, st>>>(a);                                \
+            YV_LAUNCH_CHECK("few_front");                                                                        \
+        }                                                                                                        \
+        if (two) few_experts_kernel<WFV, true, true, TWO><<<grid, kAllThreads, 0, st>>>(a);                      \
+        else if (one) few_experts_kernel<WFV, true, true, 1><<<grid, kAllThreads, 0, st>>>(a);                   \
+        else if (ldsx) few_experts_kernel<WFV, true, false, 1><<<grid, kAllThreads, 0, st>>>(a);                 \
+        else few_experts_kernel<WFV, false, false, 1><<<grid, kAllThreads, 0, st>>>(a);                          \
+        YV_LAUNCH_CHECK("few_experts");                                                                          \
     } while (0)
     switch (w->format) {
         case YVMOE_W_F32: YV_FEW(YVMOE_W_F32); break;

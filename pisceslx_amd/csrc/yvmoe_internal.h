@@ -262,13 +262,17 @@ inline int few_splits(int H) { return H >= 4096 ? 4 : H >= 1024 ? H / 1024 : 1; 
 // work-groups: a column group's weights (of the experts that N tokens touch) at a CU's 25 GB/s, and
 // some 3 us around each item. (H 5120: 320 groups are two rounds alone, or five of quarters.)
 constexpr int kFewParts = 8, kFewGrid = 256;
+inline double few_tiles(int N, int k, int E, int S) {  // that tokens which choose at random make
+    return std::min((double)N * k, E * (1.0 - std::pow(std::max(0.0, 1.0 - (double)k / E), N)) + 0.5) + S;
+}
 inline int few_hparts(int N, int k, int E, int S, int H, int F, int wf) {
     const double each = wf == YVMOE_W_F32 ? 4 : wf == YVMOE_W_BF16 ? 2 : wf == YVMOE_W_INT4 ? 0.5 : 1;
-    const double tiles = std::min((double)N * k, E * (1.0 - std::pow(std::max(0.0, 1.0 - (double)k / E), N)) + 0.5) + S;
-    const double us = tiles * 16 * F * each / 25e3;
+    const double us = few_tiles(N, k, E, S) * 16 * F * each / 25e3;
+    // a share is a chunk of K at least, of up to two, four or eight steps of 64
+    const int most = std::min(kFewParts, ceil_div(F / 64, wf == YVMOE_W_INT4 ? 8 : each == 1 ? 4 : 2));
     int best = 1;
     double cost = 1e30;
-    for (int p = 1; p <= kFewParts; ++p) {
+    for (int p = 1; p <= most; ++p) {
         const double c = ceil_div(H / 16 * p, kFewGrid) * (us / p + 3.0) + (p > 1 ? 2.0 : 0.0);
         if (c < 0.97 * cost) {
             best = p;
@@ -289,7 +293,7 @@ inline FewWs few_ws(int N, int k, int E, int S, int H, int F, int wf, int act) {
     w.hsum = o;     o = align_up(o + (parts > 1 ? (size_t)parts * 2 * N * H * 4 : 0), 256);
     w.logits = o;   o = align_up(o + (size_t)few_splits(H) * N * router_ld(E, act) * 4, 256);
     w.xo = o;       o = align_up(o + (wf == YVMOE_W_INT4 ? (size_t)N * H * 2 : 0), 256);
-    w.h = o;        o = align_up(o + (size_t)N * (k + S) * F * (act == YVMOE_ACT_BF16 ? 2 : 4), 256);
+    w.h = o;        o = align_up(o + (size_t)N * (k + S) * F * 4, 256);  // bf16: two terms
     w.bytes = o;
     return w;
 }

@@ -361,3 +361,27 @@ def test_calls_side_by_side(cuda):
     torch.cuda.synchronize()
     for i, o in enumerate(got):
         assert torch.equal(o, want[i % len(xs)]), i
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("N,H,F", [(2, 512, 256), (5, 1024, 640), (16, 256, 896)])
+def test_bits_do_not_go_by_the_others_choices(cuda, fmt, N, H, F):
+    """A token's outputs are the same bits whatever experts the other tokens go to."""
+    E, k, S = 24, 4, 1
+    dt = torch.float32 if fmt == "f32" else torch.bfloat16
+    ex = make_experts(fmt, E, S, H, F, 71)
+    mix, x = torch.ones(1, device="cuda"), randn(72, N, H, dtype=dt)
+    g = torch.Generator(device="cuda").manual_seed(73)
+    w = torch.rand(N, k, device="cuda", generator=g)
+    first = None
+    for trial in range(4):
+        idx = torch.stack([torch.randperm(E, device="cuda", generator=g)[:k] for _ in range(N)])
+        if trial == 1:
+            idx[:] = idx[0]  # all the same experts
+        if trial == 2:
+            idx[1:] = -1     # none
+        idx[0] = torch.tensor([3, 7, 11, 23], device="cuda")
+        out, shared, _ = yvf.experts_few(x, w, idx, ex, mix)
+        if first is None:
+            first = out[0].clone(), shared[0].clone()
+        assert torch.equal(out[0], first[0]) and torch.equal(shared[0], first[1]), trial
