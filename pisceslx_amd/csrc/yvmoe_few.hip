@@ -42,10 +42,10 @@ namespace yvmoe {
 namespace {
 
 // k-steps per chunk and chunks held for two matrices and for one, without and with activations in LDS. As
-// many bytes in flight as the 168 registers of nine wavefronts hold without spilling (a spill in a loop
-// cost bf16 a half); longer chunks make the last one of a short K emptier (fp32 with two k-steps: 56 -> 70 us
-// at one token, 1024 -> 2816). More and thinner wavefronts do not help: with 11 one int8 token takes 48 us,
-// with 15 61, with 8 44.
+// many bytes in flight as the 168 registers of nine wavefronts hold without spilling in a loop (which cost
+// bf16 a half); longer chunks make the last one of a short K emptier (fp32 with two k-steps: 56 -> 70 us at one
+// token, 1024 -> 2816; bf16 with two: 2 to 5 % more from 1088 to 4096). More and thinner wavefronts do not
+// help: with 11 one int8 token takes 48 us, with 15 61, with 8 44.
 struct Depth {
     int u2, r2, u1, r1, lu2, lr2, lu1, lr1;
     constexpr int unit(int nm, bool lds) const { return nm == 2 ? (lds ? lu2 : u2) : (lds ? lu1 : u1); }
@@ -157,7 +157,7 @@ template <>
 struct Wt<YVMOE_W_BF16> {
     typedef Frag16 Raw;
     typedef ActB16 Act;
-    static constexpr Depth DEPTH = {1, 3, 2, 3, 2, 3, 2, 4};
+    static constexpr Depth DEPTH = {1, 3, 1, 4, 1, 4, 1, 4};
     static constexpr bool GROUPED = false;
     static __device__ __forceinline__ const char* ptr(const void* b, long long e, int n0, int K, int lane) {
         return block_ptr(b, e * 2, n0, K, 2048, 16, lane);
