@@ -27,10 +27,8 @@
 // written through and read past the caches (sc1): an acquire would invalidate every L2, 30 us for
 // the 4,096 wavefronts of a launch.
 //
-// Rounding: weights enter exactly (codes as bf16, scales on the fp32 sums), h as two bf16 terms (16 bits) where
-// they fit into LDS, else rounded once to bf16 (each WG reads all of h past the caches: with two terms from there 2
-// tokens of fp8 took 150 us, not 130); the outputs are rounded once at the end. One term's rounding is as large as
-// the outputs' own: errors against 64 bits 1.4 times those of two.
+// Rounding: weights enter exactly (codes as bf16, scales on the fp32 sums), h as two bf16 terms (16 bits) for
+// the second product's MFMAs; the outputs are rounded once at the end.
 #include <algorithm>
 #include <type_traits>
 
@@ -53,7 +51,7 @@ struct Depth {
 };
 
 constexpr int kFewSlots = kFewTokens * YVMOE_MAX_TOPK;
-constexpr int kFewTiles = kFewSlots + YVMOE_MAX_SHARED;
+constexpr int kFewTiles = kFewSlots + 2 * YVMOE_MAX_SHARED;
 // Wavefronts that stream weights; one more sums their products, stores h, takes items and waits, so that
 // the streams never wait for a store or an atomic (which answer after microseconds, and in the order
 // of the loads round them).
@@ -101,7 +99,6 @@ struct FewArgs {
     const void* xo; // x, for int4 in its order of columns
     void* h;        // [terms][N k + S N][F], routed rows by expert, then the shared experts' tokens
     unsigned* signals;  // Signal words, 32 apart
-    int hterms;       // terms of an h
     int hparts;       // work-groups per 16 columns of H
     int parts;        // parts of a work-group's share of K
     int* hcount;      // [H / 16]: those of them that are done
@@ -119,6 +116,14 @@ struct FewArgs {
 // GROUPED: the scale belongs to a row (int4) or 128 rows (fp8) and 128 columns, that is two k-steps.
 template <int WF>
 struct Wt;
+
+// h in two bf16 terms (16 bits), so that its rounding does not add to the outputs' own (with one term errors
+// against 64 bits are 1.4 times as large): both are rows of one operand, so that they cost no instruction. A tile
+// of the second kernel has eight rows therefore, and more of one expert's read its weights again.
+template <int WF>
+constexpr int kTerms = WF == YVMOE_W_F32 ? 1 : 2;
+template <int WF>
+constexpr int kTileRows = 16 / kTerms<WF>;
 
 // 16 bytes at an offset (none, and nothing read, past the buffer's end). FRESH: read past the caches (h,
 // which other work-groups of the launch have written).
@@ -422,45 +427,36 @@ struct Chunk {
             for (int m = 0; m < NM; ++m) rs[m] = bf16_to_f32(*(const unsigned short*)o.s[m]);
     }
 };
-// T terms of each number, the later ones `plane` bytes further on.
-template <int WF, int NM, bool LDS, int T>
+template <int WF, int NM, bool LDS>
 struct Acts {
     static constexpr int U = Wt<WF>::DEPTH.unit(NM, LDS);
-    typename Wt<WF>::Act a[U][T];
+    typename Wt<WF>::Act a[U];
     template <bool FRESH>
-    __device__ __forceinline__ void load(const Chunk<WF, NM, LDS>& q, __amdgpu_buffer_rsrc_t buf, int plane, int nks) {
+    __device__ __forceinline__ void load(const Chunk<WF, NM, LDS>& q, __amdgpu_buffer_rsrc_t buf, int nks) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int t = 0; t < T; ++t)
-                a[u][t].template load<FRESH>(buf, q.act + t * plane, min(q.c * U + u, nks - 1));
+        for (int u = 0; u < U; ++u) a[u].template load<FRESH>(buf, q.act, min(q.c * U + u, nks - 1));
     }
-    __device__ __forceinline__ void read(const Chunk<WF, NM, LDS>& q, const char* lds, int plane, int nks) {
+    __device__ __forceinline__ void read(const Chunk<WF, NM, LDS>& q, const char* lds, int nks) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int t = 0; t < T; ++t) a[u][t].read(lds + q.act + t * plane, min(q.c * U + u, nks - 1));
+        for (int u = 0; u < U; ++u) a[u].read(lds + q.act, min(q.c * U + u, nks - 1));
     }
 };
 
-// A k-step's products of a matrix, its weights converted once for all terms.
-template <int WF, int T>
-__device__ __forceinline__ void products(const typename Wt<WF>::Raw& w, const typename Wt<WF>::Act (&a)[T], f32x4& acc) {
+// A k-step's products of a matrix.
+template <int WF>
+__device__ __forceinline__ void products(const typename Wt<WF>::Raw& w, const typename Wt<WF>::Act& a, f32x4& acc) {
     if constexpr (WF == YVMOE_W_F32) {
-        Wt<WF>::mma(w, a[0], acc);
+        Wt<WF>::mma(w, a, acc);
     } else {
         const Frag16 f = Wt<WF>::frag(w);
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            acc = mfma16(a[t].f.v[0], f.v[0], acc);
-            acc = mfma16(a[t].f.v[1], f.v[1], acc);
-        }
+        acc = mfma16(a.f.v[0], f.v[0], acc);
+        acc = mfma16(a.f.v[1], f.v[1], acc);
     }
 }
 
 // ORDER: the activations are as the caller has them, not in int4's order yet.
-template <int WF, int NM, bool LDS, bool ORDER, int T>
-__device__ __forceinline__ void mma(const Chunk<WF, NM, LDS>& q, Acts<WF, NM, LDS, T>& x, int nks, f32x4 (&acc)[NM]) {
+template <int WF, int NM, bool LDS, bool ORDER>
+__device__ __forceinline__ void mma(const Chunk<WF, NM, LDS>& q, Acts<WF, NM, LDS>& x, int nks, f32x4 (&acc)[NM]) {
     typedef Wt<WF> W;
     const int c = q.c;
     constexpr int U = W::DEPTH.unit(NM, LDS);
@@ -469,7 +465,7 @@ __device__ __forceinline__ void mma(const Chunk<WF, NM, LDS>& q, Acts<WF, NM, LD
         for (int u = 0; u < U; ++u)
             if (c * U + u < nks)
 #pragma unroll
-                for (int m = 0; m < NM; ++m) products<WF, T>(q.w[u][m], x.a[u], acc[m]);
+                for (int m = 0; m < NM; ++m) products<WF>(q.w[u][m], x.a[u], acc[m]);
     } else {
 #pragma unroll
         for (int p = 0; p < U; p += 2) {
@@ -482,12 +478,11 @@ __device__ __forceinline__ void mma(const Chunk<WF, NM, LDS>& q, Acts<WF, NM, LD
                 if constexpr (WF == YVMOE_W_INT4) {
                     if constexpr (ORDER)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) x.a[u][0].f.u[h] = int4_order(x.a[u][0].f.u[h]);
-#pragma unroll
-                    for (int t = 0; t < T; ++t) W::offset(x.a[u][t], corr);
+                        for (int h = 0; h < 2; ++h) x.a[u].f.u[h] = int4_order(x.a[u].f.u[h]);
+                    W::offset(x.a[u], corr);
                 }
 #pragma unroll
-                for (int m = 0; m < NM; ++m) products<WF, T>(q.w[u][m], x.a[u], part[m]);
+                for (int m = 0; m < NM; ++m) products<WF>(q.w[u][m], x.a[u], part[m]);
             }
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
@@ -511,12 +506,12 @@ __device__ __forceinline__ int chunks(int K) {
 // moves it one on, after the end to lines that everyone reads. While a chunk is multiplied, the weights
 // of the next ones and (without LDS) the activations of the next are in flight, across items too. The
 // start is apart, so that the weights' part of it can come before a wait.
-template <int WF, int NM, class Walk, bool LDS, int T = 1, bool FRESH = false, bool ORDER = false>
+template <int WF, int NM, class Walk, bool LDS, bool FRESH = false, bool ORDER = false>
 struct Ring {
     static constexpr int kRing = Wt<WF>::DEPTH.ring(NM, LDS);
     static_assert(kRing <= kOwnItems - 1, "what the streams look ahead");
     Chunk<WF, NM, LDS> q[kRing];
-    Acts<WF, NM, LDS, T> x[LDS ? 1 : 2];
+    Acts<WF, NM, LDS> x[LDS ? 1 : 2];
     typename Walk::Place place[kRing];
 
     __device__ __forceinline__ void start_weights(Walk& w, int nks) {
@@ -527,12 +522,12 @@ struct Ring {
             w.next();
         }
     }
-    __device__ __forceinline__ void start_acts(Walk& w, int plane, int nks) {
-        if constexpr (!LDS) x[0].template load<FRESH>(q[0], w.o.buf, plane, nks);
+    __device__ __forceinline__ void start_acts(Walk& w, int nks) {
+        if constexpr (!LDS) x[0].template load<FRESH>(q[0], w.o.buf, nks);
     }
 
     template <class End>
-    __device__ __forceinline__ void run(Walk& w, const char* lds, int plane, int nks, End end) {
+    __device__ __forceinline__ void run(Walk& w, const char* lds, int nks, End end) {
         constexpr int STEPS = LDS || kRing % 2 == 0 ? kRing : 2 * kRing;
         f32x4 acc[NM];
 #pragma unroll
@@ -542,14 +537,14 @@ struct Ring {
             for (int i = 0; i < STEPS; ++i) {
                 constexpr int AHEAD = kRing - 1;
                 Chunk<WF, NM, LDS>&p = q[i % kRing], &n = q[(i + AHEAD) % kRing];
-                if constexpr (!LDS && kRing > 2) x[(i + 1) % 2].template load<FRESH>(q[(i + 1) % kRing], w.o.buf, plane, nks);
+                if constexpr (!LDS && kRing > 2) x[(i + 1) % 2].template load<FRESH>(q[(i + 1) % kRing], w.o.buf, nks);
                 n.load_weights(w.o, w.c, nks);
-                if constexpr (!LDS && kRing == 2) x[(i + 1) % 2].template load<FRESH>(n, w.o.buf, plane, nks);
+                if constexpr (!LDS && kRing == 2) x[(i + 1) % 2].template load<FRESH>(n, w.o.buf, nks);
                 place[(i + AHEAD) % kRing] = w.place();
                 w.next();
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (LDS) x[0].read(p, lds, plane, nks);
-                mma<WF, NM, LDS, ORDER, T>(p, x[LDS ? 0 : i % 2], nks, acc);
+                if constexpr (LDS) x[0].read(p, lds, nks);
+                mma<WF, NM, LDS, ORDER>(p, x[LDS ? 0 : i % 2], nks, acc);
                 if (place[i % kRing].ends) {
                     if constexpr (WF == YVMOE_W_INT8)
 #pragma unroll
@@ -581,12 +576,11 @@ __device__ __forceinline__ void sum_waves(const f32x4 (&red)[kWaves][2][64], int
     }
 }
 
-// h of four activation rows from row and one column, below row + n (int4: in its order of columns); with bf16
-// activations as one or two bf16 terms, the second nrows rows further on. PUBLISH: written through to where
-// every XCD reads it.
+// h of four activation rows from row and one column, below row + n (int4: in its order of columns), its second
+// term nrows rows further on. PUBLISH: written through to where every XCD reads it.
 template <int WF, bool PUBLISH>
-__device__ __forceinline__ void store_h(void* h, long long row, int n, int nrows, int terms, int F, int col,
-                                        const f32x4& g, const f32x4& u) {
+__device__ __forceinline__ void store_h(void* h, long long row, int n, int nrows, int F, int col, const f32x4& g,
+                                        const f32x4& u) {
     const int at = WF == YVMOE_W_INT4 ? int4_place(col) : col;
     auto put = [&](auto* p, auto v) {
         if constexpr (PUBLISH) __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -603,8 +597,7 @@ __device__ __forceinline__ void store_h(void* h, long long row, int n, int nrows
             const unsigned short hi = f32_to_bf16_rne(f);
             const bool finite = (hi & 0x7f80u) != 0x7f80u;
             put(p, hi);
-            if (terms > 1)
-                put(p + (long long)nrows * F, finite ? f32_to_bf16_rne(f - bf16_to_f32(hi)) : (unsigned short)0);
+            put(p + (long long)nrows * F, finite ? f32_to_bf16_rne(f - bf16_to_f32(hi)) : (unsigned short)0);
         }
     }
 }
@@ -687,11 +680,11 @@ __device__ __forceinline__ int gate_up(const FewArgs& a, At at, GateUpItems item
     if (wave < kWaves) {
         typedef GateUpWalk<WF, LDS, At> Walk;
         Walk w(a, PUBLISH ? a.xo : a.x, at, items, wave, lane);
-        Ring<WF, 2, Walk, LDS, 1, false, !PUBLISH> ring;
+        Ring<WF, 2, Walk, LDS, false, !PUBLISH> ring;
         ring.start_weights(w, a.H / 64);
-        ring.start_acts(w, 0, a.H / 64);
+        ring.start_acts(w, a.H / 64);
         int it = 0;
-        ring.run(w, lds, 0, a.H / 64, [&](const typename Walk::Place&, const f32x4 (&acc)[2]) {
+        ring.run(w, lds, a.H / 64, [&](const typename Walk::Place&, const f32x4 (&acc)[2]) {
             red[it & 1][wave][0][lane] = acc[0];
             red[it & 1][wave][1][lane] = acc[1];
             __syncthreads();
@@ -712,7 +705,7 @@ __device__ __forceinline__ int gate_up(const FewArgs& a, At at, GateUpItems item
         f32x4 sum[2];
         sum_waves<2>(red[it & 1], lane, sum);
         const int g = lane >> 4;
-        store_h<WF, PUBLISH>(a.h, row0 + 4 * g, n - 4 * g, a.N * (a.k + a.S), a.hterms, a.F, n0 + (lane & 15), sum[0], sum[1]);
+        store_h<WF, PUBLISH>(a.h, row0 + 4 * g, n - 4 * g, a.N * (a.k + a.S), a.F, n0 + (lane & 15), sum[0], sum[1]);
         more = items.advance();
     } while (more);
     return items.it;
@@ -761,8 +754,8 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_front_kernel(FewArgs a) {
         if (wave < kWaves && w.c < w.end) {
             Ring<RF, 1, RouterWalk<RF>, false> ring;
             ring.start_weights(w, nks);
-            ring.start_acts(w, 0, nks);
-            ring.run(w, nullptr, 0, nks, [&](const typename RouterWalk<RF>::Place&, const f32x4 (&acc)[1]) {
+            ring.start_acts(w, nks);
+            ring.run(w, nullptr, nks, [&](const typename RouterWalk<RF>::Place&, const f32x4 (&acc)[1]) {
                 red[0][wave][0][lane] = acc[0];
             });
         }
@@ -800,7 +793,6 @@ struct FewTables {
     short pos[kFewSlots];     // its row, -1: none
     short slot[kFewSlots];    // slot of each routed row
     short first[kFewSlots];   // a routed row's place among its expert's
-    short tile[kFewSlots];    // tile of each routed row
     short tile_e[kFewTiles], tile_row0[kFewTiles], tile_n[kFewTiles];
     float score[kFewTokens];
     int counts[YVMOE_MAX_EXPERTS];
@@ -895,8 +887,9 @@ __device__ __forceinline__ void topk_wave(const float* lg, const float* bias, in
     my_w0 = ej / tot;
 }
 
-// The routing of up to 16 tokens, from the logits or as given, and the tiles: up to 16 rows of one
+// The routing of up to 16 tokens, from the logits or as given, and the tiles: up to ROWS rows of one
 // expert each. Every work-group computes it; the first one also writes it out.
+template <int ROWS>
 __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, FewLogits& lg, bool writer) {
 #pragma clang fp contract(off)
     const int tid = threadIdx.x, N = a.N, E = a.E, k = a.k, ns = N * k;
@@ -1037,7 +1030,7 @@ __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, FewL
     bool start = false;
     int below = 0;
     if (tid < kFewSlots) {
-        start = tid < nrows && (t.first[tid] & 15) == 0;
+        start = tid < nrows && t.first[tid] % ROWS == 0;
         const unsigned long long m = __ballot(start);
         below = __popcll(m & ((1ull << (tid & 63)) - 1ull));
         if ((tid & 63) == 0) t.wave_starts[tid >> 6] = __popcll(m);
@@ -1055,18 +1048,15 @@ __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, FewL
         const int e = t.expert[t.slot[tid]];
         t.tile_e[i] = (short)e;
         t.tile_row0[i] = (short)tid;
-        t.tile_n[i] = (short)min(16, t.counts[e] - t.first[tid]);
-    }
-    if (tid < nrows) {  // the tile that starts here, or the last one that started before
-        int i = below + (start ? 1 : 0) - 1;
-        for (int w = 0; w < (tid >> 6); ++w) i += t.wave_starts[w];
-        t.tile[tid] = (short)i;
+        t.tile_n[i] = (short)min(ROWS, t.counts[e] - t.first[tid]);
     }
     const int ntiles = t.wave_starts[0] + t.wave_starts[1] + t.wave_starts[2] + t.wave_starts[3];
-    if (tid < a.S) {
-        t.tile_e[ntiles + tid] = (short)(E + tid);
-        t.tile_row0[ntiles + tid] = (short)(ns + tid * N);
-        t.tile_n[ntiles + tid] = (short)N;
+    const int each = (N + ROWS - 1) / ROWS;
+    if (tid < a.S * each) {
+        const int e = tid / each, from = (tid - e * each) * ROWS;
+        t.tile_e[ntiles + tid] = (short)(E + e);
+        t.tile_row0[ntiles + tid] = (short)(ns + e * N + from);
+        t.tile_n[ntiles + tid] = (short)min(ROWS, N - from);
     }
     if (tid == 0) t.ntiles = ntiles;
     __syncthreads();
@@ -1211,7 +1201,8 @@ struct DownWalk {
         n = __builtin_amdgcn_readfirstlane(t.tile_n[tile]);
         row = part * nrows + row0;
         o.set(0, a.w_down, a.s_down, e, a.E + a.S, a.H, a.F, items.n0(), lane);
-        o.template rows<LDS>(a.h, nrows, (lane & 15) < n ? row0 + (lane & 15) : -1, a.F, lane);
+        const int r = lane % kTileRows<WF>, term = lane % 16 / kTileRows<WF>;
+        o.template rows<LDS>(a.h, kTerms<WF> * nrows, r < n ? term * nrows + row0 + r : -1, a.F, lane);
         const int cut = items.share() * parts + part, cuts = items.hparts * parts;
         c = cut * nch / cuts;
         c1 = (cut + 1) * nch / cuts;
@@ -1219,7 +1210,7 @@ struct DownWalk {
     // no unit: a chunk past the end, from lines that everyone reads
     __device__ __forceinline__ void nothing() {
         o.set(0, a.w_down, a.s_down, 0, a.E + a.S, a.H, a.F, 0, lane);
-        o.template rows<LDS>(a.h, nrows, -1, a.F, lane);
+        o.template rows<LDS>(a.h, kTerms<WF> * nrows, -1, a.F, lane);
         c = nch;
         c1 = nch + 1;
         row = 0;
@@ -1323,7 +1314,7 @@ __host__ __device__ inline int h_bytes(int terms, int nrows, int bytes) {
     return (terms * nrows * (bytes + kRowPad) + 127) / 128 * 128;
 }
 
-template <int WF, bool LDSX, bool LDSH, int T>
+template <int WF, bool LDSX, bool LDSH>
 __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) {
     constexpr int BYTES = WF == YVMOE_W_F32 ? 4 : 2;
     __shared__ FewTables t;
@@ -1336,7 +1327,7 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, grid = gridDim.x;
     if constexpr (LDSX) stage_rows<false>(a.xo, a.N, a.H * BYTES, pool, wave, lane);
-    few_routing(a, t, lg, blockIdx.x == 0);
+    few_routing<kTileRows<WF>>(a, t, lg, blockIdx.x == 0);
     if (a.N == 0) return;
     if constexpr (LDSX) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1359,13 +1350,13 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
     const int used = nitems > kOwnItems * grid ? grid : rounds > 0 ? (nitems + rounds - 1) / rounds : 0;
     const int handed = max(0, nitems - kOwnItems * used), hitems = a.H / 16 * a.hparts;
     if ((int)blockIdx.x >= used && (int)blockIdx.x >= hitems) return;
-    const int ntiles = t.ntiles + a.S, nrows = ns + a.S * a.N;
+    const int ntiles = t.ntiles + a.S * ((a.N + kTileRows<WF> - 1) / kTileRows<WF>), nrows = ns + a.S * a.N;
     const DownItems down{(int)blockIdx.x, grid, hitems, a.hparts};
     const int yrows = nrows * a.parts;
-    float* y = (float*)(pool + (LDSH ? h_bytes(T, nrows, a.F * BYTES) : 0));
+    float* y = (float*)(pool + (LDSH ? h_bytes(kTerms<WF>, nrows, a.F * BYTES) : 0));
     auto stage_h = [&]() {
         if constexpr (LDSH) {
-            stage_rows<true>(a.h, T * nrows, a.F * BYTES, pool, wave, lane);
+            stage_rows<true>(a.h, kTerms<WF> * nrows, a.F * BYTES, pool, wave, lane);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
         }
@@ -1385,20 +1376,24 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
         if (wave < kWaves) {
             typedef DownWalk<WF, LDSH> Walk;
             Walk w(a, t, down, nrows, ntiles, wave, lane);
-            Ring<WF, 1, Walk, LDSH, T, true> ring;
+            Ring<WF, 1, Walk, LDSH, true> ring;
             ring.start_weights(w, a.F / 64);  // no h is needed for these
             __syncthreads();
             share = __builtin_amdgcn_readfirstlane(t.help);
             if (share >= 0) continue;
             stage_h();
-            const int plane = nrows * (a.F * BYTES + kRowPad);
-            ring.start_acts(w, plane, a.F / 64);
+            ring.start_acts(w, a.F / 64);
             int it = 0;
-            ring.run(w, pool, plane, a.F / 64, [&](const typename Walk::Place& p, const f32x4 (&acc)[1]) {
-                if (p.unit)
+            ring.run(w, pool, a.F / 64, [&](const typename Walk::Place& p, const f32x4 (&acc)[1]) {
+                if (p.unit) {
+                    f32x4 v = acc[0];
+                    if constexpr (kTerms<WF> == 2)  // rows 8 .. 15 are the second terms'
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = v[i] + __shfl_xor(v[i], 32);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (4 * (lane >> 4) + i < p.n) y[((it & 1) * yrows + p.row + 4 * (lane >> 4) + i) * 16 + r] = acc[0][i];
+                        if (4 * (lane >> 4) + i < p.n) y[((it & 1) * yrows + p.row + 4 * (lane >> 4) + i) * 16 + r] = v[i];
+                }
                 if (p.item_ends) {
                     __syncthreads();
                     ++it;
@@ -1479,26 +1474,21 @@ int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, cons
     const int esz = act == YVMOE_ACT_BF16 ? 2 : 4;
     const int nrows = N * (k + S);
     const bool ldsx = (long long)N * (H * esz + kRowPad) <= kPoolBytes - kEndBytes;
-    auto fits = [&](int terms) {  // h and two sets of partial outputs
-        return ldsx && (long long)terms * nrows * (F * esz + kRowPad) + 128 <= kPoolBytes - 128 * nrows;
-    };
-    const bool two = act == YVMOE_ACT_BF16 && fits(2), one = fits(1);
-    a.hterms = two ? 2 : 1;
-    const int room = std::min(kYRows, two || one ? (kPoolBytes - h_bytes(a.hterms, nrows, F * esz)) / 128 : kYRows);
-    const int tiles = (int)few_tiles(N, k, E, S);
-#define YV_FEW(WFV)                                                                                              \
-    do {                                                                                                         \
-        constexpr int TWO = WFV == YVMOE_W_F32 ? 1 : 2;                                                          \
-        a.parts = few_parts(tiles, nrows, ceil_div(F / 64, Wt<WFV>::DEPTH.unit(1, two || one)), a.hparts, room); \
-        if (N > 0) {                                                                                             \
-            few_front_kernel<WFV><<<std::max(front, 1), kAllThreads, 0, st>>>(a);                                \
-            YV_LAUNCH_CHECK("few_front");                                                                        \
-        }                                                                                                        \
-        if (two) few_experts_kernel<WFV, true, true, TWO><<<grid, kAllThreads, 0, st>>>(a);                      \
-        else if (one) few_experts_kernel<WFV, true, true, 1><<<grid, kAllThreads, 0, st>>>(a);                   \
-        else if (ldsx) few_experts_kernel<WFV, true, false, 1><<<grid, kAllThreads, 0, st>>>(a);                 \
-        else few_experts_kernel<WFV, false, false, 1><<<grid, kAllThreads, 0, st>>>(a);                          \
-        YV_LAUNCH_CHECK("few_experts");                                                                          \
+    const int terms = act == YVMOE_ACT_BF16 ? 2 : 1;
+    const bool ldsh = ldsx && (long long)terms * nrows * (F * esz + kRowPad) + 128 <= kPoolBytes - 128 * nrows;
+    const int room = std::min(kYRows, ldsh ? (kPoolBytes - h_bytes(terms, nrows, F * esz)) / 128 : kYRows);
+    const int tiles = (int)few_tiles(N, k, E, 0) + S * ceil_div(N, 16 / terms);
+#define YV_FEW(WFV)                                                                                       \
+    do {                                                                                                  \
+        a.parts = few_parts(tiles, nrows, ceil_div(F / 64, Wt<WFV>::DEPTH.unit(1, ldsh)), a.hparts, room); \
+        if (N > 0) {                                                                                      \
+            few_front_kernel<WFV><<<std::max(front, 1), kAllThreads, 0, st>>>(a);                         \
+            YV_LAUNCH_CHECK("few_front");                                                                 \
+        }                                                                                                 \
+        if (ldsh) few_experts_kernel<WFV, true, true><<<grid, kAllThreads, 0, st>>>(a);                   \
+        else if (ldsx) few_experts_kernel<WFV, true, false><<<grid, kAllThreads, 0, st>>>(a);             \
+        else few_experts_kernel<WFV, false, false><<<grid, kAllThreads, 0, st>>>(a);                      \
+        YV_LAUNCH_CHECK("few_experts");                                                                   \
     } while (0)
     switch (w->format) {
         case YVMOE_W_F32: YV_FEW(YVMOE_W_F32); break;

@@ -365,7 +365,7 @@ def moe_forward_few(x2d: torch.Tensor, router: RouterState, experts: PackedExper
                     mix: Optional[torch.Tensor], skip: Optional[torch.Tensor],
                     workspace: Optional[torch.Tensor] = None):
     """moe_forward for up to 16 tokens in two kernels (yvmoe_forward_few), with fewer roundings:
-    weights enter exactly, h keeps 16 bits or (many tokens) is rounded once, the outputs once. ``workspace`` is scratch of
+    weights enter exactly, h keeps 16 bits, the outputs are rounded once. ``workspace`` is scratch of
     few_workspace_bytes (allocated here when None or too small); calls that overlap in time need
     one each. Returns (out [N,H], shared_out [N,H] or None, Routing)."""
     dev = _require_cuda(x2d, router.w_router, mix, skip, *experts.tensors())
