@@ -275,12 +275,12 @@ int32_t yvmoe_forward_static(const void* x, int32_t act_dtype, int32_t n_tokens,
 
 /*
  * The layer for a few tokens (0 <= N <= YVMOE_FEW_TOKENS) in two kernels, for decoding one or a few
- * sequences. Routing, formats, shapes, results and limits are yvmoe_forward's, with fewer roundings: quantized
- * weights enter the products exactly (yvmoe_forward rounds bf16(q * s)), gate and up stay fp32, h keeps
- * 16 bits (two bf16 terms), expert outputs and their weighted sum stay fp32, and out and shared_out are
- * each rounded once. How sums are cut goes by
- * sizes alone: a token's bits do not depend on the experts that the others choose. Router logits are fp32 sums in an order of their own (a tie within the last bits may
- * fall the other way). Equal calls give equal bits.
+ * sequences. Routing, formats, shapes, results and limits are yvmoe_forward's (ffn below 2^22), with fewer
+ * roundings: quantized weights enter the products exactly (yvmoe_forward rounds bf16(q * s)), gate and up
+ * stay fp32, h keeps 16 bits (two bf16 terms), expert outputs and their weighted sum stay fp32, and out and
+ * shared_out are each rounded once. Router logits are fp32 sums in an order of their own (a tie within the
+ * last bits may fall the other way). Equal calls give equal bits, and a token's outputs do not depend on the
+ * experts that the others choose: how sums are cut goes by sizes alone.
  *
  * yvmoe_forward_few: the whole layer with YvStableMoEGate's routing.
  * yvmoe_experts_few: the routed and shared experts, the weighted sum and the skip residual for a

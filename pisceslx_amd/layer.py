@@ -20,8 +20,9 @@ reference keys ``experts.{e}.{gate,up,down}_proj.weight``,
 
 ``few_tokens`` (or ``cfg.moe_few_tokens``, 0 to 16, default 0): calls of up to that many tokens take
 the few-token form (``functional.moe_forward_few``; after YvMoEGate's own call, ``experts_few``),
-which rounds less often, so its results differ from the general form's in the last bits. It is faster
-at 1 and 2 tokens (int8, H 4096: 44 and 61 us, general 51 and 66; int4 up to 4) and not in fp32. Longer
+which rounds less often, so its results differ from the general form's in the last bits. With
+router="stable" it is faster at 1 and 2 tokens (int8, H 4096: 44 and 58 us, general 51 and 66; int8 and
+int4 up to 4), with YvMoEGate and in fp32 about level. Longer
 calls are as without it.
 """
 from __future__ import annotations
