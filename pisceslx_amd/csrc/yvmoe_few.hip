@@ -13,7 +13,7 @@
 //    sums, and the gate/up products of the shared experts; it also clears the counters of 2.
 // 2. few_experts_kernel: every work-group computes the routing from the logits by itself (N·k <= 256
 //    slots in LDS; cheaper than another launch), then the gate/up products of the routed experts as
-//    (16-row tile, 16 columns of F) items, and once all of them are there each work-group takes 16
+//    (tile, 16 columns of F) items, and once all of them are there each work-group takes 16
 //    columns of H of *all* tiles, so that the weighted sum, the shared mixture and the skip residual
 //    end in its LDS: no expert output leaves the chip. Where H gives too few work-groups, up to eight
 //    share 16 columns, and the last one to finish adds up their sums, in their order.
@@ -1241,7 +1241,8 @@ struct DownWalk {
 // of 16 columns for every token, from the partial outputs y; shared between work-groups, the sum of
 // their sums by the last of them.
 template <int WF>
-__device__ __forceinline__ void combine(const FewArgs& a, const Term* list, const DownItems& d, const float* y, int lane) {
+__device__ __forceinline__ void combine(const FewArgs& a, const Term* list, const DownItems& d, const float* y,
+                                        int lane) {
     constexpr bool F32 = WF == YVMOE_W_F32;
     const int c = lane & 15, ns = a.N * a.k, n0 = d.n0(), parts = a.parts;
     const long long stride = (long long)a.N * a.H;
@@ -1392,7 +1393,8 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
                         for (int i = 0; i < 4; ++i) v[i] = v[i] + __shfl_xor(v[i], 32);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (4 * (lane >> 4) + i < p.n) y[((it & 1) * yrows + p.row + 4 * (lane >> 4) + i) * 16 + r] = v[i];
+                        if (4 * (lane >> 4) + i < p.n)
+                            y[((it & 1) * yrows + p.row + 4 * (lane >> 4) + i) * 16 + r] = v[i];
                 }
                 if (p.item_ends) {
                     __syncthreads();

@@ -319,7 +319,7 @@ class PackedLinear:
                                self.scales.data_ptr())
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
-        """The dense [out][in] weight (for checkers)."""
+        """The dense [out][in] weight (for tests)."""
         ob, groups = self.codes.shape[:2]
         w = self.codes.view(torch.int32).view(ob, groups, 4, 16, 4, 1)     # [g][r][dword]
         shift = torch.tensor([0, 8, 16, 24, 4, 12, 20, 28], dtype=torch.int32, device=w.device)

@@ -385,3 +385,21 @@ def test_bits_do_not_go_by_the_others_choices(cuda, fmt, N, H, F):
         if first is None:
             first = out[0].clone(), shared[0].clone()
         assert torch.equal(out[0], first[0]) and torch.equal(shared[0], first[1]), trial
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("N,E,k,S,H,F", [(16, 20, 16, 8, 128, 128), (16, 256, 16, 8, 256, 384), (9, 3, 3, 8, 640, 128)])
+def test_the_most_slots(cuda, fmt, N, E, k, S, H, F):
+    """As many slots, shared experts and rows of one expert as there can be."""
+    print(f"most slots {fmt} {N} {E} {k} {S} {H} {F}", flush=True)
+    dt = torch.float32 if fmt == "f32" else torch.bfloat16
+    ex = make_experts(fmt, E, S, H, F, 81)
+    g = torch.Generator(device="cuda").manual_seed(82)
+    mix, x, skip = torch.rand(S, device="cuda", generator=g), randn(83, N, H, dtype=dt), randn(84, N, H, dtype=dt)
+    w = torch.rand(N, k, device="cuda", generator=g)
+    idx = torch.stack([torch.randperm(E, device="cuda", generator=g)[:k] for _ in range(N)])
+    out, shared, invalid = yvf.experts_few(x, w, idx, ex, mix, skip)
+    ref, sref, tol, stol = reference(x, w.double(), idx, ex, mix.double(), skip)
+    check(out, ref, tol, "out")
+    check(shared, sref, stol, "shared")
+    assert int(invalid) == 0
