@@ -58,7 +58,7 @@ constexpr int kFewTiles = kFewSlots + 2 * YVMOE_MAX_SHARED;
 constexpr int kWaves = 8, kThreads = 64 * kWaves, kAllThreads = kThreads + 64;
 constexpr int kYRows = 512;            // rows of partial expert outputs that a work-group holds
 constexpr int kGrid = kFewGrid;  // most work-groups of the second kernel: one per CU
-constexpr int kPatience = 4096;  // looks at a signal, about half a microsecond each, before helping
+constexpr int kPatience = 1024;  // looks at a signal, between half and one microsecond each, before helping
 
 constexpr int kOwnItems = 5;  // gate/up items that a work-group takes without asking (GateUpItems)
 constexpr int kMarkWords = kGrid / 32, kGoLines = 32;
@@ -1153,7 +1153,7 @@ __device__ __forceinline__ int wait_done(const FewArgs& a, int used, int lane) {
             const int l = __ffsll(turned != 0 ? turned : open) - 1;
             return __builtin_amdgcn_readlane(32 * lane + __ffs(~m) - 1, l);
         }
-        if (round >= 1 << 9) return -1;  // only if another call has cleared the words
+        if (round >= 1 << 11) return -1;  // only if another call has cleared the words
     }
 }
 
