@@ -24,6 +24,7 @@
 
 #include "yvmoe_frag.h"
 #include "yvmoe_internal.h"
+#include "yvmoe_linear_stream.h"
 
 namespace yvmoe {
 namespace {
@@ -197,23 +198,20 @@ __global__ __launch_bounds__(512, 4) void int4_few_kernel(LinArgs a) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r = lane & 15;
-    const int sets = (a.blocks + RB - 1) / RB;
-    const int items = (sets - 1 - (int)blockIdx.x) / (int)gridDim.x + 1;
     struct W {
         uint4 w[RB];
         unsigned short s[RB];
     };
-    int ahead_item = 0, ahead_kg = min(wave, a.groups - 1);
+    CodeStream<RB> ahead(a.blocks, a.groups, wave, blockIdx.x, gridDim.x);
+    const int items = ahead.items;
     auto load_w = [&](W& q) {  // after the last group: that one again, not used
-        const int set = (int)blockIdx.x + ahead_item * (int)gridDim.x;
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            const long long at = (long long)min(set * RB + b, a.blocks - 1) * a.groups + ahead_kg;
+            const long long at = ahead.at(b);
             q.w[b] = nt_load16(a.codes + at * 1024 + lane * 16);
             q.s[b] = a.scales[at * 16 + r];
         }
-        if (ahead_kg + 8 < a.groups) ahead_kg += 8;
-        else if (ahead_item + 1 < items) ahead_item += 1, ahead_kg = wave;
+        ahead.next();
     };
     W q[D];
 #pragma unroll
