@@ -290,6 +290,9 @@ int32_t yvmoe_forward_static(const void* x, int32_t act_dtype, int32_t n_tokens,
  * (int32 device scalar, may be NULL) receives their number. With num_shared == 0 and skip NULL this
  * is yvmoe_dispatch.
  *   mix, skip, shared_out: as for yvmoe_combine.
+ * out, shared_out and the workspace may overlap neither each other nor x, mix or a given routing
+ * (work-groups write out while others still read those); skip may be out or shared_out itself, and
+ * may overlap them and the workspace in no other way. Such calls are refused.
  * workspace: yvmoe_few_workspace_bytes() bytes, which nothing need initialise; calls that overlap in
  * time need workspaces of their own. (Overlapping calls on one workspace end, but out is undefined.)
  */

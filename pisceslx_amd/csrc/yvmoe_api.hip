@@ -436,6 +436,38 @@ static int check_few(const void* x, int act, int N, int k, const yvmoe_expert_we
     return YVMOE_OK;
 }
 
+struct Range {
+    const void* p;  // NULL: none
+    size_t bytes;
+    bool overlaps(const Range& o) const {
+        return p != nullptr && o.p != nullptr && bytes > 0 && o.bytes > 0 &&
+               (uintptr_t)p < (uintptr_t)o.p + o.bytes && (uintptr_t)o.p < (uintptr_t)p + bytes;
+    }
+};
+
+// What the few-token kernels write is apart from what they read: a work-group that starts late reads x and the
+// routing after others have written their columns of out. skip alone is read by the lane that writes the
+// same element, right before.
+static int check_few_ranges(const void* x, int act, int N, int k, const yvmoe_expert_weights* w, const void* rweights,
+                            int weight_dtype, const int64_t* rindices, const float* mix, const void* skip,
+                            const void* out, const void* shared_out, const void* workspace) {
+    const size_t esz = act == YVMOE_ACT_F32 ? 4 : 2, rows = esz * N * w->hidden, slots = (size_t)N * k;
+    const Range o{out, rows}, s{shared_out, rows}, sk{skip, rows};
+    const Range ws{workspace, few_ws(N, k, w->num_routed, w->num_shared, w->hidden, w->ffn, w->format, act).bytes};
+    const Range in[] = {{x, rows},
+                        {rweights, slots * (weight_dtype == YVMOE_ACT_F32 ? 4 : 2)},
+                        {rindices, slots * 8},
+                        {mix, (size_t)w->num_shared * 4}};
+    for (const Range& r : in)
+        YV_REQUIRE(!o.overlaps(r) && !s.overlaps(r) && !ws.overlaps(r), YVMOE_ERR_ARG,
+                   "out, shared_out or the workspace overlaps an input");
+    YV_REQUIRE(!o.overlaps(s) && !o.overlaps(ws) && !s.overlaps(ws), YVMOE_ERR_ARG,
+               "two of out, shared_out and the workspace overlap");
+    YV_REQUIRE((skip == out || !sk.overlaps(o)) && (skip == shared_out || !sk.overlaps(s)) && !sk.overlaps(ws),
+               YVMOE_ERR_ARG, "skip overlaps what the call writes (it may be out or shared_out itself)");
+    return YVMOE_OK;
+}
+
 int32_t yvmoe_forward_few(const void* x, int32_t act_dtype, int32_t n_tokens,
                           const yvmoe_router* router, const yvmoe_expert_weights* experts,
                           const float* mix, const void* skip, void* out, void* shared_out,
@@ -456,6 +488,9 @@ int32_t yvmoe_forward_few(const void* x, int32_t act_dtype, int32_t n_tokens,
     if (!router->fixed_shape_mode && router->dynamic_capacity)
         YV_REQUIRE(router->b1 && router->w2 && router->b2, YVMOE_ERR_ARG,
                    "dynamic capacity needs the predictor's weights");
+    rc = check_few_ranges(x, act_dtype, n_tokens, router->top_k, experts, nullptr, 0, nullptr, mix, skip, out,
+                          shared_out, workspace);
+    if (rc) return rc;
     return few_launch(x, act_dtype, n_tokens, router->top_k, router, nullptr, 0, nullptr, experts, mix, skip, out,
                       shared_out, routing, nullptr, (char*)workspace, (hipStream_t)stream);
 }
@@ -471,9 +506,12 @@ int32_t yvmoe_experts_few(const void* x, int32_t act_dtype, int32_t n_tokens,
                "slots_per_token=%d outside [1, %d]", slots_per_token, YVMOE_MAX_TOPK);
     YV_REQUIRE(weight_dtype == YVMOE_ACT_F32 || weight_dtype == YVMOE_ACT_BF16, YVMOE_ERR_DTYPE,
                "routing weights must be fp32 or bf16 (got dtype %d)", weight_dtype);
-    const int rc = check_few(x, act_dtype, n_tokens, slots_per_token, experts, mix, out, workspace, workspace_bytes);
+    int rc = check_few(x, act_dtype, n_tokens, slots_per_token, experts, mix, out, workspace, workspace_bytes);
     if (rc) return rc;
     YV_REQUIRE(n_tokens == 0 || (routing_weights && expert_indices), YVMOE_ERR_ARG, "NULL pointer");
+    rc = check_few_ranges(x, act_dtype, n_tokens, slots_per_token, experts, routing_weights, weight_dtype, expert_indices,
+                          mix, skip, out, shared_out, workspace);
+    if (rc) return rc;
     return few_launch(x, act_dtype, n_tokens, slots_per_token, nullptr, routing_weights,
                       weight_dtype == YVMOE_ACT_BF16, expert_indices, experts, mix, skip, out, shared_out, nullptr,
                       invalid, (char*)workspace, (hipStream_t)stream);
