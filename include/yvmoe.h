@@ -421,8 +421,9 @@ int32_t yvmoe_rmsnorm(const void* x, int32_t act_dtype, int32_t n_tokens, int32_
  *   products, rounded once to the activation dtype.
  * x [N][in], bias [out] or NULL and out [N][out] in the activation dtype, row-major, at any address
  * that suits their elements; in_features and out_features from 1 to 2^24, n_rows from 0 to 2^30,
- * n_rows x out_features up to about 2^36. out may not overlap x. A row of x with an infinity (fp32:
- * or a number beyond 3.39e38) or NaN gives NaN in all its outputs.
+ * n_rows x out_features up to about 2^36. out may overlap neither x nor the weight, and bias only if
+ * it is bias itself, of one row. A row of x with an infinity (fp32: or a number beyond 3.39e38) or NaN
+ * gives NaN in all its outputs.
  *   codes [ceil(out/16)][ceil(in/128)] blocks of 1 KB, each 16 rows x 128 columns: byte
  *         16 (16 g + r) starts row r's columns 32 g .. 32 g + 31 (g = 0..3), eight of them in each
  *         of four dwords, columns 0 .. 3 of the eight in its bytes' lower nibbles, 4 .. 7 in the upper;

@@ -754,9 +754,14 @@ int32_t yvmoe_int4_linear(const void* x, int32_t act_dtype, int32_t n_rows,
                "codes must be 16-byte and scales 8-byte aligned");
     YV_REQUIRE(((uintptr_t)x | (uintptr_t)bias | (uintptr_t)out) % (act_dtype == YVMOE_ACT_F32 ? 4 : 2) == 0,
                YVMOE_ERR_ARG, "x, bias and out must be aligned to their elements");
-    const uintptr_t esz = act_dtype == YVMOE_ACT_F32 ? 4 : 2, xa = (uintptr_t)x, oa = (uintptr_t)out;
-    YV_REQUIRE(oa + esz * n_rows * weight->out_features <= xa || xa + esz * n_rows * weight->in_features <= oa,
-               YVMOE_ERR_ARG, "out overlaps x");
+    const size_t esz = act_dtype == YVMOE_ACT_F32 ? 4 : 2, K = weight->in_features, O = weight->out_features;
+    const size_t groups = (size_t)ceil_div(weight->out_features, 16) * ceil_div(weight->in_features, 128);
+    const Range o{out, esz * n_rows * O};
+    YV_REQUIRE(!o.overlaps({x, esz * n_rows * K}), YVMOE_ERR_ARG, "out overlaps x");
+    YV_REQUIRE(!o.overlaps({weight->codes, groups * 1024}) && !o.overlaps({weight->scales, groups * 32}), YVMOE_ERR_ARG,
+               "out overlaps the weight");
+    // of one row each element is read by the lane that writes it
+    YV_REQUIRE((bias == out && n_rows == 1) || !o.overlaps({bias, esz * O}), YVMOE_ERR_ARG, "out overlaps bias");
     return int4_linear_launch(x, act_dtype, n_rows, weight, bias, out, (hipStream_t)stream);
 }
 

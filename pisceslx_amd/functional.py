@@ -608,8 +608,8 @@ def int4_linear(x: torch.Tensor, weight: PackedLinear, bias: Optional[torch.Tens
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [..., in] · Wᵀ (+ bias [out]) with a 4-bit weight (quant.pack_linear), in fp32 sums of exact
     products rounded once to x's dtype (bf16 or fp32), which bias and ``out`` share. Any number of
-    rows; ``out`` [..., out] must not overlap x. An infinity or NaN in a row of x makes all its outputs
-    NaN."""
+    rows; ``out`` [..., out] must not overlap x or the weight, nor bias unless it is bias, of one row. An
+    infinity or NaN in a row of x makes all its outputs NaN."""
     K, O = weight.in_features, weight.out_features
     shape, dt = x.shape, x.dtype
     if x.dim() == 0 or shape[-1] != K:
