@@ -607,13 +607,16 @@ def rms_norm(x: torch.Tensor, norms, out: Optional[torch.Tensor] = None) -> torc
 def int4_linear(x: torch.Tensor, weight: PackedLinear, bias: Optional[torch.Tensor] = None,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [..., in] · Wᵀ (+ bias [out]) with a 4-bit weight (quant.pack_linear), in fp32 sums of exact
-    products rounded once to x's dtype (bf16 or fp32), which bias and ``out`` share. Any number of
+    products rounded once to x's dtype (bf16 or fp32), which bias and ``out`` share. Up to 2^30
     rows; ``out`` [..., out] must not overlap x or the weight, nor bias unless it is bias, of one row. An
     infinity or NaN in a row of x makes all its outputs NaN."""
     K, O = weight.in_features, weight.out_features
     shape, dt = x.shape, x.dtype
     if x.dim() == 0 or shape[-1] != K:
         raise ValueError(f"x must be [..., {K}], got {tuple(shape)}")
+    rows = x.numel() // K
+    if rows > 1 << 30:
+        raise ValueError(f"{rows} rows: a call takes up to 2^30")
     dev = _require_cuda(x, weight.codes, weight.scales, bias, out)
     act = _act(dt)
     if bias is not None and (bias.dtype != dt or bias.numel() != O):
@@ -624,7 +627,7 @@ def int4_linear(x: torch.Tensor, weight: PackedLinear, bias: Optional[torch.Tens
     elif out.shape != want or out.dtype != dt:
         raise ValueError(f"out must be {dt} {tuple(want)}")
     w = weight.struct()
-    rc = _lib.lib().yvmoe_int4_linear(x.data_ptr(), act, x.numel() // K, ctypes.byref(w), _ptr(bias),
+    rc = _lib.lib().yvmoe_int4_linear(x.data_ptr(), act, rows, ctypes.byref(w), _ptr(bias),
                                       out.data_ptr(), _stream(dev))
     if rc:
         _lib.check(rc, "yvmoe_int4_linear")
