@@ -310,6 +310,17 @@ class PackedLinear:
     codes: torch.Tensor
     scales: torch.Tensor
 
+    def __post_init__(self):
+        blocks, groups = -(-self.out_features // 16), -(-self.in_features // 128)
+        if blocks < 1 or groups < 1:
+            raise ValueError(f"a linear layer needs features, got in {self.in_features}, out {self.out_features}")
+        if self.codes.shape != (blocks, groups, 1024) or self.codes.dtype != torch.uint8:
+            raise ValueError(f"codes must be uint8 [{blocks}, {groups}, 1024], got {self.codes.dtype} "
+                             f"{tuple(self.codes.shape)}")
+        if self.scales.shape != (blocks, groups, 16) or self.scales.dtype != torch.bfloat16:
+            raise ValueError(f"scales must be bfloat16 [{blocks}, {groups}, 16], got {self.scales.dtype} "
+                             f"{tuple(self.scales.shape)}")
+
     def to(self, device) -> "PackedLinear":
         return PackedLinear(self.in_features, self.out_features, self.codes.to(device),
                             self.scales.to(device))
