@@ -62,15 +62,17 @@ class YvInt4Linear(nn.Module):
 
     def load_reference_state_dict(self, src, name: str) -> None:
         """The Linear ``name`` of a reference state dict, full precision or quantized
-        (``checkpoint.linear_weight``), packed; its ``bias`` where the layer has one."""
+        (``checkpoint.linear_weight``), packed, and its ``bias``, which the checkpoint has if and only if the
+        layer does."""
+        key = f"{name}.bias"
+        if self.bias is not None and key not in src:
+            raise KeyError(f"{key}: not in the checkpoint")
+        if self.bias is None and key in src:
+            raise ValueError(f"{key}: the layer has no bias")
         self.set_weight(pack_linear(linear_weight(src, name).to(self.codes.device)))
         if self.bias is not None:
-            key = f"{name}.bias"
-            if key in src:
-                with torch.no_grad():
-                    self.bias.copy_(src.get(key) if isinstance(src, StateSource) else src[key])
-            else:
-                raise KeyError(f"{key}: not in the checkpoint")
+            with torch.no_grad():
+                self.bias.copy_(src.get(key) if isinstance(src, StateSource) else src[key])
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self.training:
