@@ -294,7 +294,8 @@ int32_t yvmoe_forward_static(const void* x, int32_t act_dtype, int32_t n_tokens,
  * (work-groups write out while others still read those); skip may be out or shared_out itself, and
  * may overlap them and the workspace in no other way. Such calls are refused.
  * workspace: yvmoe_few_workspace_bytes() bytes, which nothing need initialise; calls that overlap in
- * time need workspaces of their own. (Overlapping calls on one workspace end, but out is undefined.)
+ * time need workspaces of their own. (Overlapping calls on one workspace end, but out is undefined;
+ * columns whose work-group has given up waiting, after seconds, are NaN.)
  */
 #define YVMOE_FEW_TOKENS 16
 size_t yvmoe_few_workspace_bytes(int32_t n_tokens, int32_t act_dtype, int32_t slots_per_token,

@@ -30,6 +30,7 @@
 // Rounding: weights enter exactly (codes as bf16, scales on the fp32 sums), h as two bf16 terms (16 bits) for
 // the second product's MFMAs; the outputs are rounded once at the end.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "yvmoe_frag.h"
@@ -58,7 +59,13 @@ constexpr int kFewTiles = kFewSlots + 2 * YVMOE_MAX_SHARED;
 constexpr int kWaves = 8, kThreads = 64 * kWaves, kAllThreads = kThreads + 64;
 constexpr int kYRows = 512;            // rows of partial expert outputs that a work-group holds
 constexpr int kGrid = kFewGrid;  // most work-groups of the second kernel: one per CU
-constexpr int kPatience = 1024;  // looks at a signal, between half and one microsecond each, before helping
+// Looks at a signal, between half and one microsecond each, before helping, and rounds of them after which a wait
+// with nothing to help with is given up (seconds).
+constexpr int kPatience = 1024, kMostRounds = 1 << 11;
+enum Waited { WAIT_DONE = -1, WAIT_GIVEN_UP = -2 };
+// What a SIG_GO word holds: GO_DONE once all is done, before that 0 or how a test wants the wait.
+enum Go { GO_DONE = 1, GO_ONE_LOOK = 2, GO_NO_WAIT = 4 };
+std::atomic<int> wait_mode{0};
 
 constexpr int kOwnItems = 5;  // gate/up items that a work-group takes without asking (GateUpItems)
 constexpr int kMarkWords = kGrid / 32, kGoLines = 32;
@@ -69,7 +76,7 @@ enum Signal {
     SIG_FINISHED = kMarkWords,   // items handed out that are done
     SIG_ROOT,                    // of the above, how many are complete
     SIG_TICKET,                  // items handed out
-    SIG_GO,                      // kGoLines words: all is done
+    SIG_GO,                      // kGoLines words: all is done (Go)
     SIG_COUNT = SIG_GO + kGoLines
 };
 constexpr int kSignalBytes = SIG_COUNT * 128;
@@ -103,6 +110,7 @@ struct FewArgs {
     int parts;        // parts of a work-group's share of K
     int* hcount;      // [H / 16]: those of them that are done
     float* hsum;      // [hparts][2][N][H]: their sums of the routed and of the shared experts
+    int wait_mode;    // what the first kernel puts into the SIG_GO words
 };
 
 // ---------------------------------------------------------------- weights and activations
@@ -734,7 +742,7 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_front_kernel(FewArgs a) {
     const int r = lane & 15;
     int b = blockIdx.x;
     if (b == 0) {
-        for (int i = threadIdx.x; i < SIG_COUNT; i += kAllThreads) a.signals[32 * i] = 0;
+        for (int i = threadIdx.x; i < SIG_COUNT; i += kAllThreads) a.signals[32 * i] = i < SIG_GO ? 0 : a.wait_mode;
         if (a.hparts > 1)
             for (int i = threadIdx.x; i < a.H / 16; i += kAllThreads) a.hcount[i] = 0;
     }
@@ -1127,20 +1135,22 @@ __device__ __forceinline__ void signal_done(const FewArgs& a, int share, int use
                                complete == all;
     }
     if (__builtin_amdgcn_readfirstlane(complete) != 0 && lane < kGoLines)
-        __hip_atomic_store(word(SIG_GO + lane), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(word(SIG_GO + lane), (unsigned)GO_DONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Waits until all is done (-1), or kPatience looks: then a share whose mark is missing, if there is one.
-// Called by one wavefront.
+// Waits until all is done, or kPatience looks: then a share whose mark is missing, if there is one. With none
+// missing some other work-group holds items that were handed out, and the wait goes on for kMostRounds: only
+// another call that has cleared the words meanwhile brings it there. Called by one wavefront.
 __device__ __forceinline__ int wait_done(const FewArgs& a, int used, int lane) {
     unsigned* go = a.signals + 32 * (SIG_GO + blockIdx.x % kGoLines);
     for (int round = 0;; ++round) {
-        for (int i = 0; i < kPatience; ++i) {
-            if (__builtin_amdgcn_readfirstlane(
-                    __hip_atomic_load(go, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) != 0)
-                return -1;
+        unsigned now = 0;
+        for (int i = 0; i < kPatience && now == 0; ++i) {
+            now = __builtin_amdgcn_readfirstlane(__hip_atomic_load(go, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            if (now == GO_DONE) return WAIT_DONE;
             __builtin_amdgcn_s_sleep(8);
         }
+        if (now == GO_NO_WAIT) return WAIT_GIVEN_UP;
         unsigned m = ~0u;
         if (lane * 32 < used) {
             m = __hip_atomic_load(a.signals + 32 * (SIG_MARKS + lane), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -1153,7 +1163,7 @@ __device__ __forceinline__ int wait_done(const FewArgs& a, int used, int lane) {
             const int l = __ffsll(turned != 0 ? turned : open) - 1;
             return __builtin_amdgcn_readlane(32 * lane + __ffs(~m) - 1, l);
         }
-        if (round >= 1 << 11) return -1;  // only if another call has cleared the words
+        if (round >= (now == 0 ? kMostRounds : kPatience * kMostRounds)) return WAIT_GIVEN_UP;
     }
 }
 
@@ -1404,7 +1414,9 @@ __global__ __launch_bounds__(kAllThreads, 3) void few_experts_kernel(FewArgs a) 
             return;
         }
         list_terms(a, t, terms, nrows, lane);
-        const int m = nitems > 0 ? wait_done(a, used, lane) : -1;
+        const int m = nitems > 0 ? wait_done(a, used, lane) : WAIT_DONE;
+        if (m == WAIT_GIVEN_UP)  // h is not all there: the work-group's columns are no numbers
+            for (int i = lane; i < kYRows; i += 64) terms[i] = Term{__builtin_nanf(""), 0};
         if (lane == 0) t.help = m;
         __syncthreads();
         share = m;
@@ -1435,6 +1447,12 @@ int few_parts(int tiles, int rows, int nch, int shares, int room) {
 }
 
 }  // namespace
+
+// For tests: 1 makes a work-group help after one look (by default one that has waited a millisecond does), 2 has
+// the waits given up at once, 0 is the default.
+extern "C" void yvmoe_few_set_wait(int mode) {
+    wait_mode = mode == 1 ? GO_ONE_LOOK : mode == 2 ? GO_NO_WAIT : 0;
+}
 
 int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, const void* rweights, int rweights_bf16,
                const int64_t* rindices, const yvmoe_expert_weights* w, const float* mix, const void* skip, void* out,
@@ -1468,6 +1486,7 @@ int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, cons
     a.hparts = few_hparts(N, k, E, S, H, F, w->format);
     a.hcount = (int*)(ws + L.hcount);
     a.hsum = (float*)(ws + L.hsum);
+    a.wait_mode = wait_mode;
     int front = (a.self ? a.ncols / 16 * a.nsplit : 0) + S * (F / 16);
     if (w->format == YVMOE_W_INT4) front = std::max(front, ceil_div(N * (H / 8), kAllThreads));
     // two work-groups per CU, fewer where neither half has work for them
