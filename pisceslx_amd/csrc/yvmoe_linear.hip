@@ -349,8 +349,9 @@ __global__ __launch_bounds__(512, 4) void int4_few_kernel(LinArgs a) {
 // them, D - 1 steps ahead, once for the TB MFMAs of every term. The sums of the WK wavefronts meet in LDS.
 //
 // FOLD: with 64 x 64 products per wavefront the MFMAs of -8 / 512 Σ x would be a fifth of all. There the
-// wavefronts that share rows share them, and every 32 groups Σ_groups s (-8 Σ x) is one more product, with
-// the scales (bf16 already) as one operand and the sums in three bf16 terms (24 bits) as the other. That takes
+// wavefronts that share rows share them, and every 32 groups Σ_groups 512 s (-8 / 512 Σ x) is one more product, with
+// the scales (bf16 after the factor too) as one operand and the sums in three bf16 terms (24 bits) as the other
+// (the factor on the scales, as elsewhere, so that large rows overflow here no sooner than there). That takes
 // the additions out of the group's end as well: 8192 x 8192 at 4096 rows 672 -> 593 us (927 TFLOP/s), and
 // slower where a wavefront has 64 x 16 (100 x 4096 x 28672: 59 -> 68 us).
 template <bool F32, int TB, int RB, int WO, int WT, int D, int ROWS>
@@ -432,17 +433,16 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
     for (int b = 0; b < RB; ++b)
 #pragma unroll
         for (int t = 0; t < TB; ++t) acc[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // acc += s (-8 Σ x) over n groups
+    // acc += 512 s (-8 / 512 Σ x) over n groups
     auto fold = [&](int g0, int n) {
         bf16x8 sc[RB];
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            unsigned short e[8];
+            float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = scales[b][(long long)min(g0 + 8 * g + i, a.groups - 1) * 16];
+            for (int i = 0; i < 8; ++i) e[i] = scale512(scales[b][(long long)min(g0 + 8 * g + i, a.groups - 1) * 16]);
             Frag8 f;
-            f.u = make_uint4(e[0] | (unsigned)e[1] << 16, e[2] | (unsigned)e[3] << 16, e[4] | (unsigned)e[5] << 16,
-                             e[6] | (unsigned)e[7] << 16);
+            f.u = make_uint4(pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7]));
             sc[b] = f.v;
         }
 #pragma unroll
@@ -499,7 +499,7 @@ __global__ __launch_bounds__(512, 2) void int4_rows_kernel(LinArgs a) {
             if (r == 0)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    sums[((wt * TB + wr) * 16 + 4 * g + i) * SUMLD + step % SUMS] = 512.0f * sum[i];
+                    sums[((wt * TB + wr) * 16 + 4 * g + i) * SUMLD + step % SUMS] = sum[i];
         } else {
             bf16x8 c[RB][4];
 #pragma unroll
