@@ -151,6 +151,7 @@ typedef struct {
 /*
  * Routing results (device buffers, caller-allocated).
  *   weights [N][k] fp32, indices [N][k] int64 : the gate's (weights, top_idx)
+ *       (a token whose probabilities are all NaN: experts 0 .. k-1, weights NaN)
  *   counts [E], offsets [E+1] int32 : bincount and exclusive prefix sum
  *   perm [N*k] int32 : flat slot t*k+j at each expert-sorted position (stable argsort)
  *   pos [N*k] int32  : inverse of perm

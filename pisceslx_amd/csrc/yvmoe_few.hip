@@ -880,11 +880,11 @@ __device__ __forceinline__ void topk_wave(const float* lg, const float* bias, in
             const unsigned long long who = __ballot(key[i] == b);
             if (who != 0) id = 64 * i + __ffsll(who) - 1;
         }
-        if (b == 0) id = 0x7fffffff;
+        if (b == 0) id = j;  // all probabilities are NaN
 #pragma unroll
         for (int i = 0; i < NV; ++i) key[i] = lane + 64 * i == id ? 0u : key[i];
         if (lane == j) {
-            my_ts = b != 0 ? __uint_as_float(b - 1u) : -1.0f;
+            my_ts = b != 0 ? __uint_as_float(b - 1u) : __builtin_nanf("");
             my_id = id;
         }
     }
@@ -954,7 +954,7 @@ __device__ __forceinline__ void few_routing(const FewArgs& a, FewTables& t, FewL
                 else if (E <= 128) topk_wave<2>(lg.z[job], bias, lane, E, k, id, p, w);
                 else topk_wave<4>(lg.z[job], bias, lane, E, k, id, p, w);
                 if (lane < k) {
-                    t.expert[job * k + lane] = id < E ? (short)id : (short)-1;
+                    t.expert[job * k + lane] = (short)id;
                     t.p[job * k + lane] = p;
                     t.w[job * k + lane] = w;
                     if (writer) a.out_routing.indices[job * k + lane] = id;
@@ -1111,8 +1111,7 @@ __device__ __forceinline__ void list_terms(const FewArgs& a, const FewTables& t,
             row = ns + e * a.N + tok;
             w = a.mix[e];
         }
-        // logits that are not numbers choose nothing: the token's output is none either
-        list[i] = row >= 0 ? Term{w, q * nrows + row} : a.self ? Term{__builtin_nanf(""), 0} : Term{0.0f, -1};
+        list[i] = row >= 0 ? Term{w, q * nrows + row} : Term{0.0f, -1};
     }
 }
 

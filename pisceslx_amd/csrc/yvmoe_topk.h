@@ -131,9 +131,10 @@ __device__ __forceinline__ void topk_token(LogitFn logit, const float* __restric
     } while (0)
         YV_BFLY16(YV_KEYSTEP);
 #undef YV_KEYSTEP
-        // no candidate left (only with NaN probabilities): probability -1, index INT_MAX
-        const float bv = b != 0ull ? __uint_as_float((unsigned)(b >> 32)) : -1.0f;
-        const int be = b != 0ull ? (int)~(unsigned)b : 0x7fffffff;
+        // No candidate: every probability is NaN (the exponentials' sum was 0), and the j-th choice is expert j,
+        // of a probability that is no number. Callers index by it, so it is one of the experts.
+        const float bv = b != 0ull ? __uint_as_float((unsigned)(b >> 32)) : __builtin_nanf("");
+        const int be = b != 0ull ? (int)~(unsigned)b : j;
 #pragma unroll
         for (int i = 0; i < NV; ++i) key[i] = key[i] == b ? 0ull : key[i];  // the owner takes it
         if (j == 0) ts0 = bv;
