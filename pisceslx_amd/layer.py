@@ -210,7 +210,12 @@ class YvDynamicMoELayer(nn.Module):
         if has_shared:
             buf = self._apply_skip_residual_buffer((B, Sq, H))
             skip = None if buf is None else buf.reshape(-1, H)
-        ws = self._workspace if self._workspace is not None and self._workspace.device == x.device else None
+        # A captured call takes a workspace out of the graph's memory: the layer's own may be replaced by a
+        # longer call's and freed while the graph still writes to it.
+        capturing = x.is_cuda and torch.cuda.is_current_stream_capturing()
+        ws = self._workspace
+        if capturing or (ws is not None and ws.device != x.device):
+            ws = None
         if 0 < x2d.shape[0] <= self.few_tokens:
             out, shared_out, routing, loss, ws = self._forward_few(x, x2d, act, skip, modal_id, ws)
         elif self._router_kind == "moegate":
@@ -231,7 +236,8 @@ class YvDynamicMoELayer(nn.Module):
             out, shared_out, routing = yvf.moe_forward(x2d, st, self.experts_packed, self._mix(), skip,
                                                        workspace=ws)
             loss = torch.tensor(0.0, device=x.device, dtype=x.dtype)
-        self._workspace = ws
+        if not capturing:
+            self._workspace = ws
         if has_shared:
             self._skip_buffer = shared_out.view(B, Sq, H)
         self.last_routing = routing
