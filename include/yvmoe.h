@@ -276,12 +276,13 @@ int32_t yvmoe_forward_static(const void* x, int32_t act_dtype, int32_t n_tokens,
 
 /*
  * The layer for a few tokens (0 <= N <= YVMOE_FEW_TOKENS) in two kernels, for decoding one or a few
- * sequences. Routing, formats, shapes, results and limits are yvmoe_forward's (ffn below 2^22), with fewer
- * roundings: quantized weights enter the products exactly (yvmoe_forward rounds bf16(q * s)), gate and up
- * stay fp32, h keeps 16 bits (two bf16 terms), expert outputs and their weighted sum stay fp32, and out and
- * shared_out are each rounded once. Router logits are fp32 sums in an order of their own (a tie within the
- * last bits may fall the other way). Equal calls give equal bits, and a token's outputs do not depend on the
- * experts that the others choose: how sums are cut goes by sizes alone.
+ * sequences. Routing, formats, shapes, results and limits are yvmoe_forward's, and N (k + S) ffn and
+ * N hidden below 2^28, with fewer roundings: quantized weights enter the products exactly
+ * (yvmoe_forward rounds bf16(q * s)), gate and up stay fp32, h keeps 16 bits (two bf16 terms), expert
+ * outputs and their weighted sum stay fp32, and out and shared_out are each rounded once. Router logits
+ * are fp32 sums in an order of their own (a tie within the last bits may fall the other way). Equal
+ * calls give equal bits, and a token's outputs do not depend on the experts that the others choose:
+ * how sums are cut goes by sizes alone. int4: an infinity in a token's x or h makes what comes of it NaN.
  *
  * yvmoe_forward_few: the whole layer with YvStableMoEGate's routing.
  * yvmoe_experts_few: the routed and shared experts, the weighted sum and the skip residual for a
@@ -425,7 +426,7 @@ int32_t yvmoe_rmsnorm(const void* x, int32_t act_dtype, int32_t n_tokens, int32_
  * that suits their elements; in_features and out_features from 1 to 2^24, n_rows from 0 to 2^30,
  * n_rows x out_features up to about 2^36. out may overlap neither x nor the weight, and bias only if
  * it is bias itself, of one row. A row of x with an infinity (fp32: or a number beyond 3.39e38) or NaN
- * gives NaN in all its outputs.
+ * gives NaN in all its outputs; fp32 numbers below 2^-112 lose their last bits (2^-118: 1e-5 of the outputs).
  *   codes [ceil(out/16)][ceil(in/128)] blocks of 1 KB, each 16 rows x 128 columns: byte
  *         16 (16 g + r) starts row r's columns 32 g .. 32 g + 31 (g = 0..3), eight of them in each
  *         of four dwords, columns 0 .. 3 of the eight in its bytes' lower nibbles, 4 .. 7 in the upper;

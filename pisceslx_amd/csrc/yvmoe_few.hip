@@ -24,8 +24,9 @@
 // run and wait for nothing; those of the first kind are computed by a work-group that has waited long
 // for their mark (the same bits, so doing them twice is harmless). So the wait ends whichever part of
 // the grid is resident, also beside other kernels that wait. What work-groups hand to each other is
-// written through and read past the caches (sc1): an acquire would invalidate every L2, 30 us for
-// the 4,096 wavefronts of a launch.
+// written through and read past the caches (sc1): an acquire in every wavefront would invalidate the L2s each
+// time, which cost 30 us in a form of 4,096 wavefronts. A wait that nothing ends is given up after seconds, and
+// the columns of that work-group are NaN.
 //
 // Rounding: weights enter exactly (codes as bf16, scales on the fp32 sums), h as two bf16 terms (16 bits) for
 // the second product's MFMAs; the outputs are rounded once at the end.
@@ -1488,7 +1489,7 @@ int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, cons
     a.wait_mode = wait_mode;
     int front = (a.self ? a.ncols / 16 * a.nsplit : 0) + S * (F / 16);
     if (w->format == YVMOE_W_INT4) front = std::max(front, ceil_div(N * (H / 8), kAllThreads));
-    // two work-groups per CU, fewer where neither half has work for them
+    // one work-group per CU (LDS has no room for a second), fewer where neither half has work for them
     const int items = std::max(std::min(N * k, E) * (F / 16), H / 16 * a.hparts);
     const int grid = N == 0 ? 1 : std::min(kGrid, items);
     const int esz = act == YVMOE_ACT_BF16 ? 2 : 4;
