@@ -40,6 +40,8 @@
  *                           model/moe/layer.py:867-963 (inference)
  *   yvmoe_int4_linear    -> _YvQuantizedLinear.forward model/utils/quantization.py:486-496 with
  *                           the codes of quantize_to_int4_blockwise opss/quantize/engine.py:889-941
+ *   yvmoe_swiglu_forward, yvmoe_swiglu_backward
+ *                        -> YvSwiGLUExpert.forward model/moe/expert.py:475-489 and its gradients
  *   yvmoe_rmsnorm        -> YvRMSNorm.forward model/core/norms.py:206-208 via
  *                           fused_rms_norm opss/kernels/fused_rms_norm.py:42; two in a
  *                           row = YvHybridBlock's norm_fusion then norm_mlp
@@ -443,6 +445,39 @@ typedef struct {
 
 int32_t yvmoe_int4_linear(const void* x, int32_t act_dtype, int32_t n_rows,
                           const yvmoe_int4_matrix* weight, const void* bias, void* out, void* stream);
+
+/*
+ * Gated feed-forward block on full-precision weights (one expert of the layer, dense), row-major:
+ *   g = x w_gateᵀ, u = x w_upᵀ, h = silu(g) u, out = h w_downᵀ
+ * x and out [N][hidden], w_gate and w_up [ffn][hidden], w_down [hidden][ffn], all in the activation dtype and
+ * 16-byte aligned. bf16: h is rounded once, as an operand, and the output once; sums and everything between
+ * are fp32. fp32: operands as three bf16 terms (24 bits); an infinity or a number beyond bf16's largest
+ * (3.39e38) among them gives NaN, numbers below 2^-110 lose their last bits.
+ * saved: yvmoe_swiglu_saved_bytes() for the backward pass (g and u in fp32), or NULL; 16-byte aligned.
+ *
+ * Its gradients, from dy [N][hidden] and the forward call's x, weights and saved:
+ *   dh = dy w_down, s = 1 / (1 + exp(-g)), du = dh g s, dg = dh u s (1 + g (1 - s)),
+ *   dx = dg w_gate + du w_up, dw_gate = dgᵀ x, dw_up = duᵀ x, dw_down = dyᵀ h
+ * in the activation dtype, each rounded once (bf16: dg, du and h once, as operands). A gradient whose pointer
+ * is NULL is not computed. Outputs may overlap neither each other nor an input. All sums are in a fixed order:
+ * the same call gives the same bits. n_rows from 0 (gradients of the weights are then zero) to 2^24, hidden and
+ * ffn from 1 to 2^20, any two of n_rows, hidden and 2 ffn with a product of at most 2^39.
+ */
+typedef struct {
+    int32_t hidden;
+    int32_t ffn;
+    const void* w_gate;
+    const void* w_up;
+    const void* w_down;
+} yvmoe_swiglu_weights;
+
+size_t yvmoe_swiglu_saved_bytes(int32_t n_rows, int32_t ffn);
+size_t yvmoe_swiglu_workspace_bytes(int32_t n_rows, int32_t act_dtype, int32_t hidden, int32_t ffn, int32_t backward);
+int32_t yvmoe_swiglu_forward(const void* x, int32_t act_dtype, int32_t n_rows, const yvmoe_swiglu_weights* weights,
+                             float* saved, void* out, void* workspace, size_t workspace_bytes, void* stream);
+int32_t yvmoe_swiglu_backward(const void* dy, const void* x, const float* saved, int32_t act_dtype, int32_t n_rows,
+                              const yvmoe_swiglu_weights* weights, void* dx, void* dw_gate, void* dw_up,
+                              void* dw_down, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The whole layer with YvMoEGate as its router, as YvDynamicMoELayer builds it

@@ -62,6 +62,10 @@ EXPORTED_SYMBOLS = (
     "yvmoe_forward_few",
     "yvmoe_experts_few",
     "yvmoe_int4_linear",
+    "yvmoe_swiglu_saved_bytes",
+    "yvmoe_swiglu_workspace_bytes",
+    "yvmoe_swiglu_forward",
+    "yvmoe_swiglu_backward",
 )
 
 # YvMoEGate auxiliary heads (YVMOE_HEAD_*)
@@ -133,6 +137,17 @@ class Int4Matrix(ctypes.Structure):
         ("out_features", ctypes.c_int32),
         ("codes", ctypes.c_void_p),
         ("scales", ctypes.c_void_p),
+    ]
+
+
+class SwiGLUWeights(ctypes.Structure):
+    """yvmoe_swiglu_weights (include/yvmoe.h)."""
+    _fields_ = [
+        ("hidden", ctypes.c_int32),
+        ("ffn", ctypes.c_int32),
+        ("w_gate", ctypes.c_void_p),
+        ("w_up", ctypes.c_void_p),
+        ("w_down", ctypes.c_void_p),
     ]
 
 
@@ -220,6 +235,15 @@ def _declare(l: ctypes.CDLL) -> None:
                                        ctypes.POINTER(Routing), vp]
     l.yvmoe_int4_linear.restype = i32
     l.yvmoe_int4_linear.argtypes = [vp, i32, i32, ctypes.POINTER(Int4Matrix), vp, vp, vp]
+    l.yvmoe_swiglu_saved_bytes.restype = sz
+    l.yvmoe_swiglu_saved_bytes.argtypes = [i32, i32]
+    l.yvmoe_swiglu_workspace_bytes.restype = sz
+    l.yvmoe_swiglu_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
+    l.yvmoe_swiglu_forward.restype = i32
+    l.yvmoe_swiglu_forward.argtypes = [vp, i32, i32, ctypes.POINTER(SwiGLUWeights), vp, vp, vp, sz, vp]
+    l.yvmoe_swiglu_backward.restype = i32
+    l.yvmoe_swiglu_backward.argtypes = [vp, vp, vp, i32, i32, ctypes.POINTER(SwiGLUWeights), vp, vp, vp, vp, vp,
+                                        sz, vp]
     l.yvmoe_few_workspace_bytes.restype = sz
     l.yvmoe_few_workspace_bytes.argtypes = [i32, i32, i32, ctypes.POINTER(ExpertWeights)]
     l.yvmoe_forward_few.restype = i32

@@ -765,4 +765,99 @@ int32_t yvmoe_int4_linear(const void* x, int32_t act_dtype, int32_t n_rows,
     return int4_linear_launch(x, act_dtype, n_rows, weight, bias, out, (hipStream_t)stream);
 }
 
+// Sizes of a gated block that its kernels and grids hold.
+static int check_swiglu_sizes(int act, int n, int hidden, int ffn) {
+    YV_REQUIRE(act == YVMOE_ACT_F32 || act == YVMOE_ACT_BF16, YVMOE_ERR_DTYPE, "unknown activation dtype %d", act);
+    YV_REQUIRE(n >= 0 && n <= (1 << 24), YVMOE_ERR_ARG, "n_rows=%d outside [0, 2^24]", n);
+    YV_REQUIRE(hidden >= 1 && hidden <= (1 << 20) && ffn >= 1 && ffn <= (1 << 20), YVMOE_ERR_SHAPE,
+               "hidden=%d, ffn=%d outside [1, 2^20]", hidden, ffn);
+    const long long most = 1ll << 39, a = n, b = hidden, c = 2ll * ffn;
+    YV_REQUIRE(a * b <= most && a * c <= most && b * c <= most, YVMOE_ERR_SHAPE,
+               "n_rows=%d, hidden=%d, ffn=%d is too much for one call", n, hidden, ffn);
+    return YVMOE_OK;
+}
+
+size_t yvmoe_swiglu_saved_bytes(int32_t n_rows, int32_t ffn) {
+    return n_rows > 0 && ffn > 0 ? swiglu_saved_bytes(n_rows, ffn) : 0;
+}
+
+size_t yvmoe_swiglu_workspace_bytes(int32_t n_rows, int32_t act_dtype, int32_t hidden, int32_t ffn, int32_t backward) {
+    clear_error();
+    if (check_swiglu_sizes(act_dtype, n_rows, hidden, ffn)) return 0;
+    const yvmoe_swiglu_weights w{hidden, ffn, nullptr, nullptr, nullptr};
+    size_t bytes = 0;
+    if (backward)
+        swiglu_backward_launch(nullptr, nullptr, nullptr, act_dtype, n_rows, &w, nullptr, nullptr, nullptr, nullptr,
+                               nullptr, &bytes, nullptr);
+    else
+        swiglu_forward_launch(nullptr, act_dtype, n_rows, &w, nullptr, nullptr, nullptr, &bytes, nullptr);
+    return bytes;
+}
+
+// Ranges of a gated block's inputs.
+struct SwiGLURanges {
+    size_t row, mat;  // bytes of [N][hidden] and of a weight
+    Range in[6];      // x, dy or NULL, gate, up, down, saved or NULL
+};
+static SwiGLURanges swiglu_ranges(const void* x, const void* dy, const void* saved, int act, int n,
+                                  const yvmoe_swiglu_weights* w) {
+    const size_t e = act == YVMOE_ACT_F32 ? 4 : 2;
+    const size_t row = e * n * w->hidden, mat = e * w->hidden * w->ffn;
+    return {row, mat, {{x, row}, {dy, dy ? row : 0}, {w->w_gate, mat}, {w->w_up, mat}, {w->w_down, mat},
+                       {saved, saved ? swiglu_saved_bytes(n, w->ffn) : 0}}};
+}
+
+int32_t yvmoe_swiglu_forward(const void* x, int32_t act_dtype, int32_t n_rows, const yvmoe_swiglu_weights* weights,
+                             float* saved, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    YV_REQUIRE(weights != nullptr, YVMOE_ERR_ARG, "weights is NULL");
+    if (const int rc = check_swiglu_sizes(act_dtype, n_rows, weights->hidden, weights->ffn)) return rc;
+    if (n_rows == 0) return YVMOE_OK;
+    YV_REQUIRE(weights->w_gate && weights->w_up && weights->w_down && x && out && workspace, YVMOE_ERR_ARG,
+               "NULL pointer");
+    YV_REQUIRE(((uintptr_t)weights->w_gate | (uintptr_t)weights->w_up | (uintptr_t)weights->w_down | (uintptr_t)x |
+                (uintptr_t)out | (uintptr_t)saved | (uintptr_t)workspace) % 16 == 0,
+               YVMOE_ERR_ARG, "tensors and the workspace must be 16-byte aligned");
+    const size_t need = yvmoe_swiglu_workspace_bytes(n_rows, act_dtype, weights->hidden, weights->ffn, 0);
+    YV_REQUIRE(workspace_bytes >= need, YVMOE_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes,
+               need);
+    const SwiGLURanges r = swiglu_ranges(x, nullptr, nullptr, act_dtype, n_rows, weights);
+    const Range o{out, r.row}, s{saved, saved ? swiglu_saved_bytes(n_rows, weights->ffn) : 0}, ws{workspace, need};
+    for (const Range& i : r.in)
+        YV_REQUIRE(!o.overlaps(i) && !s.overlaps(i) && !ws.overlaps(i), YVMOE_ERR_ARG,
+                   "out, saved or the workspace overlaps an input");
+    YV_REQUIRE(!o.overlaps(s) && !o.overlaps(ws) && !s.overlaps(ws), YVMOE_ERR_ARG,
+               "out, saved and the workspace overlap");
+    return swiglu_forward_launch(x, act_dtype, n_rows, weights, saved, out, (char*)workspace, nullptr,
+                                 (hipStream_t)stream);
+}
+
+int32_t yvmoe_swiglu_backward(const void* dy, const void* x, const float* saved, int32_t act_dtype, int32_t n_rows,
+                              const yvmoe_swiglu_weights* weights, void* dx, void* dw_gate, void* dw_up,
+                              void* dw_down, void* workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    YV_REQUIRE(weights != nullptr, YVMOE_ERR_ARG, "weights is NULL");
+    if (const int rc = check_swiglu_sizes(act_dtype, n_rows, weights->hidden, weights->ffn)) return rc;
+    YV_REQUIRE(weights->w_gate && weights->w_up && weights->w_down, YVMOE_ERR_ARG, "NULL pointer");
+    YV_REQUIRE(n_rows == 0 || (dy && x && saved), YVMOE_ERR_ARG, "NULL pointer");
+    YV_REQUIRE(((uintptr_t)weights->w_gate | (uintptr_t)weights->w_up | (uintptr_t)weights->w_down | (uintptr_t)dy |
+                (uintptr_t)x | (uintptr_t)saved | (uintptr_t)dx | (uintptr_t)dw_gate | (uintptr_t)dw_up |
+                (uintptr_t)dw_down | (uintptr_t)workspace) % 16 == 0,
+               YVMOE_ERR_ARG, "tensors and the workspace must be 16-byte aligned");
+    const size_t need = yvmoe_swiglu_workspace_bytes(n_rows, act_dtype, weights->hidden, weights->ffn, 1);
+    YV_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), YVMOE_ERR_WORKSPACE,
+               "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
+    const SwiGLURanges r = swiglu_ranges(x, dy, saved, act_dtype, n_rows, weights);
+    const Range out[5] = {{dx, dx ? r.row : 0}, {dw_gate, dw_gate ? r.mat : 0}, {dw_up, dw_up ? r.mat : 0},
+                          {dw_down, dw_down ? r.mat : 0}, {workspace, need}};
+    for (int i = 0; i < 5; ++i) {
+        for (const Range& in : r.in)
+            YV_REQUIRE(!out[i].overlaps(in), YVMOE_ERR_ARG, "a gradient or the workspace overlaps an input");
+        for (int j = 0; j < i; ++j)
+            YV_REQUIRE(!out[i].overlaps(out[j]), YVMOE_ERR_ARG, "gradients or the workspace overlap");
+    }
+    return swiglu_backward_launch(dy, x, saved, act_dtype, n_rows, weights, dx, dw_gate, dw_up, dw_down,
+                                  (char*)workspace, nullptr, (hipStream_t)stream);
+}
+
 }  // extern "C"

@@ -488,5 +488,13 @@ int few_launch(const void* x, int act, int N, int k, const yvmoe_router* r, cons
 // Linear layer with 4-bit weights (yvmoe_linear.hip).
 int int4_linear_launch(const void* x, int act, int N, const yvmoe_int4_matrix* w, const void* bias, void* out,
                        hipStream_t st);
+// Gated feed-forward block on full-precision weights (yvmoe_swiglu.hip). With bytes nothing is launched:
+// *bytes is the size of the workspace.
+size_t swiglu_saved_bytes(int N, int F);
+int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weights* w, float* saved, void* out,
+                          char* ws, size_t* bytes, hipStream_t st);
+int swiglu_backward_launch(const void* dy, const void* x, const float* saved, int act, int N,
+                           const yvmoe_swiglu_weights* w, void* dx, void* dwg, void* dwu, void* dwd, char* ws,
+                           size_t* bytes, hipStream_t st);
 
 }  // namespace yvmoe

@@ -1,0 +1,583 @@
+// Gated feed-forward block on full-precision weights, forward and backward, for gfx950:
+//
+//   g = x Wgᵀ, u = x Wuᵀ, h = silu(g) u, y = h Wdᵀ
+//   dh = dy Wd, s = 1 / (1 + exp(-g)), du = dh g s, dg = dh u s (1 + g (1 - s))
+//   dx = dg Wg + du Wu, dWg = dgᵀ x, dWu = duᵀ x, dWd = dyᵀ h
+//
+// (the expert of model/moe/expert.py:475-489 and its gradients).
+//
+// Products. Every product runs on v_mfma_f32_16x16x32_bf16 with fp32 sums. bf16 operands go in as they are.
+// An fp32 operand is the sum of three bf16 terms (24 bits), and a product the six of the nine term products
+// that reach fp32's last bits, the smallest first, so that the running sum is small while they are added.
+// Roundings of the bf16 form: h, dg and du once each, where they become operands, and the outputs; g and u are
+// kept for the backward pass in fp32 (in bf16 the gradients of the gate and up weights would be twice as far
+// from the exact ones: 3.7e-3 relative instead of 2.4e-3). The fp32 form rounds h, dg and du to their 24 bits.
+#include <algorithm>
+
+#include "yvmoe_frag.h"
+#include "yvmoe_internal.h"
+
+namespace yvmoe {
+namespace {
+
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_t;
+
+constexpr int kSeg = 12;      // operand pairs of a launch: 6 term products x 2 matrices
+constexpr int kChunk = 64;    // contraction elements per LDS stage
+
+enum Epi { kOut, kSwiGLU, kGrad };
+
+// Rows by contraction ("KC": the contraction index is contiguous) or contraction by rows ("MC").
+struct TileArgs {
+    int M, N;            // output rows and columns (kSwiGLU: columns of h)
+    int ka, kb;          // contraction elements of A and of B; beyond them both count as zero
+    int lda, ldb;        // elements between rows in memory
+    int nseg;
+    int ncb, total;      // column blocks, tiles
+    const char* a[kSeg];
+    const char* b[kSeg];
+    const char* b1[6];   // kSwiGLU: the up matrix
+    // kOut: rows [0, split) to out, rows [split_at, ...) to out1 at row - split_at (split_at >= split)
+    void* out;
+    void* out1;
+    int ldo, split, split_at, f32;
+    // kSwiGLU, kGrad: planes of bf16 terms (1, fp32: 3), elements between planes
+    int planes;
+    long long plane_h, plane_d;
+    unsigned short* h;   // [planes][M][ldh]
+    unsigned short* d;   // [planes][M][2 ldh]: dg, then du
+    float* gu;           // [2][M][ldh], kSwiGLU may have none
+    int ldh;
+};
+
+// s_waitcnt immediates (gfx9 encoding)
+constexpr int vm_only(int n) { return (n & 0xf) | ((n >> 4) << 14) | (0x7 << 4) | (0xf << 8); }
+constexpr int lgkm0() { return 0xf | (0x3 << 14) | (0x7 << 4); }
+
+// 16 bytes per lane from base + off to LDS at m0 + 16 lane; an offset of kNone reads zeros: the buffer's
+// bounds are 2^31 bytes, which no other offset reaches (the host checks), and no lane reads behind a tensor.
+constexpr unsigned kNone = 0xfffffff0u;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void load_lds(const char* base, unsigned off, unsigned m0) {
+    const unsigned long long p = (unsigned long long)base;
+    const i32x4 rsrc = {(int)(unsigned)p, (int)(unsigned)(p >> 32) & 0xffff, (int)0x80000000u, 0x00020000};
+    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ void mfma_acc(f32x4& acc, const bf16x8& a, const bf16x8& b) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+
+__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+
+// v as the sum of three bf16 numbers (one: v rounded), written to planes of p
+__device__ __forceinline__ void put_terms(unsigned short* p, long long plane, int planes, const float (&v)[4]) {
+    float r[4] = {v[0], v[1], v[2], v[3]};
+    for (int t = 0; t < planes; ++t) {
+        const unsigned lo = pack_bf16(r[0], r[1]), hi = pack_bf16(r[2], r[3]);
+        *(uint2*)(p + t * plane) = make_uint2(lo, hi);
+        r[0] -= bf16_to_f32((unsigned short)(lo & 0xffff)), r[1] -= bf16_to_f32((unsigned short)(lo >> 16));
+        r[2] -= bf16_to_f32((unsigned short)(hi & 0xffff)), r[3] -= bf16_to_f32((unsigned short)(hi >> 16));
+    }
+}
+
+// One operand's part of a stage: TW rows (or columns) of 64 contraction elements.
+// KC: [TW][64], 128-byte rows in 16-byte pieces, piece c of row r at c ^ (r & 7) ^ (r >> 3 & 1).
+// MC: [64][TW], rows of TW elements in 32-byte pairs, pair p of row k at p ^ f(k), f(k) = (k & 3) | (k >> 1 & 4)
+//     (64 wide: k & 3): the four rows that 16 lanes read together then lie in different banks.
+template <bool MC, int TW>
+struct Stage {
+    static constexpr int BYTES = TW * kChunk * 2;
+    static constexpr int LOADS = BYTES / 1024 / 4;  // of a wavefront
+    static constexpr int FM = TW >= 128 ? 7 : 3;
+    unsigned off[LOADS];
+    const char* base;
+    long long step;  // bytes per chunk
+
+    // row0: first row of the tile in the operand, rows: how many the operand has
+    __device__ __forceinline__ void init(int wave, int lane, int row0, int rows, int ld) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int blk = wave * LOADS + j;
+            if (MC) {
+                constexpr int RPL = 512 / TW;  // contraction rows of a load
+                constexpr int PPR = TW / 8;    // 16-byte pieces of a row
+                const int k = blk * RPL + lane / PPR, piece = lane % PPR;
+                const int f = ((k & 3) | (k >> 1 & 4)) & FM;
+                const int m = row0 + ((((piece >> 1) ^ f) << 1 | (piece & 1)) << 3);
+                off[j] = m < rows ? (unsigned)(((long long)k * ld + m) * 2) : kNone;
+            } else {
+                const int r = blk * 8 + lane / 8;
+                const int c = (lane % 8) ^ (r & 7) ^ (r >> 3 & 1);
+                off[j] = row0 + r < rows ? (unsigned)((r * (long long)ld + c * 8) * 2) : kNone;
+            }
+        }
+        step = MC ? (long long)kChunk * ld * 2 : kChunk * 2;
+    }
+    // the lane's first contraction element of load j
+    __device__ __forceinline__ static int k_of(int wave, int lane, int j) {
+        const int blk = wave * LOADS + j;
+        if (MC) return blk * (512 / TW) + lane / (TW / 8);
+        const int r = blk * 8 + lane / 8;
+        return ((lane % 8) ^ (r & 7) ^ (r >> 3 & 1)) * 8;
+    }
+    // load j of the chunk that starts `left` elements before the operand's end
+    __device__ __forceinline__ void load(int wave, int lane, int j, const char* at, int left, unsigned lds) const {
+        unsigned o = off[j];
+        if (left < kChunk) o = k_of(wave, lane, j) < left ? o : kNone;
+        load_lds(at, o, lds + (wave * LOADS + j) * 1024);
+    }
+};
+
+// Fragment of the MFMA step s (32 contraction elements) for the 16 rows from r0: lane 16 g + r gets row r0 + r,
+// elements 8 g .. 8 g + 7 of the step.
+template <bool MC, int TW>
+struct Reader {
+    int at;  // lane's byte for r0 = the wavefront's first row, s = 0
+    __device__ __forceinline__ void init(int lane, int r0) {
+        const int g = lane >> 4, i = lane & 15;
+        if (MC) {
+            const int f = ((i >> 2) | (g & 1) << 2) & Stage<MC, TW>::FM;
+            at = (8 * g + (i >> 2)) * TW * 2 + ((((r0 >> 4) ^ f)) << 5) + (i & 3) * 8;
+        } else {
+            const int r = r0 + i;
+            at = r * 128 + ((g ^ (r & 7) ^ (r >> 3 & 1)) << 4);
+        }
+    }
+    // blocks of 16 rows are counted from the wavefront's first, which is a multiple of their number
+    __device__ __forceinline__ bf16x8 read(const unsigned char* stage, int s, int blk) const {
+        if (MC) {
+            const unsigned char* p = stage + (at ^ blk << 5) + s * 32 * TW * 2;
+            union { s16x4 h[2]; bf16x8 v; } f;
+            f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)p);
+            f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(p + 4 * TW * 2));
+            return f.v;
+        }
+        return *(const bf16x8*)(stage + (at ^ s << 6) + blk * 2048);
+    }
+};
+
+// One tile of 32 MB rows x 32 NB columns (kSwiGLU: 16 NB columns of h, gate and up) by four wavefronts in a
+// 2 x 2 grid, each 16 MB x 16 NB: MB x NB blocks of 16 x 16, fp32 sums in AGPRs (an MFMA in inline assembly
+// with the sum as one tied AGPR operand, so that the register allocator copies none). Chunks of 64
+// contraction elements move to LDS by direct loads through two stages; the MFMAs of a chunk run in two
+// halves with the next half's fragment reads and the loads of the chunk after next among them, one barrier
+// between the halves. The columns' operand is the MFMA's first, so that a lane holds four consecutive
+// columns of one row.
+template <int EPI, bool AMC, bool BMC, int MB, int NB>
+__global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
+    constexpr int TM = 32 * MB, TN = 32 * NB;
+    constexpr int T = MB * NB, R = MB + NB;
+    constexpr bool DUAL = EPI == kSwiGLU;
+    typedef Stage<AMC, TM> SA;
+    typedef Stage<BMC, TN> SB;
+    constexpr int DA = SA::LOADS, D = SA::LOADS + SB::LOADS;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[2][SA::BYTES + SB::BYTES];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave >> 1, wc = wave & 1;
+    // tiles, column block fastest, in 8 contiguous ranges (one per XCD)
+    const int per = (p.total + 7) / 8;
+    const int local = blockIdx.x / 8;
+    const int item = (blockIdx.x % 8) * per + local;
+    if (local >= per || item >= p.total) return;
+    const int m0 = (item / p.ncb) * TM;
+    const int n0 = (item % p.ncb) * (DUAL ? TN / 2 : TN);
+
+    SA sa;
+    SB sb;
+    sa.init(wave, lane, m0, p.M, p.lda);
+    // kSwiGLU: tile columns 0 .. TN / 2 - 1 are gate rows, the others the same up rows: wavefronts 0 and 1 load
+    // the gate's half, 2 and 3 the up's
+    sb.init(DUAL ? wave & 1 : wave, lane, n0, p.N, p.ldb);
+    if (DUAL) {
+        // a half is LOADS loads of two wavefronts: rows count from the half's start
+        static_assert(!DUAL || !BMC, "the forward pass reads weights row by row");
+    }
+    const long long a_tile = AMC ? (long long)m0 * 2 : (long long)m0 * p.lda * 2;
+    const long long b_tile = BMC ? (long long)n0 * 2 : (long long)n0 * p.ldb * 2;
+    // KC offsets count rows from the tile, MC offsets columns from the matrix: see Stage::init
+    const unsigned lds0 = (unsigned)(size_t)(lds_ptr_t)&lds[0][0];
+    const int cps = (max(p.ka, p.kb) + kChunk - 1) / kChunk;  // chunks per segment
+    const int chunks = cps * p.nseg;
+
+    // the next chunk to load: segment and place in it
+    int seg = 0, at = 0;
+    const char *pa = p.a[0] + (AMC ? 0 : a_tile), *pb = (DUAL && wave >= 2 ? p.b1[0] : p.b[0]) + (BMC ? 0 : b_tile);
+    auto load = [&](int st, int j) {
+        const unsigned base = lds0 + st * (SA::BYTES + SB::BYTES);
+        if (j < DA) {
+            sa.load(wave, lane, j, pa, p.ka - at, base);
+        } else {
+            if (DUAL) {
+                unsigned o = sb.off[j - DA];
+                if (p.kb - at < kChunk) o = SB::k_of(wave & 1, lane, j - DA) < p.kb - at ? o : kNone;
+                load_lds(pb, o, base + SA::BYTES + (wave * SB::LOADS + j - DA) * 1024);
+            } else {
+                sb.load(wave, lane, j - DA, pb, p.kb - at, base + SA::BYTES);
+            }
+        }
+    };
+    auto advance = [&]() {
+        at += kChunk;
+        pa += sa.step;
+        pb += sb.step;
+        if (at >= cps * kChunk && seg + 1 < p.nseg) {
+            ++seg;
+            at = 0;
+            pa = p.a[seg] + (AMC ? 0 : a_tile);
+            pb = (DUAL && wave >= 2 ? p.b1[seg % 6] : p.b[seg]) + (BMC ? 0 : b_tile);
+        }
+    };
+
+    Reader<AMC, TM> ra;
+    Reader<BMC, TN> rb;
+    ra.init(lane, wr * 16 * MB);
+    // kSwiGLU: the wavefront's first NB / 2 blocks are gate columns, the others the up columns of the same
+    rb.init(lane, DUAL ? wc * 8 * NB : wc * 16 * NB);
+    f32x4 acc[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bf16x8 fa[2][MB], fb[2][NB];
+    auto read = [&](int st, int s, int q) {
+        if (q < NB) {
+            const int blk = DUAL && q >= NB / 2 ? q - NB / 2 + NB : q;
+            fb[s][q] = rb.read(&lds[st][SA::BYTES], s, blk);
+        } else {
+            fa[s][q - NB] = ra.read(&lds[st][0], s, q - NB);
+        }
+    };
+    if (chunks > 0) {
+#pragma unroll
+        for (int j = 0; j < D; ++j) load(0, j);
+        if (chunks > 1) advance();
+#pragma unroll
+        for (int j = 0; j < D; ++j) load(1, j);
+        __builtin_amdgcn_s_waitcnt(vm_only(D));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int q = 0; q < R; ++q) read(0, 0, q);
+        for (int c = 0; c < chunks; ++c) {
+            const int st = c & 1;
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                mfma_acc(acc[i % MB][i / MB], fb[0][i / MB], fa[0][i % MB]);
+#pragma unroll
+                for (int q = (i * R) / T; q < ((i + 1) * R) / T; ++q) read(st, 1, q);
+            }
+            // this wavefront has read chunk c and holds its loads of chunk c + 1: the barrier frees the stage
+            // for chunk c + 2 and publishes chunk c + 1
+            __builtin_amdgcn_s_waitcnt(vm_only(0));
+            __builtin_amdgcn_s_waitcnt(lgkm0());
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            // past the last chunk the loads repeat it and the reads see an idle stage; neither is used
+            if (c + 2 < chunks) advance();
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                mfma_acc(acc[i % MB][i / MB], fb[1][i / MB], fa[1][i % MB]);
+#pragma unroll
+                for (int q = (i * R) / T; q < ((i + 1) * R) / T; ++q) read(st ^ 1, 0, q);
+#pragma unroll
+                for (int j = (i * D) / T; j < ((i + 1) * D) / T; ++j) load(st, j);
+            }
+        }
+        // the repeated loads land before the work-group ends; wait states between the last MFMAs and the
+        // reads of their sums
+        __builtin_amdgcn_s_waitcnt(vm_only(0));
+    }
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+
+    // block (i, j): row 16 i + lane % 16, columns 16 j + 4 g .. + 3
+    const int g4 = 4 * (lane >> 4);
+    if constexpr (EPI == kOut) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            const int m = m0 + wr * 16 * MB + 16 * i + (lane & 15);
+            const bool first = m < p.split, second = m >= p.split_at && m < p.M;
+            const long long row = first ? m : m - p.split_at;
+            void* o = first ? p.out : p.out1;
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const int n = n0 + wc * 16 * NB + 16 * j + g4;
+                const f32x4 v = acc[i][j];
+                if (!(first || second) || n >= p.N) continue;
+                const long long e = row * p.ldo + n;
+                if (n + 4 <= p.N && p.ldo % 4 == 0) {
+                    if (p.f32) *(f32x4*)((float*)o + e) = v;
+                    else *(uint2*)((unsigned short*)o + e) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (n + q < p.N) {
+                            if (p.f32) ((float*)o)[e + q] = v[q];
+                            else ((unsigned short*)o)[e + q] = f32_to_bf16_rne(v[q]);
+                        }
+                }
+            }
+        }
+    } else {
+        const long long gu_plane = (long long)p.M * p.ldh;
+        constexpr int NH = DUAL ? NB / 2 : NB;
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            const int m = m0 + wr * 16 * MB + 16 * i + (lane & 15);
+#pragma unroll
+            for (int j = 0; j < NH; ++j) {
+                const int n = n0 + wc * 16 * NH + 16 * j + g4;
+                // columns from N to ldh are sums of zeros and written as such: they are operands of products
+                if (m >= p.M || n >= p.ldh) continue;
+                const long long e = (long long)m * p.ldh + n;
+                float h[4];
+                if constexpr (DUAL) {
+                    const f32x4 g = acc[i][j], u = acc[i][j + NH];
+                    if (p.gu != nullptr) {
+                        *(f32x4*)(p.gu + e) = g;
+                        *(f32x4*)(p.gu + gu_plane + e) = u;
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) h[q] = silu(g[q]) * u[q];
+                } else {
+                    const f32x4 dh = acc[i][j], g = *(const f32x4*)(p.gu + e), u = *(const f32x4*)(p.gu + gu_plane + e);
+                    float dg[4], du[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float s = sigmoid(g[q]), a = g[q] * s;
+                        h[q] = a * u[q];
+                        du[q] = dh[q] * a;
+                        dg[q] = dh[q] * u[q] * (s + a * (1.0f - s));
+                    }
+                    unsigned short* d = p.d + (long long)m * 2 * p.ldh + n;
+                    put_terms(d, p.plane_d, p.planes, dg);
+                    put_terms(d + p.ldh, p.plane_d, p.planes, du);
+                }
+                put_terms(p.h + e, p.plane_h, p.planes, h);
+            }
+        }
+    }
+}
+
+// Rows of any width to planes of bf16 terms whose rows are a multiple of 8 wide, zeros behind the last column.
+template <bool F32>
+__global__ __launch_bounds__(256) void swiglu_pack_kernel(const void* src, int cols, int ld, long long pieces,
+                                                          unsigned short* dst, long long plane) {
+    const int per = ld / 8;
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < pieces; e += (long long)gridDim.x * 256) {
+        const long long row = e / per;
+        const int c = (int)(e - row * per) * 8;
+        float v[2][4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const long long at = row * cols + c + i;
+            v[i / 4][i % 4] = c + i >= cols ? 0.0f
+                              : F32         ? ((const float*)src)[at]
+                                            : bf16_to_f32(((const unsigned short*)src)[at]);
+        }
+        put_terms(dst + row * ld + c, plane, F32 ? 3 : 1, v[0]);
+        put_terms(dst + row * ld + c + 4, plane, F32 ? 3 : 1, v[1]);
+    }
+}
+
+// ------------------------------------------------------------------ host
+// Term products of an fp32 product, smallest first: (term of A, term of B).
+constexpr int kTermA[6] = {2, 0, 1, 1, 0, 0};
+constexpr int kTermB[6] = {0, 2, 1, 0, 1, 0};
+
+inline int up8(int v) { return (v + 7) / 8 * 8; }
+
+// An operand as planes of bf16: the tensor itself, or its packed copy in the workspace.
+struct Operand {
+    const char* p;
+    int ld;
+    long long plane;  // bytes
+};
+
+// Parts of a workspace; dry: sizes only, nothing is launched.
+struct Carve {
+    char* base;
+    bool dry;
+    size_t used = 0;
+    char* take(size_t bytes) {
+        char* r = dry ? nullptr : base + used;
+        used += align_up(bytes, 256);
+        return r;
+    }
+};
+
+inline bool needs_pack(int act, int cols) { return act == YVMOE_ACT_F32 || cols % 8 != 0; }
+inline size_t pack_bytes(int act, long long rows, int cols) {
+    return (size_t)rows * up8(cols) * 2 * (act == YVMOE_ACT_F32 ? 3 : 1);
+}
+
+Operand operand(const void* t, int act, long long rows, int cols, Carve& ws, hipStream_t st) {
+    if (!needs_pack(act, cols)) return {(const char*)t, cols, 0};
+    char* dst = ws.take(pack_bytes(act, rows, cols));
+    const Operand o{dst, up8(cols), (long long)rows * up8(cols) * 2};
+    if (ws.dry || rows == 0) return o;
+    const long long pieces = rows * (up8(cols) / 8);
+    const unsigned blocks = (unsigned)std::min<long long>((pieces + 255) / 256, 16384);
+    if (act == YVMOE_ACT_F32)
+        swiglu_pack_kernel<true><<<blocks, 256, 0, st>>>(t, cols, o.ld, pieces, (unsigned short*)dst, o.plane / 2);
+    else
+        swiglu_pack_kernel<false><<<blocks, 256, 0, st>>>(t, cols, o.ld, pieces, (unsigned short*)dst, o.plane / 2);
+    return o;
+}
+
+// Adds the operand pairs of A · Bᵀ (with b1: gate and up) to a launch.
+void add_product(TileArgs& p, int act, const Operand& a, const Operand& b, const Operand* b1 = nullptr) {
+    const int n = act == YVMOE_ACT_F32 ? 6 : 1;
+    for (int t = 0; t < n; ++t) {
+        const int ta = n == 1 ? 0 : kTermA[t], tb = n == 1 ? 0 : kTermB[t];
+        p.a[p.nseg] = a.p + ta * a.plane;
+        p.b[p.nseg] = b.p + tb * b.plane;
+        if (b1 != nullptr) p.b1[t] = b1->p + tb * b1->plane;
+        ++p.nseg;
+    }
+    p.lda = a.ld;
+    p.ldb = b.ld;
+}
+
+template <int EPI, bool AMC, bool BMC, int MB, int NB>
+void tile_grid(TileArgs p, hipStream_t st) {
+    const int cols = EPI == kSwiGLU ? 16 * NB : 32 * NB;
+    p.ncb = ceil_div(p.N, cols);
+    p.total = ceil_div(p.M, 32 * MB) * p.ncb;
+    swiglu_tile_kernel<EPI, AMC, BMC, MB, NB><<<(unsigned)(ceil_div(p.total, 8) * 8), 256, 0, st>>>(p);
+}
+
+template <int EPI, bool AMC, bool BMC>
+void tile_launch(const TileArgs& p, hipStream_t st) {
+    if (p.M <= 0 || p.N <= 0) return;
+    const long long cols = EPI == kSwiGLU ? 2ll * p.N : p.N;
+    auto tiles = [&](int t) { return ((p.M + t - 1) / t) * ((cols + t - 1) / t); };
+    if (tiles(256) >= 192) tile_grid<EPI, AMC, BMC, 8, 8>(p, st);
+    else if (tiles(128) >= 192) tile_grid<EPI, AMC, BMC, 4, 4>(p, st);
+    else tile_grid<EPI, AMC, BMC, 2, 2>(p, st);
+}
+
+}  // namespace
+
+size_t swiglu_saved_bytes(int N, int F) { return (size_t)2 * N * up8(F) * 4; }
+
+// With bytes nothing is launched: *bytes is the size of the workspace.
+int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weights* w, float* saved, void* out,
+                          char* ws, size_t* bytes, hipStream_t st) {
+    const int H = w->hidden, F = w->ffn, F8 = up8(F), planes = act == YVMOE_ACT_F32 ? 3 : 1;
+    Carve c{ws, bytes != nullptr};
+    const Operand ox = operand(x, act, N, H, c, st), og = operand(w->w_gate, act, F, H, c, st),
+                  ou = operand(w->w_up, act, F, H, c, st), od = operand(w->w_down, act, H, F, c, st);
+    const long long plane = (long long)N * F8;
+    unsigned short* h = (unsigned short*)c.take((size_t)plane * 2 * planes);
+    if (bytes != nullptr) *bytes = c.used;
+    if (c.dry || N == 0) return YVMOE_OK;
+    TileArgs p{};
+    p.M = N;
+    p.N = F;
+    p.ka = p.kb = ox.ld;
+    add_product(p, act, ox, og, &ou);
+    p.planes = planes;
+    p.h = h;
+    p.plane_h = plane;
+    p.gu = saved;
+    p.ldh = F8;
+    tile_launch<kSwiGLU, false, false>(p, st);
+    TileArgs q{};
+    q.M = N;
+    q.N = H;
+    q.ka = q.kb = F8;
+    add_product(q, act, Operand{(const char*)h, F8, plane * 2}, od);
+    q.out = out;
+    q.ldo = H;
+    q.split = q.split_at = N;
+    q.f32 = act == YVMOE_ACT_F32;
+    tile_launch<kOut, false, false>(q, st);
+    YV_LAUNCH_CHECK("swiglu_forward");
+    return YVMOE_OK;
+}
+
+int swiglu_backward_launch(const void* dy, const void* x, const float* saved, int act, int N,
+                           const yvmoe_swiglu_weights* w, void* dx, void* dwg, void* dwu, void* dwd, char* ws,
+                           size_t* bytes, hipStream_t st) {
+    const int H = w->hidden, F = w->ffn, F8 = up8(F), planes = act == YVMOE_ACT_F32 ? 3 : 1;
+    const int f32 = act == YVMOE_ACT_F32;
+    Carve c{ws, bytes != nullptr};
+    const long long plane = (long long)N * F8;
+    const Operand ody = operand(dy, act, N, H, c, st), od = operand(w->w_down, act, H, F, c, st);
+    unsigned short* h = (unsigned short*)c.take((size_t)plane * 2 * planes);
+    unsigned short* d = (unsigned short*)c.take((size_t)plane * 4 * planes);
+    Operand ox{}, og{}, ou{};
+    if (c.dry || dwg != nullptr || dwu != nullptr) ox = operand(x, act, N, H, c, st);
+    if (c.dry || dx != nullptr) {
+        og = operand(w->w_gate, act, F, H, c, st);
+        ou = operand(w->w_up, act, F, H, c, st);
+    }
+    if (bytes != nullptr) *bytes = c.used;
+    if (c.dry) return YVMOE_OK;
+    const Operand oh{(const char*)h, F8, plane * 2}, odg{(const char*)d, 2 * F8, plane * 4},
+        odu{(const char*)(d + F8), 2 * F8, plane * 4};
+    TileArgs p{};
+    p.M = N;
+    p.N = F;
+    p.ka = ody.ld;
+    p.kb = H;
+    add_product(p, act, ody, od);
+    p.planes = planes;
+    p.h = h;
+    p.plane_h = plane;
+    p.d = d;
+    p.plane_d = plane * 2;
+    p.gu = const_cast<float*>(saved);
+    p.ldh = F8;
+    tile_launch<kGrad, false, true>(p, st);
+    if (dx != nullptr) {
+        TileArgs q{};
+        q.M = N;
+        q.N = H;
+        q.ka = F8;
+        q.kb = F;
+        // the smallest term products of both matrices first
+        add_product(q, act, odg, og);
+        add_product(q, act, odu, ou);
+        q.out = dx;
+        q.ldo = H;
+        q.split = q.split_at = N;
+        q.f32 = f32;
+        tile_launch<kOut, false, true>(q, st);
+    }
+    if (dwg != nullptr || dwu != nullptr) {
+        const bool both = dwg != nullptr && dwu != nullptr;
+        TileArgs q{};
+        q.M = both ? F8 + F : F;
+        q.N = H;
+        q.ka = q.kb = N;
+        add_product(q, act, dwg != nullptr ? odg : odu, ox);
+        q.out = dwg != nullptr ? dwg : dwu;
+        q.out1 = dwu;
+        q.ldo = H;
+        q.split = F;
+        q.split_at = both ? F8 : F;
+        q.f32 = f32;
+        tile_launch<kOut, true, true>(q, st);
+    }
+    if (dwd != nullptr) {
+        TileArgs q{};
+        q.M = H;
+        q.N = F;
+        q.ka = q.kb = N;
+        add_product(q, act, ody, oh);
+        q.out = dwd;
+        q.ldo = F;
+        q.split = q.split_at = H;
+        q.f32 = f32;
+        tile_launch<kOut, true, true>(q, st);
+    }
+    YV_LAUNCH_CHECK("swiglu_backward");
+    return YVMOE_OK;
+}
+
+}  // namespace yvmoe

@@ -5,6 +5,7 @@ of them has a CPU or PyTorch fallback — a call on CPU tensors raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from dataclasses import dataclass
@@ -632,3 +633,100 @@ def int4_linear(x: torch.Tensor, weight: PackedLinear, bias: Optional[torch.Tens
     if rc:
         _lib.check(rc, "yvmoe_int4_linear")
     return out
+
+
+# ---------------------------------------------------------------- gated feed-forward block
+def _on(dev: torch.device):
+    """A guard for launches on ``dev`` where another device is current."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
+    """_require_cuda, on one device."""
+    dev = _require_cuda(*ts)
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {t.device} and {dev}")
+    return dev
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` at a 16-byte address (a copy where a view starts elsewhere)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _swiglu_forward(x2d, w_gate, w_up, w_down, keep: bool):
+    """(out, what the backward pass needs or None) of rows [N, H]."""
+    l, (N, H), F, dt, dev = _lib.lib(), x2d.shape, w_gate.shape[0], x2d.dtype, x2d.device
+    act = _act(dt)
+    out = torch.empty_like(x2d)
+    w = _lib.SwiGLUWeights(H, F, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr())
+    nbytes = l.yvmoe_swiglu_workspace_bytes(N, act, H, F, 0)
+    if nbytes == 0 and N > 0:
+        raise ValueError(f"swiglu: {l.yvmoe_last_error().decode(errors='replace')}")
+    saved = torch.empty(l.yvmoe_swiglu_saved_bytes(N, F) // 4, dtype=torch.float32, device=dev) if keep else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = l.yvmoe_swiglu_forward(x2d.data_ptr(), act, N, ctypes.byref(w), _ptr(saved), out.data_ptr(),
+                                    ws.data_ptr(), nbytes, _stream(dev))
+    if rc:
+        _lib.check(rc, "yvmoe_swiglu_forward")
+    return out, saved
+
+
+class _SwiGLU(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x2d, w_gate, w_up, w_down):
+        out, saved = _swiglu_forward(x2d, w_gate, w_up, w_down, True)
+        ctx.save_for_backward(x2d, w_gate, w_up, w_down, saved)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, wg, wu, wd, saved = ctx.saved_tensors
+        l, (N, H), F, dev = _lib.lib(), x.shape, wg.shape[0], x.device
+        act = _act(x.dtype)
+        dy = _aligned(dy.contiguous())
+        grads = [torch.empty_like(t) if need else None
+                 for t, need in zip((x, wg, wu, wd), ctx.needs_input_grad)]
+        w = _lib.SwiGLUWeights(H, F, wg.data_ptr(), wu.data_ptr(), wd.data_ptr())
+        nbytes = l.yvmoe_swiglu_workspace_bytes(N, act, H, F, 1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with _on(dev):
+            rc = l.yvmoe_swiglu_backward(dy.data_ptr(), x.data_ptr(), saved.data_ptr(), act, N, ctypes.byref(w),
+                                         *map(_ptr, grads), ws.data_ptr(), nbytes, _stream(dev))
+        if rc:
+            _lib.check(rc, "yvmoe_swiglu_backward")
+        return tuple(grads)
+
+
+def swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> torch.Tensor:
+    """The gated feed-forward block of one dense expert (YvSwiGLUExpert.forward,
+    model/moe/expert.py:475-489): (silu(x w_gateᵀ) · (x w_upᵀ)) w_downᵀ, with gradients of x and the weights.
+
+    x [..., H], w_gate and w_up [F, H], w_down [H, F] (nn.Linear.weight), all bf16 or all fp32, contiguous;
+    any sizes up to 2^24 rows and 2^20 features. Sums are fp32; bf16 rounds the activated product and the two
+    gradients before it once each, as operands, and the outputs. For the backward pass the call keeps x and the
+    two projections in fp32 (8 bytes a row and feature of F). The gradients are not differentiable again.
+    """
+    if w_gate.dim() != 2 or w_up.shape != w_gate.shape or tuple(w_down.shape) != tuple(w_gate.shape[::-1]):
+        raise ValueError(f"weights must be [F, H], [F, H], [H, F], got {tuple(w_gate.shape)}, "
+                         f"{tuple(w_up.shape)}, {tuple(w_down.shape)}")
+    F, H = w_gate.shape
+    if F < 1 or H < 1:
+        raise ValueError(f"a gated block needs features, got hidden {H}, ffn {F}")
+    if x.dim() == 0 or x.shape[-1] != H:
+        raise ValueError(f"x must be [..., {H}], got {tuple(x.shape)}")
+    if not (x.dtype == w_gate.dtype == w_up.dtype == w_down.dtype):
+        raise ValueError(f"x and the weights must have one dtype, got {x.dtype}, {w_gate.dtype}, {w_up.dtype}, "
+                         f"{w_down.dtype}")
+    _act(x.dtype)
+    _same_device(x, w_gate, w_up, w_down)
+    ts = [_aligned(t) for t in (x, w_gate, w_up, w_down)]
+    x2d = ts[0].reshape(-1, H)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        out = _SwiGLU.apply(x2d, *ts[1:])
+    else:
+        out, _ = _swiglu_forward(x2d, *ts[1:], False)
+    return out.view(x.shape)
