@@ -40,6 +40,10 @@
  *                           model/moe/layer.py:867-963 (inference)
  *   yvmoe_int4_linear    -> _YvQuantizedLinear.forward model/utils/quantization.py:486-496 with
  *                           the codes of quantize_to_int4_blockwise opss/quantize/engine.py:889-941
+ *   yvmoe_quantize_fp8_rows, yvmoe_fp8_linear, yvmoe_fp8_linear_rows, yvmoe_fp8_swiglu
+ *                        -> PiscesLxFP8QuantizationEngine.quantize_to_fp8 opss/quantize/engine.py:841-883
+ *                           with a scale per 128 values, and nn.Linear and YvSwiGLUExpert.forward
+ *                           model/moe/expert.py:475-489 on such weights and rows
  *   yvmoe_swiglu_forward, yvmoe_swiglu_backward
  *                        -> YvSwiGLUExpert.forward model/moe/expert.py:475-489 and its gradients
  *   yvmoe_rmsnorm        -> YvRMSNorm.forward model/core/norms.py:206-208 via
@@ -445,6 +449,56 @@ typedef struct {
 
 int32_t yvmoe_int4_linear(const void* x, int32_t act_dtype, int32_t n_rows,
                           const yvmoe_int4_matrix* weight, const void* bias, void* out, void* stream);
+
+/*
+ * Rows in 8-bit floating point with a scale per 128 values: for the values of row n and the group b of columns
+ * 128 b .. 128 b + 127 (the last group may be shorter),
+ *   scales[b][n] = max(max |x| / 448, 1e-12), codes = e4m3fn(x / scale), rounded to nearest even, both divisions
+ *   in fp32. A group with an infinity or NaN has that scale and a NaN among its codes, so that every product
+ *   with it is NaN.
+ * x [N][features] in act_dtype at any address that suits its elements; codes [N][G][128] (columns behind the last
+ * one are zero), 16-byte aligned, scales [G][N] fp32, 4-byte aligned, G = ceil(features / 128). n_rows from 0 to
+ * 2^24, features from 1 to 2^20. Neither output may overlap x.
+ */
+int32_t yvmoe_quantize_fp8_rows(const void* x, int32_t act_dtype, int32_t n_rows, int32_t features, void* codes,
+                                float* scales, void* stream);
+
+/*
+ * Linear layer on e4m3fn weights with a scale per 128 x 128 block, products in 8-bit floating point:
+ *   out[n][o] = sum_b xs[b][n] ws[o / 128][b] sum_(k in b) xq[n][k] wq[o][k] + bias[o]
+ * in fp32 sums, rounded once to bf16 (the matrix unit's sum of 128 products keeps about 16 bits).
+ *   codes  [ceil(out/16)][ceil(in/128)][2] blocks of 1 KB, each 16 rows x 64 columns: byte 16 (16 g + r) starts
+ *          row r's columns 16 g .. 16 g + 15 (the order of the experts' matrices); rows past out_features and
+ *          columns past in_features are zero; 16-byte aligned
+ *   scales [ceil(out/128)][ceil(in/128)] fp32
+ *   pisceslx_amd/quant.py pack_fp8_linear() writes this order.
+ * yvmoe_fp8_linear takes bf16 rows x [N][in] and rounds them to 8 bits first (yvmoe_quantize_fp8_rows, in the
+ * workspace of yvmoe_fp8_linear_workspace_bytes, 16-byte aligned), yvmoe_fp8_linear_rows takes rows that are.
+ * bias [out] bf16 or NULL; out [N][out] bf16, 8-byte aligned. in_features, out_features from 1 to 2^20, n_rows from 0
+ * to 2^24, n_rows x out_features up to 2^36. out and the workspace overlap no input.
+ */
+typedef struct {
+    int32_t in_features;
+    int32_t out_features;
+    const void* codes;
+    const float* scales;
+} yvmoe_fp8_matrix;
+
+size_t yvmoe_fp8_linear_workspace_bytes(int32_t n_rows, int32_t in_features);
+int32_t yvmoe_fp8_linear(const void* x, int32_t n_rows, const yvmoe_fp8_matrix* weight, const void* bias, void* out,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int32_t yvmoe_fp8_linear_rows(const void* codes, const float* scales, int32_t n_rows, const yvmoe_fp8_matrix* weight,
+                              const void* bias, void* out, void* stream);
+
+/*
+ * Gated feed-forward block on such weights: g = x gateᵀ, u = x upᵀ, h = silu(g) u, out = h downᵀ, each product as
+ * in yvmoe_fp8_linear; g, u and h are fp32, h is rounded to 8 bits as rows are. x and out [N][hidden] bf16, gate
+ * and up [ffn][hidden], down [hidden][ffn]. Limits as above.
+ */
+size_t yvmoe_fp8_swiglu_workspace_bytes(int32_t n_rows, int32_t hidden, int32_t ffn);
+int32_t yvmoe_fp8_swiglu(const void* x, int32_t n_rows, const yvmoe_fp8_matrix* gate, const yvmoe_fp8_matrix* up,
+                         const yvmoe_fp8_matrix* down, void* out, void* workspace, size_t workspace_bytes,
+                         void* stream);
 
 /*
  * Gated feed-forward block on full-precision weights (one expert of the layer, dense), row-major:

@@ -62,6 +62,12 @@ EXPORTED_SYMBOLS = (
     "yvmoe_forward_few",
     "yvmoe_experts_few",
     "yvmoe_int4_linear",
+    "yvmoe_quantize_fp8_rows",
+    "yvmoe_fp8_linear_workspace_bytes",
+    "yvmoe_fp8_linear",
+    "yvmoe_fp8_linear_rows",
+    "yvmoe_fp8_swiglu_workspace_bytes",
+    "yvmoe_fp8_swiglu",
     "yvmoe_swiglu_saved_bytes",
     "yvmoe_swiglu_workspace_bytes",
     "yvmoe_swiglu_forward",
@@ -132,6 +138,16 @@ class RMSNormParams(ctypes.Structure):
 
 class Int4Matrix(ctypes.Structure):
     """yvmoe_int4_matrix (include/yvmoe.h)."""
+    _fields_ = [
+        ("in_features", ctypes.c_int32),
+        ("out_features", ctypes.c_int32),
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+    ]
+
+
+class Fp8Matrix(ctypes.Structure):
+    """yvmoe_fp8_matrix (include/yvmoe.h)."""
     _fields_ = [
         ("in_features", ctypes.c_int32),
         ("out_features", ctypes.c_int32),
@@ -235,6 +251,19 @@ def _declare(l: ctypes.CDLL) -> None:
                                        ctypes.POINTER(Routing), vp]
     l.yvmoe_int4_linear.restype = i32
     l.yvmoe_int4_linear.argtypes = [vp, i32, i32, ctypes.POINTER(Int4Matrix), vp, vp, vp]
+    mat = ctypes.POINTER(Fp8Matrix)
+    l.yvmoe_quantize_fp8_rows.restype = i32
+    l.yvmoe_quantize_fp8_rows.argtypes = [vp, i32, i32, i32, vp, vp, vp]
+    l.yvmoe_fp8_linear_workspace_bytes.restype = sz
+    l.yvmoe_fp8_linear_workspace_bytes.argtypes = [i32, i32]
+    l.yvmoe_fp8_linear.restype = i32
+    l.yvmoe_fp8_linear.argtypes = [vp, i32, mat, vp, vp, vp, sz, vp]
+    l.yvmoe_fp8_linear_rows.restype = i32
+    l.yvmoe_fp8_linear_rows.argtypes = [vp, vp, i32, mat, vp, vp, vp]
+    l.yvmoe_fp8_swiglu_workspace_bytes.restype = sz
+    l.yvmoe_fp8_swiglu_workspace_bytes.argtypes = [i32, i32, i32]
+    l.yvmoe_fp8_swiglu.restype = i32
+    l.yvmoe_fp8_swiglu.argtypes = [vp, i32, mat, mat, mat, vp, vp, sz, vp]
     l.yvmoe_swiglu_saved_bytes.restype = sz
     l.yvmoe_swiglu_saved_bytes.argtypes = [i32, i32]
     l.yvmoe_swiglu_workspace_bytes.restype = sz

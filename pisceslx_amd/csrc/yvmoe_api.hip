@@ -765,6 +765,117 @@ int32_t yvmoe_int4_linear(const void* x, int32_t act_dtype, int32_t n_rows,
     return int4_linear_launch(x, act_dtype, n_rows, weight, bias, out, (hipStream_t)stream);
 }
 
+// A weight of 8-bit products, and n rows of it.
+static int check_fp8_matrix(const yvmoe_fp8_matrix* w, int n, const char* name) {
+    YV_REQUIRE(w != nullptr, YVMOE_ERR_ARG, "%s is NULL", name);
+    YV_REQUIRE(n >= 0 && n <= (1 << 24), YVMOE_ERR_ARG, "n_rows=%d outside [0, 2^24]", n);
+    YV_REQUIRE(w->in_features >= 1 && w->in_features <= (1 << 20) && w->out_features >= 1 &&
+                   w->out_features <= (1 << 20),
+               YVMOE_ERR_SHAPE, "%s: in_features=%d, out_features=%d outside [1, 2^20]", name, w->in_features,
+               w->out_features);
+    YV_REQUIRE((long long)n * w->out_features <= 1ll << 36, YVMOE_ERR_SHAPE,
+               "%s: n_rows=%d x out_features=%d is too much for one call", name, n, w->out_features);
+    if (n == 0) return YVMOE_OK;
+    YV_REQUIRE(w->codes && w->scales, YVMOE_ERR_ARG, "%s: NULL pointer", name);
+    YV_REQUIRE((uintptr_t)w->codes % 16 == 0 && (uintptr_t)w->scales % 4 == 0, YVMOE_ERR_ARG,
+               "%s: codes must be 16-byte and scales 4-byte aligned", name);
+    return YVMOE_OK;
+}
+static bool overlaps_fp8_matrix(const Range& o, const yvmoe_fp8_matrix* w) {
+    const size_t groups = ceil_div(w->in_features, 128);
+    return o.overlaps({w->codes, (size_t)ceil_div(w->out_features, 16) * groups * 2048}) ||
+           o.overlaps({w->scales, (size_t)ceil_div(w->out_features, 128) * groups * 4});
+}
+
+int32_t yvmoe_quantize_fp8_rows(const void* x, int32_t act_dtype, int32_t n_rows, int32_t features, void* codes,
+                                float* scales, void* stream) {
+    clear_error();
+    YV_REQUIRE(act_dtype == YVMOE_ACT_F32 || act_dtype == YVMOE_ACT_BF16, YVMOE_ERR_DTYPE,
+               "unknown activation dtype %d", act_dtype);
+    YV_REQUIRE(n_rows >= 0 && n_rows <= (1 << 24), YVMOE_ERR_ARG, "n_rows=%d outside [0, 2^24]", n_rows);
+    YV_REQUIRE(features >= 1 && features <= (1 << 20), YVMOE_ERR_SHAPE, "features=%d outside [1, 2^20]", features);
+    if (n_rows == 0) return YVMOE_OK;
+    YV_REQUIRE(x && codes && scales, YVMOE_ERR_ARG, "NULL pointer");
+    const size_t esz = act_dtype == YVMOE_ACT_F32 ? 4 : 2, groups = ceil_div(features, 128);
+    YV_REQUIRE((uintptr_t)x % esz == 0 && (uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 4 == 0, YVMOE_ERR_ARG,
+               "x and scales must be aligned to their elements, codes to 16 bytes");
+    const Range in{x, esz * n_rows * features}, c{codes, groups * 128 * n_rows}, s{scales, groups * 4 * n_rows};
+    YV_REQUIRE(!c.overlaps(in) && !s.overlaps(in) && !c.overlaps(s), YVMOE_ERR_ARG, "x, codes and scales overlap");
+    return fp8_rows_launch(x, act_dtype, n_rows, features, codes, scales, (hipStream_t)stream);
+}
+
+size_t yvmoe_fp8_linear_workspace_bytes(int32_t n_rows, int32_t in_features) {
+    return n_rows > 0 && in_features > 0 ? fp8_linear_ws(n_rows, in_features) : 0;
+}
+
+int32_t yvmoe_fp8_linear(const void* x, int32_t n_rows, const yvmoe_fp8_matrix* weight, const void* bias, void* out,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    if (const int rc = check_fp8_matrix(weight, n_rows, "weight")) return rc;
+    if (n_rows == 0) return YVMOE_OK;
+    YV_REQUIRE(x && out && workspace, YVMOE_ERR_ARG, "NULL pointer");
+    YV_REQUIRE(((uintptr_t)x | (uintptr_t)bias) % 2 == 0 && (uintptr_t)out % 8 == 0 && (uintptr_t)workspace % 16 == 0,
+               YVMOE_ERR_ARG, "x and bias must be 2-byte, out 8-byte and the workspace 16-byte aligned");
+    const size_t need = fp8_linear_ws(n_rows, weight->in_features);
+    YV_REQUIRE(workspace_bytes >= need, YVMOE_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes,
+               need);
+    const Range in{x, (size_t)n_rows * weight->in_features * 2}, b{bias, (size_t)weight->out_features * 2},
+        o{out, (size_t)n_rows * weight->out_features * 2}, ws{workspace, need};
+    for (const Range& r : {o, ws})
+        YV_REQUIRE(!r.overlaps(in) && !r.overlaps(b) && !overlaps_fp8_matrix(r, weight), YVMOE_ERR_ARG,
+                   "out or the workspace overlaps an input");
+    YV_REQUIRE(!o.overlaps(ws), YVMOE_ERR_ARG, "out overlaps the workspace");
+    return fp8_linear_launch(x, n_rows, weight, bias, out, (char*)workspace, (hipStream_t)stream);
+}
+
+int32_t yvmoe_fp8_linear_rows(const void* codes, const float* scales, int32_t n_rows, const yvmoe_fp8_matrix* weight,
+                              const void* bias, void* out, void* stream) {
+    clear_error();
+    if (const int rc = check_fp8_matrix(weight, n_rows, "weight")) return rc;
+    if (n_rows == 0) return YVMOE_OK;
+    YV_REQUIRE(codes && scales && out, YVMOE_ERR_ARG, "NULL pointer");
+    YV_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 4 == 0 && (uintptr_t)bias % 2 == 0 &&
+                   (uintptr_t)out % 8 == 0,
+               YVMOE_ERR_ARG, "codes must be 16-byte, scales 4-byte, bias 2-byte and out 8-byte aligned");
+    const size_t groups = ceil_div(weight->in_features, 128);
+    const Range o{out, (size_t)n_rows * weight->out_features * 2};
+    YV_REQUIRE(!o.overlaps({codes, groups * 128 * n_rows}) && !o.overlaps({scales, groups * 4 * n_rows}) &&
+                   !o.overlaps({bias, (size_t)weight->out_features * 2}) && !overlaps_fp8_matrix(o, weight),
+               YVMOE_ERR_ARG, "out overlaps an input");
+    return fp8_product_launch(codes, scales, n_rows, weight, bias, out, (hipStream_t)stream);
+}
+
+size_t yvmoe_fp8_swiglu_workspace_bytes(int32_t n_rows, int32_t hidden, int32_t ffn) {
+    return n_rows > 0 && hidden > 0 && ffn > 0 ? fp8_swiglu_ws(n_rows, hidden, ffn) : 0;
+}
+
+int32_t yvmoe_fp8_swiglu(const void* x, int32_t n_rows, const yvmoe_fp8_matrix* gate, const yvmoe_fp8_matrix* up,
+                         const yvmoe_fp8_matrix* down, void* out, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+    clear_error();
+    if (const int rc = check_fp8_matrix(gate, n_rows, "gate")) return rc;
+    if (const int rc = check_fp8_matrix(up, n_rows, "up")) return rc;
+    if (const int rc = check_fp8_matrix(down, n_rows, "down")) return rc;
+    const int H = gate->in_features, F = gate->out_features;
+    YV_REQUIRE(up->in_features == H && up->out_features == F && down->in_features == F && down->out_features == H,
+               YVMOE_ERR_SHAPE, "gate %d x %d, up %d x %d, down %d x %d are no gated block", F, H, up->out_features,
+               up->in_features, down->out_features, down->in_features);
+    if (n_rows == 0) return YVMOE_OK;
+    YV_REQUIRE(x && out && workspace, YVMOE_ERR_ARG, "NULL pointer");
+    YV_REQUIRE((uintptr_t)x % 2 == 0 && (uintptr_t)out % 8 == 0 && (uintptr_t)workspace % 16 == 0, YVMOE_ERR_ARG,
+               "x must be 2-byte, out 8-byte and the workspace 16-byte aligned");
+    const size_t need = fp8_swiglu_ws(n_rows, H, F);
+    YV_REQUIRE(workspace_bytes >= need, YVMOE_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes,
+               need);
+    const Range in{x, (size_t)n_rows * H * 2}, o{out, (size_t)n_rows * H * 2}, ws{workspace, need};
+    for (const yvmoe_fp8_matrix* w : {gate, up, down})
+        YV_REQUIRE(!overlaps_fp8_matrix(o, w) && !overlaps_fp8_matrix(ws, w), YVMOE_ERR_ARG,
+                   "out or the workspace overlaps a weight");
+    YV_REQUIRE(!o.overlaps(in) && !ws.overlaps(in) && !o.overlaps(ws), YVMOE_ERR_ARG,
+               "x, out and the workspace overlap");
+    return fp8_swiglu_launch(x, n_rows, gate, up, down, out, (char*)workspace, (hipStream_t)stream);
+}
+
 // Sizes of a gated block that its kernels and grids hold.
 static int check_swiglu_sizes(int act, int n, int hidden, int ffn) {
     YV_REQUIRE(act == YVMOE_ACT_F32 || act == YVMOE_ACT_BF16, YVMOE_ERR_DTYPE, "unknown activation dtype %d", act);

@@ -1,0 +1,530 @@
+// 8-bit floating point products with a scale per 128 values, for gfx950:
+//
+//   rows     s[b][n] = max(max |x[n][k in b]| / 448, 1e-12), q[n][k] = e4m3(x[n][k] / s[b][n])
+//   linear   y[n][o] = Σ_b s[b][n] w[o / 128][b] Σ_{k in b} q[n][k] c[o][k] + bias[o]
+//   block    g, u = linear(x; gate), linear(x; up), h = silu(g) u, y = linear(h; down)
+//
+// (the format of opss/quantize/engine.py:841-883 with a scale per 128 x 128 weights and per 128 values of a row).
+//
+// Products. v_mfma_f32_16x16x128_f8f6f4 on a block of 128 contraction elements from a sum of zero, then the block's
+// two scales times that sum onto the fp32 result: 4 multiply-adds a lane beside 32 cycles of the matrix unit. 16
+// weight rows are the first operand, so a lane holds four consecutive outputs of one row, and the row's scale is one
+// number a lane. The unit's sum of 128 products keeps about 16 bits: against 64 bits its results are off by 1.4e-5
+// relative (normal values; the same for v_mfma_f32_16x16x32_fp8_fp8, four of them in a row), a hundredth of a bf16
+// output's own rounding, which is why outputs are bf16 only.
+//
+// Weights lie in blocks of 16 rows x 64 columns, 1 KB, lane l = 16 g + r's 16 bytes at 16 l: row r, columns
+// 16 g .. 16 g + 15 (the order of the experts' matrices); two consecutive blocks are an operand of 128, in which
+// lane group g holds elements 16 g .. + 15 and 64 + 16 g .. + 15.
+#include <algorithm>
+
+#include "yvmoe_frag.h"
+#include "yvmoe_internal.h"
+
+namespace yvmoe {
+namespace {
+
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kBlock = 128;
+constexpr float kMax = 448.0f, kMinScale = 1e-12f;
+
+union Op8 {  // an operand of 128 elements: two pieces of 16 bytes
+    uint4 u[2];
+    i32x8 v;
+};
+__device__ __forceinline__ f32x4 mfma8(const Op8& a, const Op8& b) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+
+// The scale of values whose largest size has the bits m. NaN (its bits are above every other's) stays NaN.
+__device__ __forceinline__ float scale_of(unsigned m) {
+    const float s = __uint_as_float(m) / kMax;
+    return s < kMinScale ? kMinScale : s;
+}
+// e4m3 codes of four values over s, lowest first
+__device__ __forceinline__ unsigned codes4(float a, float b, float c, float d, float s) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a / s, b / s, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c / s, d / s, w, true);
+}
+__device__ __forceinline__ unsigned size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// ------------------------------------------------------------------ rows
+// 16 lanes a group of 128, 8 values a lane; rows ld apart. VEC: rows of whole 16-byte pieces at 16-byte addresses.
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(256) void fp8_rows_kernel(const void* x, int N, int K, int ld, int groups,
+                                                       unsigned char* codes, float* scales) {
+    const long long items = (long long)N * groups;
+    for (long long it = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); it < items; it += (long long)gridDim.x * 16) {
+        const int n = (int)(it / groups), b = (int)(it - (long long)n * groups);
+        const int k = b * kBlock + (threadIdx.x & 15) * 8;
+        const long long at = (long long)n * ld + k;
+        float v[8];
+        if (VEC) {
+            if (k < K) {
+                if (F32) {
+                    const float4 lo = *(const float4*)((const float*)x + at);
+                    float4 hi = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (k + 4 < K) hi = *(const float4*)((const float*)x + at + 4);
+                    v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+                } else {
+                    const uint4 u = *(const uint4*)((const unsigned short*)x + at);
+                    const unsigned d[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32((unsigned short)(d[i / 2] >> 16 * (i & 1)));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = k + i >= K ? 0.0f : F32 ? ((const float*)x)[at + i] : bf16_to_f32(((const unsigned short*)x)[at + i]);
+        }
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, size_bits(v[i]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 16));
+        const float s = scale_of(m);
+        *(uint2*)(codes + ((long long)n * groups + b) * kBlock + (threadIdx.x & 15) * 8) =
+            make_uint2(codes4(v[0], v[1], v[2], v[3], s), codes4(v[4], v[5], v[6], v[7], s));
+        if ((threadIdx.x & 15) == 0) scales[(long long)b * N + n] = s;
+    }
+}
+
+// ------------------------------------------------------------------ products
+enum Epi { kLinear, kSwiGLU };
+
+struct Fp8Args {
+    const char* codes;    // rows [N][groups * 128]
+    const float* scales;  // [groups][N]
+    int N, O, groups, blocks;      // outputs (kSwiGLU: columns of h), blocks of 16
+    const char* w[2];              // [blocks][groups] of 2 KB; kSwiGLU: gate, up
+    const float* ws[2];            // [ceil(O / 128)][groups]
+    const unsigned short* bias;    // [O] or NULL
+    unsigned short* out;           // [N][O]
+    float* h;                      // kSwiGLU: [N][ldh], ldh = O rounded up to 128
+    unsigned char* hq;             // or its codes [N][ldh] and scales [ldh / 128][N]
+    float* hs;
+    int ldh;
+    int ncb, total;
+};
+
+__device__ __forceinline__ uint4 load16(const char* p) { return *(const uint4*)p; }
+
+// Few rows (16 MR at most): a work-group of eight wavefronts owns 16 outputs (kSwiGLU: gate and up), the wavefronts
+// deal out the blocks of 128 contraction elements and add their sums in LDS, in order. Bound by the stream of the
+// weights, which go to registers in their stored order; rows come from L2.
+template <int EPI, int MR>
+__global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Args p) {
+    constexpr int NM = EPI == kSwiGLU ? 2 : 1;  // matrices
+    __shared__ f32x4 part[8][NM * MR][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int blk = blockIdx.x;
+    const int row = lane & 15;
+    f32x4 acc[NM][MR];
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int r = 0; r < MR; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int b = wave; b < p.groups; b += 8) {
+        Op8 w[NM], a[MR];
+        float s[MR];
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            const char* at = p.w[m] + ((long long)blk * p.groups + b) * 2048 + lane * 16;
+            w[m].u[0] = nt_load16(at);
+            w[m].u[1] = nt_load16(at + 1024);
+        }
+#pragma unroll
+        for (int r = 0; r < MR; ++r) {
+            // rows past the last one are read as it is; their sums are not stored
+            const int n = min(16 * r + row, p.N - 1);
+            const char* at = p.codes + ((long long)n * p.groups + b) * kBlock + (lane >> 4) * 16;
+            a[r].u[0] = load16(at);
+            a[r].u[1] = load16(at + 64);
+            s[r] = p.scales[(long long)b * p.N + n];
+        }
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            const float ws = p.ws[m][(long long)(blk >> 3) * p.groups + b];
+#pragma unroll
+            for (int r = 0; r < MR; ++r) {
+                const f32x4 d = mfma8(w[m], a[r]);
+                const float f = s[r] * ws;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[m][r][i] = fmaf(d[i], f, acc[m][r][i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int r = 0; r < MR; ++r) part[wave][m * MR + r][lane] = acc[m][r];
+    __syncthreads();
+    // wavefront r finishes rows 16 r .. + 15
+    if (wave >= MR) return;
+    f32x4 v[NM];
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+        v[m] = part[0][m * MR + wave][lane];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v[m] = v[m] + part[k][m * MR + wave][lane];
+    }
+    const int n = 16 * wave + row, o = blk * 16 + 4 * (lane >> 4);
+    if (n >= p.N) return;
+    if constexpr (EPI == kSwiGLU) {
+        f32x4 h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = silu(v[0][i]) * v[1][i];
+        *(f32x4*)(p.h + (long long)n * p.ldh + o) = h;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (o + i < p.O) {
+                const float b = p.bias != nullptr ? bf16_to_f32(p.bias[o + i]) : 0.0f;
+                p.out[(long long)n * p.O + o + i] = f32_to_bf16_rne(v[0][i] + b);
+            }
+    }
+}
+
+// s_waitcnt immediate (gfx9 encoding): vmcnt <= n only
+constexpr int vm_only(int n) { return (n & 0xf) | ((n >> 4) << 14) | (0x7 << 4) | (0xf << 8); }
+
+// Direct loads to LDS at m0 + 16 (4) x lane, from base + off; an offset of kNone reads zeros (the buffer's bounds are
+// 2^31 bytes, which no other offset reaches, and no lane reads behind a tensor).
+constexpr unsigned kNone = 0xfffffff0u;
+__device__ __forceinline__ i32x4 rsrc_of(const void* base) {
+    const unsigned long long p = (unsigned long long)base;
+    return i32x4{(int)(unsigned)p, (int)(unsigned)(p >> 32) & 0xffff, (int)0x80000000u, 0x00020000};
+}
+__device__ __forceinline__ void load_lds16(const void* base, unsigned off, unsigned m0) {
+    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc_of(base)), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ void load_lds4(const void* base, unsigned off, unsigned m0) {
+    asm volatile("buffer_load_dword %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc_of(base)), "{m0}"(m0) : "memory");
+}
+
+// Tiles: WR x WC wavefronts of 16 MB rows x 16 NB columns each (kSwiGLU: the wavefront's first NB / 2 blocks are gate
+// columns, the others the up columns of the same h columns). A step is a block of 128 contraction elements: rows
+// (swizzled 128-byte lines), weights (stored order) and both scales go to LDS by direct loads, one step ahead of the
+// products, in two stages with one barrier a step.
+template <int EPI, int WR, int WC, int MB, int NB>
+__global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
+    constexpr int NW = WR * WC, TM = WR * 16 * MB, TN = WC * 16 * NB;
+    constexpr bool DUAL = EPI == kSwiGLU;
+    constexpr int A_BYTES = TM * kBlock, B_BYTES = TN * kBlock;
+    constexpr int DA = A_BYTES / 1024 / NW, DB = B_BYTES / 1024 / NW;
+    constexpr int STAGE = A_BYTES + B_BYTES + NW * 256;  // and 64 scales of every wavefront's load
+    static_assert(TM / 64 < NW && DA * NW * 1024 == A_BYTES && DB * NW * 1024 == B_BYTES, "loads deal out evenly");
+    static_assert(16 * NB <= kBlock, "a wavefront's columns share their weight scales");
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[2][STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave / WC, wc = wave % WC;
+    const int per = (p.total + 7) / 8, local = blockIdx.x / 8;
+    const int item = (blockIdx.x % 8) * per + local;
+    if (local >= per || item >= p.total) return;
+    const int m0 = (item / p.ncb) * TM;
+    const int n0 = (item % p.ncb) * (DUAL ? TN / 2 : TN);
+    const long long ldx = (long long)p.groups * kBlock, ldw = (long long)p.groups * 2048;
+
+    // rows: line r = 8 blk + lane / 8, piece c at c ^ (r & 7) ^ (r >> 3 & 1)
+    unsigned a_off[DA], b_off[DB];
+#pragma unroll
+    for (int j = 0; j < DA; ++j) {
+        const int r = (wave * DA + j) * 8 + lane / 8;
+        const int c = (lane % 8) ^ (r & 7) ^ (r >> 3 & 1);
+        a_off[j] = m0 + r < p.N ? (unsigned)(r * ldx + c * 16) : kNone;
+    }
+    // weights: piece q = half q & 1 of the tile's block q / 2; kSwiGLU: the tile's second half are up blocks
+    const int q0 = wave * DB;
+    const bool up = DUAL && q0 >= TN / 16;  // uniform: a wavefront's pieces are of one matrix
+    static_assert(!DUAL || (TN / 16) % DB == 0, "a wavefront's pieces are of one matrix");
+#pragma unroll
+    for (int j = 0; j < DB; ++j) {
+        const int q = q0 + j - (up ? TN / 16 : 0);
+        const int blk = q >> 1;
+        b_off[j] = (n0 >> 4) + blk < p.blocks ? (unsigned)(blk * ldw + (q & 1) * 1024 + lane * 16) : kNone;
+    }
+    const char* pa = p.codes + m0 * ldx;
+    const char* pb = (up ? p.w[1] : p.w[0]) + (n0 >> 4) * ldw;
+    // scales: wavefront w loads those of rows 64 w .., the next one the weights' (lane i: of columns 128 i .., kSwiGLU:
+    // gate and up), the others none
+    const float* ps = p.scales;
+    unsigned s_off = kNone;
+    long long s_step = 4ll * p.N;
+    if (wave < TM / 64) {
+        ps += m0 + wave * 64;
+        if (m0 + wave * 64 + lane < p.N) s_off = lane * 4;
+    } else if (wave == TM / 64) {
+        s_step = 4;
+        const int ob = n0 / kBlock;
+        ps = p.ws[0] + (long long)ob * p.groups;
+        if (DUAL) {
+            // two tensors: lane 0 reads the gate's, and the up's go with a base of their own (below)
+            s_off = lane == 0 ? 0 : kNone;
+        } else if (lane < (TN + kBlock - 1) / kBlock && (ob + lane) * kBlock < p.O) {
+            s_off = (unsigned)(4ll * lane * p.groups);
+        }
+    } else if (DUAL && wave == TM / 64 + 1) {
+        s_step = 4;
+        ps = p.ws[1] + (long long)(n0 / kBlock) * p.groups;
+        s_off = lane == 0 ? 0 : kNone;
+    }
+    const char* psc = (const char*)ps;
+    const unsigned lds0 = (unsigned)(size_t)(lds_ptr_t)&lds[0][0];
+    auto load = [&](int st) {
+        const unsigned base = lds0 + st * STAGE;
+#pragma unroll
+        for (int j = 0; j < DA; ++j) load_lds16(pa, a_off[j], base + (wave * DA + j) * 1024);
+#pragma unroll
+        for (int j = 0; j < DB; ++j) load_lds16(pb, b_off[j], base + A_BYTES + (q0 + j) * 1024);
+        load_lds4(psc, s_off, base + A_BYTES + B_BYTES + wave * 256);
+        pa += kBlock;
+        pb += 2048;
+        psc += s_step;
+    };
+
+    const int g = lane >> 4, r16 = lane & 15;
+    const int ar = wr * 16 * MB + r16;
+    const int a_rd = ar * 128 + ((g ^ (ar & 7) ^ (ar >> 3 & 1)) << 4);  // the second piece: ^ 64
+    // tile block of the wavefront's column block j
+    auto block_of = [&](int j) { return DUAL ? (j < NB / 2 ? wc * (NB / 2) + j : TN / 32 + wc * (NB / 2) + j - NB / 2) : wc * NB + j; };
+    f32x4 acc[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    load(0);
+    for (int b = 0; b < p.groups; ++b) {
+        const int st = b & 1;
+        // this wavefront's loads of step b have landed, and after the barrier everybody's, and step b - 1 is read
+        __builtin_amdgcn_s_waitcnt(vm_only(0));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (b + 1 < p.groups) load(st ^ 1);
+        const unsigned char* A = &lds[st][0];
+        const unsigned char* B = A + A_BYTES;
+        const float* S = (const float*)(B + B_BYTES);
+        Op8 a[MB];
+        float f[MB], f1[MB];
+        const float w0 = S[DUAL ? TM : TM + (wc * 16 * NB) / kBlock], w1 = DUAL ? S[TM + 64] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            a[i].u[0] = *(const uint4*)(A + a_rd + i * 2048);
+            a[i].u[1] = *(const uint4*)(A + (a_rd ^ 64) + i * 2048);
+            const float s = S[ar + 16 * i];
+            f[i] = s * w0;
+            f1[i] = s * w1;
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            Op8 w;
+            const unsigned char* at = B + block_of(j) * 2048 + lane * 16;
+            w.u[0] = *(const uint4*)at;
+            w.u[1] = *(const uint4*)(at + 1024);
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const f32x4 d = mfma8(w, a[i]);
+                const float s = DUAL && j >= NB / 2 ? f1[i] : f[i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], s, acc[i][j][e]);
+            }
+        }
+    }
+
+    // block (i, j): row 16 i + lane % 16, columns 16 j + 4 g .. + 3
+    if constexpr (!DUAL) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int o = n0 + (wc * NB + j) * 16 + 4 * g;
+            float bias[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bias[e] = p.bias != nullptr && o + e < p.O ? bf16_to_f32(p.bias[o + e]) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const int n = m0 + ar + 16 * i;
+                if (n >= p.N) continue;
+                unsigned short* dst = p.out + (long long)n * p.O + o;
+                const unsigned lo = pack_bf16(acc[i][j][0] + bias[0], acc[i][j][1] + bias[1]),
+                               hi = pack_bf16(acc[i][j][2] + bias[2], acc[i][j][3] + bias[3]);
+                if (o + 4 <= p.O && p.O % 4 == 0) {
+                    *(uint2*)dst = make_uint2(lo, hi);
+                } else {
+                    const unsigned v[2] = {lo, hi};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (o + e < p.O) dst[e] = (unsigned short)(v[e / 2] >> 16 * (e & 1));
+                }
+            }
+        }
+    } else {
+        constexpr int NH = NB / 2;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NH; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = silu(acc[i][j][e]) * acc[i][j + NH][e];
+        if constexpr (TN / 2 == kBlock) {
+            // the tile holds whole groups of h: their largest sizes through LDS, then codes
+            unsigned(*top)[TM] = (unsigned(*)[TM])&lds[0][0];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                unsigned m = 0;
+#pragma unroll
+                for (int j = 0; j < NH; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m = max(m, size_bits(acc[i][j][e]));
+                m = max(m, (unsigned)__shfl_xor((int)m, 16));
+                m = max(m, (unsigned)__shfl_xor((int)m, 32));
+                if (g == 0) top[wc][ar + 16 * i] = m;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const int n = m0 + ar + 16 * i;
+                if (n >= p.N) continue;
+                unsigned m = top[0][ar + 16 * i];
+#pragma unroll
+                for (int c = 1; c < WC; ++c) m = max(m, top[c][ar + 16 * i]);
+                const float s = scale_of(m);
+#pragma unroll
+                for (int j = 0; j < NH; ++j)
+                    *(unsigned*)(p.hq + (long long)n * p.ldh + n0 + (wc * NH + j) * 16 + 4 * g) =
+                        codes4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], s);
+                if (g == 0 && wc == 0) p.hs[(long long)(n0 / kBlock) * p.N + n] = s;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const int n = m0 + ar + 16 * i;
+                if (n >= p.N) continue;
+#pragma unroll
+                for (int j = 0; j < NH; ++j) *(f32x4*)(p.h + (long long)n * p.ldh + n0 + (wc * NH + j) * 16 + 4 * g) = acc[i][j];
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host
+inline int groups_of(int k) { return (k + kBlock - 1) / kBlock; }
+
+void rows_launch(const void* x, int act, int N, int K, int ld, void* codes, float* scales, hipStream_t st) {
+    const int groups = groups_of(K);
+    const unsigned blocks = (unsigned)std::min<long long>(((long long)N * groups + 15) / 16, 1 << 16);
+    const int piece = act == YVMOE_ACT_F32 ? 4 : 8;
+    const bool vec = (uintptr_t)x % 16 == 0 && K % piece == 0 && ld % piece == 0;
+    unsigned char* c = (unsigned char*)codes;
+    if (act == YVMOE_ACT_F32) {
+        if (vec) fp8_rows_kernel<true, true><<<blocks, 256, 0, st>>>(x, N, K, ld, groups, c, scales);
+        else fp8_rows_kernel<true, false><<<blocks, 256, 0, st>>>(x, N, K, ld, groups, c, scales);
+    } else {
+        if (vec) fp8_rows_kernel<false, true><<<blocks, 256, 0, st>>>(x, N, K, ld, groups, c, scales);
+        else fp8_rows_kernel<false, false><<<blocks, 256, 0, st>>>(x, N, K, ld, groups, c, scales);
+    }
+}
+
+constexpr int kFewRows = 64;
+
+template <int EPI, int WR, int WC, int MB, int NB>
+void tile_grid(Fp8Args p, hipStream_t st) {
+    constexpr int TM = WR * 16 * MB, TN = WC * 16 * NB;
+    p.ncb = ceil_div(p.O, EPI == kSwiGLU ? TN / 2 : TN);
+    p.total = ceil_div(p.N, TM) * p.ncb;
+    fp8_tile_kernel<EPI, WR, WC, MB, NB><<<(unsigned)(ceil_div(p.total, 8) * 8), 64 * WR * WC, 0, st>>>(p);
+}
+
+// Whether kSwiGLU writes codes of h (else h in fp32).
+inline bool wide_tiles(int N, int cols) { return (long long)ceil_div(N, 256) * ceil_div(cols, 256) >= 160; }
+inline bool swiglu_codes(int N, int F) { return N > kFewRows && wide_tiles(N, 2 * F); }
+
+template <int EPI>
+void product_launch(const Fp8Args& p, hipStream_t st) {
+    if (p.N <= kFewRows) {
+        if (p.N <= 16) fp8_few_kernel<EPI, 1><<<(unsigned)p.blocks, 512, 0, st>>>(p);
+        else if (p.N <= 32) fp8_few_kernel<EPI, 2><<<(unsigned)p.blocks, 512, 0, st>>>(p);
+        else fp8_few_kernel<EPI, 4><<<(unsigned)p.blocks, 512, 0, st>>>(p);
+    } else if (wide_tiles(p.N, EPI == kSwiGLU ? 2 * p.O : p.O)) {
+        tile_grid<EPI, 4, 2, 4, 8>(p, st);
+    } else {
+        tile_grid<EPI, 2, 2, 2, 4>(p, st);
+    }
+}
+
+Fp8Args product_of(const void* codes, const float* scales, int N, const yvmoe_fp8_matrix* w) {
+    Fp8Args p{};
+    p.codes = (const char*)codes;
+    p.scales = scales;
+    p.N = N;
+    p.O = w->out_features;
+    p.groups = groups_of(w->in_features);
+    p.blocks = ceil_div(w->out_features, 16);
+    p.w[0] = (const char*)w->codes;
+    p.ws[0] = (const float*)w->scales;
+    return p;
+}
+
+inline size_t codes_bytes(int N, int K) { return align_up((size_t)N * groups_of(K) * kBlock, 256); }
+inline size_t scales_bytes(int N, int K) { return align_up((size_t)N * groups_of(K) * 4, 256); }
+
+}  // namespace
+
+int fp8_rows_launch(const void* x, int act, int N, int K, void* codes, float* scales, hipStream_t st) {
+    rows_launch(x, act, N, K, K, codes, scales, st);
+    YV_LAUNCH_CHECK("fp8 rows");
+    return YVMOE_OK;
+}
+
+size_t fp8_linear_ws(int N, int K) { return codes_bytes(N, K) + scales_bytes(N, K); }
+
+int fp8_product_launch(const void* codes, const float* scales, int N, const yvmoe_fp8_matrix* w, const void* bias,
+                       void* out, hipStream_t st) {
+    Fp8Args p = product_of(codes, scales, N, w);
+    p.bias = (const unsigned short*)bias;
+    p.out = (unsigned short*)out;
+    product_launch<kLinear>(p, st);
+    YV_LAUNCH_CHECK("fp8 linear");
+    return YVMOE_OK;
+}
+
+int fp8_linear_launch(const void* x, int N, const yvmoe_fp8_matrix* w, const void* bias, void* out, char* ws,
+                      hipStream_t st) {
+    float* scales = (float*)(ws + codes_bytes(N, w->in_features));
+    rows_launch(x, YVMOE_ACT_BF16, N, w->in_features, w->in_features, ws, scales, st);
+    return fp8_product_launch(ws, scales, N, w, bias, out, st);
+}
+
+size_t fp8_swiglu_ws(int N, int H, int F) {
+    return fp8_linear_ws(N, H) + fp8_linear_ws(N, F) +
+           (swiglu_codes(N, F) ? 0 : align_up((size_t)N * groups_of(F) * kBlock * 4, 256));
+}
+
+int fp8_swiglu_launch(const void* x, int N, const yvmoe_fp8_matrix* gate, const yvmoe_fp8_matrix* up,
+                      const yvmoe_fp8_matrix* down, void* out, char* ws, hipStream_t st) {
+    const int H = gate->in_features, F = gate->out_features;
+    char* xq = ws;
+    float* xs = (float*)(xq + codes_bytes(N, H));
+    char* hq = (char*)xs + scales_bytes(N, H);
+    float* hs = (float*)(hq + codes_bytes(N, F));
+    float* h = (float*)((char*)hs + scales_bytes(N, F));
+    rows_launch(x, YVMOE_ACT_BF16, N, H, H, xq, xs, st);
+    Fp8Args p = product_of(xq, xs, N, gate);
+    p.w[1] = (const char*)up->codes;
+    p.ws[1] = (const float*)up->scales;
+    p.ldh = groups_of(F) * kBlock;
+    p.h = h;
+    p.hq = (unsigned char*)hq;
+    p.hs = hs;
+    product_launch<kSwiGLU>(p, st);
+    if (!swiglu_codes(N, F)) rows_launch(h, YVMOE_ACT_F32, N, F, p.ldh, hq, hs, st);
+    return fp8_product_launch(hq, hs, N, down, nullptr, out, st);
+}
+
+}  // namespace yvmoe

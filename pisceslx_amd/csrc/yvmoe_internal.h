@@ -497,4 +497,15 @@ int swiglu_backward_launch(const void* dy, const void* x, const float* saved, in
                            const yvmoe_swiglu_weights* w, void* dx, void* dwg, void* dwu, void* dwd, char* ws,
                            size_t* bytes, hipStream_t st);
 
+// 8-bit floating point rows, linear layer and gated block (yvmoe_fp8.hip).
+int fp8_rows_launch(const void* x, int act, int N, int K, void* codes, float* scales, hipStream_t st);
+int fp8_product_launch(const void* codes, const float* scales, int N, const yvmoe_fp8_matrix* w, const void* bias,
+                       void* out, hipStream_t st);
+size_t fp8_linear_ws(int N, int K);
+int fp8_linear_launch(const void* x, int N, const yvmoe_fp8_matrix* w, const void* bias, void* out, char* ws,
+                      hipStream_t st);
+size_t fp8_swiglu_ws(int N, int H, int F);
+int fp8_swiglu_launch(const void* x, int N, const yvmoe_fp8_matrix* gate, const yvmoe_fp8_matrix* up,
+                      const yvmoe_fp8_matrix* down, void* out, char* ws, hipStream_t st);
+
 }  // namespace yvmoe

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .quant import PackedExperts, PackedLinear
+from .quant import Fp8Rows, PackedExperts, PackedFp8Linear, PackedLinear
 
 
 def _act(dtype: torch.dtype) -> int:
@@ -635,7 +635,7 @@ def int4_linear(x: torch.Tensor, weight: PackedLinear, bias: Optional[torch.Tens
     return out
 
 
-# ---------------------------------------------------------------- gated feed-forward block
+# ---------------------------------------------------------------- 8-bit floating point
 def _on(dev: torch.device):
     """A guard for launches on ``dev`` where another device is current."""
     return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
@@ -650,6 +650,98 @@ def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
+def quantize_fp8_rows(x: torch.Tensor) -> Fp8Rows:
+    """Rows of x [..., features] (bf16 or fp32) in e4m3fn with a scale per 128 values, the left operand of
+    fp8_linear: scale = max(max|x| / 448, 1e-12), code = e4m3fn(x / scale), in fp32 divisions and rounded to
+    nearest even (quantize_to_fp8, opss/quantize/engine.py:841-883, per 128 values). A group with an infinity or
+    NaN makes every product of its row NaN. Up to 2^24 rows of up to 2^20 features."""
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"x must be [..., features], got {tuple(x.shape)}")
+    dev, act, K = _same_device(x), _act(x.dtype), x.shape[-1]
+    N, groups = x.numel() // K, -(-K // 128)
+    rows = Fp8Rows(K, torch.empty(N, groups * 128, dtype=torch.float8_e4m3fn, device=dev),
+                   torch.empty(groups, N, dtype=torch.float32, device=dev))
+    with _on(dev):
+        rc = _lib.lib().yvmoe_quantize_fp8_rows(x.data_ptr(), act, N, K, rows.codes.data_ptr(),
+                                                rows.scales.data_ptr(), _stream(dev))
+    if rc:
+        _lib.check(rc, "yvmoe_quantize_fp8_rows")
+    return rows
+
+
+def _fp8_out(out: Optional[torch.Tensor], shape, dev) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    if tuple(out.shape) != tuple(shape) or out.dtype != torch.bfloat16:
+        raise ValueError(f"out must be bfloat16 {tuple(shape)}")
+    return out
+
+
+def fp8_linear(x, weight: PackedFp8Linear, bias: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x · Wᵀ (+ bias [out] bf16) with both operands in 8-bit floating point: W in e4m3fn with a scale per
+    128 x 128 block (quant.pack_fp8_linear), x [..., in] bf16, rounded to e4m3fn with a scale per 128 values in
+    the call, or rows that are already (Fp8Rows). fp32 sums, rounded once to bf16 [..., out]; the matrix unit
+    keeps about 16 bits of a block's sum, so there are no fp32 outputs. Up to 2^24 rows. ``out`` must
+    overlap no input."""
+    K, O = weight.in_features, weight.out_features
+    rows = isinstance(x, Fp8Rows)
+    if rows:
+        if x.features != K:
+            raise ValueError(f"rows have {x.features} features, the weight {K}")
+        lead, dev = (x.codes.shape[0],), _same_device(x.codes, x.scales, weight.codes, weight.scales, bias, out)
+    else:
+        if x.dim() == 0 or x.shape[-1] != K:
+            raise ValueError(f"x must be [..., {K}], got {tuple(x.shape)}")
+        if x.dtype != torch.bfloat16:
+            raise ValueError(f"x must be bfloat16 or Fp8Rows, got {x.dtype}")
+        lead, dev = x.shape[:-1], _same_device(x, weight.codes, weight.scales, bias, out)
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != O):
+        raise ValueError(f"bias must be bfloat16 [{O}]")
+    out = _fp8_out(out, (*lead, O), dev)
+    l, w, N = _lib.lib(), weight.struct(), out.numel() // O
+    with _on(dev):
+        if rows:
+            rc = l.yvmoe_fp8_linear_rows(x.codes.data_ptr(), x.scales.data_ptr(), N, ctypes.byref(w), _ptr(bias),
+                                         out.data_ptr(), _stream(dev))
+        else:
+            nbytes = l.yvmoe_fp8_linear_workspace_bytes(N, K)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            rc = l.yvmoe_fp8_linear(x.data_ptr(), N, ctypes.byref(w), _ptr(bias), out.data_ptr(), ws.data_ptr(),
+                                    nbytes, _stream(dev))
+    if rc:
+        _lib.check(rc, "yvmoe_fp8_linear")
+    return out
+
+
+def fp8_swiglu(x: torch.Tensor, gate: PackedFp8Linear, up: PackedFp8Linear, down: PackedFp8Linear,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gated feed-forward block (:func:`swiglu`) on 8-bit weights: products as in :func:`fp8_linear`, the
+    activated product in fp32 and rounded to e4m3fn with a scale per 128 values. x [..., H] and the result
+    bf16, gate and up F x H, down H x F. Inference only. ``out`` must overlap no input."""
+    H, F = gate.in_features, gate.out_features
+    if (up.in_features, up.out_features, down.in_features, down.out_features) != (H, F, F, H):
+        raise ValueError(f"gate {F} x {H}, up {up.out_features} x {up.in_features}, down {down.out_features} x "
+                         f"{down.in_features} are no gated block")
+    if x.dim() == 0 or x.shape[-1] != H:
+        raise ValueError(f"x must be [..., {H}], got {tuple(x.shape)}")
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"x must be bfloat16, got {x.dtype}")
+    dev = _same_device(x, gate.codes, gate.scales, up.codes, up.scales, down.codes, down.scales, out)
+    out = _fp8_out(out, x.shape, dev)
+    l, N = _lib.lib(), x.numel() // H
+    g, u, d = gate.struct(), up.struct(), down.struct()
+    nbytes = l.yvmoe_fp8_swiglu_workspace_bytes(N, H, F)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = l.yvmoe_fp8_swiglu(x.data_ptr(), N, ctypes.byref(g), ctypes.byref(u), ctypes.byref(d), out.data_ptr(),
+                                ws.data_ptr(), nbytes, _stream(dev))
+    if rc:
+        _lib.check(rc, "yvmoe_fp8_swiglu")
+    return out
+
+
+# ---------------------------------------------------------------- gated feed-forward block
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """``t`` at a 16-byte address (a copy where a view starts elsewhere)."""
     return t if t.data_ptr() % 16 == 0 else t.clone()

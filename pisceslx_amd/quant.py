@@ -373,6 +373,94 @@ def pack_linear(w: torch.Tensor) -> PackedLinear:
     return pack_linear_codes(q, s, inn)
 
 
+# ------------------------------------------------------------------ linear layers, fp8 128x128
+@dataclass
+class PackedFp8Linear:
+    """A linear layer's weight in e4m3fn with a scale per 128 x 128 block, in the order yvmoe_fp8_linear reads
+    (include/yvmoe.h): codes [out/16][in/128] blocks of 2 KB, scales [out/128][in/128] fp32, all counts
+    rounded up. Any in_features and out_features. An expert's matrix in fp8 (PackedExperts) has this order."""
+
+    in_features: int
+    out_features: int
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self):
+        if self.in_features < 1 or self.out_features < 1:
+            raise ValueError(f"a linear layer needs features, got in {self.in_features}, out {self.out_features}")
+        groups = -(-self.in_features // 128)
+        want = (-(-self.out_features // 16), groups, 2048)
+        if self.codes.shape != want or self.codes.dtype != torch.uint8:
+            raise ValueError(f"codes must be uint8 {list(want)}, got {self.codes.dtype} {tuple(self.codes.shape)}")
+        want = (-(-self.out_features // 128), groups)
+        if self.scales.shape != want or self.scales.dtype != torch.float32:
+            raise ValueError(f"scales must be float32 {list(want)}, got {self.scales.dtype} "
+                             f"{tuple(self.scales.shape)}")
+
+    def to(self, device) -> "PackedFp8Linear":
+        return PackedFp8Linear(self.in_features, self.out_features, self.codes.to(device), self.scales.to(device))
+
+    def struct(self) -> _lib.Fp8Matrix:
+        return _lib.Fp8Matrix(self.in_features, self.out_features, self.codes.data_ptr(), self.scales.data_ptr())
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """The dense [out][in] weight (for tests)."""
+        ob, groups = self.codes.shape[:2]
+        q = unblock_matrix(self.codes.view(ob * 16, groups * 128), _lib.W_FP8).view(torch.float8_e4m3fn).float()
+        s = self.scales.repeat_interleave(128, 0)[:ob * 16].repeat_interleave(128, 1)
+        return (q * s)[:self.out_features, :self.in_features].to(dtype)
+
+
+def pack_fp8_linear_codes(codes: torch.Tensor, scales: torch.Tensor, in_features: int) -> PackedFp8Linear:
+    """A PackedFp8Linear of codes in the fp8 format (:func:`quantize_fp8`), but of any size: codes [out][in]
+    (float8_e4m3fn, or their bytes as uint8) and scales [out/128][in/128] fp32, rounded up."""
+    if codes.dim() != 2 or codes.dtype not in (torch.uint8, torch.float8_e4m3fn) or codes.shape[1] != in_features:
+        raise ValueError(f"codes must be uint8 or float8_e4m3fn [out, {in_features}], got {codes.dtype} "
+                         f"{tuple(codes.shape)}")
+    q, out = codes.view(torch.uint8), codes.shape[0]
+    pad = (0, -in_features % 128, 0, -out % 16)
+    if any(pad):
+        q = torch.nn.functional.pad(q, pad)
+    b = block_matrix(q, _lib.W_FP8).view(q.shape[0] // 16, q.shape[1] // 128, 2048)
+    return PackedFp8Linear(in_features, out, b, scales.contiguous())
+
+
+def pack_fp8_linear(w: torch.Tensor) -> PackedFp8Linear:
+    """Quantize a [out][in] weight (nn.Linear.weight) to e4m3fn with a scale per 128 x 128 block and pack it."""
+    if w.dim() != 2:
+        raise ValueError(f"a linear weight is [out, in], got {tuple(w.shape)}")
+    out, inn = w.shape
+    pad = (0, -inn % 128, 0, -out % 128)
+    q, s = quantize_fp8(torch.nn.functional.pad(w.float(), pad) if any(pad) else w)
+    return pack_fp8_linear_codes(q[:out, :inn], s, inn)
+
+
+@dataclass
+class Fp8Rows:
+    """Rows in e4m3fn with a scale per 128 values (functional.quantize_fp8_rows): codes
+    [rows][ceil(features / 128) * 128] float8_e4m3fn (zero behind the last feature), scales
+    [ceil(features / 128)][rows] fp32."""
+
+    features: int
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self):
+        groups = -(-self.features // 128)
+        if (self.features < 1 or self.codes.dim() != 2 or self.codes.shape[1] != groups * 128
+                or self.codes.dtype != torch.float8_e4m3fn):
+            raise ValueError(f"codes must be float8_e4m3fn [rows, {groups * 128}], got {self.codes.dtype} "
+                             f"{tuple(self.codes.shape)}")
+        if self.scales.shape != (groups, self.codes.shape[0]) or self.scales.dtype != torch.float32:
+            raise ValueError(f"scales must be float32 [{groups}, {self.codes.shape[0]}], got {self.scales.dtype} "
+                             f"{tuple(self.scales.shape)}")
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """The dense [rows][features] values (for tests)."""
+        s = self.scales.t().repeat_interleave(128, 1)
+        return (self.codes.float() * s)[:, :self.features].to(dtype)
+
+
 # ------------------------------------------------------------------ router
 def split_bf16x3(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """fp32 w -> (hi, mid, lo) bf16 with hi + mid + lo == w to within one fp32 ulp."""
