@@ -362,6 +362,158 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     }
 }
 
+// ------------------------------------------------------------------ few rows
+// Up to 64 rows of the forward pass: bound by the stream of the weights, which are read as they lie. A work-group of
+// eight wavefronts owns 16 columns (kSwiGLU: gate and up), the wavefronts deal out the contraction in spans of kSpan
+// steps and add their sums in LDS, in order. Lane 16 g + r reads 16 bytes of weight row r and of row r of x, so a
+// step is 32 (fp32: 16) elements and a span of four 256 consecutive bytes of every weight row; any alignment. fp32 runs
+// on the fp32 MFMAs: four a step, each on one element of the lanes' four.
+struct FewArgs {
+    const void* x;
+    int N, K, ldx;
+    const void* w[2];       // [O][K]
+    int O;
+    void* out;              // kOut: [N][O]; kSwiGLU: h [N][ldh], in x's type
+    float* gu;              // kSwiGLU: [2][N][ldh] or none
+    int ldh;
+};
+constexpr int kSpan = 4;
+
+struct __attribute__((packed, aligned(2))) Any16 {
+    unsigned v[4];
+};
+template <bool F32>
+struct Piece {  // 16 bytes of a row
+    union {
+        uint4 u;
+        bf16x8 b;
+        float f[4];
+        unsigned short s[8];
+    };
+    static constexpr int E = F32 ? 4 : 8, STEP = 4 * E;
+    __device__ __forceinline__ void load(const void* p, size_t at) {
+        const Any16 a = *(const Any16*)((const char*)p + at * (F32 ? 4 : 2));
+        u = make_uint4(a.v[0], a.v[1], a.v[2], a.v[3]);
+    }
+    // the first `left` elements, zeros behind them
+    __device__ __forceinline__ void load_end(const void* p, size_t at, int left) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (F32) f[e] = e < left ? ((const float*)p)[at + e] : 0.0f;
+            else s[e] = e < left ? ((const unsigned short*)p)[at + e] : 0;
+        }
+    }
+};
+template <bool F32>
+__device__ __forceinline__ f32x4 few_mfma(const Piece<F32>& a, const Piece<F32>& b, f32x4 c) {
+    if constexpr (F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.f[e], b.f[e], c, 0, 0, 0);
+        return c;
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.b, b.b, c, 0, 0, 0);
+    }
+}
+
+template <int EPI, bool F32, int MR>
+__global__ __launch_bounds__(512) void swiglu_few_kernel(FewArgs p) {
+    constexpr int NM = EPI == kSwiGLU ? 2 : 1;
+    typedef Piece<F32> P;
+    __shared__ f32x4 part[8][NM * MR][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, r = lane & 15;
+    // rows past the last one read it again: their sums are not stored
+    const size_t wrow = (size_t)min((int)blockIdx.x * 16 + r, p.O - 1) * p.K;
+    size_t xrow[MR];
+#pragma unroll
+    for (int i = 0; i < MR; ++i) xrow[i] = (size_t)min(16 * i + r, p.N - 1) * p.ldx;
+    f32x4 acc[NM][MR];
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int i = 0; i < MR; ++i) acc[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int steps = p.K / P::STEP, spans = (steps + kSpan - 1) / kSpan;
+    for (int sp = wave; sp < spans; sp += 8) {
+        const int s0 = sp * kSpan;
+        P w[NM][kSpan], x[MR][kSpan];
+        if (s0 + kSpan <= steps) {
+#pragma unroll
+            for (int s = 0; s < kSpan; ++s) {
+                const size_t k = (size_t)(s0 + s) * P::STEP + g * P::E;
+#pragma unroll
+                for (int m = 0; m < NM; ++m) w[m][s].load(p.w[m], wrow + k);
+#pragma unroll
+                for (int i = 0; i < MR; ++i) x[i][s].load(p.x, xrow[i] + k);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // all of the span's loads in flight
+#pragma unroll
+            for (int s = 0; s < kSpan; ++s)
+#pragma unroll
+                for (int m = 0; m < NM; ++m)
+#pragma unroll
+                    for (int i = 0; i < MR; ++i) acc[m][i] = few_mfma<F32>(w[m][s], x[i][s], acc[m][i]);
+        } else {
+            for (int s = s0; s < steps; ++s) {
+                const size_t k = (size_t)s * P::STEP + g * P::E;
+#pragma unroll
+                for (int m = 0; m < NM; ++m) w[m][0].load(p.w[m], wrow + k);
+#pragma unroll
+                for (int i = 0; i < MR; ++i) x[i][0].load(p.x, xrow[i] + k);
+#pragma unroll
+                for (int m = 0; m < NM; ++m)
+#pragma unroll
+                    for (int i = 0; i < MR; ++i) acc[m][i] = few_mfma<F32>(w[m][0], x[i][0], acc[m][i]);
+            }
+        }
+    }
+    if (steps * P::STEP < p.K && wave == spans % 8) {
+        // the rest of the rows, less than a step
+        const size_t k = (size_t)steps * P::STEP + g * P::E;
+        const int left = p.K - (int)k;
+        P w[NM], x[MR];
+#pragma unroll
+        for (int m = 0; m < NM; ++m) w[m].load_end(p.w[m], wrow + k, left);
+#pragma unroll
+        for (int i = 0; i < MR; ++i) x[i].load_end(p.x, xrow[i] + k, left);
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+            for (int i = 0; i < MR; ++i) acc[m][i] = few_mfma<F32>(w[m], x[i], acc[m][i]);
+    }
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int i = 0; i < MR; ++i) part[wave][m * MR + i][lane] = acc[m][i];
+    __syncthreads();
+    if (wave >= MR) return;  // wavefront i finishes rows 16 i .. + 15
+    f32x4 v[NM];
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+        v[m] = part[0][m * MR + wave][lane];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v[m] = v[m] + part[k][m * MR + wave][lane];
+    }
+    const int n = 16 * wave + r, o = blockIdx.x * 16 + 4 * g;
+    if (n >= p.N) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (EPI == kSwiGLU) {
+            const size_t at = (size_t)n * p.ldh + o + e;
+            const bool in = o + e < p.O;
+            if (o + e >= p.ldh) continue;
+            // behind the last column: zeros, as the tiles write them
+            const float a = in ? v[0][e] : 0.0f, u = in ? v[NM - 1][e] : 0.0f, h = silu(a) * u;
+            if (p.gu != nullptr) p.gu[at] = a, p.gu[(size_t)p.N * p.ldh + at] = u;
+            if (F32) ((float*)p.out)[at] = h;
+            else ((unsigned short*)p.out)[at] = f32_to_bf16_rne(h);
+        } else if (o + e < p.O) {
+            const size_t at = (size_t)n * p.O + o + e;
+            if (F32) ((float*)p.out)[at] = v[0][e];
+            else ((unsigned short*)p.out)[at] = f32_to_bf16_rne(v[0][e]);
+        }
+    }
+}
+
 // Rows of any width to planes of bf16 terms whose rows are a multiple of 8 wide, zeros behind the last column.
 template <bool F32>
 __global__ __launch_bounds__(256) void swiglu_pack_kernel(const void* src, int cols, int ld, long long pieces,
@@ -460,6 +612,16 @@ void tile_launch(const TileArgs& p, hipStream_t st) {
     else tile_grid<EPI, AMC, BMC, 2, 2>(p, st);
 }
 
+constexpr int kFewRows = 64;
+
+template <int EPI, bool F32>
+void few_launch(const FewArgs& p, hipStream_t st) {
+    const unsigned blocks = (unsigned)ceil_div(p.O, 16);
+    if (p.N <= 16) swiglu_few_kernel<EPI, F32, 1><<<blocks, 512, 0, st>>>(p);
+    else if (p.N <= 32) swiglu_few_kernel<EPI, F32, 2><<<blocks, 512, 0, st>>>(p);
+    else swiglu_few_kernel<EPI, F32, 4><<<blocks, 512, 0, st>>>(p);
+}
+
 }  // namespace
 
 size_t swiglu_saved_bytes(int N, int F) { return (size_t)2 * N * up8(F) * 4; }
@@ -469,6 +631,18 @@ int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weig
                           char* ws, size_t* bytes, hipStream_t st) {
     const int H = w->hidden, F = w->ffn, F8 = up8(F), planes = act == YVMOE_ACT_F32 ? 3 : 1;
     Carve c{ws, bytes != nullptr};
+    if (N <= kFewRows) {
+        const bool f32 = act == YVMOE_ACT_F32;
+        void* h = c.take((size_t)N * F8 * (f32 ? 4 : 2));
+        if (bytes != nullptr) *bytes = c.used;
+        if (c.dry || N == 0) return YVMOE_OK;
+        const FewArgs p{x, N, H, H, {w->w_gate, w->w_up}, F, h, saved, F8};
+        const FewArgs q{h, N, F, F8, {w->w_down, nullptr}, H, out, nullptr, 0};
+        if (f32) few_launch<kSwiGLU, true>(p, st), few_launch<kOut, true>(q, st);
+        else few_launch<kSwiGLU, false>(p, st), few_launch<kOut, false>(q, st);
+        YV_LAUNCH_CHECK("swiglu_forward");
+        return YVMOE_OK;
+    }
     const Operand ox = operand(x, act, N, H, c, st), og = operand(w->w_gate, act, F, H, c, st),
                   ou = operand(w->w_up, act, F, H, c, st), od = operand(w->w_down, act, H, F, c, st);
     const long long plane = (long long)N * F8;
