@@ -35,10 +35,13 @@ struct TileArgs {
     int ka, kb;          // contraction elements of A and of B; beyond them both count as zero
     int lda, ldb;        // elements between rows in memory
     int nseg;
-    int ncb, total;      // column blocks, tiles
+    int ncb, tiles, total;  // column blocks, tiles, tiles x splits
+    int split_chunks;       // kOut: chunks of a split of the contraction (all of them: one split)
+    float* part;            // kOut with several splits: their sums [split][M][ldp]
+    int ldp;
     const char* a[kSeg];
     const char* b[kSeg];
-    const char* b1[6];   // kSwiGLU: the up matrix
+    const char* b1[kSeg];  // kSwiGLU: the up matrix
     // kOut: rows [0, split) to out, rows [split_at, ...) to out1 at row - split_at (split_at >= split)
     void* out;
     void* out1;
@@ -182,8 +185,10 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     const int local = blockIdx.x / 8;
     const int item = (blockIdx.x % 8) * per + local;
     if (local >= per || item >= p.total) return;
-    const int m0 = (item / p.ncb) * TM;
-    const int n0 = (item % p.ncb) * (DUAL ? TN / 2 : TN);
+    // splits slowest: tiles of one split, which run together, share their operands
+    const int split = EPI == kOut ? item / p.tiles : 0, tile = EPI == kOut ? item % p.tiles : item;
+    const int m0 = (tile / p.ncb) * TM;
+    const int n0 = (tile % p.ncb) * (DUAL ? TN / 2 : TN);
 
     SA sa;
     SB sb;
@@ -200,11 +205,17 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     // KC offsets count rows from the tile, MC offsets columns from the matrix: see Stage::init
     const unsigned lds0 = (unsigned)(size_t)(lds_ptr_t)&lds[0][0];
     const int cps = (max(p.ka, p.kb) + kChunk - 1) / kChunk;  // chunks per segment
-    const int chunks = cps * p.nseg;
+    int chunks = cps * p.nseg;
 
     // the next chunk to load: segment and place in it
     int seg = 0, at = 0;
-    const char *pa = p.a[0] + (AMC ? 0 : a_tile), *pb = (DUAL && wave >= 2 ? p.b1[0] : p.b[0]) + (BMC ? 0 : b_tile);
+    if constexpr (EPI == kOut) {
+        const int first = split * p.split_chunks;
+        chunks = min(p.split_chunks, chunks - first);
+        if (first > 0) seg = first / cps, at = (first - seg * cps) * kChunk;
+    }
+    const char *pa = p.a[seg] + (AMC ? 0 : a_tile) + (at / kChunk) * sa.step,
+               *pb = (DUAL && wave >= 2 ? p.b1[seg] : p.b[seg]) + (BMC ? 0 : b_tile) + (at / kChunk) * sb.step;
     auto load = [&](int st, int j) {
         const unsigned base = lds0 + st * (SA::BYTES + SB::BYTES);
         if (j < DA) {
@@ -227,7 +238,7 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
             ++seg;
             at = 0;
             pa = p.a[seg] + (AMC ? 0 : a_tile);
-            pb = (DUAL && wave >= 2 ? p.b1[seg % 6] : p.b[seg]) + (BMC ? 0 : b_tile);
+            pb = (DUAL && wave >= 2 ? p.b1[seg] : p.b[seg]) + (BMC ? 0 : b_tile);
         }
     };
 
@@ -296,6 +307,19 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     // block (i, j): row 16 i + lane % 16, columns 16 j + 4 g .. + 3
     const int g4 = 4 * (lane >> 4);
     if constexpr (EPI == kOut) {
+        if (p.part != nullptr) {
+            float* part = p.part + (long long)split * p.M * p.ldp;
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const int m = m0 + wr * 16 * MB + 16 * i + (lane & 15);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    const int n = n0 + wc * 16 * NB + 16 * j + g4;
+                    if (m < p.M && n < p.ldp) *(f32x4*)(part + (long long)m * p.ldp + n) = acc[i][j];
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
             const int m = m0 + wr * 16 * MB + 16 * i + (lane & 15);
@@ -514,24 +538,77 @@ __global__ __launch_bounds__(512) void swiglu_few_kernel(FewArgs p) {
     }
 }
 
-// Rows of any width to planes of bf16 terms whose rows are a multiple of 8 wide, zeros behind the last column.
-template <bool F32>
-__global__ __launch_bounds__(256) void swiglu_pack_kernel(const void* src, int cols, int ld, long long pieces,
-                                                          unsigned short* dst, long long plane) {
-    const int per = ld / 8;
-    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < pieces; e += (long long)gridDim.x * 256) {
-        const long long row = e / per;
-        const int c = (int)(e - row * per) * 8;
-        float v[2][4];
+// Sums of the splits, in order, to the output.
+__global__ __launch_bounds__(256) void swiglu_sum_kernel(TileArgs p, int splits) {
+    const int per = p.ldp / 4;
+    const long long total = (long long)p.M * per, plane = (long long)p.M * p.ldp;
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
+        const int m = (int)(e / per), n = (int)(e - (long long)m * per) * 4;
+        const float* at = p.part + (long long)m * p.ldp + n;
+        f32x4 v = *(const f32x4*)at;
+        for (int s = 1; s < splits; ++s) v = v + *(const f32x4*)(at + s * plane);
+        const bool first = m < p.split;
+        if (!first && m < p.split_at) continue;
+        void* o = first ? p.out : p.out1;
+        const long long d = (long long)(first ? m : m - p.split_at) * p.ldo + n;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const long long at = row * cols + c + i;
-            v[i / 4][i % 4] = c + i >= cols ? 0.0f
-                              : F32         ? ((const float*)src)[at]
-                                            : bf16_to_f32(((const unsigned short*)src)[at]);
+        for (int q = 0; q < 4; ++q)
+            if (n + q < p.N) {
+                if (p.f32) ((float*)o)[d + q] = v[q];
+                else ((unsigned short*)o)[d + q] = f32_to_bf16_rne(v[q]);
+            }
+    }
+}
+
+// Tensors of rows of any width to planes of bf16 terms whose rows are a multiple of 8 wide, zeros behind the last
+// column: up to five tensors a launch, 8 values a thread.
+struct PackArgs {
+    int n;
+    long long pieces;  // of all tensors
+    struct {
+        const void* src;
+        unsigned short* dst;
+        long long end, plane;  // pieces up to this tensor's last one, elements between planes
+        int cols, ld;
+    } t[5];
+};
+template <bool F32>
+__global__ __launch_bounds__(256) void swiglu_pack_kernel(PackArgs a) {
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < a.pieces; e += (long long)gridDim.x * 256) {
+        int k = 0;
+        while (e >= a.t[k].end) ++k;
+        const auto& t = a.t[k];
+        const long long i = e - (k > 0 ? a.t[k - 1].end : 0);
+        const int per = t.ld / 8;
+        const long long row = i / per;
+        const int c = (int)(i - row * per) * 8;
+        const size_t at = (size_t)row * t.cols + c;
+        Piece<F32> v[F32 ? 2 : 1];
+#pragma unroll
+        for (int q = 0; q < (F32 ? 2 : 1); ++q) {
+            if (c + 8 <= t.cols) v[q].load(t.src, at + 4 * q);
+            else v[q].load_end(t.src, at + 4 * q, t.cols - c - 4 * q);
         }
-        put_terms(dst + row * ld + c, plane, F32 ? 3 : 1, v[0]);
-        put_terms(dst + row * ld + c + 4, plane, F32 ? 3 : 1, v[1]);
+        unsigned short* dst = t.dst + row * t.ld + c;
+        if constexpr (F32) {
+            // the terms of eight values, a plane's 16 bytes at a time
+            float r[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) r[q] = v[q / 4].f[q % 4];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                unsigned d[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    d[q] = pack_bf16(r[2 * q], r[2 * q + 1]);
+                    r[2 * q] -= bf16_to_f32((unsigned short)(d[q] & 0xffff));
+                    r[2 * q + 1] -= bf16_to_f32((unsigned short)(d[q] >> 16));
+                }
+                *(uint4*)(dst + p * t.plane) = make_uint4(d[0], d[1], d[2], d[3]);
+            }
+        } else {
+            *(uint4*)dst = v[0].u;
+        }
     }
 }
 
@@ -541,44 +618,44 @@ constexpr int kTermA[6] = {2, 0, 1, 1, 0, 0};
 constexpr int kTermB[6] = {0, 2, 1, 0, 1, 0};
 
 inline int up8(int v) { return (v + 7) / 8 * 8; }
+inline int up4(int v) { return (v + 3) / 4 * 4; }
 
-// An operand as planes of bf16: the tensor itself, or its packed copy in the workspace.
+// An operand as planes of bf16 terms.
 struct Operand {
     const char* p;
     int ld;
     long long plane;  // bytes
 };
 
-// Parts of a workspace; dry: sizes only, nothing is launched.
+// Parts of a workspace, and the tensors to be packed into them; dry: sizes only, nothing is launched.
 struct Carve {
     char* base;
     bool dry;
+    int act;
     size_t used = 0;
+    PackArgs packs{};
     char* take(size_t bytes) {
         char* r = dry ? nullptr : base + used;
         used += align_up(bytes, 256);
         return r;
     }
+    // rows x cols as an operand: itself, where a row is whole 16-byte pieces of bf16
+    Operand operand(const void* t, long long rows, int cols) {
+        if (act == YVMOE_ACT_BF16 && cols % 8 == 0) return {(const char*)t, cols, 0};
+        const int ld = up8(cols);
+        char* dst = take((size_t)rows * ld * 2 * (act == YVMOE_ACT_F32 ? 3 : 1));
+        const long long pieces = rows * (ld / 8);
+        packs.pieces += pieces;
+        packs.t[packs.n++] = {t, (unsigned short*)dst, packs.pieces, rows * ld, cols, ld};
+        return {dst, ld, rows * ld * 2};
+    }
+    void pack(hipStream_t st) const {
+        if (packs.pieces == 0) return;
+        const unsigned blocks = (unsigned)std::min<long long>((packs.pieces + 255) / 256, 1 << 16);
+        if (act == YVMOE_ACT_F32) swiglu_pack_kernel<true><<<blocks, 256, 0, st>>>(packs);
+        else swiglu_pack_kernel<false><<<blocks, 256, 0, st>>>(packs);
+    }
 };
-
-inline bool needs_pack(int act, int cols) { return act == YVMOE_ACT_F32 || cols % 8 != 0; }
-inline size_t pack_bytes(int act, long long rows, int cols) {
-    return (size_t)rows * up8(cols) * 2 * (act == YVMOE_ACT_F32 ? 3 : 1);
-}
-
-Operand operand(const void* t, int act, long long rows, int cols, Carve& ws, hipStream_t st) {
-    if (!needs_pack(act, cols)) return {(const char*)t, cols, 0};
-    char* dst = ws.take(pack_bytes(act, rows, cols));
-    const Operand o{dst, up8(cols), (long long)rows * up8(cols) * 2};
-    if (ws.dry || rows == 0) return o;
-    const long long pieces = rows * (up8(cols) / 8);
-    const unsigned blocks = (unsigned)std::min<long long>((pieces + 255) / 256, 16384);
-    if (act == YVMOE_ACT_F32)
-        swiglu_pack_kernel<true><<<blocks, 256, 0, st>>>(t, cols, o.ld, pieces, (unsigned short*)dst, o.plane / 2);
-    else
-        swiglu_pack_kernel<false><<<blocks, 256, 0, st>>>(t, cols, o.ld, pieces, (unsigned short*)dst, o.plane / 2);
-    return o;
-}
 
 // Adds the operand pairs of A · Bᵀ (with b1: gate and up) to a launch.
 void add_product(TileArgs& p, int act, const Operand& a, const Operand& b, const Operand* b1 = nullptr) {
@@ -594,22 +671,66 @@ void add_product(TileArgs& p, int act, const Operand& a, const Operand& b, const
     p.ldb = b.ld;
 }
 
+// Tile and number of splits of the contraction for M x N outputs (kSwiGLU: N twice the columns of h) of `chunks`
+// chunks: the least of an estimate. A CU's work-group takes `alone` us a chunk when it runs by itself and `shared` us of
+// the CU's time beside others (measured: 256 1.45 and 1.79 under full load, 128 0.84 and 0.42 to 0.60, 64 0.63 and
+// 0.28 to 0.34); splits cost a launch and their sums' traffic.
+struct Plan {
+    int tile, splits;
+};
+Plan plan_of(int M, int N, int chunks, bool may_split) {
+    static const struct { int tile; float alone, shared; } kinds[3] = {{256, 1.6f, 1.75f}, {128, 0.84f, 0.5f}, {64, 0.63f, 0.3f}};
+    Plan best{256, 1};
+    float least = 1e30f;
+    for (const auto& k : kinds) {
+        const long long tiles = (long long)((M + k.tile - 1) / k.tile) * ((N + k.tile - 1) / k.tile);
+        for (int s = 1; s <= (may_split ? 16 : 1) && (s == 1 || chunks / s >= 4); ++s) {
+            const float per_cu = (float)((tiles * s + 255) / 256);
+            const int len = (chunks + s - 1) / s;
+            float us = std::max(k.alone, per_cu * k.shared) * len;
+            if (s > 1) us += 4.0f + (float)s * M * N * 8.0f / 4e6f;
+            if (us < least) least = us, best = {k.tile, s};
+        }
+    }
+    // splits of whole chunks: as many as are not empty
+    best.splits = ceil_div(chunks, ceil_div(std::max(chunks, 1), best.splits));
+    best.splits = std::max(best.splits, 1);
+    return best;
+}
+
+inline int chunks_of(const TileArgs& p) { return ceil_div(std::max(p.ka, p.kb), kChunk) * p.nseg; }
+// Bytes of the partial sums of an M x N output.
+size_t part_bytes(int M, int N, int k, int nseg) {
+    const Plan q = plan_of(M, N, ceil_div(k, kChunk) * nseg, true);
+    return q.splits > 1 ? (size_t)q.splits * M * up4(N) * 4 : 0;
+}
+
 template <int EPI, bool AMC, bool BMC, int MB, int NB>
-void tile_grid(TileArgs p, hipStream_t st) {
+void tile_grid(TileArgs p, int splits, hipStream_t st) {
     const int cols = EPI == kSwiGLU ? 16 * NB : 32 * NB;
     p.ncb = ceil_div(p.N, cols);
-    p.total = ceil_div(p.M, 32 * MB) * p.ncb;
+    p.tiles = ceil_div(p.M, 32 * MB) * p.ncb;
+    p.total = p.tiles * splits;
     swiglu_tile_kernel<EPI, AMC, BMC, MB, NB><<<(unsigned)(ceil_div(p.total, 8) * 8), 256, 0, st>>>(p);
 }
 
 template <int EPI, bool AMC, bool BMC>
-void tile_launch(const TileArgs& p, hipStream_t st) {
+void tile_launch(TileArgs p, float* part, hipStream_t st) {
     if (p.M <= 0 || p.N <= 0) return;
-    const long long cols = EPI == kSwiGLU ? 2ll * p.N : p.N;
-    auto tiles = [&](int t) { return ((p.M + t - 1) / t) * ((cols + t - 1) / t); };
-    if (tiles(256) >= 192) tile_grid<EPI, AMC, BMC, 8, 8>(p, st);
-    else if (tiles(128) >= 192) tile_grid<EPI, AMC, BMC, 4, 4>(p, st);
-    else tile_grid<EPI, AMC, BMC, 2, 2>(p, st);
+    const int chunks = chunks_of(p);
+    const Plan q = plan_of(p.M, EPI == kSwiGLU ? 2 * p.N : p.N, chunks, EPI == kOut);
+    p.split_chunks = ceil_div(std::max(chunks, 1), q.splits);
+    if (q.splits > 1) {
+        p.part = part;
+        p.ldp = up4(p.N);
+    }
+    if (q.tile == 256) tile_grid<EPI, AMC, BMC, 8, 8>(p, q.splits, st);
+    else if (q.tile == 128) tile_grid<EPI, AMC, BMC, 4, 4>(p, q.splits, st);
+    else tile_grid<EPI, AMC, BMC, 2, 2>(p, q.splits, st);
+    if (q.splits > 1) {
+        const long long quads = (long long)p.M * (p.ldp / 4);
+        swiglu_sum_kernel<<<(unsigned)std::min<long long>((quads + 255) / 256, 8192), 256, 0, st>>>(p, q.splits);
+    }
 }
 
 constexpr int kFewRows = 64;
@@ -630,7 +751,7 @@ size_t swiglu_saved_bytes(int N, int F) { return (size_t)2 * N * up8(F) * 4; }
 int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weights* w, float* saved, void* out,
                           char* ws, size_t* bytes, hipStream_t st) {
     const int H = w->hidden, F = w->ffn, F8 = up8(F), planes = act == YVMOE_ACT_F32 ? 3 : 1;
-    Carve c{ws, bytes != nullptr};
+    Carve c{ws, bytes != nullptr, act};
     if (N <= kFewRows) {
         const bool f32 = act == YVMOE_ACT_F32;
         void* h = c.take((size_t)N * F8 * (f32 ? 4 : 2));
@@ -643,12 +764,14 @@ int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weig
         YV_LAUNCH_CHECK("swiglu_forward");
         return YVMOE_OK;
     }
-    const Operand ox = operand(x, act, N, H, c, st), og = operand(w->w_gate, act, F, H, c, st),
-                  ou = operand(w->w_up, act, F, H, c, st), od = operand(w->w_down, act, H, F, c, st);
+    const Operand ox = c.operand(x, N, H), og = c.operand(w->w_gate, F, H), ou = c.operand(w->w_up, F, H),
+                  od = c.operand(w->w_down, H, F);
     const long long plane = (long long)N * F8;
     unsigned short* h = (unsigned short*)c.take((size_t)plane * 2 * planes);
+    float* part = (float*)c.take(part_bytes(N, H, F8, planes == 3 ? 6 : 1));
     if (bytes != nullptr) *bytes = c.used;
     if (c.dry || N == 0) return YVMOE_OK;
+    c.pack(st);
     TileArgs p{};
     p.M = N;
     p.N = F;
@@ -659,7 +782,7 @@ int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weig
     p.plane_h = plane;
     p.gu = saved;
     p.ldh = F8;
-    tile_launch<kSwiGLU, false, false>(p, st);
+    tile_launch<kSwiGLU, false, false>(p, nullptr, st);
     TileArgs q{};
     q.M = N;
     q.N = H;
@@ -669,7 +792,7 @@ int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weig
     q.ldo = H;
     q.split = q.split_at = N;
     q.f32 = act == YVMOE_ACT_F32;
-    tile_launch<kOut, false, false>(q, st);
+    tile_launch<kOut, false, false>(q, part, st);
     YV_LAUNCH_CHECK("swiglu_forward");
     return YVMOE_OK;
 }
@@ -679,19 +802,23 @@ int swiglu_backward_launch(const void* dy, const void* x, const float* saved, in
                            size_t* bytes, hipStream_t st) {
     const int H = w->hidden, F = w->ffn, F8 = up8(F), planes = act == YVMOE_ACT_F32 ? 3 : 1;
     const int f32 = act == YVMOE_ACT_F32;
-    Carve c{ws, bytes != nullptr};
+    Carve c{ws, bytes != nullptr, act};
     const long long plane = (long long)N * F8;
-    const Operand ody = operand(dy, act, N, H, c, st), od = operand(w->w_down, act, H, F, c, st);
+    const Operand ody = c.operand(dy, N, H), od = c.operand(w->w_down, H, F);
     unsigned short* h = (unsigned short*)c.take((size_t)plane * 2 * planes);
     unsigned short* d = (unsigned short*)c.take((size_t)plane * 4 * planes);
     Operand ox{}, og{}, ou{};
-    if (c.dry || dwg != nullptr || dwu != nullptr) ox = operand(x, act, N, H, c, st);
+    if (c.dry || dwg != nullptr || dwu != nullptr) ox = c.operand(x, N, H);
     if (c.dry || dx != nullptr) {
-        og = operand(w->w_gate, act, F, H, c, st);
-        ou = operand(w->w_up, act, F, H, c, st);
+        og = c.operand(w->w_gate, F, H);
+        ou = c.operand(w->w_up, F, H);
     }
+    const int terms = f32 ? 6 : 1;
+    float* part = (float*)c.take(std::max({part_bytes(N, H, F8, 2 * terms), part_bytes(F8 + F, H, N, terms),
+                                           part_bytes(F, H, N, terms), part_bytes(H, F, N, terms)}));
     if (bytes != nullptr) *bytes = c.used;
     if (c.dry) return YVMOE_OK;
+    c.pack(st);
     const Operand oh{(const char*)h, F8, plane * 2}, odg{(const char*)d, 2 * F8, plane * 4},
         odu{(const char*)(d + F8), 2 * F8, plane * 4};
     TileArgs p{};
@@ -707,21 +834,27 @@ int swiglu_backward_launch(const void* dy, const void* x, const float* saved, in
     p.plane_d = plane * 2;
     p.gu = const_cast<float*>(saved);
     p.ldh = F8;
-    tile_launch<kGrad, false, true>(p, st);
+    tile_launch<kGrad, false, true>(p, nullptr, st);
     if (dx != nullptr) {
         TileArgs q{};
         q.M = N;
         q.N = H;
         q.ka = F8;
         q.kb = F;
-        // the smallest term products of both matrices first
         add_product(q, act, odg, og);
         add_product(q, act, odu, ou);
+        if (f32) {  // both matrices' smallest terms first
+            const TileArgs in = q;
+            for (int t = 0; t < 12; ++t) {
+                q.a[t] = in.a[t / 2 + 6 * (t & 1)];
+                q.b[t] = in.b[t / 2 + 6 * (t & 1)];
+            }
+        }
         q.out = dx;
         q.ldo = H;
         q.split = q.split_at = N;
         q.f32 = f32;
-        tile_launch<kOut, false, true>(q, st);
+        tile_launch<kOut, false, true>(q, part, st);
     }
     if (dwg != nullptr || dwu != nullptr) {
         const bool both = dwg != nullptr && dwu != nullptr;
@@ -736,7 +869,7 @@ int swiglu_backward_launch(const void* dy, const void* x, const float* saved, in
         q.split = F;
         q.split_at = both ? F8 : F;
         q.f32 = f32;
-        tile_launch<kOut, true, true>(q, st);
+        tile_launch<kOut, true, true>(q, part, st);
     }
     if (dwd != nullptr) {
         TileArgs q{};
@@ -748,7 +881,7 @@ int swiglu_backward_launch(const void* dy, const void* x, const float* saved, in
         q.ldo = F;
         q.split = q.split_at = H;
         q.f32 = f32;
-        tile_launch<kOut, true, true>(q, st);
+        tile_launch<kOut, true, true>(q, part, st);
     }
     YV_LAUNCH_CHECK("swiglu_backward");
     return YVMOE_OK;
