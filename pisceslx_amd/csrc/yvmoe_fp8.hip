@@ -52,47 +52,87 @@ __device__ __forceinline__ unsigned codes4(float a, float b, float c, float d, f
 __device__ __forceinline__ unsigned size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // ------------------------------------------------------------------ rows
-// 16 lanes a group of 128, 8 values a lane; rows ld apart. VEC: rows of whole 16-byte pieces at 16-byte addresses.
-template <bool F32, bool VEC>
-__global__ __launch_bounds__(256) void fp8_rows_kernel(const void* x, int N, int K, int ld, int groups,
+struct __attribute__((packed, aligned(2))) Any16 {  // 16 bytes at any address
+    unsigned v[4];
+};
+// Eight values from element `at` of a tensor, those from `left` on zero.
+template <bool F32>
+__device__ __forceinline__ void load8(const void* x, size_t at, int left, float (&v)[8]) {
+    if (left >= 8) {
+        if (F32) {
+            const Any16 a = *(const Any16*)((const float*)x + at), b = *(const Any16*)((const float*)x + at + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(a.v[i]), v[4 + i] = __uint_as_float(b.v[i]);
+        } else {
+            const Any16 a = *(const Any16*)((const unsigned short*)x + at);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32((unsigned short)(a.v[i / 2] >> 16 * (i & 1)));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = i >= left ? 0.0f : F32 ? ((const float*)x)[at + i] : bf16_to_f32(((const unsigned short*)x)[at + i]);
+    }
+}
+
+// Where h comes from: h itself (parts = 0), or g and u as sums of `parts` fp32 planes each, [parts][2][N][ld].
+struct Hidden {
+    const float* p;
+    int parts, ld;
+    long long plane;  // N ld
+};
+__device__ __forceinline__ void load8(const Hidden& h, size_t at, int left, float (&v)[8]) {
+    if (h.parts == 0) return load8<true>(h.p, at, left, v);
+    // columns behind the last one hold sums of zeros (ld is a multiple of 128)
+    f32x4 s[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) s[m][q] = *(const f32x4*)(h.p + m * h.plane + at + 4 * q);
+    for (int k = 1; k < h.parts; ++k)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) s[m][q] = s[m][q] + *(const f32x4*)(h.p + (2 * k + m) * h.plane + at + 4 * q);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i >= left ? 0.0f : silu(s[0][i / 4][i % 4]) * s[1][i / 4][i % 4];
+}
+
+// 16 lanes hold a group of 128, eight values each: its scale, and the lane's codes.
+__device__ __forceinline__ float quantize8(const float (&v)[8], uint2& codes) {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, size_bits(v[i]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 16));
+    const float s = scale_of(m);
+    codes = make_uint2(codes4(v[0], v[1], v[2], v[3], s), codes4(v[4], v[5], v[6], v[7], s));
+    return s;
+}
+
+enum Source { kCodes, kBf16, kF32, kHidden };
+// Values of row n, group b that the lane holds.
+template <int SRC>
+__device__ __forceinline__ void values8(const void* x, const Hidden& h, int n, int K, int b, int lane16, float (&v)[8]) {
+    const int k = b * kBlock + lane16 * 8;
+    if (SRC == kHidden) load8(h, (size_t)n * h.ld + k, K - k, v);
+    else load8<SRC == kF32>(x, (size_t)n * K + k, K - k, v);
+}
+
+// One pass over the rows, bound by memory.
+template <int SRC>
+__global__ __launch_bounds__(256) void fp8_rows_kernel(const void* x, Hidden h, int N, int K, int groups,
                                                        unsigned char* codes, float* scales) {
     const long long items = (long long)N * groups;
+    const int l = threadIdx.x & 15;
     for (long long it = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); it < items; it += (long long)gridDim.x * 16) {
         const int n = (int)(it / groups), b = (int)(it - (long long)n * groups);
-        const int k = b * kBlock + (threadIdx.x & 15) * 8;
-        const long long at = (long long)n * ld + k;
         float v[8];
-        if (VEC) {
-            if (k < K) {
-                if (F32) {
-                    const float4 lo = *(const float4*)((const float*)x + at);
-                    float4 hi = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (k + 4 < K) hi = *(const float4*)((const float*)x + at + 4);
-                    v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-                } else {
-                    const uint4 u = *(const uint4*)((const unsigned short*)x + at);
-                    const unsigned d[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32((unsigned short)(d[i / 2] >> 16 * (i & 1)));
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = k + i >= K ? 0.0f : F32 ? ((const float*)x)[at + i] : bf16_to_f32(((const unsigned short*)x)[at + i]);
-        }
-        unsigned m = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, size_bits(v[i]));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 16));
-        const float s = scale_of(m);
-        *(uint2*)(codes + ((long long)n * groups + b) * kBlock + (threadIdx.x & 15) * 8) =
-            make_uint2(codes4(v[0], v[1], v[2], v[3], s), codes4(v[4], v[5], v[6], v[7], s));
-        if ((threadIdx.x & 15) == 0) scales[(long long)b * N + n] = s;
+        values8<SRC>(x, h, n, K, b, l, v);
+        uint2 c;
+        const float s = quantize8(v, c);
+        *(uint2*)(codes + it * kBlock + l * 8) = c;
+        if (l == 0) scales[(long long)b * N + n] = s;
     }
 }
 
@@ -107,7 +147,11 @@ struct Fp8Args {
     const float* ws[2];            // [ceil(O / 128)][groups]
     const unsigned short* bias;    // [O] or NULL
     unsigned short* out;           // [N][O]
-    float* h;                      // kSwiGLU: [N][ldh], ldh = O rounded up to 128
+    const void* x;                 // few rows: rounded to 8 bits in the kernel, [N][K]
+    Hidden hidden;                 // or the rows' source
+    int K;
+    float* h;                      // kSwiGLU: [N][ldh], ldh = O rounded up to 128; or sums of g and u (Hidden)
+    int parts;                     // kSwiGLU, few rows: splits of the contraction (1: h itself)
     unsigned char* hq;             // or its codes [N][ldh] and scales [ldh / 128][N]
     float* hs;
     int ldh;
@@ -118,49 +162,103 @@ __device__ __forceinline__ uint4 load16(const char* p) { return *(const uint4*)p
 
 // Few rows (16 MR at most): a work-group of eight wavefronts owns 16 outputs (kSwiGLU: gate and up), the wavefronts
 // deal out the blocks of 128 contraction elements and add their sums in LDS, in order. Bound by the stream of the
-// weights, which go to registers in their stored order; rows come from L2.
-template <int EPI, int MR>
+// weights, which go to registers in their stored order, kAhead steps ahead. SRC: the rows' codes come from L2, or the
+// work-group makes them in LDS while its first weights are on their way (a launch and a round trip less; each
+// work-group repeats the work, so only for few values).
+template <int EPI, int MR, int SRC>
 __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Args p) {
     constexpr int NM = EPI == kSwiGLU ? 2 : 1;  // matrices
-    __shared__ f32x4 part[8][NM * MR][64];
+    constexpr int kAhead = MR == 1 ? 4 : 2;
+    extern __shared__ __attribute__((aligned(16))) unsigned char few_lds[];
+    f32x4(*part)[NM * MR][64] = (f32x4(*)[NM * MR][64])few_lds;
+    unsigned char* lcodes = few_lds + sizeof(f32x4) * 8 * NM * MR * 64;  // [N][pitch]
+    const int pitch = p.groups * kBlock + 16;
+    float* lscales = (float*)(lcodes + (size_t)p.N * pitch);             // [N][groups]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int blk = blockIdx.x;
+    const int blk = EPI == kSwiGLU ? blockIdx.x % p.blocks : blockIdx.x;
+    const int split = EPI == kSwiGLU ? blockIdx.x / p.blocks : 0, stride = EPI == kSwiGLU ? 8 * p.parts : 8;
     const int row = lane & 15;
+    struct Step {
+        Op8 w[NM], a[MR];
+        float s[MR], ws[NM];
+    } buf[kAhead];
+    // step t of the wavefront: block first + t stride
+    const int first = split * 8 + wave;
+    const int steps = first < p.groups ? (p.groups - first + stride - 1) / stride : 0;
+    auto load = [&](Step& q, int t) {
+        const int b = first + t * stride;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            const char* at = p.w[m] + ((long long)blk * p.groups + b) * 2048 + lane * 16;
+            q.w[m].u[0] = nt_load16(at);
+            q.w[m].u[1] = nt_load16(at + 1024);
+            q.ws[m] = p.ws[m][(long long)(blk >> 3) * p.groups + b];
+        }
+        if constexpr (SRC == kCodes) {
+#pragma unroll
+            for (int r = 0; r < MR; ++r) {
+                // rows past the last one read it again; their sums are not stored
+                const int n = min(16 * r + row, p.N - 1);
+                const char* at = p.codes + ((long long)n * p.groups + b) * kBlock + (lane >> 4) * 16;
+                q.a[r].u[0] = load16(at);
+                q.a[r].u[1] = load16(at + 64);
+                q.s[r] = p.scales[(long long)b * p.N + n];
+            }
+        }
+    };
     f32x4 acc[NM][MR];
 #pragma unroll
     for (int m = 0; m < NM; ++m)
 #pragma unroll
         for (int r = 0; r < MR; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int b = wave; b < p.groups; b += 8) {
-        Op8 w[NM], a[MR];
-        float s[MR];
-#pragma unroll
-        for (int m = 0; m < NM; ++m) {
-            const char* at = p.w[m] + ((long long)blk * p.groups + b) * 2048 + lane * 16;
-            w[m].u[0] = nt_load16(at);
-            w[m].u[1] = nt_load16(at + 1024);
+    auto add = [&](Step& q, int t) {
+        if constexpr (SRC != kCodes) {
+            const int b = first + t * stride, n = min(row, p.N - 1);
+            const unsigned char* at = lcodes + n * pitch + b * kBlock + (lane >> 4) * 16;
+            q.a[0].u[0] = *(const uint4*)at;
+            q.a[0].u[1] = *(const uint4*)(at + 64);
+            q.s[0] = lscales[n * p.groups + b];
         }
 #pragma unroll
-        for (int r = 0; r < MR; ++r) {
-            // rows past the last one are read as it is; their sums are not stored
-            const int n = min(16 * r + row, p.N - 1);
-            const char* at = p.codes + ((long long)n * p.groups + b) * kBlock + (lane >> 4) * 16;
-            a[r].u[0] = load16(at);
-            a[r].u[1] = load16(at + 64);
-            s[r] = p.scales[(long long)b * p.N + n];
-        }
-#pragma unroll
-        for (int m = 0; m < NM; ++m) {
-            const float ws = p.ws[m][(long long)(blk >> 3) * p.groups + b];
+        for (int m = 0; m < NM; ++m)
 #pragma unroll
             for (int r = 0; r < MR; ++r) {
-                const f32x4 d = mfma8(w[m], a[r]);
-                const float f = s[r] * ws;
+                const f32x4 d = mfma8(q.w[m], q.a[r]);
+                const float f = q.s[r] * q.ws[m];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[m][r][i] = fmaf(d[i], f, acc[m][r][i]);
             }
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (i < steps) load(buf[i], i);
+    if constexpr (SRC != kCodes) {
+        const int l = threadIdx.x & 15;
+        for (int it = threadIdx.x >> 4; it < p.N * p.groups; it += 32) {
+            const int n = it / p.groups, b = it - n * p.groups;
+            float v[8];
+            values8<SRC>(p.x, p.hidden, n, p.K, b, l, v);
+            uint2 c;
+            const float s = quantize8(v, c);
+            *(uint2*)(lcodes + n * pitch + b * kBlock + l * 8) = c;
+            if (l == 0) lscales[it] = s;
         }
+        __syncthreads();
     }
+    int t = 0;
+    for (; t + 2 * kAhead <= steps; t += kAhead)
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            add(buf[i], t + i);
+            load(buf[i], t + kAhead + i);
+        }
+    for (; t < steps; t += kAhead)
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (t + i < steps) {
+                add(buf[i], t + i);
+                if (t + kAhead + i < steps) load(buf[i], t + kAhead + i);
+            }
 #pragma unroll
     for (int m = 0; m < NM; ++m)
 #pragma unroll
@@ -178,10 +276,16 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Args p) {
     const int n = 16 * wave + row, o = blk * 16 + 4 * (lane >> 4);
     if (n >= p.N) return;
     if constexpr (EPI == kSwiGLU) {
-        f32x4 h;
+        const long long at = (long long)n * p.ldh + o, plane = (long long)p.N * p.ldh;
+        if (p.parts == 1) {
+            f32x4 h;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = silu(v[0][i]) * v[1][i];
-        *(f32x4*)(p.h + (long long)n * p.ldh + o) = h;
+            for (int i = 0; i < 4; ++i) h[i] = silu(v[0][i]) * v[NM - 1][i];
+            *(f32x4*)(p.h + at) = h;
+        } else {
+            *(f32x4*)(p.h + 2 * split * plane + at) = v[0];
+            *(f32x4*)(p.h + (2 * split + 1) * plane + at) = v[NM - 1];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -209,6 +313,12 @@ __device__ __forceinline__ void load_lds4(const void* base, unsigned off, unsign
     asm volatile("buffer_load_dword %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc_of(base)), "{m0}"(m0) : "memory");
 }
 
+constexpr int kBand = 8;
+
+// 16-byte piece c of a 128-byte row r lies at c ^ swizzle(r): the 16 lanes that read together, of two neighbouring lane
+// groups g and 16 rows, then lie in different banks.
+__device__ __forceinline__ int swizzle(int r) { return (r >> 1 & 3) | ((r ^ r >> 3) & 1) << 2; }
+
 // Tiles: WR x WC wavefronts of 16 MB rows x 16 NB columns each (kSwiGLU: the wavefront's first NB / 2 blocks are gate
 // columns, the others the up columns of the same h columns). A step is a block of 128 contraction elements: rows
 // (swizzled 128-byte lines), weights (stored order) and both scales go to LDS by direct loads, one step ahead of the
@@ -228,16 +338,20 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
     const int per = (p.total + 7) / 8, local = blockIdx.x / 8;
     const int item = (blockIdx.x % 8) * per + local;
     if (local >= per || item >= p.total) return;
-    const int m0 = (item / p.ncb) * TM;
-    const int n0 = (item % p.ncb) * (DUAL ? TN / 2 : TN);
+    // eight row blocks and all columns, row block fastest, then the next eight: the tiles that an XCD works on at a
+    // time (32 in a row) share 8 panels of rows and 4 of columns, not one and 32
+    const int band = item / (kBand * p.ncb), in = item - band * kBand * p.ncb;
+    const int height = min(kBand, (p.N + TM - 1) / TM - band * kBand);
+    const int m0 = (band * kBand + in % height) * TM;
+    const int n0 = (in / height) * (DUAL ? TN / 2 : TN);
     const long long ldx = (long long)p.groups * kBlock, ldw = (long long)p.groups * 2048;
 
-    // rows: line r = 8 blk + lane / 8, piece c at c ^ (r & 7) ^ (r >> 3 & 1)
+    // rows: line r = 8 blk + lane / 8, piece c at c ^ swizzle(r)
     unsigned a_off[DA], b_off[DB];
 #pragma unroll
     for (int j = 0; j < DA; ++j) {
         const int r = (wave * DA + j) * 8 + lane / 8;
-        const int c = (lane % 8) ^ (r & 7) ^ (r >> 3 & 1);
+        const int c = (lane % 8) ^ swizzle(r);
         a_off[j] = m0 + r < p.N ? (unsigned)(r * ldx + c * 16) : kNone;
     }
     // weights: piece q = half q & 1 of the tile's block q / 2; kSwiGLU: the tile's second half are up blocks
@@ -291,7 +405,7 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
 
     const int g = lane >> 4, r16 = lane & 15;
     const int ar = wr * 16 * MB + r16;
-    const int a_rd = ar * 128 + ((g ^ (ar & 7) ^ (ar >> 3 & 1)) << 4);  // the second piece: ^ 64
+    const int a_rd = ar * 128 + ((g ^ swizzle(ar)) << 4);  // the second piece: ^ 64
     // tile block of the wavefront's column block j
     auto block_of = [&](int j) { return DUAL ? (j < NB / 2 ? wc * (NB / 2) + j : TN / 32 + wc * (NB / 2) + j - NB / 2) : wc * NB + j; };
     f32x4 acc[MB][NB];
@@ -416,22 +530,33 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
 // ------------------------------------------------------------------ host
 inline int groups_of(int k) { return (k + kBlock - 1) / kBlock; }
 
-void rows_launch(const void* x, int act, int N, int K, int ld, void* codes, float* scales, hipStream_t st) {
+template <int SRC>
+void rows_launch(const void* x, const Hidden& h, int N, int K, void* codes, float* scales, hipStream_t st) {
     const int groups = groups_of(K);
     const unsigned blocks = (unsigned)std::min<long long>(((long long)N * groups + 15) / 16, 1 << 16);
-    const int piece = act == YVMOE_ACT_F32 ? 4 : 8;
-    const bool vec = (uintptr_t)x % 16 == 0 && K % piece == 0 && ld % piece == 0;
-    unsigned char* c = (unsigned char*)codes;
-    if (act == YVMOE_ACT_F32) {
-        if (vec) fp8_rows_kernel<true, true><<<blocks, 256, 0, st>>>(x, N, K, ld, groups, c, scales);
-        else fp8_rows_kernel<true, false><<<blocks, 256, 0, st>>>(x, N, K, ld, groups, c, scales);
-    } else {
-        if (vec) fp8_rows_kernel<false, true><<<blocks, 256, 0, st>>>(x, N, K, ld, groups, c, scales);
-        else fp8_rows_kernel<false, false><<<blocks, 256, 0, st>>>(x, N, K, ld, groups, c, scales);
-    }
+    fp8_rows_kernel<SRC><<<blocks, 256, 0, st>>>(x, h, N, K, groups, (unsigned char*)codes, scales);
 }
 
 constexpr int kFewRows = 64;
+
+// Rows whose codes the few-row kernel makes itself: at most three groups for 16 of its lanes, one after the other (1 x
+// 4096 x 4096: 5.2 us against 2.4 + 4.9 in two launches, 7 x 5000 x 3001, nine groups, 12.7 against 2.8 + 5.5), and
+// at most 16 MB read by all work-groups together.
+inline bool own_rows(int N, int K, int blocks, int bytes) {
+    return N <= 16 && (long long)N * groups_of(K) <= 96 && (long long)N * K * bytes * blocks <= 16 << 20;
+}
+// Splits of the contraction of g and u in the few-row kernel: where blocks of outputs leave CUs idle.
+inline int few_parts(int blocks, int groups) {
+    return std::max(1, std::min({4, (256 + blocks / 2) / blocks, groups / 8}));
+}
+
+template <int EPI, int MR, int SRC>
+void few_grid(const Fp8Args& p, hipStream_t st) {
+    const size_t lds = sizeof(f32x4) * 8 * (EPI == kSwiGLU ? 2 : 1) * MR * 64 +
+                       (SRC == kCodes ? 0 : (size_t)p.N * (p.groups * (kBlock + 4) + 16));
+    const unsigned grid = (unsigned)(p.blocks * (EPI == kSwiGLU ? p.parts : 1));
+    fp8_few_kernel<EPI, MR, SRC><<<grid, 512, lds, st>>>(p);
+}
 
 template <int EPI, int WR, int WC, int MB, int NB>
 void tile_grid(Fp8Args p, hipStream_t st) {
@@ -445,12 +570,14 @@ void tile_grid(Fp8Args p, hipStream_t st) {
 inline bool wide_tiles(int N, int cols) { return (long long)ceil_div(N, 256) * ceil_div(cols, 256) >= 160; }
 inline bool swiglu_codes(int N, int F) { return N > kFewRows && wide_tiles(N, 2 * F); }
 
+// Rows as codes.
 template <int EPI>
 void product_launch(const Fp8Args& p, hipStream_t st) {
     if (p.N <= kFewRows) {
-        if (p.N <= 16) fp8_few_kernel<EPI, 1><<<(unsigned)p.blocks, 512, 0, st>>>(p);
-        else if (p.N <= 32) fp8_few_kernel<EPI, 2><<<(unsigned)p.blocks, 512, 0, st>>>(p);
-        else fp8_few_kernel<EPI, 4><<<(unsigned)p.blocks, 512, 0, st>>>(p);
+        if (p.N <= 16) few_grid<EPI, 1, kCodes>(p, st);
+        else if (p.N <= 32) few_grid<EPI, 2, kCodes>(p, st);
+        else if (p.N <= 48) few_grid<EPI, 3, kCodes>(p, st);
+        else few_grid<EPI, 4, kCodes>(p, st);
     } else if (wide_tiles(p.N, EPI == kSwiGLU ? 2 * p.O : p.O)) {
         tile_grid<EPI, 4, 2, 4, 8>(p, st);
     } else {
@@ -463,6 +590,7 @@ Fp8Args product_of(const void* codes, const float* scales, int N, const yvmoe_fp
     p.codes = (const char*)codes;
     p.scales = scales;
     p.N = N;
+    p.K = w->in_features;
     p.O = w->out_features;
     p.groups = groups_of(w->in_features);
     p.blocks = ceil_div(w->out_features, 16);
@@ -477,7 +605,8 @@ inline size_t scales_bytes(int N, int K) { return align_up((size_t)N * groups_of
 }  // namespace
 
 int fp8_rows_launch(const void* x, int act, int N, int K, void* codes, float* scales, hipStream_t st) {
-    rows_launch(x, act, N, K, K, codes, scales, st);
+    if (act == YVMOE_ACT_F32) rows_launch<kF32>(x, Hidden{}, N, K, codes, scales, st);
+    else rows_launch<kBf16>(x, Hidden{}, N, K, codes, scales, st);
     YV_LAUNCH_CHECK("fp8 rows");
     return YVMOE_OK;
 }
@@ -497,13 +626,24 @@ int fp8_product_launch(const void* codes, const float* scales, int N, const yvmo
 int fp8_linear_launch(const void* x, int N, const yvmoe_fp8_matrix* w, const void* bias, void* out, char* ws,
                       hipStream_t st) {
     float* scales = (float*)(ws + codes_bytes(N, w->in_features));
-    rows_launch(x, YVMOE_ACT_BF16, N, w->in_features, w->in_features, ws, scales, st);
-    return fp8_product_launch(ws, scales, N, w, bias, out, st);
+    Fp8Args p = product_of(ws, scales, N, w);
+    p.bias = (const unsigned short*)bias;
+    p.out = (unsigned short*)out;
+    p.x = x;
+    if (own_rows(N, p.K, p.blocks, 2)) {
+        few_grid<kLinear, 1, kBf16>(p, st);
+    } else {
+        rows_launch<kBf16>(x, Hidden{}, N, p.K, ws, scales, st);
+        product_launch<kLinear>(p, st);
+    }
+    YV_LAUNCH_CHECK("fp8 linear");
+    return YVMOE_OK;
 }
 
 size_t fp8_swiglu_ws(int N, int H, int F) {
+    const int parts = N <= kFewRows ? few_parts(ceil_div(F, 16), groups_of(H)) : 1;
     return fp8_linear_ws(N, H) + fp8_linear_ws(N, F) +
-           (swiglu_codes(N, F) ? 0 : align_up((size_t)N * groups_of(F) * kBlock * 4, 256));
+           (swiglu_codes(N, F) ? 0 : align_up((size_t)(parts > 1 ? 2 * parts : 1) * N * groups_of(F) * kBlock * 4, 256));
 }
 
 int fp8_swiglu_launch(const void* x, int N, const yvmoe_fp8_matrix* gate, const yvmoe_fp8_matrix* up,
@@ -514,7 +654,6 @@ int fp8_swiglu_launch(const void* x, int N, const yvmoe_fp8_matrix* gate, const 
     char* hq = (char*)xs + scales_bytes(N, H);
     float* hs = (float*)(hq + codes_bytes(N, F));
     float* h = (float*)((char*)hs + scales_bytes(N, F));
-    rows_launch(x, YVMOE_ACT_BF16, N, H, H, xq, xs, st);
     Fp8Args p = product_of(xq, xs, N, gate);
     p.w[1] = (const char*)up->codes;
     p.ws[1] = (const float*)up->scales;
@@ -522,9 +661,26 @@ int fp8_swiglu_launch(const void* x, int N, const yvmoe_fp8_matrix* gate, const 
     p.h = h;
     p.hq = (unsigned char*)hq;
     p.hs = hs;
-    product_launch<kSwiGLU>(p, st);
-    if (!swiglu_codes(N, F)) rows_launch(h, YVMOE_ACT_F32, N, F, p.ldh, hq, hs, st);
-    return fp8_product_launch(hq, hs, N, down, nullptr, out, st);
+    p.x = x;
+    p.parts = N <= kFewRows ? few_parts(p.blocks, p.groups) : 1;
+    if (own_rows(N, H, p.blocks * p.parts, 2)) {
+        few_grid<kSwiGLU, 1, kBf16>(p, st);
+    } else {
+        rows_launch<kBf16>(x, Hidden{}, N, H, xq, xs, st);
+        product_launch<kSwiGLU>(p, st);
+    }
+    const Hidden hidden{h, p.parts > 1 ? p.parts : 0, p.ldh, (long long)N * p.ldh};
+    Fp8Args q = product_of(hq, hs, N, down);
+    q.out = (unsigned short*)out;
+    q.hidden = hidden;
+    if (own_rows(N, F, q.blocks, p.parts > 1 ? 8 * p.parts : 4)) {
+        few_grid<kLinear, 1, kHidden>(q, st);
+    } else {
+        if (!swiglu_codes(N, F)) rows_launch<kHidden>(nullptr, hidden, N, F, hq, hs, st);
+        product_launch<kLinear>(q, st);
+    }
+    YV_LAUNCH_CHECK("fp8 swiglu");
+    return YVMOE_OK;
 }
 
 }  // namespace yvmoe

@@ -27,6 +27,8 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4_t;
 constexpr int kSeg = 12;      // operand pairs of a launch: 6 term products x 2 matrices
 constexpr int kChunk = 64;    // contraction elements per LDS stage
 
+constexpr int kBand = 8;      // row blocks that neighbouring tiles share columns over
+
 enum Epi { kOut, kSwiGLU, kGrad };
 
 // Rows by contraction ("KC": the contraction index is contiguous) or contraction by rows ("MC").
@@ -85,8 +87,11 @@ __device__ __forceinline__ void put_terms(unsigned short* p, long long plane, in
     }
 }
 
+__device__ __forceinline__ int swizzle(int r) { return (r >> 1 & 3) | ((r ^ r >> 3) & 1) << 2; }
+
 // One operand's part of a stage: TW rows (or columns) of 64 contraction elements.
-// KC: [TW][64], 128-byte rows in 16-byte pieces, piece c of row r at c ^ (r & 7) ^ (r >> 3 & 1).
+// KC: [TW][64], 128-byte rows in 16-byte pieces, piece c of row r at c ^ swizzle(r): the 16 lanes that read together,
+//     of two neighbouring lane groups and 16 rows, then lie in different banks.
 // MC: [64][TW], rows of TW elements in 32-byte pairs, pair p of row k at p ^ f(k), f(k) = (k & 3) | (k >> 1 & 4)
 //     (64 wide: k & 3): the four rows that 16 lanes read together then lie in different banks.
 template <bool MC, int TW>
@@ -112,7 +117,7 @@ struct Stage {
                 off[j] = m < rows ? (unsigned)(((long long)k * ld + m) * 2) : kNone;
             } else {
                 const int r = blk * 8 + lane / 8;
-                const int c = (lane % 8) ^ (r & 7) ^ (r >> 3 & 1);
+                const int c = (lane % 8) ^ swizzle(r);
                 off[j] = row0 + r < rows ? (unsigned)((r * (long long)ld + c * 8) * 2) : kNone;
             }
         }
@@ -123,7 +128,7 @@ struct Stage {
         const int blk = wave * LOADS + j;
         if (MC) return blk * (512 / TW) + lane / (TW / 8);
         const int r = blk * 8 + lane / 8;
-        return ((lane % 8) ^ (r & 7) ^ (r >> 3 & 1)) * 8;
+        return ((lane % 8) ^ swizzle(r)) * 8;
     }
     // load j of the chunk that starts `left` elements before the operand's end
     __device__ __forceinline__ void load(int wave, int lane, int j, const char* at, int left, unsigned lds) const {
@@ -145,7 +150,7 @@ struct Reader {
             at = (8 * g + (i >> 2)) * TW * 2 + ((((r0 >> 4) ^ f)) << 5) + (i & 3) * 8;
         } else {
             const int r = r0 + i;
-            at = r * 128 + ((g ^ (r & 7) ^ (r >> 3 & 1)) << 4);
+            at = r * 128 + ((g ^ swizzle(r)) << 4);
         }
     }
     // blocks of 16 rows are counted from the wavefront's first, which is a multiple of their number
@@ -180,15 +185,19 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave >> 1, wc = wave & 1;
-    // tiles, column block fastest, in 8 contiguous ranges (one per XCD)
+    // tiles in 8 contiguous ranges (one per XCD)
     const int per = (p.total + 7) / 8;
     const int local = blockIdx.x / 8;
     const int item = (blockIdx.x % 8) * per + local;
     if (local >= per || item >= p.total) return;
     // splits slowest: tiles of one split, which run together, share their operands
     const int split = EPI == kOut ? item / p.tiles : 0, tile = EPI == kOut ? item % p.tiles : item;
-    const int m0 = (tile / p.ncb) * TM;
-    const int n0 = (tile % p.ncb) * (DUAL ? TN / 2 : TN);
+    // eight row blocks and all columns, row block fastest, then the next eight: the tiles that an XCD works on at a
+    // time (32 in a row) share 8 panels of rows and 4 of columns, not one and 32
+    const int band = tile / (kBand * p.ncb), in = tile - band * kBand * p.ncb;
+    const int height = min(kBand, (p.M + TM - 1) / TM - band * kBand);
+    const int m0 = (band * kBand + in % height) * TM;
+    const int n0 = (in / height) * (DUAL ? TN / 2 : TN);
 
     SA sa;
     SB sb;
