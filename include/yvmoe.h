@@ -472,8 +472,8 @@ int32_t yvmoe_quantize_fp8_rows(const void* x, int32_t act_dtype, int32_t n_rows
  *          columns past in_features are zero; 16-byte aligned
  *   scales [ceil(out/128)][ceil(in/128)] fp32
  *   pisceslx_amd/quant.py pack_fp8_linear() writes this order.
- * yvmoe_fp8_linear takes bf16 rows x [N][in] and rounds them to 8 bits first (yvmoe_quantize_fp8_rows, in the
- * workspace of yvmoe_fp8_linear_workspace_bytes, 16-byte aligned), yvmoe_fp8_linear_rows takes rows that are.
+ * yvmoe_fp8_linear takes bf16 rows x [N][in] and rounds them to 8 bits first (yvmoe_quantize_fp8_rows, in its
+ * workspace), yvmoe_fp8_linear_rows takes rows that are. Workspaces are 16-byte aligned (0 bytes: may be NULL).
  * bias [out] bf16 or NULL; out [N][out] bf16, 8-byte aligned. in_features, out_features from 1 to 2^20, n_rows from 0
  * to 2^24, n_rows x out_features up to 2^36. out and the workspace overlap no input.
  */
@@ -484,11 +484,12 @@ typedef struct {
     const float* scales;
 } yvmoe_fp8_matrix;
 
-size_t yvmoe_fp8_linear_workspace_bytes(int32_t n_rows, int32_t in_features);
+size_t yvmoe_fp8_linear_workspace_bytes(int32_t n_rows, int32_t in_features, int32_t out_features);
+size_t yvmoe_fp8_linear_rows_workspace_bytes(int32_t n_rows, int32_t in_features, int32_t out_features);
 int32_t yvmoe_fp8_linear(const void* x, int32_t n_rows, const yvmoe_fp8_matrix* weight, const void* bias, void* out,
                          void* workspace, size_t workspace_bytes, void* stream);
 int32_t yvmoe_fp8_linear_rows(const void* codes, const float* scales, int32_t n_rows, const yvmoe_fp8_matrix* weight,
-                              const void* bias, void* out, void* stream);
+                              const void* bias, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Gated feed-forward block on such weights: g = x gateᵀ, u = x upᵀ, h = silu(g) u, out = h downᵀ, each product as

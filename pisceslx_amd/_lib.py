@@ -64,6 +64,7 @@ EXPORTED_SYMBOLS = (
     "yvmoe_int4_linear",
     "yvmoe_quantize_fp8_rows",
     "yvmoe_fp8_linear_workspace_bytes",
+    "yvmoe_fp8_linear_rows_workspace_bytes",
     "yvmoe_fp8_linear",
     "yvmoe_fp8_linear_rows",
     "yvmoe_fp8_swiglu_workspace_bytes",
@@ -255,11 +256,13 @@ def _declare(l: ctypes.CDLL) -> None:
     l.yvmoe_quantize_fp8_rows.restype = i32
     l.yvmoe_quantize_fp8_rows.argtypes = [vp, i32, i32, i32, vp, vp, vp]
     l.yvmoe_fp8_linear_workspace_bytes.restype = sz
-    l.yvmoe_fp8_linear_workspace_bytes.argtypes = [i32, i32]
+    l.yvmoe_fp8_linear_workspace_bytes.argtypes = [i32, i32, i32]
+    l.yvmoe_fp8_linear_rows_workspace_bytes.restype = sz
+    l.yvmoe_fp8_linear_rows_workspace_bytes.argtypes = [i32, i32, i32]
     l.yvmoe_fp8_linear.restype = i32
     l.yvmoe_fp8_linear.argtypes = [vp, i32, mat, vp, vp, vp, sz, vp]
     l.yvmoe_fp8_linear_rows.restype = i32
-    l.yvmoe_fp8_linear_rows.argtypes = [vp, vp, i32, mat, vp, vp, vp]
+    l.yvmoe_fp8_linear_rows.argtypes = [vp, vp, i32, mat, vp, vp, vp, sz, vp]
     l.yvmoe_fp8_swiglu_workspace_bytes.restype = sz
     l.yvmoe_fp8_swiglu_workspace_bytes.argtypes = [i32, i32, i32]
     l.yvmoe_fp8_swiglu.restype = i32

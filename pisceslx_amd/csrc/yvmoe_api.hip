@@ -804,8 +804,12 @@ int32_t yvmoe_quantize_fp8_rows(const void* x, int32_t act_dtype, int32_t n_rows
     return fp8_rows_launch(x, act_dtype, n_rows, features, codes, scales, (hipStream_t)stream);
 }
 
-size_t yvmoe_fp8_linear_workspace_bytes(int32_t n_rows, int32_t in_features) {
-    return n_rows > 0 && in_features > 0 ? fp8_linear_ws(n_rows, in_features) : 0;
+size_t yvmoe_fp8_linear_workspace_bytes(int32_t n_rows, int32_t in_features, int32_t out_features) {
+    return n_rows > 0 && in_features > 0 && out_features > 0 ? fp8_linear_ws(n_rows, in_features, out_features) : 0;
+}
+
+size_t yvmoe_fp8_linear_rows_workspace_bytes(int32_t n_rows, int32_t in_features, int32_t out_features) {
+    return n_rows > 0 && in_features > 0 && out_features > 0 ? fp8_product_ws(n_rows, in_features, out_features) : 0;
 }
 
 int32_t yvmoe_fp8_linear(const void* x, int32_t n_rows, const yvmoe_fp8_matrix* weight, const void* bias, void* out,
@@ -816,7 +820,7 @@ int32_t yvmoe_fp8_linear(const void* x, int32_t n_rows, const yvmoe_fp8_matrix* 
     YV_REQUIRE(x && out && workspace, YVMOE_ERR_ARG, "NULL pointer");
     YV_REQUIRE(((uintptr_t)x | (uintptr_t)bias) % 2 == 0 && (uintptr_t)out % 8 == 0 && (uintptr_t)workspace % 16 == 0,
                YVMOE_ERR_ARG, "x and bias must be 2-byte, out 8-byte and the workspace 16-byte aligned");
-    const size_t need = fp8_linear_ws(n_rows, weight->in_features);
+    const size_t need = fp8_linear_ws(n_rows, weight->in_features, weight->out_features);
     YV_REQUIRE(workspace_bytes >= need, YVMOE_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes,
                need);
     const Range in{x, (size_t)n_rows * weight->in_features * 2}, b{bias, (size_t)weight->out_features * 2},
@@ -829,7 +833,7 @@ int32_t yvmoe_fp8_linear(const void* x, int32_t n_rows, const yvmoe_fp8_matrix* 
 }
 
 int32_t yvmoe_fp8_linear_rows(const void* codes, const float* scales, int32_t n_rows, const yvmoe_fp8_matrix* weight,
-                              const void* bias, void* out, void* stream) {
+                              const void* bias, void* out, void* workspace, size_t workspace_bytes, void* stream) {
     clear_error();
     if (const int rc = check_fp8_matrix(weight, n_rows, "weight")) return rc;
     if (n_rows == 0) return YVMOE_OK;
@@ -837,12 +841,18 @@ int32_t yvmoe_fp8_linear_rows(const void* codes, const float* scales, int32_t n_
     YV_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 4 == 0 && (uintptr_t)bias % 2 == 0 &&
                    (uintptr_t)out % 8 == 0,
                YVMOE_ERR_ARG, "codes must be 16-byte, scales 4-byte, bias 2-byte and out 8-byte aligned");
+    const size_t need = fp8_product_ws(n_rows, weight->in_features, weight->out_features);
+    YV_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), YVMOE_ERR_WORKSPACE,
+               "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
+    YV_REQUIRE((uintptr_t)workspace % 16 == 0, YVMOE_ERR_ARG, "the workspace must be 16-byte aligned");
     const size_t groups = ceil_div(weight->in_features, 128);
-    const Range o{out, (size_t)n_rows * weight->out_features * 2};
-    YV_REQUIRE(!o.overlaps({codes, groups * 128 * n_rows}) && !o.overlaps({scales, groups * 4 * n_rows}) &&
-                   !o.overlaps({bias, (size_t)weight->out_features * 2}) && !overlaps_fp8_matrix(o, weight),
-               YVMOE_ERR_ARG, "out overlaps an input");
-    return fp8_product_launch(codes, scales, n_rows, weight, bias, out, (hipStream_t)stream);
+    const Range o{out, (size_t)n_rows * weight->out_features * 2}, ws{workspace, need};
+    for (const Range& r : {o, ws})
+        YV_REQUIRE(!r.overlaps({codes, groups * 128 * n_rows}) && !r.overlaps({scales, groups * 4 * n_rows}) &&
+                       !r.overlaps({bias, (size_t)weight->out_features * 2}) && !overlaps_fp8_matrix(r, weight),
+                   YVMOE_ERR_ARG, "out or the workspace overlaps an input");
+    YV_REQUIRE(!o.overlaps(ws), YVMOE_ERR_ARG, "out overlaps the workspace");
+    return fp8_product_launch(codes, scales, n_rows, weight, bias, out, (char*)workspace, (hipStream_t)stream);
 }
 
 size_t yvmoe_fp8_swiglu_workspace_bytes(int32_t n_rows, int32_t hidden, int32_t ffn) {

@@ -151,11 +151,14 @@ struct Fp8Args {
     Hidden hidden;                 // or the rows' source
     int K;
     float* h;                      // kSwiGLU: [N][ldh], ldh = O rounded up to 128; or sums of g and u (Hidden)
-    int parts;                     // kSwiGLU, few rows: splits of the contraction (1: h itself)
+    int parts;                     // splits of the contraction
+    float* part;                   // kLinear with several: their sums [parts][N][ldp]
+    int ldp;
     unsigned char* hq;             // or its codes [N][ldh] and scales [ldh / 128][N]
     float* hs;
     int ldh;
-    int ncb, total;
+    int ncb, tiles, total;         // column blocks, tiles, tiles x splits
+    int len;                       // blocks of 128 contraction elements of a tile's split
 };
 
 __device__ __forceinline__ uint4 load16(const char* p) { return *(const uint4*)p; }
@@ -175,8 +178,7 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Args p) {
     const int pitch = p.groups * kBlock + 16;
     float* lscales = (float*)(lcodes + (size_t)p.N * pitch);             // [N][groups]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int blk = EPI == kSwiGLU ? blockIdx.x % p.blocks : blockIdx.x;
-    const int split = EPI == kSwiGLU ? blockIdx.x / p.blocks : 0, stride = EPI == kSwiGLU ? 8 * p.parts : 8;
+    const int blk = blockIdx.x % p.blocks, split = blockIdx.x / p.blocks, stride = 8 * p.parts;
     const int row = lane & 15;
     struct Step {
         Op8 w[NM], a[MR];
@@ -286,6 +288,8 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Args p) {
             *(f32x4*)(p.h + 2 * split * plane + at) = v[0];
             *(f32x4*)(p.h + (2 * split + 1) * plane + at) = v[NM - 1];
         }
+    } else if (p.parts > 1) {
+        *(f32x4*)(p.part + ((long long)split * p.N + n) * p.ldp + o) = v[0];
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -340,7 +344,8 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
     if (local >= per || item >= p.total) return;
     // eight row blocks and all columns, row block fastest, then the next eight: the tiles that an XCD works on at a
     // time (32 in a row) share 8 panels of rows and 4 of columns, not one and 32
-    const int band = item / (kBand * p.ncb), in = item - band * kBand * p.ncb;
+    const int split = item / p.tiles, tile = item - split * p.tiles;
+    const int band = tile / (kBand * p.ncb), in = tile - band * kBand * p.ncb;
     const int height = min(kBand, (p.N + TM - 1) / TM - band * kBand);
     const int m0 = (band * kBand + in % height) * TM;
     const int n0 = (in / height) * (DUAL ? TN / 2 : TN);
@@ -390,6 +395,10 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
         s_off = lane == 0 ? 0 : kNone;
     }
     const char* psc = (const char*)ps;
+    const int first = split * p.len, steps = min(p.len, p.groups - first);
+    pa += (long long)first * kBlock;
+    pb += (long long)first * 2048;
+    psc += first * s_step;
     const unsigned lds0 = (unsigned)(size_t)(lds_ptr_t)&lds[0][0];
     auto load = [&](int st) {
         const unsigned base = lds0 + st * STAGE;
@@ -414,14 +423,14 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     load(0);
-    for (int b = 0; b < p.groups; ++b) {
+    for (int b = 0; b < steps; ++b) {
         const int st = b & 1;
         // this wavefront's loads of step b have landed, and after the barrier everybody's, and step b - 1 is read
         __builtin_amdgcn_s_waitcnt(vm_only(0));
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (b + 1 < p.groups) load(st ^ 1);
+        if (b + 1 < steps) load(st ^ 1);
         const unsigned char* A = &lds[st][0];
         const unsigned char* B = A + A_BYTES;
         const float* S = (const float*)(B + B_BYTES);
@@ -453,6 +462,21 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
     }
 
     // block (i, j): row 16 i + lane % 16, columns 16 j + 4 g .. + 3
+    if (p.parts > 1) {
+        const int ld = DUAL ? p.ldh : p.ldp;
+        float* part = DUAL ? p.h + 2 * split * (long long)p.N * ld : p.part + split * (long long)p.N * ld;
+        constexpr int NH = DUAL ? NB / 2 : NB;
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            const int n = m0 + ar + 16 * i;
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const int o = n0 + (wc * NH + j % NH) * 16 + 4 * g;
+                if (n < p.N && o < ld) *(f32x4*)(part + (j / NH * (long long)p.N + n) * ld + o) = acc[i][j];
+            }
+        }
+        return;
+    }
     if constexpr (!DUAL) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
@@ -527,6 +551,24 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
     }
 }
 
+// Sums of the splits, in order, and the bias.
+__global__ __launch_bounds__(256) void fp8_sum_kernel(Fp8Args p) {
+    const int per = p.ldp / 4;
+    const long long total = (long long)p.N * per, plane = (long long)p.N * p.ldp;
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
+        const int n = (int)(e / per), o = (int)(e - (long long)n * per) * 4;
+        const float* at = p.part + (long long)n * p.ldp + o;
+        f32x4 v = *(const f32x4*)at;
+        for (int s = 1; s < p.parts; ++s) v = v + *(const f32x4*)(at + s * plane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (o + i < p.O) {
+                const float b = p.bias != nullptr ? bf16_to_f32(p.bias[o + i]) : 0.0f;
+                p.out[(long long)n * p.O + o + i] = f32_to_bf16_rne(v[i] + b);
+            }
+    }
+}
+
 // ------------------------------------------------------------------ host
 inline int groups_of(int k) { return (k + kBlock - 1) / kBlock; }
 
@@ -537,7 +579,9 @@ void rows_launch(const void* x, const Hidden& h, int N, int K, void* codes, floa
     fp8_rows_kernel<SRC><<<blocks, 256, 0, st>>>(x, h, N, K, groups, (unsigned char*)codes, scales);
 }
 
-constexpr int kFewRows = 64;
+// Each block of 16 outputs reads all rows from L2: with many blocks, tiles take over from 33 rows on (1024 x 16384: 64
+// rows 18.1 us, 65 in tiles 11.4; 4096 x 4096: 15.1 and 15.4).
+inline bool few_rows(int N, int blocks) { return N <= (blocks > 512 ? 32 : 64); }
 
 // Rows whose codes the few-row kernel makes itself: at most three groups for 16 of its lanes, one after the other (1 x
 // 4096 x 4096: 5.2 us against 2.4 + 4.9 in two launches, 7 x 5000 x 3001, nine groups, 12.7 against 2.8 + 5.5), and
@@ -545,43 +589,78 @@ constexpr int kFewRows = 64;
 inline bool own_rows(int N, int K, int blocks, int bytes) {
     return N <= 16 && (long long)N * groups_of(K) <= 96 && (long long)N * K * bytes * blocks <= 16 << 20;
 }
-// Splits of the contraction of g and u in the few-row kernel: where blocks of outputs leave CUs idle.
-inline int few_parts(int blocks, int groups) {
-    return std::max(1, std::min({4, (256 + blocks / 2) / blocks, groups / 8}));
+// Form of a product of N rows with `cols` weight rows (kSwiGLU: gate and up) over `groups` blocks of 128, and splits
+// of the contraction: the least of an estimate. Few rows: a block of 16 outputs is a work-group, whose eight
+// wavefronts take a step of 128 in `step` us, and splits pay their sums' launch (g and u: the pass over h, which is
+// there anyway). Tiles: a CU's work-group takes `alone` us a step by itself, `shared` us of the CU's time beside others.
+struct Plan {
+    int tile;    // rows of a tile, 0: few rows
+    int splits;
+    int len;     // steps of a split
+};
+Plan plan_of(int N, int cols, int groups, bool dual) {
+    Plan best{0, 1, groups};
+    const int blocks = ceil_div(cols, dual ? 32 : 16);
+    if (few_rows(N, blocks)) {
+        // enough work-groups for the CUs, at least a step for every wavefront; without a pass over h at least eight
+        best.splits = std::max(1, std::min({4, (256 + blocks / 2) / blocks, groups / (dual ? 8 : 32)}));
+        return best;
+    }
+    static const struct { int rows, cols; float alone, shared; } kinds[2] = {{256, 256, 2.1f, 2.2f}, {64, 128, 0.58f, 0.38f}};
+    float least = 1e30f;
+    for (const auto& k : kinds) {
+        const long long tiles = (long long)ceil_div(N, k.rows) * ceil_div(cols, k.cols);
+        const int most = k.rows == 256 && dual ? 1 : 16;  // 256 columns are a group of h: they go on as codes
+        for (int s = 1; s <= most && (s == 1 || groups / s >= 4); ++s) {
+            const int len = ceil_div(groups, s);
+            float us = std::max(k.alone, (float)((tiles * s + 255) / 256) * k.shared) * len;
+            if (s > 1) us += (dual ? 0.0f : 4.0f) + (float)s * N * cols * 8.0f / 4e6f;
+            if (us < least) least = us, best = {k.rows, ceil_div(groups, len), len};
+        }
+    }
+    return best;
+}
+inline bool swiglu_codes(const Plan& q) { return q.tile == 256; }  // h leaves the kernel as codes
+// Bytes of the sums of kLinear's splits.
+inline size_t part_bytes(int N, int O, int groups) {
+    const Plan q = plan_of(N, O, groups, false);
+    return q.splits > 1 ? align_up((size_t)q.splits * N * ceil_div(O, 16) * 16 * 4, 256) : 0;
 }
 
 template <int EPI, int MR, int SRC>
 void few_grid(const Fp8Args& p, hipStream_t st) {
     const size_t lds = sizeof(f32x4) * 8 * (EPI == kSwiGLU ? 2 : 1) * MR * 64 +
                        (SRC == kCodes ? 0 : (size_t)p.N * (p.groups * (kBlock + 4) + 16));
-    const unsigned grid = (unsigned)(p.blocks * (EPI == kSwiGLU ? p.parts : 1));
-    fp8_few_kernel<EPI, MR, SRC><<<grid, 512, lds, st>>>(p);
+    fp8_few_kernel<EPI, MR, SRC><<<(unsigned)(p.blocks * p.parts), 512, lds, st>>>(p);
 }
 
 template <int EPI, int WR, int WC, int MB, int NB>
 void tile_grid(Fp8Args p, hipStream_t st) {
     constexpr int TM = WR * 16 * MB, TN = WC * 16 * NB;
     p.ncb = ceil_div(p.O, EPI == kSwiGLU ? TN / 2 : TN);
-    p.total = ceil_div(p.N, TM) * p.ncb;
+    p.tiles = ceil_div(p.N, TM) * p.ncb;
+    p.total = p.tiles * p.parts;
     fp8_tile_kernel<EPI, WR, WC, MB, NB><<<(unsigned)(ceil_div(p.total, 8) * 8), 64 * WR * WC, 0, st>>>(p);
 }
 
-// Whether kSwiGLU writes codes of h (else h in fp32).
-inline bool wide_tiles(int N, int cols) { return (long long)ceil_div(N, 256) * ceil_div(cols, 256) >= 160; }
-inline bool swiglu_codes(int N, int F) { return N > kFewRows && wide_tiles(N, 2 * F); }
-
-// Rows as codes.
-template <int EPI>
-void product_launch(const Fp8Args& p, hipStream_t st) {
-    if (p.N <= kFewRows) {
-        if (p.N <= 16) few_grid<EPI, 1, kCodes>(p, st);
-        else if (p.N <= 32) few_grid<EPI, 2, kCodes>(p, st);
-        else if (p.N <= 48) few_grid<EPI, 3, kCodes>(p, st);
-        else few_grid<EPI, 4, kCodes>(p, st);
-    } else if (wide_tiles(p.N, EPI == kSwiGLU ? 2 * p.O : p.O)) {
-        tile_grid<EPI, 4, 2, 4, 8>(p, st);
-    } else {
-        tile_grid<EPI, 2, 2, 2, 4>(p, st);
+// Rows as codes, or (few rows, SRC) made into codes in the kernel; part: the workspace of kLinear's splits.
+template <int EPI, int SRC = kCodes>
+void product_launch(Fp8Args p, float* part, hipStream_t st) {
+    const Plan q = plan_of(p.N, EPI == kSwiGLU ? 2 * p.O : p.O, p.groups, EPI == kSwiGLU);
+    p.parts = q.splits;
+    p.len = q.len;
+    p.part = part;
+    p.ldp = p.blocks * 16;
+    if (SRC != kCodes) few_grid<EPI, 1, SRC>(p, st);
+    else if (q.tile == 0 && p.N <= 16) few_grid<EPI, 1, kCodes>(p, st);
+    else if (q.tile == 0 && p.N <= 32) few_grid<EPI, 2, kCodes>(p, st);
+    else if (q.tile == 0 && p.N <= 48) few_grid<EPI, 3, kCodes>(p, st);
+    else if (q.tile == 0) few_grid<EPI, 4, kCodes>(p, st);
+    else if (q.tile == 256) tile_grid<EPI, 4, 2, 4, 8>(p, st);
+    else tile_grid<EPI, 2, 2, 2, 4>(p, st);
+    if (EPI == kLinear && p.parts > 1) {
+        const long long quads = (long long)p.N * (p.ldp / 4);
+        fp8_sum_kernel<<<(unsigned)std::min<long long>((quads + 255) / 256, 8192), 256, 0, st>>>(p);
     }
 }
 
@@ -611,14 +690,15 @@ int fp8_rows_launch(const void* x, int act, int N, int K, void* codes, float* sc
     return YVMOE_OK;
 }
 
-size_t fp8_linear_ws(int N, int K) { return codes_bytes(N, K) + scales_bytes(N, K); }
+size_t fp8_product_ws(int N, int K, int O) { return part_bytes(N, O, groups_of(K)); }
+size_t fp8_linear_ws(int N, int K, int O) { return codes_bytes(N, K) + scales_bytes(N, K) + fp8_product_ws(N, K, O); }
 
 int fp8_product_launch(const void* codes, const float* scales, int N, const yvmoe_fp8_matrix* w, const void* bias,
-                       void* out, hipStream_t st) {
+                       void* out, char* ws, hipStream_t st) {
     Fp8Args p = product_of(codes, scales, N, w);
     p.bias = (const unsigned short*)bias;
     p.out = (unsigned short*)out;
-    product_launch<kLinear>(p, st);
+    product_launch<kLinear>(p, (float*)ws, st);
     YV_LAUNCH_CHECK("fp8 linear");
     return YVMOE_OK;
 }
@@ -626,24 +706,26 @@ int fp8_product_launch(const void* codes, const float* scales, int N, const yvmo
 int fp8_linear_launch(const void* x, int N, const yvmoe_fp8_matrix* w, const void* bias, void* out, char* ws,
                       hipStream_t st) {
     float* scales = (float*)(ws + codes_bytes(N, w->in_features));
+    float* part = (float*)((char*)scales + scales_bytes(N, w->in_features));
     Fp8Args p = product_of(ws, scales, N, w);
     p.bias = (const unsigned short*)bias;
     p.out = (unsigned short*)out;
     p.x = x;
     if (own_rows(N, p.K, p.blocks, 2)) {
-        few_grid<kLinear, 1, kBf16>(p, st);
+        product_launch<kLinear, kBf16>(p, part, st);
     } else {
         rows_launch<kBf16>(x, Hidden{}, N, p.K, ws, scales, st);
-        product_launch<kLinear>(p, st);
+        product_launch<kLinear>(p, part, st);
     }
     YV_LAUNCH_CHECK("fp8 linear");
     return YVMOE_OK;
 }
 
 size_t fp8_swiglu_ws(int N, int H, int F) {
-    const int parts = N <= kFewRows ? few_parts(ceil_div(F, 16), groups_of(H)) : 1;
-    return fp8_linear_ws(N, H) + fp8_linear_ws(N, F) +
-           (swiglu_codes(N, F) ? 0 : align_up((size_t)(parts > 1 ? 2 * parts : 1) * N * groups_of(F) * kBlock * 4, 256));
+    const Plan q = plan_of(N, 2 * F, groups_of(H), true);
+    const size_t h = (size_t)N * groups_of(F) * kBlock * 4;
+    return fp8_linear_ws(N, F, H) + codes_bytes(N, H) + scales_bytes(N, H) +
+           (swiglu_codes(q) ? 0 : align_up((q.splits > 1 ? 2 * q.splits : 1) * h, 256));
 }
 
 int fp8_swiglu_launch(const void* x, int N, const yvmoe_fp8_matrix* gate, const yvmoe_fp8_matrix* up,
@@ -653,7 +735,8 @@ int fp8_swiglu_launch(const void* x, int N, const yvmoe_fp8_matrix* gate, const 
     float* xs = (float*)(xq + codes_bytes(N, H));
     char* hq = (char*)xs + scales_bytes(N, H);
     float* hs = (float*)(hq + codes_bytes(N, F));
-    float* h = (float*)((char*)hs + scales_bytes(N, F));
+    float* part = (float*)((char*)hs + scales_bytes(N, F));
+    float* h = (float*)((char*)part + fp8_product_ws(N, F, H));
     Fp8Args p = product_of(xq, xs, N, gate);
     p.w[1] = (const char*)up->codes;
     p.ws[1] = (const float*)up->scales;
@@ -662,22 +745,22 @@ int fp8_swiglu_launch(const void* x, int N, const yvmoe_fp8_matrix* gate, const 
     p.hq = (unsigned char*)hq;
     p.hs = hs;
     p.x = x;
-    p.parts = N <= kFewRows ? few_parts(p.blocks, p.groups) : 1;
-    if (own_rows(N, H, p.blocks * p.parts, 2)) {
-        few_grid<kSwiGLU, 1, kBf16>(p, st);
+    const Plan plan = plan_of(N, 2 * F, p.groups, true);
+    if (own_rows(N, H, p.blocks * plan.splits, 2)) {
+        product_launch<kSwiGLU, kBf16>(p, nullptr, st);
     } else {
         rows_launch<kBf16>(x, Hidden{}, N, H, xq, xs, st);
-        product_launch<kSwiGLU>(p, st);
+        product_launch<kSwiGLU>(p, nullptr, st);
     }
-    const Hidden hidden{h, p.parts > 1 ? p.parts : 0, p.ldh, (long long)N * p.ldh};
+    const Hidden hidden{h, plan.splits > 1 ? plan.splits : 0, p.ldh, (long long)N * p.ldh};
     Fp8Args q = product_of(hq, hs, N, down);
     q.out = (unsigned short*)out;
     q.hidden = hidden;
-    if (own_rows(N, F, q.blocks, p.parts > 1 ? 8 * p.parts : 4)) {
-        few_grid<kLinear, 1, kHidden>(q, st);
+    if (own_rows(N, F, q.blocks, plan.splits > 1 ? 8 * plan.splits : 4)) {
+        product_launch<kLinear, kHidden>(q, part, st);
     } else {
-        if (!swiglu_codes(N, F)) rows_launch<kHidden>(nullptr, hidden, N, F, hq, hs, st);
-        product_launch<kLinear>(q, st);
+        if (!swiglu_codes(plan)) rows_launch<kHidden>(nullptr, hidden, N, F, hq, hs, st);
+        product_launch<kLinear>(q, part, st);
     }
     YV_LAUNCH_CHECK("fp8 swiglu");
     return YVMOE_OK;

@@ -499,9 +499,10 @@ int swiglu_backward_launch(const void* dy, const void* x, const float* saved, in
 
 // 8-bit floating point rows, linear layer and gated block (yvmoe_fp8.hip).
 int fp8_rows_launch(const void* x, int act, int N, int K, void* codes, float* scales, hipStream_t st);
+size_t fp8_product_ws(int N, int K, int O);
 int fp8_product_launch(const void* codes, const float* scales, int N, const yvmoe_fp8_matrix* w, const void* bias,
-                       void* out, hipStream_t st);
-size_t fp8_linear_ws(int N, int K);
+                       void* out, char* ws, hipStream_t st);
+size_t fp8_linear_ws(int N, int K, int O);
 int fp8_linear_launch(const void* x, int N, const yvmoe_fp8_matrix* w, const void* bias, void* out, char* ws,
                       hipStream_t st);
 size_t fp8_swiglu_ws(int N, int H, int F);

@@ -700,15 +700,15 @@ def fp8_linear(x, weight: PackedFp8Linear, bias: Optional[torch.Tensor] = None,
         raise ValueError(f"bias must be bfloat16 [{O}]")
     out = _fp8_out(out, (*lead, O), dev)
     l, w, N = _lib.lib(), weight.struct(), out.numel() // O
+    need = l.yvmoe_fp8_linear_rows_workspace_bytes if rows else l.yvmoe_fp8_linear_workspace_bytes
+    nbytes = need(N, K, O)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    tail = (N, ctypes.byref(w), _ptr(bias), out.data_ptr(), ws.data_ptr(), nbytes, _stream(dev))
     with _on(dev):
         if rows:
-            rc = l.yvmoe_fp8_linear_rows(x.codes.data_ptr(), x.scales.data_ptr(), N, ctypes.byref(w), _ptr(bias),
-                                         out.data_ptr(), _stream(dev))
+            rc = l.yvmoe_fp8_linear_rows(x.codes.data_ptr(), x.scales.data_ptr(), *tail)
         else:
-            nbytes = l.yvmoe_fp8_linear_workspace_bytes(N, K)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            rc = l.yvmoe_fp8_linear(x.data_ptr(), N, ctypes.byref(w), _ptr(bias), out.data_ptr(), ws.data_ptr(),
-                                    nbytes, _stream(dev))
+            rc = l.yvmoe_fp8_linear(x.data_ptr(), *tail)
     if rc:
         _lib.check(rc, "yvmoe_fp8_linear")
     return out
