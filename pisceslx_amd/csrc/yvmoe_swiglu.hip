@@ -27,34 +27,42 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4_t;
 constexpr int kSeg = 12;      // operand pairs of a launch: 6 term products x 2 matrices
 constexpr int kChunk = 64;    // contraction elements per LDS stage
 
+constexpr int kDirectRows = 1024;  // rows up to which fp32 weights are not packed
 constexpr int kBand = 8;      // row blocks that neighbouring tiles share columns over
+
+// Term products of an fp32 product, smallest first: (term of A, term of B).
+constexpr int kTermA[6] = {2, 0, 1, 1, 0, 0};
+constexpr int kTermB[6] = {0, 2, 1, 0, 1, 0};
 
 enum Epi { kOut, kSwiGLU, kGrad };
 
-// Rows by contraction ("KC": the contraction index is contiguous) or contraction by rows ("MC").
-struct TileArgs {
+// What becomes of a product's sums.
+struct Finish {
     int M, N;            // output rows and columns (kSwiGLU: columns of h)
-    int ka, kb;          // contraction elements of A and of B; beyond them both count as zero
-    int lda, ldb;        // elements between rows in memory
-    int nseg;
-    int ncb, tiles, total;  // column blocks, tiles, tiles x splits
-    int split_chunks;       // kOut: chunks of a split of the contraction (all of them: one split)
-    float* part;            // kOut with several splits: their sums [split][M][ldp]
+    float* part;         // with several splits their sums [split][M][ldp], kSwiGLU [split][2][M][ldp]
     int ldp;
-    const char* a[kSeg];
-    const char* b[kSeg];
-    const char* b1[kSeg];  // kSwiGLU: the up matrix
     // kOut: rows [0, split) to out, rows [split_at, ...) to out1 at row - split_at (split_at >= split)
     void* out;
     void* out1;
     int ldo, split, split_at, f32;
-    // kSwiGLU, kGrad: planes of bf16 terms (1, fp32: 3), elements between planes
-    int planes;
+    // kSwiGLU, kGrad: h [M][ldh] and d = dg, du [M][2 ldh] (Planes; elements between them), and g and u, which kSwiGLU
+    // may not have to keep
     long long plane_h, plane_d;
-    unsigned short* h;   // [planes][M][ldh]
-    unsigned short* d;   // [planes][M][2 ldh]: dg, then du
-    float* gu;           // [2][M][ldh], kSwiGLU may have none
+    char* h;
+    char* d;
+    float* gu;           // [2][M][ldh]
     int ldh;
+};
+// Operands in memory: rows by contraction ("KC": the contraction index is contiguous) or contraction by rows ("MC").
+struct TileArgs : Finish {
+    int ka, kb;          // contraction elements of A and of B; beyond them both count as zero
+    int lda, ldb;        // elements between rows in memory
+    int nseg;
+    int ncb, tiles, total;  // column blocks, tiles, tiles x splits
+    int split_chunks;       // chunks of a split of the contraction (all of them: one split)
+    const char* a[kSeg];
+    const char* b[kSeg];
+    const char* b1[kSeg];  // kSwiGLU: the up matrix
 };
 
 // s_waitcnt immediates (gfx9 encoding)
@@ -76,10 +84,19 @@ __device__ __forceinline__ void mfma_acc(f32x4& acc, const bf16x8& a, const bf16
 
 __device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
 
-// v as the sum of three bf16 numbers (one: v rounded), written to planes of p
-__device__ __forceinline__ void put_terms(unsigned short* p, long long plane, int planes, const float (&v)[4]) {
+// How h and d are stored: one bf16 plane (rounded), three (a value is the sum of three bf16 numbers), or fp32.
+enum Planes { kOne = 1, kThree = 3, kFp32 = 0 };
+// Four values to element e of h or d.
+template <int PL>
+__device__ __forceinline__ void put(char* base, long long e, long long plane, const float (&v)[4]) {
+    if (PL == kFp32) {
+        *(f32x4*)((float*)base + e) = f32x4{v[0], v[1], v[2], v[3]};
+        return;
+    }
+    unsigned short* p = (unsigned short*)base + e;
     float r[4] = {v[0], v[1], v[2], v[3]};
-    for (int t = 0; t < planes; ++t) {
+#pragma unroll
+    for (int t = 0; t < PL; ++t) {
         const unsigned lo = pack_bf16(r[0], r[1]), hi = pack_bf16(r[2], r[3]);
         *(uint2*)(p + t * plane) = make_uint2(lo, hi);
         r[0] -= bf16_to_f32((unsigned short)(lo & 0xffff)), r[1] -= bf16_to_f32((unsigned short)(lo >> 16));
@@ -87,53 +104,144 @@ __device__ __forceinline__ void put_terms(unsigned short* p, long long plane, in
     }
 }
 
-__device__ __forceinline__ int swizzle(int r) { return (r >> 1 & 3) | ((r ^ r >> 3) & 1) << 2; }
+// What becomes of four sums of row m, columns n .. n + 3.
+__device__ __forceinline__ void finish_out(const Finish& p, int m, int n, f32x4 v) {
+    const bool first = m < p.split;
+    if ((!first && m < p.split_at) || m >= p.M || n >= p.N) return;
+    void* o = first ? p.out : p.out1;
+    const long long e = (long long)(first ? m : m - p.split_at) * p.ldo + n;
+    if (n + 4 <= p.N && p.ldo % 4 == 0) {
+        if (p.f32) *(f32x4*)((float*)o + e) = v;
+        else *(uint2*)((unsigned short*)o + e) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (n + q < p.N) {
+                if (p.f32) ((float*)o)[e + q] = v[q];
+                else ((unsigned short*)o)[e + q] = f32_to_bf16_rne(v[q]);
+            }
+    }
+}
+// Columns from N to ldh are sums of zeros and written as such: they are operands of products.
+template <int PL>
+__device__ __forceinline__ void finish_swiglu(const Finish& p, int m, int n, f32x4 g, f32x4 u) {
+    if (m >= p.M || n >= p.ldh) return;
+    const long long e = (long long)m * p.ldh + n;
+    if (p.gu != nullptr) {
+        *(f32x4*)(p.gu + e) = g;
+        *(f32x4*)(p.gu + (long long)p.M * p.ldh + e) = u;
+    }
+    float h[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) h[q] = silu(g[q]) * u[q];
+    put<PL>(p.h, e, p.plane_h, h);
+}
+template <int PL>
+__device__ __forceinline__ void finish_grad(const Finish& p, int m, int n, f32x4 dh) {
+    if (m >= p.M || n >= p.ldh) return;
+    const long long e = (long long)m * p.ldh + n;
+    const f32x4 g = *(const f32x4*)(p.gu + e), u = *(const f32x4*)(p.gu + (long long)p.M * p.ldh + e);
+    float dg[4], du[4], h[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const float s = sigmoid(g[q]), a = g[q] * s;
+        h[q] = a * u[q];
+        du[q] = dh[q] * a;
+        dg[q] = dh[q] * u[q] * (s + a * (1.0f - s));
+    }
+    const long long ed = (long long)m * 2 * p.ldh + n;
+    put<PL>(p.d, ed, p.plane_d, dg);
+    put<PL>(p.d, ed + p.ldh, p.plane_d, du);
+    put<PL>(p.h, e, p.plane_h, h);
+}
+// Block AT of a wavefront and those after it. Written out by recursion: `#pragma unroll` gives up on bodies as long as
+// these, and the sums would then go through memory.
+template <int EPI, int PL, int MB, int NB, int AT = 0>
+__device__ __forceinline__ void finish_blocks(const Finish& p, const f32x4 (&acc)[MB][NB], int m, int n) {
+    constexpr int NH = EPI == kSwiGLU ? NB / 2 : NB, i = AT / NH, j = AT % NH;
+    if constexpr (EPI == kOut) finish_out(p, m + 16 * i, n + 16 * j, acc[i][j]);
+    else if constexpr (EPI == kGrad) finish_grad<PL>(p, m + 16 * i, n + 16 * j, acc[i][j]);
+    else finish_swiglu<PL>(p, m + 16 * i, n + 16 * j, acc[i][j], acc[i][j + NH]);
+    asm volatile("" ::: "memory");  // one block's addresses at a time
+    if constexpr (AT + 1 < MB * NH) finish_blocks<EPI, PL, MB, NB, AT + 1>(p, acc, m, n);
+}
+// A wavefront's blocks: (i, j) holds row m + 16 i, columns n + 16 j .. + 3 (kSwiGLU: of gate, then of up).
+template <int EPI, int PL, int MB, int NB>
+__device__ __forceinline__ void finish(const Finish& p, const f32x4 (&acc)[MB][NB], int m, int n, int split) {
+    constexpr int NH = EPI == kSwiGLU ? NB / 2 : NB;
+    if (p.part != nullptr) {
+        float* part = p.part + (long long)split * (EPI == kSwiGLU ? 2 : 1) * p.M * p.ldp;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const int r = m + 16 * i, c = n + 16 * (j % NH);
+                if (r < p.M && c < p.ldp) *(f32x4*)(part + (j / NH * (long long)p.M + r) * p.ldp + c) = acc[i][j];
+            }
+        return;
+    }
+    finish_blocks<EPI, PL>(p, acc, m, n);
+}
 
-// One operand's part of a stage: TW rows (or columns) of 64 contraction elements.
-// KC: [TW][64], 128-byte rows in 16-byte pieces, piece c of row r at c ^ swizzle(r): the 16 lanes that read together,
-//     of two neighbouring lane groups and 16 rows, then lie in different banks.
-// MC: [64][TW], rows of TW elements in 32-byte pairs, pair p of row k at p ^ f(k), f(k) = (k & 3) | (k >> 1 & 4)
-//     (64 wide: k & 3): the four rows that 16 lanes read together then lie in different banks.
-template <bool MC, int TW>
+// Of bf16, whose lane groups g read pieces g, and of fp32, where they read pieces 2 g.
+template <bool F32>
+__device__ __forceinline__ int swizzle(int r) {
+    return F32 ? (r ^ r >> 3 & 1) & 7 : (r >> 1 & 3) | ((r ^ r >> 3) & 1) << 2;
+}
+
+// One operand's part of a stage: TW rows (or columns) of a chunk, 64 contraction elements of bf16 or 32 of fp32.
+// KC: 128-byte rows in 16-byte pieces, piece c of row r at c ^ swizzle(r): the 16 lanes that read together, of two
+//     neighbouring lane groups and 16 rows, then lie in different banks.
+// MC: rows of TW elements, in groups of 16 elements (bf16: pairs of pieces, fp32: four), group p of row k at p ^ f(k).
+//     bf16: f(k) = (k & 3) | (k >> 1 & 4) (64 wide: k & 3), so that the four rows that 16 lanes read together lie in
+//     different banks; fp32: f(k) = k >> 3 & 3, the four lane groups' rows.
+template <bool MC, int TW, bool F32 = false>
 struct Stage {
-    static constexpr int BYTES = TW * kChunk * 2;
+    static constexpr int BYTES = TW * 128;
     static constexpr int LOADS = BYTES / 1024 / 4;  // of a wavefront
-    static constexpr int FM = TW >= 128 ? 7 : 3;
+    static constexpr int ES = F32 ? 4 : 2, CHUNK = 128 / ES, PE = 16 / ES;
+    static constexpr int ROW = TW * ES;             // MC: bytes of a row, pieces of a load's rows
+    static constexpr int RPL = ROW > 1024 ? 1 : 1024 / ROW, PPR = ROW / 16;
+    static_assert(ROW <= 1024, "a load holds whole rows");
     unsigned off[LOADS];
-    const char* base;
     long long step;  // bytes per chunk
 
+    __device__ __forceinline__ static int f(int k) {
+        return F32 ? k >> 3 & 3 : ((k & 3) | (k >> 1 & 4)) & (TW >= 128 ? 7 : 3);
+    }
+    // the first of the lane's elements in load j of a wavefront: row of the tile and contraction element
+    __device__ __forceinline__ static void place(int wave, int lane, int j, int& m, int& k) {
+        const int blk = wave * LOADS + j;
+        if (MC) {
+            constexpr int GP = 16 / PE;  // pieces of a group
+            const int piece = lane % PPR;
+            k = blk * RPL + lane / PPR;
+            m = ((piece / GP ^ f(k)) * GP + piece % GP) * PE;
+        } else {
+            m = blk * 8 + lane / 8;
+            k = ((lane % 8) ^ swizzle<F32>(m)) * PE;
+        }
+    }
     // row0: first row of the tile in the operand, rows: how many the operand has
     __device__ __forceinline__ void init(int wave, int lane, int row0, int rows, int ld) {
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
-            const int blk = wave * LOADS + j;
-            if (MC) {
-                constexpr int RPL = 512 / TW;  // contraction rows of a load
-                constexpr int PPR = TW / 8;    // 16-byte pieces of a row
-                const int k = blk * RPL + lane / PPR, piece = lane % PPR;
-                const int f = ((k & 3) | (k >> 1 & 4)) & FM;
-                const int m = row0 + ((((piece >> 1) ^ f) << 1 | (piece & 1)) << 3);
-                off[j] = m < rows ? (unsigned)(((long long)k * ld + m) * 2) : kNone;
-            } else {
-                const int r = blk * 8 + lane / 8;
-                const int c = (lane % 8) ^ swizzle(r);
-                off[j] = row0 + r < rows ? (unsigned)((r * (long long)ld + c * 8) * 2) : kNone;
-            }
+            int m, k;
+            place(wave, lane, j, m, k);
+            // KC offsets count rows from the tile, MC offsets columns from the matrix
+            const long long e = MC ? (long long)k * ld + row0 + m : (long long)m * ld + k;
+            off[j] = row0 + m < rows ? (unsigned)(e * ES) : kNone;
         }
-        step = MC ? (long long)kChunk * ld * 2 : kChunk * 2;
+        step = MC ? (long long)CHUNK * ld * ES : 128;
     }
-    // the lane's first contraction element of load j
-    __device__ __forceinline__ static int k_of(int wave, int lane, int j) {
-        const int blk = wave * LOADS + j;
-        if (MC) return blk * (512 / TW) + lane / (TW / 8);
-        const int r = blk * 8 + lane / 8;
-        return ((lane % 8) ^ swizzle(r)) * 8;
-    }
-    // load j of the chunk that starts `left` elements before the operand's end
-    __device__ __forceinline__ void load(int wave, int lane, int j, const char* at, int left, unsigned lds) const {
+    // load j of the chunk that starts `left` elements before the operand's end; `as`: the wavefront whose rows it takes
+    __device__ __forceinline__ void load(int wave, int as, int lane, int j, const char* at, int left, unsigned lds) const {
         unsigned o = off[j];
-        if (left < kChunk) o = k_of(wave, lane, j) < left ? o : kNone;
+        if (left < CHUNK) {
+            int m, k;
+            place(as, lane, j, m, k);
+            o = k < left ? o : kNone;
+        }
         load_lds(at, o, lds + (wave * LOADS + j) * 1024);
     }
 };
@@ -146,11 +254,11 @@ struct Reader {
     __device__ __forceinline__ void init(int lane, int r0) {
         const int g = lane >> 4, i = lane & 15;
         if (MC) {
-            const int f = ((i >> 2) | (g & 1) << 2) & Stage<MC, TW>::FM;
-            at = (8 * g + (i >> 2)) * TW * 2 + ((((r0 >> 4) ^ f)) << 5) + (i & 3) * 8;
+            const int k = 8 * g + (i >> 2);
+            at = k * TW * 2 + (((r0 >> 4) ^ Stage<MC, TW>::f(k)) << 5) + (i & 3) * 8;
         } else {
             const int r = r0 + i;
-            at = r * 128 + ((g ^ swizzle(r)) << 4);
+            at = r * 128 + ((g ^ swizzle<false>(r)) << 4);
         }
     }
     // blocks of 16 rows are counted from the wavefront's first, which is a multiple of their number
@@ -165,6 +273,48 @@ struct Reader {
         return *(const bf16x8*)(stage + (at ^ s << 6) + blk * 2048);
     }
 };
+// The same of fp32, whose chunk is one step, as three bf16 terms: cut off, not rounded, so that two take a mask and a
+// subtraction each, and all 24 bits are kept.
+template <bool MC, int TW>
+struct Reader32 {
+    int at;
+    __device__ __forceinline__ void init(int lane, int r0) {
+        const int g = lane >> 4, i = lane & 15;
+        if (MC) {
+            at = 8 * g * TW * 4 + (((r0 >> 4) ^ Stage<MC, TW, true>::f(8 * g)) << 6) + i * 4;
+        } else {
+            const int r = r0 + i;
+            at = r * 128 + (((2 * g) ^ swizzle<true>(r)) << 4);
+        }
+    }
+    __device__ __forceinline__ void read(const unsigned char* stage, int blk, float (&v)[8]) const {
+        if (MC) {
+            const unsigned char* p = stage + (at ^ blk << 6);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = *(const float*)(p + e * TW * 4);
+        } else {
+            const float4 lo = *(const float4*)(stage + at + blk * 2048), hi = *(const float4*)(stage + (at ^ 16) + blk * 2048);
+            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+        }
+    }
+    __device__ __forceinline__ static void terms(const float (&v)[8], bf16x8 (&t)[3]) {
+        union { unsigned u[4]; bf16x8 b; } f;
+        float r[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = v[e];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // the upper halves of two values
+                f.u[e] = __builtin_amdgcn_perm(__float_as_uint(r[2 * e + 1]), __float_as_uint(r[2 * e]), 0x07060302u);
+            t[k] = f.b;
+            if (k < 2) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[e] -= __uint_as_float(__float_as_uint(r[e]) & 0xffff0000u);
+            }
+        }
+    }
+};
 
 // One tile of 32 MB rows x 32 NB columns (kSwiGLU: 16 NB columns of h, gate and up) by four wavefronts in a
 // 2 x 2 grid, each 16 MB x 16 NB: MB x NB blocks of 16 x 16, fp32 sums in AGPRs (an MFMA in inline assembly
@@ -173,7 +323,7 @@ struct Reader {
 // halves with the next half's fragment reads and the loads of the chunk after next among them, one barrier
 // between the halves. The columns' operand is the MFMA's first, so that a lane holds four consecutive
 // columns of one row.
-template <int EPI, bool AMC, bool BMC, int MB, int NB>
+template <int EPI, int PL, bool AMC, bool BMC, int MB, int NB>
 __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     constexpr int TM = 32 * MB, TN = 32 * NB;
     constexpr int T = MB * NB, R = MB + NB;
@@ -191,7 +341,7 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     const int item = (blockIdx.x % 8) * per + local;
     if (local >= per || item >= p.total) return;
     // splits slowest: tiles of one split, which run together, share their operands
-    const int split = EPI == kOut ? item / p.tiles : 0, tile = EPI == kOut ? item % p.tiles : item;
+    const int split = item / p.tiles, tile = item - split * p.tiles;
     // eight row blocks and all columns, row block fastest, then the next eight: the tiles that an XCD works on at a
     // time (32 in a row) share 8 panels of rows and 4 of columns, not one and 32
     const int band = tile / (kBand * p.ncb), in = tile - band * kBand * p.ncb;
@@ -205,38 +355,26 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     // kSwiGLU: tile columns 0 .. TN / 2 - 1 are gate rows, the others the same up rows: wavefronts 0 and 1 load
     // the gate's half, 2 and 3 the up's
     sb.init(DUAL ? wave & 1 : wave, lane, n0, p.N, p.ldb);
-    if (DUAL) {
-        // a half is LOADS loads of two wavefronts: rows count from the half's start
-        static_assert(!DUAL || !BMC, "the forward pass reads weights row by row");
-    }
+    static_assert(!DUAL || !BMC, "the forward pass reads weights row by row");
     const long long a_tile = AMC ? (long long)m0 * 2 : (long long)m0 * p.lda * 2;
     const long long b_tile = BMC ? (long long)n0 * 2 : (long long)n0 * p.ldb * 2;
-    // KC offsets count rows from the tile, MC offsets columns from the matrix: see Stage::init
     const unsigned lds0 = (unsigned)(size_t)(lds_ptr_t)&lds[0][0];
     const int cps = (max(p.ka, p.kb) + kChunk - 1) / kChunk;  // chunks per segment
     int chunks = cps * p.nseg;
 
     // the next chunk to load: segment and place in it
     int seg = 0, at = 0;
-    if constexpr (EPI == kOut) {
-        const int first = split * p.split_chunks;
-        chunks = min(p.split_chunks, chunks - first);
-        if (first > 0) seg = first / cps, at = (first - seg * cps) * kChunk;
-    }
+    const int first = split * p.split_chunks;
+    chunks = min(p.split_chunks, chunks - first);
+    if (first > 0) seg = first / cps, at = (first - seg * cps) * kChunk;
     const char *pa = p.a[seg] + (AMC ? 0 : a_tile) + (at / kChunk) * sa.step,
                *pb = (DUAL && wave >= 2 ? p.b1[seg] : p.b[seg]) + (BMC ? 0 : b_tile) + (at / kChunk) * sb.step;
     auto load = [&](int st, int j) {
         const unsigned base = lds0 + st * (SA::BYTES + SB::BYTES);
         if (j < DA) {
-            sa.load(wave, lane, j, pa, p.ka - at, base);
+            sa.load(wave, wave, lane, j, pa, p.ka - at, base);
         } else {
-            if (DUAL) {
-                unsigned o = sb.off[j - DA];
-                if (p.kb - at < kChunk) o = SB::k_of(wave & 1, lane, j - DA) < p.kb - at ? o : kNone;
-                load_lds(pb, o, base + SA::BYTES + (wave * SB::LOADS + j - DA) * 1024);
-            } else {
-                sb.load(wave, lane, j - DA, pb, p.kb - at, base + SA::BYTES);
-            }
+            sb.load(wave, DUAL ? wave & 1 : wave, lane, j - DA, pb, p.kb - at, base + SA::BYTES);
         }
     };
     auto advance = [&]() {
@@ -313,86 +451,104 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     }
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
 
-    // block (i, j): row 16 i + lane % 16, columns 16 j + 4 g .. + 3
-    const int g4 = 4 * (lane >> 4);
-    if constexpr (EPI == kOut) {
-        if (p.part != nullptr) {
-            float* part = p.part + (long long)split * p.M * p.ldp;
+    const Finish fin = p;  // apart from the arguments that the loop indexes
+    finish<EPI, PL>(fin, acc, m0 + wr * 16 * MB + (lane & 15),
+                     n0 + wc * 16 * (DUAL ? NB / 2 : NB) + 4 * (lane >> 4), split);
+}
+
+// fp32 operands as they lie, for rows that are too few to pay for packing the weights: a tile of 64 rows x 128 columns
+// (kSwiGLU: 64 columns of h), four wavefronts in a 2 x 2 grid of 32 rows x 64 columns, chunks of 32 contraction
+// elements in two stages. A fragment becomes three bf16 terms in registers (44 instructions of the VALU beside the 6
+// MFMAs that each pair of fragments takes), the small term products and the large ones have sums of their own. Three
+// work-groups share a CU, so one's conversion runs beside another's products and loads.
+template <int EPI, bool BMC>
+__global__ __launch_bounds__(256) void swiglu_f32_kernel(TileArgs p) {
+    constexpr int MB = 2, NB = 4, TM = 64, TN = 128;
+    constexpr bool DUAL = EPI == kSwiGLU;
+    typedef Stage<false, TM, true> SA;
+    typedef Stage<BMC, TN, true> SB;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[2][SA::BYTES + SB::BYTES];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave >> 1, wc = wave & 1;
+    const int per = (p.total + 7) / 8;
+    const int local = blockIdx.x / 8;
+    const int item = (blockIdx.x % 8) * per + local;
+    if (local >= per || item >= p.total) return;
+    const int split = item / p.tiles, tile = item - split * p.tiles;
+    const int band = tile / (kBand * p.ncb), in = tile - band * kBand * p.ncb;
+    const int height = min(kBand, (p.M + TM - 1) / TM - band * kBand);
+    const int m0 = (band * kBand + in % height) * TM;
+    const int n0 = (in / height) * (DUAL ? TN / 2 : TN);
+    SA sa;
+    SB sb;
+    sa.init(wave, lane, m0, p.M, p.lda);
+    sb.init(DUAL ? wave & 1 : wave, lane, n0, p.N, p.ldb);  // kSwiGLU: as in swiglu_tile_kernel
+    const long long a_tile = (long long)m0 * p.lda * 4, b_tile = BMC ? 0 : (long long)n0 * p.ldb * 4;
+    const unsigned lds0 = (unsigned)(size_t)(lds_ptr_t)&lds[0][0];
+    const int cps = (max(p.ka, p.kb) + SA::CHUNK - 1) / SA::CHUNK;
+    const int first = split * p.split_chunks;
+    const int chunks = min(p.split_chunks, cps * p.nseg - first);
+    int seg = first / cps, c0 = first - seg * cps;  // segment and chunk of it to load next
+    auto load = [&](int st) {
+        const char* pa = p.a[seg] + a_tile + c0 * sa.step;
+        const char* pb = (DUAL && wave >= 2 ? p.b1[seg] : p.b[seg]) + b_tile + c0 * sb.step;
+        const unsigned base = lds0 + st * (SA::BYTES + SB::BYTES);
+        const int left = SA::CHUNK * c0;
+#pragma unroll
+        for (int j = 0; j < SA::LOADS; ++j) sa.load(wave, wave, lane, j, pa, p.ka - left, base);
+#pragma unroll
+        for (int j = 0; j < SB::LOADS; ++j)
+            sb.load(wave, DUAL ? wave & 1 : wave, lane, j, pb, p.kb - left, base + SA::BYTES);
+        if (++c0 == cps) c0 = 0, ++seg;
+    };
+    Reader32<false, TM> ra;
+    Reader32<BMC, TN> rb;
+    ra.init(lane, wr * 16 * MB);
+    rb.init(lane, DUAL ? wc * 8 * NB : wc * 16 * NB);
+    f32x4 large[MB][NB], small[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) large[i][j] = small[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (chunks > 0) load(0);
+    for (int c = 0; c < chunks; ++c) {
+        const int st = c & 1;
+        // this wavefront's loads of chunk c have landed, and after the barrier everybody's, and chunk c - 1 is read
+        __builtin_amdgcn_s_waitcnt(vm_only(0));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (c + 1 < chunks) load(st ^ 1);
+        bf16x8 a[MB][3];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            float v[8];
+            ra.read(&lds[st][0], i, v);
+            ra.terms(v, a[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            float v[8];
+            bf16x8 b[3];
+            rb.read(&lds[st][SA::BYTES], DUAL && j >= NB / 2 ? j - NB / 2 + NB : j, v);
+            rb.terms(v, b);
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
-                const int m = m0 + wr * 16 * MB + 16 * i + (lane & 15);
 #pragma unroll
-                for (int j = 0; j < NB; ++j) {
-                    const int n = n0 + wc * 16 * NB + 16 * j + g4;
-                    if (m < p.M && n < p.ldp) *(f32x4*)(part + (long long)m * p.ldp + n) = acc[i][j];
-                }
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
-            const int m = m0 + wr * 16 * MB + 16 * i + (lane & 15);
-            const bool first = m < p.split, second = m >= p.split_at && m < p.M;
-            const long long row = first ? m : m - p.split_at;
-            void* o = first ? p.out : p.out1;
-#pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                const int n = n0 + wc * 16 * NB + 16 * j + g4;
-                const f32x4 v = acc[i][j];
-                if (!(first || second) || n >= p.N) continue;
-                const long long e = row * p.ldo + n;
-                if (n + 4 <= p.N && p.ldo % 4 == 0) {
-                    if (p.f32) *(f32x4*)((float*)o + e) = v;
-                    else *(uint2*)((unsigned short*)o + e) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (n + q < p.N) {
-                            if (p.f32) ((float*)o)[e + q] = v[q];
-                            else ((unsigned short*)o)[e + q] = f32_to_bf16_rne(v[q]);
-                        }
-                }
-            }
-        }
-    } else {
-        const long long gu_plane = (long long)p.M * p.ldh;
-        constexpr int NH = DUAL ? NB / 2 : NB;
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
-            const int m = m0 + wr * 16 * MB + 16 * i + (lane & 15);
-#pragma unroll
-            for (int j = 0; j < NH; ++j) {
-                const int n = n0 + wc * 16 * NH + 16 * j + g4;
-                // columns from N to ldh are sums of zeros and written as such: they are operands of products
-                if (m >= p.M || n >= p.ldh) continue;
-                const long long e = (long long)m * p.ldh + n;
-                float h[4];
-                if constexpr (DUAL) {
-                    const f32x4 g = acc[i][j], u = acc[i][j + NH];
-                    if (p.gu != nullptr) {
-                        *(f32x4*)(p.gu + e) = g;
-                        *(f32x4*)(p.gu + gu_plane + e) = u;
-                    }
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) h[q] = silu(g[q]) * u[q];
-                } else {
-                    const f32x4 dh = acc[i][j], g = *(const f32x4*)(p.gu + e), u = *(const f32x4*)(p.gu + gu_plane + e);
-                    float dg[4], du[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float s = sigmoid(g[q]), a = g[q] * s;
-                        h[q] = a * u[q];
-                        du[q] = dh[q] * a;
-                        dg[q] = dh[q] * u[q] * (s + a * (1.0f - s));
-                    }
-                    unsigned short* d = p.d + (long long)m * 2 * p.ldh + n;
-                    put_terms(d, p.plane_d, p.planes, dg);
-                    put_terms(d + p.ldh, p.plane_d, p.planes, du);
-                }
-                put_terms(p.h + e, p.plane_h, p.planes, h);
+                for (int t = 0; t < 5; ++t)
+                    small[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[kTermB[t]], a[i][kTermA[t]], small[i][j], 0, 0, 0);
+                large[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[0], a[i][0], large[i][j], 0, 0, 0);
             }
         }
     }
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) large[i][j] = large[i][j] + small[i][j];
+    const Finish fin = p;
+    finish<EPI, kFp32>(fin, large, m0 + wr * 16 * MB + (lane & 15),
+                     n0 + wc * 16 * (DUAL ? NB / 2 : NB) + 4 * (lane >> 4), split);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -547,25 +703,24 @@ __global__ __launch_bounds__(512) void swiglu_few_kernel(FewArgs p) {
     }
 }
 
-// Sums of the splits, in order, to the output.
-__global__ __launch_bounds__(256) void swiglu_sum_kernel(TileArgs p, int splits) {
+// Sums of the splits, in order, and what becomes of them.
+template <int EPI, int PL>
+__global__ __launch_bounds__(256) void swiglu_sum_kernel(Finish p, int splits) {
+    constexpr int NM = EPI == kSwiGLU ? 2 : 1;
     const int per = p.ldp / 4;
     const long long total = (long long)p.M * per, plane = (long long)p.M * p.ldp;
     for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
         const int m = (int)(e / per), n = (int)(e - (long long)m * per) * 4;
         const float* at = p.part + (long long)m * p.ldp + n;
-        f32x4 v = *(const f32x4*)at;
-        for (int s = 1; s < splits; ++s) v = v + *(const f32x4*)(at + s * plane);
-        const bool first = m < p.split;
-        if (!first && m < p.split_at) continue;
-        void* o = first ? p.out : p.out1;
-        const long long d = (long long)(first ? m : m - p.split_at) * p.ldo + n;
+        f32x4 v[NM];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (n + q < p.N) {
-                if (p.f32) ((float*)o)[d + q] = v[q];
-                else ((unsigned short*)o)[d + q] = f32_to_bf16_rne(v[q]);
-            }
+        for (int k = 0; k < NM; ++k) v[k] = *(const f32x4*)(at + k * plane);
+        for (int s = 1; s < splits; ++s)
+#pragma unroll
+            for (int k = 0; k < NM; ++k) v[k] = v[k] + *(const f32x4*)(at + (s * NM + k) * plane);
+        if constexpr (EPI == kOut) finish_out(p, m, n, v[0]);
+        else if constexpr (EPI == kGrad) finish_grad<PL>(p, m, n, v[0]);
+        else finish_swiglu<PL>(p, m, n, v[0], v[NM - 1]);
     }
 }
 
@@ -622,10 +777,6 @@ __global__ __launch_bounds__(256) void swiglu_pack_kernel(PackArgs a) {
 }
 
 // ------------------------------------------------------------------ host
-// Term products of an fp32 product, smallest first: (term of A, term of B).
-constexpr int kTermA[6] = {2, 0, 1, 1, 0, 0};
-constexpr int kTermB[6] = {0, 2, 1, 0, 1, 0};
-
 inline int up8(int v) { return (v + 7) / 8 * 8; }
 inline int up4(int v) { return (v + 3) / 4 * 4; }
 
@@ -641,7 +792,7 @@ struct Carve {
     char* base;
     bool dry;
     int act;
-    size_t used = 0;
+    size_t used = 0;  // where it starts in the workspace, and what is taken
     PackArgs packs{};
     char* take(size_t bytes) {
         char* r = dry ? nullptr : base + used;
@@ -666,9 +817,8 @@ struct Carve {
     }
 };
 
-// Adds the operand pairs of A · Bᵀ (with b1: gate and up) to a launch.
-void add_product(TileArgs& p, int act, const Operand& a, const Operand& b, const Operand* b1 = nullptr) {
-    const int n = act == YVMOE_ACT_F32 ? 6 : 1;
+// Adds the n = 1 or 6 operand pairs of A · Bᵀ (with b1: gate and up) to a launch.
+void add_product(TileArgs& p, int n, const Operand& a, const Operand& b, const Operand* b1 = nullptr) {
     for (int t = 0; t < n; ++t) {
         const int ta = n == 1 ? 0 : kTermA[t], tb = n == 1 ? 0 : kTermB[t];
         p.a[p.nseg] = a.p + ta * a.plane;
@@ -683,62 +833,72 @@ void add_product(TileArgs& p, int act, const Operand& a, const Operand& b, const
 // Tile and number of splits of the contraction for M x N outputs (kSwiGLU: N twice the columns of h) of `chunks`
 // chunks: the least of an estimate. A CU's work-group takes `alone` us a chunk when it runs by itself and `shared` us of
 // the CU's time beside others (measured: 256 1.45 and 1.79 under full load, 128 0.84 and 0.42 to 0.60, 64 0.63 and
-// 0.28 to 0.34); splits cost a launch and their sums' traffic.
+// 0.28 to 0.34); splits cost a launch and their sums' traffic. direct: the fp32 form, 64 x 128 and chunks of 32.
 struct Plan {
-    int tile, splits;
+    int tile, splits, len;  // len: chunks of a split
 };
-Plan plan_of(int M, int N, int chunks, bool may_split) {
-    static const struct { int tile; float alone, shared; } kinds[3] = {{256, 1.6f, 1.75f}, {128, 0.84f, 0.5f}, {64, 0.63f, 0.3f}};
-    Plan best{256, 1};
+Plan plan_of(int M, int N, int chunks, bool direct) {
+    static const struct { int rows, cols; float alone, shared; } kinds[4] = {
+        {256, 256, 1.6f, 1.75f}, {128, 128, 0.84f, 0.5f}, {64, 64, 0.63f, 0.3f}, {64, 128, 0.9f, 0.5f}};
+    Plan best{256, 1, std::max(chunks, 1)};
     float least = 1e30f;
-    for (const auto& k : kinds) {
-        const long long tiles = (long long)((M + k.tile - 1) / k.tile) * ((N + k.tile - 1) / k.tile);
-        for (int s = 1; s <= (may_split ? 16 : 1) && (s == 1 || chunks / s >= 4); ++s) {
+    for (int i = direct ? 3 : 0; i < (direct ? 4 : 3); ++i) {
+        const auto& k = kinds[i];
+        const long long tiles = (long long)((M + k.rows - 1) / k.rows) * ((N + k.cols - 1) / k.cols);
+        for (int s = 1; s <= 16 && (s == 1 || chunks / s >= 4); ++s) {
             const float per_cu = (float)((tiles * s + 255) / 256);
             const int len = (chunks + s - 1) / s;
             float us = std::max(k.alone, per_cu * k.shared) * len;
             if (s > 1) us += 4.0f + (float)s * M * N * 8.0f / 4e6f;
-            if (us < least) least = us, best = {k.tile, s};
+            if (us < least) least = us, best = {k.rows, ceil_div(chunks, std::max(len, 1)), std::max(len, 1)};
         }
     }
-    // splits of whole chunks: as many as are not empty
-    best.splits = ceil_div(chunks, ceil_div(std::max(chunks, 1), best.splits));
     best.splits = std::max(best.splits, 1);
     return best;
 }
 
-inline int chunks_of(const TileArgs& p) { return ceil_div(std::max(p.ka, p.kb), kChunk) * p.nseg; }
-// Bytes of the partial sums of an M x N output.
-size_t part_bytes(int M, int N, int k, int nseg) {
-    const Plan q = plan_of(M, N, ceil_div(k, kChunk) * nseg, true);
-    return q.splits > 1 ? (size_t)q.splits * M * up4(N) * 4 : 0;
+inline int chunks_of(int k, int nseg, bool direct) { return ceil_div(k, direct ? 32 : kChunk) * nseg; }
+// Bytes of the partial sums of an M x N product (N as in plan_of).
+size_t part_bytes(int M, int N, int k, int nseg, bool direct) {
+    const Plan q = plan_of(M, N, chunks_of(k, nseg, direct), direct);
+    return q.splits > 1 ? (size_t)q.splits * M * (N + 16) * 4 : 0;
 }
 
-template <int EPI, bool AMC, bool BMC, int MB, int NB>
+template <int EPI, int PL, bool AMC, bool BMC, int MB, int NB>
 void tile_grid(TileArgs p, int splits, hipStream_t st) {
     const int cols = EPI == kSwiGLU ? 16 * NB : 32 * NB;
     p.ncb = ceil_div(p.N, cols);
     p.tiles = ceil_div(p.M, 32 * MB) * p.ncb;
     p.total = p.tiles * splits;
-    swiglu_tile_kernel<EPI, AMC, BMC, MB, NB><<<(unsigned)(ceil_div(p.total, 8) * 8), 256, 0, st>>>(p);
+    swiglu_tile_kernel<EPI, PL, AMC, BMC, MB, NB><<<(unsigned)(ceil_div(p.total, 8) * 8), 256, 0, st>>>(p);
 }
 
-template <int EPI, bool AMC, bool BMC>
+// PL: kSwiGLU, kGrad, how h and d are stored; kOut with kFp32: the fp32 form on operands as they lie.
+template <int EPI, int PL, bool AMC, bool BMC>
 void tile_launch(TileArgs p, float* part, hipStream_t st) {
     if (p.M <= 0 || p.N <= 0) return;
-    const int chunks = chunks_of(p);
-    const Plan q = plan_of(p.M, EPI == kSwiGLU ? 2 * p.N : p.N, chunks, EPI == kOut);
-    p.split_chunks = ceil_div(std::max(chunks, 1), q.splits);
+    constexpr bool DIRECT = PL == kFp32;
+    const Plan q = plan_of(p.M, EPI == kSwiGLU ? 2 * p.N : p.N, chunks_of(std::max(p.ka, p.kb), p.nseg, DIRECT), DIRECT);
+    p.split_chunks = q.len;
     if (q.splits > 1) {
         p.part = part;
-        p.ldp = up4(p.N);
+        p.ldp = EPI == kOut ? up4(p.N) : p.ldh;
     }
-    if (q.tile == 256) tile_grid<EPI, AMC, BMC, 8, 8>(p, q.splits, st);
-    else if (q.tile == 128) tile_grid<EPI, AMC, BMC, 4, 4>(p, q.splits, st);
-    else tile_grid<EPI, AMC, BMC, 2, 2>(p, q.splits, st);
+    if constexpr (DIRECT) {
+        p.ncb = ceil_div(p.N, EPI == kSwiGLU ? 64 : 128);
+        p.tiles = ceil_div(p.M, 64) * p.ncb;
+        p.total = p.tiles * q.splits;
+        swiglu_f32_kernel<EPI, BMC><<<(unsigned)(ceil_div(p.total, 8) * 8), 256, 0, st>>>(p);
+    } else if (q.tile == 256) {
+        tile_grid<EPI, PL, AMC, BMC, 8, 8>(p, q.splits, st);
+    } else if (q.tile == 128) {
+        tile_grid<EPI, PL, AMC, BMC, 4, 4>(p, q.splits, st);
+    } else {
+        tile_grid<EPI, PL, AMC, BMC, 2, 2>(p, q.splits, st);
+    }
     if (q.splits > 1) {
         const long long quads = (long long)p.M * (p.ldp / 4);
-        swiglu_sum_kernel<<<(unsigned)std::min<long long>((quads + 255) / 256, 8192), 256, 0, st>>>(p, q.splits);
+        swiglu_sum_kernel<EPI, PL><<<(unsigned)std::min<long long>((quads + 255) / 256, 8192), 256, 0, st>>>(p, q.splits);
     }
 }
 
@@ -755,6 +915,11 @@ void few_launch(const FewArgs& p, hipStream_t st) {
 }
 
 }  // namespace
+
+// Whether fp32 operands go into the products as they lie (rows of whole 16-byte pieces).
+inline bool direct_f32(int act, int N, int H, int F) {
+    return act == YVMOE_ACT_F32 && H % 4 == 0 && F % 4 == 0 && N <= kDirectRows;
+}
 
 size_t swiglu_saved_bytes(int N, int F) { return (size_t)2 * N * up8(F) * 4; }
 
@@ -775,11 +940,19 @@ int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weig
         YV_LAUNCH_CHECK("swiglu_forward");
         return YVMOE_OK;
     }
-    const Operand ox = c.operand(x, N, H), og = c.operand(w->w_gate, F, H), ou = c.operand(w->w_up, F, H),
-                  od = c.operand(w->w_down, H, F);
+    const bool direct = direct_f32(act, N, H, F);
     const long long plane = (long long)N * F8;
-    unsigned short* h = (unsigned short*)c.take((size_t)plane * 2 * planes);
-    float* part = (float*)c.take(part_bytes(N, H, F8, planes == 3 ? 6 : 1));
+    Operand ox{(const char*)x, H, 0}, og{(const char*)w->w_gate, H, 0}, ou{(const char*)w->w_up, H, 0},
+        od{(const char*)w->w_down, F, 0};
+    if (!direct) {
+        ox = c.operand(x, N, H);
+        og = c.operand(w->w_gate, F, H);
+        ou = c.operand(w->w_up, F, H);
+        od = c.operand(w->w_down, H, F);
+    }
+    const int terms = act == YVMOE_ACT_F32 && !direct ? 6 : 1;
+    char* h = c.take((size_t)plane * (direct ? 4 : 2 * planes));
+    float* part = (float*)c.take(std::max(part_bytes(N, 2 * F, H, terms, direct), part_bytes(N, H, F8, terms, direct)));
     if (bytes != nullptr) *bytes = c.used;
     if (c.dry || N == 0) return YVMOE_OK;
     c.pack(st);
@@ -787,23 +960,26 @@ int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weig
     p.M = N;
     p.N = F;
     p.ka = p.kb = ox.ld;
-    add_product(p, act, ox, og, &ou);
-    p.planes = planes;
+    add_product(p, terms, ox, og, &ou);
     p.h = h;
     p.plane_h = plane;
     p.gu = saved;
     p.ldh = F8;
-    tile_launch<kSwiGLU, false, false>(p, nullptr, st);
     TileArgs q{};
     q.M = N;
     q.N = H;
-    q.ka = q.kb = F8;
-    add_product(q, act, Operand{(const char*)h, F8, plane * 2}, od);
+    q.ka = F8;
+    q.kb = direct ? F : F8;
+    add_product(q, terms, Operand{h, F8, plane * 2}, od);
     q.out = out;
     q.ldo = H;
     q.split = q.split_at = N;
     q.f32 = act == YVMOE_ACT_F32;
-    tile_launch<kOut, false, false>(q, part, st);
+    if (direct) tile_launch<kSwiGLU, kFp32, false, false>(p, part, st);
+    else if (planes == 3) tile_launch<kSwiGLU, kThree, false, false>(p, part, st);
+    else tile_launch<kSwiGLU, kOne, false, false>(p, part, st);
+    if (direct) tile_launch<kOut, kFp32, false, false>(q, part, st);
+    else tile_launch<kOut, kOne, false, false>(q, part, st);
     YV_LAUNCH_CHECK("swiglu_forward");
     return YVMOE_OK;
 }
@@ -811,50 +987,70 @@ int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weig
 int swiglu_backward_launch(const void* dy, const void* x, const float* saved, int act, int N,
                            const yvmoe_swiglu_weights* w, void* dx, void* dwg, void* dwu, void* dwd, char* ws,
                            size_t* bytes, hipStream_t st) {
-    const int H = w->hidden, F = w->ffn, F8 = up8(F), planes = act == YVMOE_ACT_F32 ? 3 : 1;
-    const int f32 = act == YVMOE_ACT_F32;
+    const int H = w->hidden, F = w->ffn, F8 = up8(F);
+    const int f32 = act == YVMOE_ACT_F32, planes = f32 ? 3 : 1, terms = f32 ? 6 : 1;
+    const bool direct = direct_f32(act, N, H, F);
     Carve c{ws, bytes != nullptr, act};
     const long long plane = (long long)N * F8;
-    const Operand ody = c.operand(dy, N, H), od = c.operand(w->w_down, H, F);
-    unsigned short* h = (unsigned short*)c.take((size_t)plane * 2 * planes);
-    unsigned short* d = (unsigned short*)c.take((size_t)plane * 4 * planes);
-    Operand ox{}, og{}, ou{};
-    if (c.dry || dwg != nullptr || dwu != nullptr) ox = c.operand(x, N, H);
-    if (c.dry || dx != nullptr) {
-        og = c.operand(w->w_gate, F, H);
-        ou = c.operand(w->w_up, F, H);
+    // dy and x as operands of the weights' gradients, weights and dy of dh and dx
+    const bool wgrad = c.dry || dwg != nullptr || dwu != nullptr || dwd != nullptr;
+    Operand ody{(const char*)dy, H, 0}, ox{(const char*)x, H, 0}, og{(const char*)w->w_gate, H, 0},
+        ou{(const char*)w->w_up, H, 0}, od{(const char*)w->w_down, F, 0};
+    Operand pdy = ody, oh{}, odd{};
+    if (!direct || wgrad) pdy = c.operand(dy, N, H);
+    if (!direct) {
+        ody = pdy;
+        od = c.operand(w->w_down, H, F);
+        if (c.dry || dx != nullptr) {
+            og = c.operand(w->w_gate, F, H);
+            ou = c.operand(w->w_up, F, H);
+        }
     }
-    const int terms = f32 ? 6 : 1;
-    float* part = (float*)c.take(std::max({part_bytes(N, H, F8, 2 * terms), part_bytes(F8 + F, H, N, terms),
-                                           part_bytes(F, H, N, terms), part_bytes(H, F, N, terms)}));
+    if (c.dry || dwg != nullptr || dwu != nullptr) ox = c.operand(x, N, H);
+    // h, dg and du: planes of terms, or fp32 first and packed for the weights' gradients
+    char* h = c.take((size_t)plane * (direct ? 4 : 2 * planes));
+    char* d = c.take((size_t)plane * 2 * (direct ? 4 : 2 * planes));
+    oh = Operand{h, F8, plane * 2};
+    odd = Operand{d, 2 * F8, plane * 4};
+    Carve late{c.base, c.dry, act, c.used};
+    if (direct && wgrad) {
+        oh = late.operand(h, N, F8);
+        odd = late.operand(d, N, 2 * F8);
+        c.used = late.used;
+    }
+    float* part = (float*)c.take(std::max({part_bytes(N, F, H, direct ? 1 : terms, direct),
+                                           part_bytes(N, H, F8, direct ? 2 : 2 * terms, direct),
+                                           part_bytes(F8 + F, H, N, terms, false), part_bytes(F, H, N, terms, false),
+                                           part_bytes(H, F, N, terms, false)}));
     if (bytes != nullptr) *bytes = c.used;
     if (c.dry) return YVMOE_OK;
     c.pack(st);
-    const Operand oh{(const char*)h, F8, plane * 2}, odg{(const char*)d, 2 * F8, plane * 4},
-        odu{(const char*)(d + F8), 2 * F8, plane * 4};
     TileArgs p{};
     p.M = N;
     p.N = F;
     p.ka = ody.ld;
     p.kb = H;
-    add_product(p, act, ody, od);
-    p.planes = planes;
+    add_product(p, direct ? 1 : terms, ody, od);
     p.h = h;
     p.plane_h = plane;
     p.d = d;
     p.plane_d = plane * 2;
     p.gu = const_cast<float*>(saved);
     p.ldh = F8;
-    tile_launch<kGrad, false, true>(p, nullptr, st);
+    if (direct) tile_launch<kGrad, kFp32, false, true>(p, part, st);
+    else if (planes == 3) tile_launch<kGrad, kThree, false, true>(p, part, st);
+    else tile_launch<kGrad, kOne, false, true>(p, part, st);
     if (dx != nullptr) {
         TileArgs q{};
         q.M = N;
         q.N = H;
         q.ka = F8;
         q.kb = F;
-        add_product(q, act, odg, og);
-        add_product(q, act, odu, ou);
-        if (f32) {  // both matrices' smallest terms first
+        const int e = direct ? 4 : 2;
+        const Operand dg{d, 2 * F8, plane * 4}, du{d + (size_t)F8 * e, 2 * F8, plane * 4};
+        add_product(q, direct ? 1 : terms, dg, og);
+        add_product(q, direct ? 1 : terms, du, ou);
+        if (terms > 1 && !direct) {  // both matrices' smallest terms first
             const TileArgs in = q;
             for (int t = 0; t < 12; ++t) {
                 q.a[t] = in.a[t / 2 + 6 * (t & 1)];
@@ -865,34 +1061,36 @@ int swiglu_backward_launch(const void* dy, const void* x, const float* saved, in
         q.ldo = H;
         q.split = q.split_at = N;
         q.f32 = f32;
-        tile_launch<kOut, false, true>(q, part, st);
+        if (direct) tile_launch<kOut, kFp32, false, true>(q, part, st);
+        else tile_launch<kOut, kOne, false, true>(q, part, st);
     }
+    late.pack(st);
     if (dwg != nullptr || dwu != nullptr) {
         const bool both = dwg != nullptr && dwu != nullptr;
         TileArgs q{};
         q.M = both ? F8 + F : F;
         q.N = H;
         q.ka = q.kb = N;
-        add_product(q, act, dwg != nullptr ? odg : odu, ox);
+        add_product(q, terms, dwg != nullptr ? odd : Operand{odd.p + 2 * (size_t)F8, odd.ld, odd.plane}, ox);
         q.out = dwg != nullptr ? dwg : dwu;
         q.out1 = dwu;
         q.ldo = H;
         q.split = F;
         q.split_at = both ? F8 : F;
         q.f32 = f32;
-        tile_launch<kOut, true, true>(q, part, st);
+        tile_launch<kOut, kOne, true, true>(q, part, st);
     }
     if (dwd != nullptr) {
         TileArgs q{};
         q.M = H;
         q.N = F;
         q.ka = q.kb = N;
-        add_product(q, act, ody, oh);
+        add_product(q, terms, pdy, oh);
         q.out = dwd;
         q.ldo = F;
         q.split = q.split_at = H;
         q.f32 = f32;
-        tile_launch<kOut, true, true>(q, part, st);
+        tile_launch<kOut, kOne, true, true>(q, part, st);
     }
     YV_LAUNCH_CHECK("swiglu_backward");
     return YVMOE_OK;

@@ -71,7 +71,8 @@ def step(x, wg, wu, wd, dy, cuda):
 
 
 SIZES = [(1, 1, 1), (1, 8, 8), (2, 64, 64), (3, 7, 5), (5, 128, 96), (16, 256, 320), (17, 100, 130), (33, 72, 264),
-         (64, 512, 128), (65, 63, 129), (130, 257, 255), (200, 384, 1000), (300, 1000, 272)]
+         (64, 512, 128), (65, 63, 129), (130, 257, 255), (200, 384, 1000), (300, 1000, 272),
+         (100, 100, 204), (1000, 36, 68), (66, 1028, 772), (90, 2048, 1536)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
@@ -92,7 +93,8 @@ def test_step(cuda, N, H, F, dtype):
 # tiles of 256 and 128, with full and partial ends, and the same bits twice
 @pytest.mark.parametrize("N,H,F,dtype", [(2050, 1032, 3080, torch.bfloat16), (777, 2056, 1544, torch.bfloat16),
                                          (1500, 1024, 2816, torch.float32), (515, 1001, 2003, torch.float32),
-                                         (515, 1001, 2003, torch.bfloat16)])
+                                         (515, 1001, 2003, torch.bfloat16), (1020, 516, 2052, torch.float32),
+                                         (1030, 516, 2052, torch.float32)])
 def test_step_large(cuda, N, H, F, dtype):
     t = make(N, H, F, dtype, seed=1)
     got, again = step(*t, cuda), step(*t, cuda)
