@@ -82,6 +82,9 @@ __device__ __forceinline__ void mfma_acc(f32x4& acc, const bf16x8& a, const bf16
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 
+// How many of n instructions go before MFMA i of t, spread over the first 4 / q of them.
+constexpr int among(int i, int n, int t, int q) { return i * n * q / (4 * t) < n ? i * n * q / (4 * t) : n; }
+
 __device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
 
 // How h and d are stored: one bf16 plane (rounded), three (a value is the sum of three bf16 numbers), or fp32.
@@ -320,8 +323,8 @@ struct Reader32 {
 // 2 x 2 grid, each 16 MB x 16 NB: MB x NB blocks of 16 x 16, fp32 sums in AGPRs (an MFMA in inline assembly
 // with the sum as one tied AGPR operand, so that the register allocator copies none). Chunks of 64
 // contraction elements move to LDS by direct loads through two stages; the MFMAs of a chunk run in two
-// halves with the next half's fragment reads and the loads of the chunk after next among them, one barrier
-// between the halves. The columns' operand is the MFMA's first, so that a lane holds four consecutive
+// halves with the next half's fragment reads (in the first half of them) and the loads of the chunk after next (in
+// the first quarter) among them, one barrier between the halves. The columns' operand is the MFMA's first, so that a lane holds four consecutive
 // columns of one row.
 template <int EPI, int PL, bool AMC, bool BMC, int MB, int NB>
 __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
@@ -401,11 +404,12 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
         for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     bf16x8 fa[2][MB], fb[2][NB];
     auto read = [&](int st, int s, int q) {
-        if (q < NB) {
-            const int blk = DUAL && q >= NB / 2 ? q - NB / 2 + NB : q;
-            fb[s][q] = rb.read(&lds[st][SA::BYTES], s, blk);
+        // in the order of use: the first column block, all row blocks, the other column blocks
+        if (q >= 1 && q <= MB) {
+            fa[s][q - 1] = ra.read(&lds[st][0], s, q - 1);
         } else {
-            fa[s][q - NB] = ra.read(&lds[st][0], s, q - NB);
+            const int j = q == 0 ? 0 : q - MB;
+            fb[s][j] = rb.read(&lds[st][SA::BYTES], s, DUAL && j >= NB / 2 ? j - NB / 2 + NB : j);
         }
     };
     if (chunks > 0) {
@@ -426,7 +430,7 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
             for (int i = 0; i < T; ++i) {
                 mfma_acc(acc[i % MB][i / MB], fb[0][i / MB], fa[0][i % MB]);
 #pragma unroll
-                for (int q = (i * R) / T; q < ((i + 1) * R) / T; ++q) read(st, 1, q);
+                for (int q = among(i, R, T, 5); q < among(i + 1, R, T, 5); ++q) read(st, 1, q);
             }
             // this wavefront has read chunk c and holds its loads of chunk c + 1: the barrier frees the stage
             // for chunk c + 2 and publishes chunk c + 1
@@ -440,9 +444,9 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
             for (int i = 0; i < T; ++i) {
                 mfma_acc(acc[i % MB][i / MB], fb[1][i / MB], fa[1][i % MB]);
 #pragma unroll
-                for (int q = (i * R) / T; q < ((i + 1) * R) / T; ++q) read(st ^ 1, 0, q);
+                for (int j = among(i, D, T, 4); j < among(i + 1, D, T, 4); ++j) load(st, j);
 #pragma unroll
-                for (int j = (i * D) / T; j < ((i + 1) * D) / T; ++j) load(st, j);
+                for (int q = among(i, R, T, 5); q < among(i + 1, R, T, 5); ++q) read(st ^ 1, 0, q);
             }
         }
         // the repeated loads land before the work-group ends; wait states between the last MFMAs and the
@@ -553,7 +557,7 @@ __global__ __launch_bounds__(256) void swiglu_f32_kernel(TileArgs p) {
 
 // ------------------------------------------------------------------ few rows
 // Up to 64 rows of the forward pass: bound by the stream of the weights, which are read as they lie. A work-group of
-// eight wavefronts owns 16 columns (kSwiGLU: gate and up), the wavefronts deal out the contraction in spans of kSpan
+// eight wavefronts owns 16 columns (kSwiGLU: gate and up), the wavefronts deal out the contraction in spans of SPAN
 // steps and add their sums in LDS, in order. Lane 16 g + r reads 16 bytes of weight row r and of row r of x, so a
 // step is 32 (fp32: 16) elements and a span of four 256 consecutive bytes of every weight row; any alignment. fp32 runs
 // on the fp32 MFMAs: four a step, each on one element of the lanes' four.
@@ -566,7 +570,6 @@ struct FewArgs {
     float* gu;              // kSwiGLU: [2][N][ldh] or none
     int ldh;
 };
-constexpr int kSpan = 4;
 
 struct __attribute__((packed, aligned(2))) Any16 {
     unsigned v[4];
@@ -607,6 +610,7 @@ __device__ __forceinline__ f32x4 few_mfma(const Piece<F32>& a, const Piece<F32>&
 template <int EPI, bool F32, int MR>
 __global__ __launch_bounds__(512) void swiglu_few_kernel(FewArgs p) {
     constexpr int NM = EPI == kSwiGLU ? 2 : 1;
+    constexpr int SPAN = F32 && MR == 4 ? 2 : 4;  // as many as registers hold
     typedef Piece<F32> P;
     __shared__ f32x4 part[8][NM * MR][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -621,13 +625,13 @@ __global__ __launch_bounds__(512) void swiglu_few_kernel(FewArgs p) {
     for (int m = 0; m < NM; ++m)
 #pragma unroll
         for (int i = 0; i < MR; ++i) acc[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int steps = p.K / P::STEP, spans = (steps + kSpan - 1) / kSpan;
+    const int steps = p.K / P::STEP, spans = (steps + SPAN - 1) / SPAN;
     for (int sp = wave; sp < spans; sp += 8) {
-        const int s0 = sp * kSpan;
-        P w[NM][kSpan], x[MR][kSpan];
-        if (s0 + kSpan <= steps) {
+        const int s0 = sp * SPAN;
+        P w[NM][SPAN], x[MR][SPAN];
+        if (s0 + SPAN <= steps) {
 #pragma unroll
-            for (int s = 0; s < kSpan; ++s) {
+            for (int s = 0; s < SPAN; ++s) {
                 const size_t k = (size_t)(s0 + s) * P::STEP + g * P::E;
 #pragma unroll
                 for (int m = 0; m < NM; ++m) w[m][s].load(p.w[m], wrow + k);
@@ -636,7 +640,7 @@ __global__ __launch_bounds__(512) void swiglu_few_kernel(FewArgs p) {
             }
             __builtin_amdgcn_sched_barrier(0);  // all of the span's loads in flight
 #pragma unroll
-            for (int s = 0; s < kSpan; ++s)
+            for (int s = 0; s < SPAN; ++s)
 #pragma unroll
                 for (int m = 0; m < NM; ++m)
 #pragma unroll
@@ -839,7 +843,7 @@ struct Plan {
 };
 Plan plan_of(int M, int N, int chunks, bool direct) {
     static const struct { int rows, cols; float alone, shared; } kinds[4] = {
-        {256, 256, 1.6f, 1.75f}, {128, 128, 0.84f, 0.5f}, {64, 64, 0.63f, 0.3f}, {64, 128, 0.9f, 0.5f}};
+        {256, 256, 1.6f, 1.75f}, {128, 128, 0.84f, 0.58f}, {64, 64, 0.63f, 0.3f}, {64, 128, 0.9f, 0.5f}};
     Plan best{256, 1, std::max(chunks, 1)};
     float least = 1e30f;
     for (int i = direct ? 3 : 0; i < (direct ? 4 : 3); ++i) {
@@ -902,9 +906,15 @@ void tile_launch(TileArgs p, float* part, hipStream_t st) {
     }
 }
 
+// Whether fp32 operands can go into the products as they lie: rows of whole 16-byte pieces.
+inline bool direct_f32(int act, int H, int F) { return act == YVMOE_ACT_F32 && H % 4 == 0 && F % 4 == 0; }
+
 // Each block of 16 columns reads all rows from L2: with many blocks, tiles take over from 33 rows on (4096 x 11264, bf16,
 // forward: 33 rows 101 us against about 95, 64 rows 137 against 98; 5120 x 1536: 64 rows 47 against 56).
-inline bool few_rows(int N, int F) { return N <= (F >= 8192 ? 32 : 64); }
+// fp32 from 33 on where it has tiles without packing (1024 x 2816: 33 rows 57 us, 65 in tiles 40).
+inline bool few_rows(int act, int N, int H, int F) {
+    return N <= (F >= 8192 || direct_f32(act, H, F) ? 32 : 64);
+}
 
 template <int EPI, bool F32>
 void few_launch(const FewArgs& p, hipStream_t st) {
@@ -916,11 +926,6 @@ void few_launch(const FewArgs& p, hipStream_t st) {
 
 }  // namespace
 
-// Whether fp32 operands go into the products as they lie (rows of whole 16-byte pieces).
-inline bool direct_f32(int act, int N, int H, int F) {
-    return act == YVMOE_ACT_F32 && H % 4 == 0 && F % 4 == 0 && N <= kDirectRows;
-}
-
 size_t swiglu_saved_bytes(int N, int F) { return (size_t)2 * N * up8(F) * 4; }
 
 // With bytes nothing is launched: *bytes is the size of the workspace.
@@ -928,7 +933,7 @@ int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weig
                           char* ws, size_t* bytes, hipStream_t st) {
     const int H = w->hidden, F = w->ffn, F8 = up8(F), planes = act == YVMOE_ACT_F32 ? 3 : 1;
     Carve c{ws, bytes != nullptr, act};
-    if (few_rows(N, F)) {
+    if (few_rows(act, N, H, F)) {
         const bool f32 = act == YVMOE_ACT_F32;
         void* h = c.take((size_t)N * F8 * (f32 ? 4 : 2));
         if (bytes != nullptr) *bytes = c.used;
@@ -940,7 +945,7 @@ int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weig
         YV_LAUNCH_CHECK("swiglu_forward");
         return YVMOE_OK;
     }
-    const bool direct = direct_f32(act, N, H, F);
+    const bool direct = direct_f32(act, H, F) && N <= kDirectRows;
     const long long plane = (long long)N * F8;
     Operand ox{(const char*)x, H, 0}, og{(const char*)w->w_gate, H, 0}, ou{(const char*)w->w_up, H, 0},
         od{(const char*)w->w_down, F, 0};
@@ -989,7 +994,7 @@ int swiglu_backward_launch(const void* dy, const void* x, const float* saved, in
                            size_t* bytes, hipStream_t st) {
     const int H = w->hidden, F = w->ffn, F8 = up8(F);
     const int f32 = act == YVMOE_ACT_F32, planes = f32 ? 3 : 1, terms = f32 ? 6 : 1;
-    const bool direct = direct_f32(act, N, H, F);
+    const bool direct = direct_f32(act, H, F) && N <= kDirectRows;
     Carve c{ws, bytes != nullptr, act};
     const long long plane = (long long)N * F8;
     // dy and x as operands of the weights' gradients, weights and dy of dh and dx
