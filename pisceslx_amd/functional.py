@@ -669,6 +669,11 @@ def quantize_fp8_rows(x: torch.Tensor) -> Fp8Rows:
     return rows
 
 
+def _no_gradients(x: torch.Tensor, what: str) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{what} is inference only: x requires a gradient (detach it, or use torch.no_grad)")
+
+
 def _fp8_out(out: Optional[torch.Tensor], shape, dev) -> torch.Tensor:
     if out is None:
         return torch.empty(shape, dtype=torch.bfloat16, device=dev)
@@ -682,8 +687,8 @@ def fp8_linear(x, weight: PackedFp8Linear, bias: Optional[torch.Tensor] = None,
     """x · Wᵀ (+ bias [out] bf16) with both operands in 8-bit floating point: W in e4m3fn with a scale per
     128 x 128 block (quant.pack_fp8_linear), x [..., in] bf16, rounded to e4m3fn with a scale per 128 values in
     the call, or rows that are already (Fp8Rows). fp32 sums, rounded once to bf16 [..., out]; the matrix unit
-    keeps about 16 bits of a block's sum, so there are no fp32 outputs. Up to 2^24 rows. ``out`` must
-    overlap no input."""
+    keeps about 16 bits of a block's sum, so there are no fp32 outputs. Up to 2^24 rows; inference only.
+    ``out`` must overlap no input."""
     K, O = weight.in_features, weight.out_features
     rows = isinstance(x, Fp8Rows)
     if rows:
@@ -695,6 +700,7 @@ def fp8_linear(x, weight: PackedFp8Linear, bias: Optional[torch.Tensor] = None,
             raise ValueError(f"x must be [..., {K}], got {tuple(x.shape)}")
         if x.dtype != torch.bfloat16:
             raise ValueError(f"x must be bfloat16 or Fp8Rows, got {x.dtype}")
+        _no_gradients(x, "fp8_linear")
         lead, dev = x.shape[:-1], _same_device(x, weight.codes, weight.scales, bias, out)
     if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != O):
         raise ValueError(f"bias must be bfloat16 [{O}]")
@@ -727,6 +733,7 @@ def fp8_swiglu(x: torch.Tensor, gate: PackedFp8Linear, up: PackedFp8Linear, down
         raise ValueError(f"x must be [..., {H}], got {tuple(x.shape)}")
     if x.dtype != torch.bfloat16:
         raise ValueError(f"x must be bfloat16, got {x.dtype}")
+    _no_gradients(x, "fp8_swiglu")
     dev = _same_device(x, gate.codes, gate.scales, up.codes, up.scales, down.codes, down.scales, out)
     out = _fp8_out(out, x.shape, dev)
     l, N = _lib.lib(), x.numel() // H

@@ -18,6 +18,7 @@ from typing import Any, Optional
 import torch
 import torch.nn as nn
 
+from .ffn import YvFp8SwiGLU, YvSwiGLU
 from .functional import rms_norm
 from .layer import YvDeepSeekMoELayer
 
@@ -65,16 +66,22 @@ class YvHybridBlockMLP(nn.Module):
 
     forward(hybrid_out, modal_id) -> (output, aux_loss) with
     output = hybrid_out + residual_scale_mlp * mlp(norm_mlp(norm_fusion(hybrid_out))), as the
-    block computes in eval mode (residual dropout inactive). The two norms run as one kernel.
+    block computes in eval mode (residual dropout inactive). The two norms run as one kernel. ``mlp``: a dense block
+    (YvSwiGLU, YvFp8SwiGLU) in the MoE layer's place, whose loss is 0.
     """
 
     def __init__(self, cfg: Any, device=None, dtype=None, weight_format: Optional[str] = None,
-                 router: Optional[str] = None, few_tokens: Optional[int] = None):
+                 router: Optional[str] = None, few_tokens: Optional[int] = None,
+                 mlp: Optional[nn.Module] = None):
         super().__init__()
         H = cfg.hidden_size
         self.norm_fusion = YvRMSNorm(H, device=device, dtype=dtype)
-        self.mlp = YvDeepSeekMoELayer(cfg, device=device, dtype=dtype, weight_format=weight_format,
-                                      router=router, few_tokens=few_tokens)
+        if mlp is None:
+            mlp = YvDeepSeekMoELayer(cfg, device=device, dtype=dtype, weight_format=weight_format,
+                                     router=router, few_tokens=few_tokens)
+        elif mlp.hidden_size != H:
+            raise ValueError(f"mlp has hidden_size {mlp.hidden_size}, the block {H}")
+        self.mlp = mlp
         self.norm_mlp = YvRMSNorm(H, device=device, dtype=dtype)
         self.residual_scale_mlp = nn.Parameter(
             torch.ones(1, device=device, dtype=dtype) * (2.0 * cfg.n_layer) ** -0.5)
@@ -82,8 +89,9 @@ class YvHybridBlockMLP(nn.Module):
     @torch.no_grad()
     def forward(self, hybrid_out: torch.Tensor, modal_id: Optional[torch.Tensor] = None):
         x_norm = rms_norm_chain(hybrid_out, self.norm_fusion, self.norm_mlp)
-        result = self.mlp(x_norm, modal_id=modal_id)
+        dense = isinstance(self.mlp, (YvSwiGLU, YvFp8SwiGLU))
+        result = self.mlp(x_norm) if dense else self.mlp(x_norm, modal_id=modal_id)
         mlp_out, aux_loss = result if isinstance(result, (tuple, list)) else (result, None)
         if aux_loss is None:
-            aux_loss = torch.tensor(0.0, device=hybrid_out.device, dtype=hybrid_out.dtype)
+            aux_loss = torch.zeros((), device=hybrid_out.device, dtype=hybrid_out.dtype)  # captured too
         return hybrid_out + self.residual_scale_mlp * mlp_out, aux_loss
