@@ -119,20 +119,30 @@ __device__ __forceinline__ void values8(const void* x, const Hidden& h, int n, i
     else load8<SRC == kF32>(x, (size_t)n * K + k, K - k, v);
 }
 
-// One pass over the rows, bound by memory.
-template <int SRC>
+// One pass over the rows, bound by memory: U groups for 16 lanes, all of their loads in flight at once.
+template <int SRC, int U>
 __global__ __launch_bounds__(256) void fp8_rows_kernel(const void* x, Hidden h, int N, int K, int groups,
                                                        unsigned char* codes, float* scales) {
     const long long items = (long long)N * groups;
     const int l = threadIdx.x & 15;
-    for (long long it = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); it < items; it += (long long)gridDim.x * 16) {
-        const int n = (int)(it / groups), b = (int)(it - (long long)n * groups);
-        float v[8];
-        values8<SRC>(x, h, n, K, b, l, v);
-        uint2 c;
-        const float s = quantize8(v, c);
-        *(uint2*)(codes + it * kBlock + l * 8) = c;
-        if (l == 0) scales[(long long)b * N + n] = s;
+    for (long long first = (long long)blockIdx.x * 16 * U + (threadIdx.x >> 4); first < items;
+         first += (long long)gridDim.x * 16 * U) {
+        float v[U][8];
+        int n[U], b[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const long long it = std::min(first + 16 * i, items - 1);
+            n[i] = (int)(it / groups), b[i] = (int)(it - (long long)n[i] * groups);
+            values8<SRC>(x, h, n[i], K, b[i], l, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (first + 16 * i >= items) break;
+            uint2 c;
+            const float s = quantize8(v[i], c);
+            *(uint2*)(codes + (first + 16 * i) * kBlock + l * 8) = c;
+            if (l == 0) scales[(long long)b[i] * N + n[i]] = s;
+        }
     }
 }
 
@@ -575,8 +585,13 @@ inline int groups_of(int k) { return (k + kBlock - 1) / kBlock; }
 template <int SRC>
 void rows_launch(const void* x, const Hidden& h, int N, int K, void* codes, float* scales, hipStream_t st) {
     const int groups = groups_of(K);
-    const unsigned blocks = (unsigned)std::min<long long>(((long long)N * groups + 15) / 16, 1 << 16);
-    fp8_rows_kernel<SRC><<<blocks, 256, 0, st>>>(x, h, N, K, groups, (unsigned char*)codes, scales);
+    const long long items = (long long)N * groups;
+    unsigned char* c = (unsigned char*)codes;
+    // four groups at once where there are enough of them for the CUs
+    if (SRC != kHidden && items >= 1 << 17)
+        fp8_rows_kernel<SRC, 4><<<(unsigned)std::min<long long>((items + 63) / 64, 1 << 16), 256, 0, st>>>(x, h, N, K, groups, c, scales);
+    else
+        fp8_rows_kernel<SRC, 1><<<(unsigned)std::min<long long>((items + 15) / 16, 1 << 16), 256, 0, st>>>(x, h, N, K, groups, c, scales);
 }
 
 // Each block of 16 outputs reads all rows from L2: with many blocks, tiles take over from 33 rows on (1024 x 16384: 64

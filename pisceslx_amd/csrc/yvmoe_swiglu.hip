@@ -843,7 +843,7 @@ struct Plan {
 };
 Plan plan_of(int M, int N, int chunks, bool direct) {
     static const struct { int rows, cols; float alone, shared; } kinds[4] = {
-        {256, 256, 1.6f, 1.75f}, {128, 128, 0.84f, 0.58f}, {64, 64, 0.63f, 0.3f}, {64, 128, 0.9f, 0.5f}};
+        {256, 256, 1.5f, 1.7f}, {128, 128, 0.84f, 0.58f}, {64, 64, 0.63f, 0.3f}, {64, 128, 0.9f, 0.5f}};
     Plan best{256, 1, std::max(chunks, 1)};
     float least = 1e30f;
     for (int i = direct ? 3 : 0; i < (direct ? 4 : 3); ++i) {

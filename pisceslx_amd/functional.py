@@ -5,7 +5,6 @@ of them has a CPU or PyTorch fallback — a call on CPU tensors raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from dataclasses import dataclass
@@ -636,17 +635,28 @@ def int4_linear(x: torch.Tensor, weight: PackedLinear, bias: Optional[torch.Tens
 
 
 # ---------------------------------------------------------------- 8-bit floating point
-def _on(dev: torch.device):
-    """A guard for launches on ``dev`` where another device is current."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _launch(dev: torch.device, entry, *args) -> int:
+    """Calls an entry of the library with ``dev`` as the current device."""
+    if torch._C._cuda_getDevice() == dev.index:
+        return entry(*args)
+    with torch.cuda.device(dev):
+        return entry(*args)
 
 
 def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
     """_require_cuda, on one device."""
-    dev = _require_cuda(*ts)
+    dev = None
     for t in ts:
-        if t is not None and t.device != dev:
+        if t is None:
+            continue
+        if dev is None:
+            dev = t.device
+            if dev.type != "cuda":
+                raise ValueError("libyvmoe computes on the GPU only: got a CPU tensor")
+        elif t.device != dev:
             raise ValueError(f"tensors on {t.device} and {dev}")
+        if not t.is_contiguous():
+            raise ValueError("libyvmoe needs contiguous tensors")
     return dev
 
 
@@ -661,9 +671,8 @@ def quantize_fp8_rows(x: torch.Tensor) -> Fp8Rows:
     N, groups = x.numel() // K, -(-K // 128)
     rows = Fp8Rows(K, torch.empty(N, groups * 128, dtype=torch.float8_e4m3fn, device=dev),
                    torch.empty(groups, N, dtype=torch.float32, device=dev))
-    with _on(dev):
-        rc = _lib.lib().yvmoe_quantize_fp8_rows(x.data_ptr(), act, N, K, rows.codes.data_ptr(),
-                                                rows.scales.data_ptr(), _stream(dev))
+    rc = _launch(dev, _lib.lib().yvmoe_quantize_fp8_rows, x.data_ptr(), act, N, K, rows.codes.data_ptr(),
+                 rows.scales.data_ptr(), _stream(dev))
     if rc:
         _lib.check(rc, "yvmoe_quantize_fp8_rows")
     return rows
@@ -710,11 +719,10 @@ def fp8_linear(x, weight: PackedFp8Linear, bias: Optional[torch.Tensor] = None,
     nbytes = need(N, K, O)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     tail = (N, ctypes.byref(w), _ptr(bias), out.data_ptr(), ws.data_ptr(), nbytes, _stream(dev))
-    with _on(dev):
-        if rows:
-            rc = l.yvmoe_fp8_linear_rows(x.codes.data_ptr(), x.scales.data_ptr(), *tail)
-        else:
-            rc = l.yvmoe_fp8_linear(x.data_ptr(), *tail)
+    if rows:
+        rc = _launch(dev, l.yvmoe_fp8_linear_rows, x.codes.data_ptr(), x.scales.data_ptr(), *tail)
+    else:
+        rc = _launch(dev, l.yvmoe_fp8_linear, x.data_ptr(), *tail)
     if rc:
         _lib.check(rc, "yvmoe_fp8_linear")
     return out
@@ -740,9 +748,8 @@ def fp8_swiglu(x: torch.Tensor, gate: PackedFp8Linear, up: PackedFp8Linear, down
     g, u, d = gate.struct(), up.struct(), down.struct()
     nbytes = l.yvmoe_fp8_swiglu_workspace_bytes(N, H, F)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = l.yvmoe_fp8_swiglu(x.data_ptr(), N, ctypes.byref(g), ctypes.byref(u), ctypes.byref(d), out.data_ptr(),
-                                ws.data_ptr(), nbytes, _stream(dev))
+    rc = _launch(dev, l.yvmoe_fp8_swiglu, x.data_ptr(), N, ctypes.byref(g), ctypes.byref(u), ctypes.byref(d),
+                 out.data_ptr(), ws.data_ptr(), nbytes, _stream(dev))
     if rc:
         _lib.check(rc, "yvmoe_fp8_swiglu")
     return out
@@ -765,9 +772,8 @@ def _swiglu_forward(x2d, w_gate, w_up, w_down, keep: bool):
         raise ValueError(f"swiglu: {l.yvmoe_last_error().decode(errors='replace')}")
     saved = torch.empty(l.yvmoe_swiglu_saved_bytes(N, F) // 4, dtype=torch.float32, device=dev) if keep else None
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = l.yvmoe_swiglu_forward(x2d.data_ptr(), act, N, ctypes.byref(w), _ptr(saved), out.data_ptr(),
-                                    ws.data_ptr(), nbytes, _stream(dev))
+    rc = _launch(dev, l.yvmoe_swiglu_forward, x2d.data_ptr(), act, N, ctypes.byref(w), _ptr(saved), out.data_ptr(),
+                 ws.data_ptr(), nbytes, _stream(dev))
     if rc:
         _lib.check(rc, "yvmoe_swiglu_forward")
     return out, saved
@@ -792,9 +798,8 @@ class _SwiGLU(torch.autograd.Function):
         w = _lib.SwiGLUWeights(H, F, wg.data_ptr(), wu.data_ptr(), wd.data_ptr())
         nbytes = l.yvmoe_swiglu_workspace_bytes(N, act, H, F, 1)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with _on(dev):
-            rc = l.yvmoe_swiglu_backward(dy.data_ptr(), x.data_ptr(), saved.data_ptr(), act, N, ctypes.byref(w),
-                                         *map(_ptr, grads), ws.data_ptr(), nbytes, _stream(dev))
+        rc = _launch(dev, l.yvmoe_swiglu_backward, dy.data_ptr(), x.data_ptr(), saved.data_ptr(), act, N,
+                     ctypes.byref(w), *map(_ptr, grads), ws.data_ptr(), nbytes, _stream(dev))
         if rc:
             _lib.check(rc, "yvmoe_swiglu_backward")
         return tuple(grads)
@@ -809,7 +814,7 @@ def swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: to
     gradients before it once each, as operands, and the outputs. For the backward pass the call keeps x and the
     two projections in fp32 (8 bytes a row and feature of F). The gradients are not differentiable again.
     """
-    if w_gate.dim() != 2 or w_up.shape != w_gate.shape or tuple(w_down.shape) != tuple(w_gate.shape[::-1]):
+    if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.shape != w_gate.shape[::-1]:
         raise ValueError(f"weights must be [F, H], [F, H], [H, F], got {tuple(w_gate.shape)}, "
                          f"{tuple(w_up.shape)}, {tuple(w_down.shape)}")
     F, H = w_gate.shape
@@ -822,10 +827,11 @@ def swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: to
                          f"{w_down.dtype}")
     _act(x.dtype)
     _same_device(x, w_gate, w_up, w_down)
-    ts = [_aligned(t) for t in (x, w_gate, w_up, w_down)]
-    x2d = ts[0].reshape(-1, H)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        out = _SwiGLU.apply(x2d, *ts[1:])
+    x2d = _aligned(x if x.dim() == 2 else x.view(-1, H))
+    w_gate, w_up, w_down = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+                                    or w_down.requires_grad):
+        out = _SwiGLU.apply(x2d, w_gate, w_up, w_down)
     else:
-        out, _ = _swiglu_forward(x2d, *ts[1:], False)
-    return out.view(x.shape)
+        out, _ = _swiglu_forward(x2d, w_gate, w_up, w_down, False)
+    return out if x.dim() == 2 else out.view(x.shape)
