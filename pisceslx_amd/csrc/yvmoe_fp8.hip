@@ -12,6 +12,10 @@
 // number a lane. The unit's sum of 128 products keeps about 16 bits: against 64 bits its results are off by 1.4e-5
 // relative (normal values; the same for v_mfma_f32_16x16x32_fp8_fp8, four of them in a row), a hundredth of a bf16
 // output's own rounding, which is why outputs are bf16 only.
+// Where h is rounded to 8 bits, a code whose border lies within that error of h falls on the other side: about one in a
+// thousand, by a step of up to 2^-3. Over many h they add 0.0014 relative to y's own 0.0017; over few a single one can
+// be 0.006 of y. So g and u of few rows, and of up to kExactH h, are products of the codes as bf16, on the bf16 unit at
+// half the rate, with fp32's error (111 rows x 768 x 32: y 0.0067 off 64 bits on the 8-bit unit, 0.0017 so).
 //
 // Weights lie in blocks of 16 rows x 64 columns, 1 KB, lane l = 16 g + r's 16 bytes at 16 l: row r, columns
 // 16 g .. 16 g + 15 (the order of the experts' matrices); two consecutive blocks are an operand of 128, in which
@@ -30,6 +34,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kBlock = 128;
 constexpr float kMax = 448.0f, kMinScale = 1e-12f;
+constexpr long long kExactH = 1 << 18;
 
 union Op8 {  // an operand of 128 elements: two pieces of 16 bytes
     uint4 u[2];
@@ -37,6 +42,36 @@ union Op8 {  // an operand of 128 elements: two pieces of 16 bytes
 };
 __device__ __forceinline__ f32x4 mfma8(const Op8& a, const Op8& b) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+// The same codes as bf16, which holds them exactly, in four operands of v_mfma_f32_16x16x32_bf16, whose sums are fp32's.
+struct OpB {
+    bf16x8 v[4];
+};
+__device__ __forceinline__ OpB to_bf16(const Op8& a) {
+    OpB r;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        union { unsigned u[4]; bf16x8 v; } f;
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            const int w = a.v[2 * q + d];
+            f.u[2 * d] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+            f.u[2 * d + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+        }
+        r.v[q] = f.v;
+    }
+    return r;
+}
+__device__ __forceinline__ f32x4 mfma8(const OpB& a, const OpB& b) {
+    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], c, 0, 0, 0);
+    return c;
+}
+template <bool EXACT>
+__device__ __forceinline__ auto operand(const Op8& a) {
+    if constexpr (EXACT) return to_bf16(a);
+    else return a;
 }
 
 // The scale of values whose largest size has the bits m. NaN (its bits are above every other's) stays NaN.
@@ -53,7 +88,7 @@ __device__ __forceinline__ unsigned size_bits(float v) { return __float_as_uint(
 
 // ------------------------------------------------------------------ rows
 struct __attribute__((packed, aligned(2))) Any16 {  // 16 bytes at any address
-    unsigned v[4];
+    unsigned x, y, z, w;
 };
 // Eight values from element `at` of a tensor, those from `left` on zero.
 template <bool F32>
@@ -61,12 +96,14 @@ __device__ __forceinline__ void load8(const void* x, size_t at, int left, float 
     if (left >= 8) {
         if (F32) {
             const Any16 a = *(const Any16*)((const float*)x + at), b = *(const Any16*)((const float*)x + at + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(a.v[i]), v[4 + i] = __uint_as_float(b.v[i]);
+            v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
+            v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
         } else {
             const Any16 a = *(const Any16*)((const unsigned short*)x + at);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32((unsigned short)(a.v[i / 2] >> 16 * (i & 1)));
+            v[0] = bf16_to_f32((unsigned short)a.x), v[1] = bf16_to_f32((unsigned short)(a.x >> 16));
+            v[2] = bf16_to_f32((unsigned short)a.y), v[3] = bf16_to_f32((unsigned short)(a.y >> 16));
+            v[4] = bf16_to_f32((unsigned short)a.z), v[5] = bf16_to_f32((unsigned short)(a.z >> 16));
+            v[6] = bf16_to_f32((unsigned short)a.w), v[7] = bf16_to_f32((unsigned short)(a.w >> 16));
         }
     } else {
 #pragma unroll
@@ -223,6 +260,7 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Args p) {
     for (int m = 0; m < NM; ++m)
 #pragma unroll
         for (int r = 0; r < MR; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr bool EXACT = EPI == kSwiGLU;
     auto add = [&](Step& q, int t) {
         if constexpr (SRC != kCodes) {
             const int b = first + t * stride, n = min(row, p.N - 1);
@@ -235,7 +273,7 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Args p) {
         for (int m = 0; m < NM; ++m)
 #pragma unroll
             for (int r = 0; r < MR; ++r) {
-                const f32x4 d = mfma8(q.w[m], q.a[r]);
+                const f32x4 d = mfma8(operand<EXACT>(q.w[m]), operand<EXACT>(q.a[r]));
                 const float f = q.s[r] * q.ws[m];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[m][r][i] = fmaf(d[i], f, acc[m][r][i]);
@@ -337,7 +375,7 @@ __device__ __forceinline__ int swizzle(int r) { return (r >> 1 & 3) | ((r ^ r >>
 // columns, the others the up columns of the same h columns). A step is a block of 128 contraction elements: rows
 // (swizzled 128-byte lines), weights (stored order) and both scales go to LDS by direct loads, one step ahead of the
 // products, in two stages with one barrier a step.
-template <int EPI, int WR, int WC, int MB, int NB>
+template <int EPI, int WR, int WC, int MB, int NB, bool EXACT>
 __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
     constexpr int NW = WR * WC, TM = WR * 16 * MB, TN = WC * 16 * NB;
     constexpr bool DUAL = EPI == kSwiGLU;
@@ -444,23 +482,26 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
         const unsigned char* A = &lds[st][0];
         const unsigned char* B = A + A_BYTES;
         const float* S = (const float*)(B + B_BYTES);
-        Op8 a[MB];
+        decltype(operand<EXACT>(Op8{})) a[MB];
         float f[MB], f1[MB];
         const float w0 = S[DUAL ? TM : TM + (wc * 16 * NB) / kBlock], w1 = DUAL ? S[TM + 64] : 0.0f;
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
-            a[i].u[0] = *(const uint4*)(A + a_rd + i * 2048);
-            a[i].u[1] = *(const uint4*)(A + (a_rd ^ 64) + i * 2048);
+            Op8 r;
+            r.u[0] = *(const uint4*)(A + a_rd + i * 2048);
+            r.u[1] = *(const uint4*)(A + (a_rd ^ 64) + i * 2048);
+            a[i] = operand<EXACT>(r);
             const float s = S[ar + 16 * i];
             f[i] = s * w0;
             f1[i] = s * w1;
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            Op8 w;
+            Op8 r;
             const unsigned char* at = B + block_of(j) * 2048 + lane * 16;
-            w.u[0] = *(const uint4*)at;
-            w.u[1] = *(const uint4*)(at + 1024);
+            r.u[0] = *(const uint4*)at;
+            r.u[1] = *(const uint4*)(at + 1024);
+            const auto w = operand<EXACT>(r);
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
                 const f32x4 d = mfma8(w, a[i]);
@@ -649,13 +690,13 @@ void few_grid(const Fp8Args& p, hipStream_t st) {
     fp8_few_kernel<EPI, MR, SRC><<<(unsigned)(p.blocks * p.parts), 512, lds, st>>>(p);
 }
 
-template <int EPI, int WR, int WC, int MB, int NB>
+template <int EPI, int WR, int WC, int MB, int NB, bool EXACT = false>
 void tile_grid(Fp8Args p, hipStream_t st) {
     constexpr int TM = WR * 16 * MB, TN = WC * 16 * NB;
     p.ncb = ceil_div(p.O, EPI == kSwiGLU ? TN / 2 : TN);
     p.tiles = ceil_div(p.N, TM) * p.ncb;
     p.total = p.tiles * p.parts;
-    fp8_tile_kernel<EPI, WR, WC, MB, NB><<<(unsigned)(ceil_div(p.total, 8) * 8), 64 * WR * WC, 0, st>>>(p);
+    fp8_tile_kernel<EPI, WR, WC, MB, NB, EXACT><<<(unsigned)(ceil_div(p.total, 8) * 8), 64 * WR * WC, 0, st>>>(p);
 }
 
 // Rows as codes, or (few rows, SRC) made into codes in the kernel; part: the workspace of kLinear's splits.
@@ -672,6 +713,7 @@ void product_launch(Fp8Args p, float* part, hipStream_t st) {
     else if (q.tile == 0 && p.N <= 48) few_grid<EPI, 3, kCodes>(p, st);
     else if (q.tile == 0) few_grid<EPI, 4, kCodes>(p, st);
     else if (q.tile == 256) tile_grid<EPI, 4, 2, 4, 8>(p, st);
+    else if (EPI == kSwiGLU && (long long)p.N * p.O <= kExactH) tile_grid<EPI, 2, 2, 2, 4, EPI == kSwiGLU>(p, st);
     else tile_grid<EPI, 2, 2, 2, 4>(p, st);
     if (EPI == kLinear && p.parts > 1) {
         const long long quads = (long long)p.N * (p.ldp / 4);

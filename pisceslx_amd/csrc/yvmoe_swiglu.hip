@@ -27,7 +27,6 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4_t;
 constexpr int kSeg = 12;      // operand pairs of a launch: 6 term products x 2 matrices
 constexpr int kChunk = 64;    // contraction elements per LDS stage
 
-constexpr int kDirectRows = 1024;  // rows up to which fp32 weights are not packed
 constexpr int kBand = 8;      // row blocks that neighbouring tiles share columns over
 
 // Term products of an fp32 product, smallest first: (term of A, term of B).
@@ -460,7 +459,7 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
                      n0 + wc * 16 * (DUAL ? NB / 2 : NB) + 4 * (lane >> 4), split);
 }
 
-// fp32 operands as they lie, for rows that are too few to pay for packing the weights: a tile of 64 rows x 128 columns
+// fp32 operands as they lie, where they are too few products to pay for packing: a tile of 64 rows x 128 columns
 // (kSwiGLU: 64 columns of h), four wavefronts in a 2 x 2 grid of 32 rows x 64 columns, chunks of 32 contraction
 // elements in two stages. A fragment becomes three bf16 terms in registers (44 instructions of the VALU beside the 6
 // MFMAs that each pair of fragments takes), the small term products and the large ones have sums of their own. Three
@@ -908,12 +907,20 @@ void tile_launch(TileArgs p, float* part, hipStream_t st) {
 
 // Whether fp32 operands can go into the products as they lie: rows of whole 16-byte pieces.
 inline bool direct_f32(int act, int H, int F) { return act == YVMOE_ACT_F32 && H % 4 == 0 && F % 4 == 0; }
+// And whether they do: packing reads and writes 10 bytes for each of (N + 3 F) H values, at 3.5 TB/s, and takes the
+// 36 N H F operations of the term products from about 1.0 to 1.3 PFLOP/s (4096 x 11264, forward: 800 rows direct
+// 1340 us, 1200 packed 1856).
+inline bool goes_direct(int act, int N, int H, int F) {
+    return direct_f32(act, H, F) && (double)N * F < 344.0 * ((double)N + 3.0 * F);
+}
 
 // Each block of 16 columns reads all rows from L2: with many blocks, tiles take over from 33 rows on (4096 x 11264, bf16,
 // forward: 33 rows 101 us against about 95, 64 rows 137 against 98; 5120 x 1536: 64 rows 47 against 56).
-// fp32 from 33 on where it has tiles without packing (1024 x 2816: 33 rows 57 us, 65 in tiles 40).
+// fp32, where it has tiles without packing, from 33 on (1024 x 2816: 33 rows 57 us against 33, 17 rows 26 against 33), and
+// on large weights from 17 (4096 x 11264: 17 rows 179 us against 145).
 inline bool few_rows(int act, int N, int H, int F) {
-    return N <= (F >= 8192 || direct_f32(act, H, F) ? 32 : 64);
+    if (direct_f32(act, H, F)) return N <= ((long long)H * F >= 1 << 22 ? 16 : 32);
+    return N <= (F >= 8192 ? 32 : 64);
 }
 
 template <int EPI, bool F32>
@@ -945,7 +952,7 @@ int swiglu_forward_launch(const void* x, int act, int N, const yvmoe_swiglu_weig
         YV_LAUNCH_CHECK("swiglu_forward");
         return YVMOE_OK;
     }
-    const bool direct = direct_f32(act, H, F) && N <= kDirectRows;
+    const bool direct = goes_direct(act, N, H, F);
     const long long plane = (long long)N * F8;
     Operand ox{(const char*)x, H, 0}, og{(const char*)w->w_gate, H, 0}, ou{(const char*)w->w_up, H, 0},
         od{(const char*)w->w_down, F, 0};
@@ -994,7 +1001,7 @@ int swiglu_backward_launch(const void* dy, const void* x, const float* saved, in
                            size_t* bytes, hipStream_t st) {
     const int H = w->hidden, F = w->ffn, F8 = up8(F);
     const int f32 = act == YVMOE_ACT_F32, planes = f32 ? 3 : 1, terms = f32 ? 6 : 1;
-    const bool direct = direct_f32(act, H, F) && N <= kDirectRows;
+    const bool direct = goes_direct(act, N, H, F);
     Carve c{ws, bytes != nullptr, act};
     const long long plane = (long long)N * F8;
     // dy and x as operands of the weights' gradients, weights and dy of dh and dx
