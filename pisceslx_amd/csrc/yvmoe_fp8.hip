@@ -365,6 +365,13 @@ __device__ __forceinline__ void load_lds4(const void* base, unsigned off, unsign
     asm volatile("buffer_load_dword %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc_of(base)), "{m0}"(m0) : "memory");
 }
 
+// What the lanes of a wavefront wrote to LDS before this, all of them read behind it.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 constexpr int kBand = 8;
 
 // 16-byte piece c of a 128-byte row r lies at c ^ swizzle(r): the 16 lanes that read together, of two neighbouring lane
@@ -529,6 +536,13 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
         return;
     }
     if constexpr (!DUAL) {
+        // The wavefront's outputs through LDS, so that its stores are whole lines (of 8 bytes in 16 rows each: 8192 x
+        // 4096 x 8192 272 us, so 248). Piece c of eight columns of row r lies at c ^ r.
+        constexpr int PC = 2 * NB, ROWS = 16 * MB;
+        static_assert(NW * ROWS * PC * 16 <= 2 * STAGE, "the tile in LDS");
+        unsigned char* mine = &lds[0][0] + wave * (ROWS * PC * 16);
+        auto piece = [&](int r, int c) { return mine + (r * PC + (c ^ (r & (PC - 1)))) * 16; };
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int o = n0 + (wc * NB + j) * 16 + 4 * g;
@@ -536,20 +550,26 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) bias[e] = p.bias != nullptr && o + e < p.O ? bf16_to_f32(p.bias[o + e]) : 0.0f;
 #pragma unroll
-            for (int i = 0; i < MB; ++i) {
-                const int n = m0 + ar + 16 * i;
-                if (n >= p.N) continue;
-                unsigned short* dst = p.out + (long long)n * p.O + o;
-                const unsigned lo = pack_bf16(acc[i][j][0] + bias[0], acc[i][j][1] + bias[1]),
-                               hi = pack_bf16(acc[i][j][2] + bias[2], acc[i][j][3] + bias[3]);
-                if (o + 4 <= p.O && p.O % 4 == 0) {
-                    *(uint2*)dst = make_uint2(lo, hi);
-                } else {
-                    const unsigned v[2] = {lo, hi};
+            for (int i = 0; i < MB; ++i)
+                *(uint2*)(piece(16 * i + r16, 2 * j + (g >> 1)) + (g & 1) * 8) =
+                    make_uint2(pack_bf16(acc[i][j][0] + bias[0], acc[i][j][1] + bias[1]),
+                               pack_bf16(acc[i][j][2] + bias[2], acc[i][j][3] + bias[3]));
+        }
+        wave_order();
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (o + e < p.O) dst[e] = (unsigned short)(v[e / 2] >> 16 * (e & 1));
-                }
+        for (int t = 0; t < ROWS * PC / 64; ++t) {
+            const int r = (t * 64 + lane) / PC, c = lane % PC;
+            const uint4 v = *(const uint4*)piece(r, c);
+            const int n = m0 + wr * ROWS + r, o = n0 + wc * 16 * NB + c * 8;
+            if (n >= p.N) continue;
+            unsigned short* dst = p.out + (long long)n * p.O + o;
+            if (o + 8 <= p.O) {
+                *(Any16*)dst = Any16{v.x, v.y, v.z, v.w};
+            } else {
+                const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (o + e < p.O) dst[e] = (unsigned short)(w[e / 2] >> 16 * (e & 1));
             }
         }
     } else {
@@ -576,19 +596,28 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
                 if (g == 0) top[wc][ar + 16 * i] = m;
             }
             __syncthreads();
+            // and codes through LDS as the outputs above: block j of row r at j ^ r / 4
+            unsigned char* mine = &lds[0][0] + sizeof(unsigned) * WC * TM + wave * (16 * MB * NH * 16);
+            static_assert(NH == 4 && sizeof(unsigned) * WC * TM + NW * 16 * MB * NH * 16 <= 2 * STAGE, "the codes in LDS");
+            auto piece = [&](int r, int j) { return mine + (r * NH + (j ^ (r >> 2 & 3))) * 16; };
 #pragma unroll
             for (int i = 0; i < MB; ++i) {
                 const int n = m0 + ar + 16 * i;
-                if (n >= p.N) continue;
                 unsigned m = top[0][ar + 16 * i];
 #pragma unroll
                 for (int c = 1; c < WC; ++c) m = max(m, top[c][ar + 16 * i]);
                 const float s = scale_of(m);
 #pragma unroll
                 for (int j = 0; j < NH; ++j)
-                    *(unsigned*)(p.hq + (long long)n * p.ldh + n0 + (wc * NH + j) * 16 + 4 * g) =
-                        codes4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], s);
-                if (g == 0 && wc == 0) p.hs[(long long)(n0 / kBlock) * p.N + n] = s;
+                    *(unsigned*)(piece(16 * i + r16, j) + 4 * g) = codes4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], s);
+                if (g == 0 && wc == 0 && n < p.N) p.hs[(long long)(n0 / kBlock) * p.N + n] = s;
+            }
+            wave_order();
+#pragma unroll
+            for (int t = 0; t < MB; ++t) {
+                const int r = 16 * t + lane / NH, j = lane % NH;
+                const int n = m0 + wr * 16 * MB + r;
+                if (n < p.N) *(uint4*)(p.hq + (long long)n * p.ldh + n0 + (wc * NH + j) * 16) = *(const uint4*)piece(r, j);
             }
         } else {
 #pragma unroll
@@ -628,9 +657,10 @@ void rows_launch(const void* x, const Hidden& h, int N, int K, void* codes, floa
     const int groups = groups_of(K);
     const long long items = (long long)N * groups;
     unsigned char* c = (unsigned char*)codes;
-    // four groups at once where there are enough of them for the CUs
-    if (SRC != kHidden && items >= 1 << 17)
-        fp8_rows_kernel<SRC, 4><<<(unsigned)std::min<long long>((items + 63) / 64, 1 << 16), 256, 0, st>>>(x, h, N, K, groups, c, scales);
+    // four groups at once where there are enough of them for the CUs; h, whose loads are four times as many, one
+    constexpr int U = SRC == kHidden ? 1 : 4;
+    if (U > 1 && items >= 1 << 17)
+        fp8_rows_kernel<SRC, U><<<(unsigned)std::min<long long>((items + 16 * U - 1) / (16 * U), 1 << 16), 256, 0, st>>>(x, h, N, K, groups, c, scales);
     else
         fp8_rows_kernel<SRC, 1><<<(unsigned)std::min<long long>((items + 15) / 16, 1 << 16), 256, 0, st>>>(x, h, N, K, groups, c, scales);
 }
