@@ -365,13 +365,6 @@ __device__ __forceinline__ void load_lds4(const void* base, unsigned off, unsign
     asm volatile("buffer_load_dword %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc_of(base)), "{m0}"(m0) : "memory");
 }
 
-// What the lanes of a wavefront wrote to LDS before this, all of them read behind it.
-__device__ __forceinline__ void wave_order() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 constexpr int kBand = 8;
 
 // 16-byte piece c of a 128-byte row r lies at c ^ swizzle(r): the 16 lanes that read together, of two neighbouring lane

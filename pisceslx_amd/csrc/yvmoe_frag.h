@@ -47,4 +47,11 @@ union Frag16 {  // 16 bf16 = two MFMA operands
 __device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
 
 }  // namespace
+// What the lanes of a wavefront wrote to LDS before this, all of them read behind it.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 }  // namespace yvmoe

@@ -86,8 +86,9 @@ constexpr int among(int i, int n, int t, int q) { return i * n * q / (4 * t) < n
 
 __device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
 
-// How h and d are stored: one bf16 plane (rounded), three (a value is the sum of three bf16 numbers), or fp32.
-enum Planes { kOne = 1, kThree = 3, kFp32 = 0 };
+// How h and d are stored: one bf16 plane (rounded), three (a value is the sum of three bf16 numbers), or fp32; kAlone: one
+// plane of h, and neither g and u nor sums of splits.
+enum Planes { kOne = 1, kAlone = 2, kThree = 3, kFp32 = 0 };
 // Four values to element e of h or d.
 template <int PL>
 __device__ __forceinline__ void put(char* base, long long e, long long plane, const float (&v)[4]) {
@@ -98,7 +99,7 @@ __device__ __forceinline__ void put(char* base, long long e, long long plane, co
     unsigned short* p = (unsigned short*)base + e;
     float r[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-    for (int t = 0; t < PL; ++t) {
+    for (int t = 0; t < (PL == kThree ? 3 : 1); ++t) {
         const unsigned lo = pack_bf16(r[0], r[1]), hi = pack_bf16(r[2], r[3]);
         *(uint2*)(p + t * plane) = make_uint2(lo, hi);
         r[0] -= bf16_to_f32((unsigned short)(lo & 0xffff)), r[1] -= bf16_to_f32((unsigned short)(lo >> 16));
@@ -129,7 +130,7 @@ template <int PL>
 __device__ __forceinline__ void finish_swiglu(const Finish& p, int m, int n, f32x4 g, f32x4 u) {
     if (m >= p.M || n >= p.ldh) return;
     const long long e = (long long)m * p.ldh + n;
-    if (p.gu != nullptr) {
+    if (PL != kAlone && p.gu != nullptr) {
         *(f32x4*)(p.gu + e) = g;
         *(f32x4*)(p.gu + (long long)p.M * p.ldh + e) = u;
     }
@@ -156,33 +157,67 @@ __device__ __forceinline__ void finish_grad(const Finish& p, int m, int n, f32x4
     put<PL>(p.d, ed + p.ldh, p.plane_d, du);
     put<PL>(p.h, e, p.plane_h, h);
 }
-// Block AT of a wavefront and those after it. Written out by recursion: `#pragma unroll` gives up on bodies as long as
-// these, and the sums would then go through memory.
-template <int EPI, int PL, int MB, int NB, int AT = 0>
-__device__ __forceinline__ void finish_blocks(const Finish& p, const f32x4 (&acc)[MB][NB], int m, int n) {
-    constexpr int NH = EPI == kSwiGLU ? NB / 2 : NB, i = AT / NH, j = AT % NH;
-    if constexpr (EPI == kOut) finish_out(p, m + 16 * i, n + 16 * j, acc[i][j]);
-    else if constexpr (EPI == kGrad) finish_grad<PL>(p, m + 16 * i, n + 16 * j, acc[i][j]);
-    else finish_swiglu<PL>(p, m + 16 * i, n + 16 * j, acc[i][j], acc[i][j + NH]);
-    asm volatile("" ::: "memory");  // one block's addresses at a time
-    if constexpr (AT + 1 < MB * NH) finish_blocks<EPI, PL, MB, NB, AT + 1>(p, acc, m, n);
-}
-// A wavefront's blocks: (i, j) holds row m + 16 i, columns n + 16 j .. + 3 (kSwiGLU: of gate, then of up).
-template <int EPI, int PL, int MB, int NB>
-__device__ __forceinline__ void finish(const Finish& p, const f32x4 (&acc)[MB][NB], int m, int n, int split) {
-    constexpr int NH = EPI == kSwiGLU ? NB / 2 : NB;
+// Blocks of 16 rows that a wavefront moves through LDS at a time, and their 16-byte quads: 4 x 4 NB KB fit the stages.
+constexpr int finish_rows(int mb) { return mb < 4 ? mb : 4; }
+constexpr int finish_quads(int mb, int nb) { return finish_rows(mb) * nb * 64; }
+template <int EPI, int PL>
+__device__ __forceinline__ void finish_quad(const Finish& p, int m, int n, f32x4 v, f32x4 u, int split) {
     if (p.part != nullptr) {
-        float* part = p.part + (long long)split * (EPI == kSwiGLU ? 2 : 1) * p.M * p.ldp;
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                const int r = m + 16 * i, c = n + 16 * (j % NH);
-                if (r < p.M && c < p.ldp) *(f32x4*)(part + (j / NH * (long long)p.M + r) * p.ldp + c) = acc[i][j];
-            }
-        return;
+        if (m >= p.M || n >= p.ldp) return;
+        float* to = p.part + ((long long)split * (EPI == kSwiGLU ? 2 : 1) * p.M + m) * p.ldp + n;
+        *(f32x4*)to = v;
+        if (EPI == kSwiGLU) *(f32x4*)(to + (long long)p.M * p.ldp) = u;
+    } else if constexpr (EPI == kOut) {
+        finish_out(p, m, n, v);
+    } else if constexpr (EPI == kGrad) {
+        finish_grad<PL>(p, m, n, v);
+    } else {
+        finish_swiglu<PL>(p, m, n, v, u);
     }
-    finish_blocks<EPI, PL>(p, acc, m, n);
+}
+// h of the wavefront's block AT and of those after it. Written out by recursion: `#pragma unroll` gives up on bodies as
+// long as these, and the sums would then go through memory.
+template <int MB, int NB, int AT = 0>
+__device__ __forceinline__ void finish_blocks(const Finish& p, const f32x4 (&acc)[MB][NB], int m, int n) {
+    constexpr int NH = NB / 2, i = AT / NH, j = AT % NH;
+    finish_swiglu<kAlone>(p, m + 16 * i, n + 16 * j, acc[i][j], acc[i][j + NH]);
+    asm volatile("" ::: "memory");  // one block's addresses at a time
+    if constexpr (AT + 1 < MB * NH) finish_blocks<MB, NB, AT + 1>(p, acc, m, n);
+}
+// A wavefront's blocks, from row m and column n on: lane 16 g + r of block (i, j) holds row 16 i + r, columns 16 j + 4 g
+// .. + 3 (kSwiGLU: of gate, then of up). They go through LDS, B blocks of rows at a time, so that the lanes then hold
+// whole rows and what they write and read is whole lines, not quarters of 16 (a training step of
+// 4096 x 4096 x 11264 3008 us, so 2940; fp32, 2052 x 1024 x 2816, 787 and 760). Quad c of row r lies at c ^ r. The
+// loop over the quads stays one: written out, the code would come from memory more slowly than it runs.
+template <int EPI, int PL, int MB, int NB>
+__device__ __forceinline__ void finish(const Finish& p, const f32x4 (&acc)[MB][NB], f32x4* mine, int m, int n, int split) {
+    constexpr int NH = EPI == kSwiGLU ? NB / 2 : NB, Q = 4 * NH, B = finish_rows(MB), G = B * NH < 4 ? B * NH : 4;
+    const int lane = threadIdx.x & 63;
+    // bf16 h alone: 8 bytes for 32 that LDS would move (8192 x 1024 x 2816: 149 us a block, through LDS 159)
+    if constexpr (PL == kAlone) return finish_blocks(p, acc, m + (lane & 15), n + 4 * (lane >> 4));
+    auto quad = [&](int mat, int r, int c) { return mine + (mat * 16 * B + r) * Q + (c ^ (r & 15 & (Q - 1))); };
+#pragma unroll
+    for (int i0 = 0; i0 < MB; i0 += B) {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                *quad(j / NH, 16 * i + (lane & 15), 4 * (j % NH) + (lane >> 4)) = acc[i0 + i][j];
+        wave_order();
+#pragma unroll 1
+        for (int t = 0; t < B * NH; t += G) {
+            f32x4 v[G], u[G];
+#pragma unroll
+            for (int k = 0; k < G; ++k) {
+                const int r = (64 * (t + k) + lane) / Q, c = lane % Q;
+                v[k] = *quad(0, r, c), u[k] = *quad(NB / NH - 1, r, c);
+            }
+#pragma unroll
+            for (int k = 0; k < G; ++k)
+                finish_quad<EPI, PL>(p, m + 16 * i0 + (64 * (t + k) + lane) / Q, n + 4 * (lane % Q), v[k], u[k], split);
+        }
+        wave_order();
+    }
 }
 
 // Of bf16, whose lane groups g read pieces g, and of fp32, where they read pieces 2 g.
@@ -334,6 +369,7 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     typedef Stage<BMC, TN> SB;
     constexpr int DA = SA::LOADS, D = SA::LOADS + SB::LOADS;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[2][SA::BYTES + SB::BYTES];
+    static_assert(4 * 16 * finish_quads(MB, NB) <= 2 * (SA::BYTES + SB::BYTES), "the sums in LDS");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave >> 1, wc = wave & 1;
@@ -455,8 +491,9 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
 
     const Finish fin = p;  // apart from the arguments that the loop indexes
-    finish<EPI, PL>(fin, acc, m0 + wr * 16 * MB + (lane & 15),
-                     n0 + wc * 16 * (DUAL ? NB / 2 : NB) + 4 * (lane >> 4), split);
+    __syncthreads();
+    finish<EPI, PL>(fin, acc, (f32x4*)&lds[0][0] + wave * finish_quads(MB, NB), m0 + wr * 16 * MB,
+                    n0 + wc * 16 * (DUAL ? NB / 2 : NB), split);
 }
 
 // fp32 operands as they lie, where they are too few products to pay for packing: a tile of 64 rows x 128 columns
@@ -471,6 +508,7 @@ __global__ __launch_bounds__(256) void swiglu_f32_kernel(TileArgs p) {
     typedef Stage<false, TM, true> SA;
     typedef Stage<BMC, TN, true> SB;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[2][SA::BYTES + SB::BYTES];
+    static_assert(4 * 16 * finish_quads(MB, NB) <= 2 * (SA::BYTES + SB::BYTES), "the sums in LDS");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave >> 1, wc = wave & 1;
@@ -550,8 +588,9 @@ __global__ __launch_bounds__(256) void swiglu_f32_kernel(TileArgs p) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) large[i][j] = large[i][j] + small[i][j];
     const Finish fin = p;
-    finish<EPI, kFp32>(fin, large, m0 + wr * 16 * MB + (lane & 15),
-                     n0 + wc * 16 * (DUAL ? NB / 2 : NB) + 4 * (lane >> 4), split);
+    __syncthreads();
+    finish<EPI, kFp32>(fin, large, (f32x4*)&lds[0][0] + wave * finish_quads(MB, NB), m0 + wr * 16 * MB,
+                       n0 + wc * 16 * (DUAL ? NB / 2 : NB), split);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -876,6 +915,13 @@ void tile_grid(TileArgs p, int splits, hipStream_t st) {
     swiglu_tile_kernel<EPI, PL, AMC, BMC, MB, NB><<<(unsigned)(ceil_div(p.total, 8) * 8), 256, 0, st>>>(p);
 }
 
+template <int EPI, int PL, bool AMC, bool BMC>
+void tiles_of(const TileArgs& p, const Plan& q, hipStream_t st) {
+    if (q.tile == 256) tile_grid<EPI, PL, AMC, BMC, 8, 8>(p, q.splits, st);
+    else if (q.tile == 128) tile_grid<EPI, PL, AMC, BMC, 4, 4>(p, q.splits, st);
+    else tile_grid<EPI, PL, AMC, BMC, 2, 2>(p, q.splits, st);
+}
+
 // PL: kSwiGLU, kGrad, how h and d are stored; kOut with kFp32: the fp32 form on operands as they lie.
 template <int EPI, int PL, bool AMC, bool BMC>
 void tile_launch(TileArgs p, float* part, hipStream_t st) {
@@ -892,12 +938,11 @@ void tile_launch(TileArgs p, float* part, hipStream_t st) {
         p.tiles = ceil_div(p.M, 64) * p.ncb;
         p.total = p.tiles * q.splits;
         swiglu_f32_kernel<EPI, BMC><<<(unsigned)(ceil_div(p.total, 8) * 8), 256, 0, st>>>(p);
-    } else if (q.tile == 256) {
-        tile_grid<EPI, PL, AMC, BMC, 8, 8>(p, q.splits, st);
-    } else if (q.tile == 128) {
-        tile_grid<EPI, PL, AMC, BMC, 4, 4>(p, q.splits, st);
+    } else if constexpr (EPI == kSwiGLU && PL == kOne) {
+        if (p.gu == nullptr && q.splits == 1) tiles_of<EPI, kAlone, AMC, BMC>(p, q, st);
+        else tiles_of<EPI, PL, AMC, BMC>(p, q, st);
     } else {
-        tile_grid<EPI, PL, AMC, BMC, 2, 2>(p, q.splits, st);
+        tiles_of<EPI, PL, AMC, BMC>(p, q, st);
     }
     if (q.splits > 1) {
         const long long quads = (long long)p.M * (p.ldp / 4);
