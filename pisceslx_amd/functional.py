@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import weakref
 from dataclasses import dataclass
 from typing import Optional
 
@@ -779,16 +780,34 @@ def _swiglu_forward(x2d, w_gate, w_up, w_down, keep: bool):
     return out, saved
 
 
+_training = weakref.WeakSet()  # contexts of swiglu calls whose graphs live
+
+
+def _refuse_other_streams(ctx) -> None:
+    """A leaf's gradient is added on the stream of its oldest living graph. Where that is not the stream that is being
+    captured, torch has the two wait for one another, which a capture does not survive."""
+    for other in list(_training):
+        if other.stream != ctx.stream and not other.leaves.isdisjoint(ctx.leaves):
+            raise RuntimeError("swiglu: this backward pass is being captured while a graph of the same leaves that was "
+                               "recorded on another stream lives: drop its outputs first")
+
+
 class _SwiGLU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2d, w_gate, w_up, w_down):
         out, saved = _swiglu_forward(x2d, w_gate, w_up, w_down, True)
         ctx.save_for_backward(x2d, w_gate, w_up, w_down, saved)
+        ctx.stream = _stream(x2d.device)
+        # x2d may be a view of the leaf
+        ctx.leaves = {id(t if t.is_leaf else t._base) for t in (x2d, w_gate, w_up, w_down)} - {id(None)}
+        _training.add(ctx)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.cuda.is_current_stream_capturing():
+            _refuse_other_streams(ctx)
         x, wg, wu, wd, saved = ctx.saved_tensors
         l, (N, H), F, dev = _lib.lib(), x.shape, wg.shape[0], x.device
         act = _act(x.dtype)
@@ -812,7 +831,8 @@ def swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: to
     x [..., H], w_gate and w_up [F, H], w_down [H, F] (nn.Linear.weight), all bf16 or all fp32, contiguous;
     any sizes up to 2^24 rows and 2^20 features. Sums are fp32; bf16 rounds the activated product and the two
     gradients before it once each, as operands, and the outputs. For the backward pass the call keeps x and the
-    two projections in fp32 (8 bytes a row and feature of F). The gradients are not differentiable again.
+    two projections in fp32 (8 bytes a row and feature of F). The gradients are not differentiable again. A backward
+    pass that is being captured is refused while a call's graph of the same leaves on another stream lives.
     """
     if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.shape != w_gate.shape[::-1]:
         raise ValueError(f"weights must be [F, H], [F, H], [H, F], got {tuple(w_gate.shape)}, "

@@ -1,5 +1,6 @@
 """The gated feed-forward block with gradients on the host: refusals and workspace sizes."""
 import ctypes
+import weakref
 
 import pytest
 import torch
@@ -86,3 +87,39 @@ def test_refused_in_python():
                  lambda: yvf.swiglu(torch.zeros(3, 0), torch.zeros(8, 0), torch.zeros(8, 0), torch.zeros(0, 8))):
         with pytest.raises(ValueError):
             call()
+
+
+class _Recorded:
+    """What a training call's context holds."""
+
+    def __init__(self, stream, *leaves):
+        self.stream, self.leaves = stream, {id(t) for t in leaves}
+
+
+def test_captured_backward_beside_a_living_graph(monkeypatch):
+    """A backward pass is not captured while a graph of the same leaves on another stream lives."""
+    w, other = torch.zeros(1), torch.zeros(1)
+    monkeypatch.setattr(yvf, "_training", weakref.WeakSet())
+    mine, eager, same, apart = _Recorded(7, w), _Recorded(3, w, other), _Recorded(7, w), _Recorded(3, other)
+    for c in (mine, same, apart):
+        yvf._training.add(c)
+    yvf._refuse_other_streams(mine)
+    yvf._training.add(eager)
+    with pytest.raises(RuntimeError, match="another stream lives"):
+        yvf._refuse_other_streams(mine)
+    del eager
+    yvf._refuse_other_streams(mine)
+
+
+def test_a_training_call_is_known_while_its_graph_lives(monkeypatch):
+    """The context keeps the leaves, x's behind a view too, and is forgotten with the call's outputs."""
+    monkeypatch.setattr(yvf, "_swiglu_forward", lambda x, *w: (x * 1, None))
+    monkeypatch.setattr(yvf, "_stream", lambda device: 5)
+    monkeypatch.setattr(yvf, "_training", weakref.WeakSet())
+    x, w = torch.zeros(2, 3, 4, requires_grad=True), torch.zeros(4, 4, requires_grad=True)
+    derived = w * 1
+    y = yvf._SwiGLU.apply(x.view(-1, 4), w, derived, w)
+    (ctx,) = yvf._training
+    assert ctx.stream == 5 and ctx.leaves == {id(x), id(w)}
+    del ctx, y
+    assert not yvf._training
