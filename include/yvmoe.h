@@ -506,8 +506,8 @@ int32_t yvmoe_fp8_swiglu(const void* x, int32_t n_rows, const yvmoe_fp8_matrix* 
  *   g = x w_gateᵀ, u = x w_upᵀ, h = silu(g) u, out = h w_downᵀ
  * x and out [N][hidden], w_gate and w_up [ffn][hidden], w_down [hidden][ffn], all in the activation dtype and
  * 16-byte aligned. bf16: h is rounded once, as an operand, and the output once; sums and everything between
- * are fp32. fp32: operands as three bf16 terms (24 bits); an infinity or a number beyond bf16's largest
- * (3.39e38) among them gives NaN, numbers below 2^-110 lose their last bits.
+ * are fp32. fp32: operands as three bf16 terms (24 bits); an infinity among them gives NaN, as may (by sizes) a
+ * number beyond bf16's largest (3.39e38), and numbers below 2^-110 may lose their last bits.
  * saved: yvmoe_swiglu_saved_bytes() for the backward pass (g and u in fp32), or NULL; 16-byte aligned.
  *
  * Its gradients, from dy [N][hidden] and the forward call's x, weights and saved:

@@ -374,7 +374,9 @@ __device__ __forceinline__ int swizzle(int r) { return (r >> 1 & 3) | ((r ^ r >>
 // Tiles: WR x WC wavefronts of 16 MB rows x 16 NB columns each (kSwiGLU: the wavefront's first NB / 2 blocks are gate
 // columns, the others the up columns of the same h columns). A step is a block of 128 contraction elements: rows
 // (swizzled 128-byte lines), weights (stored order) and both scales go to LDS by direct loads, one step ahead of the
-// products, in two stages with one barrier a step.
+// products, in two stages with one barrier a step. 256 x 256 tiles: 8192 x 4096 x 8192 in 248 us, 2.2 PFLOP/s, of which
+// 60 are the ends of four rounds of tiles; of the rest the scales are a tenth, the loads another, and the matrix unit by
+// itself, at the card's power, the others. Wavefronts 8 x 1, 4 x 4 or 8 x 2 and fragments read a step ahead are no faster.
 template <int EPI, int WR, int WC, int MB, int NB, bool EXACT>
 __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
     constexpr int NW = WR * WC, TM = WR * 16 * MB, TN = WC * 16 * NB;
