@@ -243,3 +243,15 @@ def test_on_another_stream(cuda):
         got = yvf.fp8_linear(x, p)
     s.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("n,o", [(2090, 4999), (2500, 5132), (130, 4107), (70, 1003)])
+def test_ends_of_tiles(cuda, n, o):
+    """Outputs of odd widths leave the tiles whole, with a bias, and nothing behind the last row is written."""
+    x, w = make_rows(n, 200, n), make_weight(o, 200, o)
+    b = torch.randn(o, generator=torch.Generator().manual_seed(o)).to(torch.bfloat16)
+    buf = torch.full((n + 3, o), 7.0, dtype=torch.bfloat16, device=cuda)
+    p = packed(w, cuda)
+    yvf.fp8_linear(x.to(cuda), p, b.to(cuda), out=buf[:n])
+    assert (buf[n:] == 7).all()
+    check_linear(buf[:n], x, w, b, f"linear {n} x 200 x {o}")

@@ -234,3 +234,13 @@ def test_on_another_stream(cuda):
     s.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("N,H,F,dtype", [(2050, 520, 3080, torch.bfloat16), (700, 1000, 1030, torch.bfloat16),
+                                         (90, 2048, 1536, torch.bfloat16), (1500, 512, 2050, torch.float32)])
+def test_without_gradients_the_same_bits(cuda, N, H, F, dtype):
+    """The forward pass that keeps nothing, in tiles of each size and split: the bits of the one that keeps g and u."""
+    x, wg, wu, wd, _ = (t.to(cuda) for t in make(N, H, F, dtype, seed=3))
+    kept = yvf.swiglu(x.requires_grad_(True), wg, wu, wd).detach()
+    with torch.no_grad():
+        assert torch.equal(yvf.swiglu(x, wg, wu, wd), kept)
