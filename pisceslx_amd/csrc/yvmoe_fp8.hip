@@ -84,6 +84,15 @@ __device__ __forceinline__ unsigned codes4(float a, float b, float c, float d, f
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(a / s, b / s, 0, false);
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c / s, d / s, w, true);
 }
+// The same of many values over one s, with its inverse: a product and a correction instead of a division.
+__device__ __forceinline__ float over(float a, float s, float inverse) {
+    const float q = a * inverse;
+    return fmaf(fmaf(-q, s, a), inverse, q);
+}
+__device__ __forceinline__ unsigned codes4(const f32x4& v, float s, float inverse) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(over(v[0], s, inverse), over(v[1], s, inverse), 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(over(v[2], s, inverse), over(v[3], s, inverse), w, true);
+}
 __device__ __forceinline__ unsigned size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // ------------------------------------------------------------------ rows
@@ -134,7 +143,7 @@ __device__ __forceinline__ void load8(const Hidden& h, size_t at, int left, floa
 #pragma unroll
             for (int q = 0; q < 2; ++q) s[m][q] = s[m][q] + *(const f32x4*)(h.p + (2 * k + m) * h.plane + at + 4 * q);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i >= left ? 0.0f : silu(s[0][i / 4][i % 4]) * s[1][i / 4][i % 4];
+    for (int i = 0; i < 8; ++i) v[i] = i >= left ? 0.0f : silu_fast(s[0][i / 4][i % 4]) * s[1][i / 4][i % 4];
 }
 
 // 16 lanes hold a group of 128, eight values each: its scale, and the lane's codes.
@@ -333,7 +342,7 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Args p) {
         if (p.parts == 1) {
             f32x4 h;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = silu(v[0][i]) * v[NM - 1][i];
+            for (int i = 0; i < 4; ++i) h[i] = silu_fast(v[0][i]) * v[NM - 1][i];
             *(f32x4*)(p.h + at) = h;
         } else {
             *(f32x4*)(p.h + 2 * split * plane + at) = v[0];
@@ -577,7 +586,7 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
 #pragma unroll
             for (int j = 0; j < NH; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = silu(acc[i][j][e]) * acc[i][j + NH][e];
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = silu_fast(acc[i][j][e]) * acc[i][j + NH][e];
         if constexpr (TN / 2 == kBlock) {
             // the tile holds whole groups of h: their largest sizes through LDS, then codes
             unsigned(*top)[TM] = (unsigned(*)[TM])&lds[0][0];
@@ -604,10 +613,9 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
                 unsigned m = top[0][ar + 16 * i];
 #pragma unroll
                 for (int c = 1; c < WC; ++c) m = max(m, top[c][ar + 16 * i]);
-                const float s = scale_of(m);
+                const float s = scale_of(m), inverse = 1.0f / s;
 #pragma unroll
-                for (int j = 0; j < NH; ++j)
-                    *(unsigned*)(piece(16 * i + r16, j) + 4 * g) = codes4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], s);
+                for (int j = 0; j < NH; ++j) *(unsigned*)(piece(16 * i + r16, j) + 4 * g) = codes4(acc[i][j], s, inverse);
                 if (g == 0 && wc == 0 && n < p.N) p.hs[(long long)(n0 / kBlock) * p.N + n] = s;
             }
             wave_order();

@@ -84,8 +84,6 @@ __device__ __forceinline__ void mfma_acc(f32x4& acc, const bf16x8& a, const bf16
 // How many of n instructions go before MFMA i of t, spread over the first 4 / q of them.
 constexpr int among(int i, int n, int t, int q) { return i * n * q / (4 * t) < n ? i * n * q / (4 * t) : n; }
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
-
 // How h and d are stored: one bf16 plane (rounded), three (a value is the sum of three bf16 numbers), or fp32; kAlone: one
 // plane of h, and neither g and u nor sums of splits. kOut: kFar, results that are read long after (past()).
 enum Planes { kOne = 1, kAlone = 2, kThree = 3, kFp32 = 0, kFar = 4 };
@@ -152,7 +150,7 @@ __device__ __forceinline__ void finish_swiglu(const Finish& p, int m, int n, f32
     }
     float h[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) h[q] = silu(g[q]) * u[q];
+    for (int q = 0; q < 4; ++q) h[q] = silu_fast(g[q]) * u[q];
     put<PL>(p.h, e, p.plane_h, h);
 }
 template <int PL>
@@ -164,7 +162,7 @@ __device__ __forceinline__ void finish_grad(const Finish& p, int m, int n, f32x4
     float dg[4], du[4], h[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        const float s = sigmoid(g[q]), a = g[q] * s;
+        const float s = sigmoid_fast(g[q]), a = g[q] * s;
         h[q] = a * u[q];
         du[q] = dh[q] * a;
         dg[q] = dh[q] * u[q] * (s + a * (1.0f - s));
@@ -752,7 +750,7 @@ __global__ __launch_bounds__(512) void swiglu_few_kernel(FewArgs p) {
             const bool in = o + e < p.O;
             if (o + e >= p.ldh) continue;
             // behind the last column: zeros, as the tiles write them
-            const float a = in ? v[0][e] : 0.0f, u = in ? v[NM - 1][e] : 0.0f, h = silu(a) * u;
+            const float a = in ? v[0][e] : 0.0f, u = in ? v[NM - 1][e] : 0.0f, h = silu_fast(a) * u;
             if (p.gu != nullptr) p.gu[at] = a, p.gu[(size_t)p.N * p.ldh + at] = u;
             if (F32) ((float*)p.out)[at] = h;
             else ((unsigned short*)p.out)[at] = f32_to_bf16_rne(h);
