@@ -79,20 +79,23 @@ __device__ __forceinline__ float scale_of(unsigned m) {
     const float s = __uint_as_float(m) / kMax;
     return s < kMinScale ? kMinScale : s;
 }
-// e4m3 codes of four values over s, lowest first
-__device__ __forceinline__ unsigned codes4(float a, float b, float c, float d, float s) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a / s, b / s, 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c / s, d / s, w, true);
-}
-// The same of many values over one s, with its inverse: a product and a correction instead of a division.
-__device__ __forceinline__ float over(float a, float s, float inverse) {
-    const float q = a * inverse;
-    return fmaf(fmaf(-q, s, a), inverse, q);
-}
-__device__ __forceinline__ unsigned codes4(const f32x4& v, float s, float inverse) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(over(v[0], s, inverse), over(v[1], s, inverse), 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(over(v[2], s, inverse), over(v[3], s, inverse), w, true);
-}
+// Values over one s and their codes. A quotient is the value times 1 / s, and its remainder times 1 / s added: off the exact
+// quotient by 2^-22 of an fp32 step before the last rounding, so that it is the rounded quotient, but perhaps where that
+// lies as near the middle of two fp32 numbers; next to the middle of two codes, where it would count, no quotient of two fp32
+// numbers whose s could do so does (by trying them all: s within 24 steps of a multiple of 1/8 of its power of two).
+struct Divisor {
+    float s, inverse;
+    __device__ __forceinline__ explicit Divisor(float by) : s(by == INFINITY ? 0.0f : by), inverse(1.0f / by) {}
+    __device__ __forceinline__ float under(float a) const {
+        const float q = a * inverse;
+        return copysignf(fmaf(fmaf(-q, s, a), inverse, q), a);  // of -0 too
+    }
+    // e4m3 codes of four values, lowest first
+    __device__ __forceinline__ unsigned codes4(float a, float b, float c, float d) const {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(under(a), under(b), 0, false);
+        return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(under(c), under(d), w, true);
+    }
+};
 __device__ __forceinline__ unsigned size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // ------------------------------------------------------------------ rows
@@ -154,7 +157,8 @@ __device__ __forceinline__ float quantize8(const float (&v)[8], uint2& codes) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 16));
     const float s = scale_of(m);
-    codes = make_uint2(codes4(v[0], v[1], v[2], v[3], s), codes4(v[4], v[5], v[6], v[7], s));
+    const Divisor by(s);
+    codes = make_uint2(by.codes4(v[0], v[1], v[2], v[3]), by.codes4(v[4], v[5], v[6], v[7]));
     return s;
 }
 
@@ -613,9 +617,11 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
                 unsigned m = top[0][ar + 16 * i];
 #pragma unroll
                 for (int c = 1; c < WC; ++c) m = max(m, top[c][ar + 16 * i]);
-                const float s = scale_of(m), inverse = 1.0f / s;
+                const float s = scale_of(m);
+                const Divisor by(s);
 #pragma unroll
-                for (int j = 0; j < NH; ++j) *(unsigned*)(piece(16 * i + r16, j) + 4 * g) = codes4(acc[i][j], s, inverse);
+                for (int j = 0; j < NH; ++j)
+                    *(unsigned*)(piece(16 * i + r16, j) + 4 * g) = by.codes4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
                 if (g == 0 && wc == 0 && n < p.N) p.hs[(long long)(n0 / kBlock) * p.N + n] = s;
             }
             wave_order();

@@ -255,3 +255,19 @@ def test_ends_of_tiles(cuda, n, o):
     yvf.fp8_linear(x.to(cuda), p, b.to(cuda), out=buf[:n])
     assert (buf[n:] == 7).all()
     check_linear(buf[:n], x, w, b, f"linear {n} x 200 x {o}")
+
+
+@pytest.mark.parametrize("n", [40, 40000])
+def test_rows_by_every_kind_of_scale(cuda, n):
+    """Codes are those of the rounded quotient, at scales of all mantissas and beside the borders between codes: each
+    group holds 448 s, which makes its scale s, and values at t / 16 s and its fp32 neighbours, t from 16 to 31."""
+    g = torch.Generator().manual_seed(n)
+    s = torch.randint(0, 1 << 23, (n,), generator=g)
+    s[::2] = (s[::2] & ~0xfffff) + torch.randint(-20, 20, (len(s[::2]),), generator=g)  # beside multiples of 1 / 8
+    s = (s.clamp(min=0).to(torch.int32) + (127 << 23)).view(torch.float32)
+    t = torch.arange(16, 32) / 16.0
+    near = (t[None] * s[:, None]).view(torch.int32)[:, :, None] + torch.arange(-3, 4, dtype=torch.int32)
+    x = torch.cat([448 * s[:, None], near.view(torch.float32).view(n, -1), torch.zeros(n, 15)], 1)
+    x = x * torch.randint(-12, 12, (n, 1), generator=g).float().exp2()
+    q, _ = ref.rows(x)
+    assert same_codes(yvf.quantize_fp8_rows(x.to(cuda)).codes, q)
