@@ -799,7 +799,8 @@ class _SwiGLU(torch.autograd.Function):
         ctx.save_for_backward(x2d, w_gate, w_up, w_down, saved)
         ctx.stream = _stream(x2d.device)
         # x2d may be a view of the leaf
-        ctx.leaves = {id(t if t.is_leaf else t._base) for t in (x2d, w_gate, w_up, w_down)} - {id(None)}
+        leaves = (t if t.is_leaf else t._base for t in (x2d, w_gate, w_up, w_down))
+        ctx.leaves = {id(t) for t in leaves if t is not None and t.requires_grad}
         _training.add(ctx)
         return out
 

@@ -123,3 +123,14 @@ def test_a_training_call_is_known_while_its_graph_lives(monkeypatch):
     assert ctx.stream == 5 and ctx.leaves == {id(x), id(w)}
     del ctx, y
     assert not yvf._training
+
+
+def test_what_needs_no_gradient_is_no_leaf(monkeypatch):
+    """Two calls that share only an input without gradients share no leaves."""
+    monkeypatch.setattr(yvf, "_swiglu_forward", lambda x, *w: (x * 1, None))
+    monkeypatch.setattr(yvf, "_stream", lambda device: 5)
+    monkeypatch.setattr(yvf, "_training", weakref.WeakSet())
+    x, w = torch.zeros(2, 4), [torch.zeros(4, 4, requires_grad=True) for _ in range(2)]
+    ys = [yvf._SwiGLU.apply(x, v, v, v) for v in w]
+    assert sorted(map(sorted, (c.leaves for c in yvf._training))) == sorted([id(v)] for v in w)
+    del ys
