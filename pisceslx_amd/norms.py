@@ -67,7 +67,8 @@ class YvHybridBlockMLP(nn.Module):
     forward(hybrid_out, modal_id) -> (output, aux_loss) with
     output = hybrid_out + residual_scale_mlp * mlp(norm_mlp(norm_fusion(hybrid_out))), as the
     block computes in eval mode (residual dropout inactive). The two norms run as one kernel. ``mlp``: a dense block
-    (YvSwiGLU, YvFp8SwiGLU) in the MoE layer's place, whose loss is 0.
+    (YvSwiGLU, YvFp8SwiGLU) in the MoE layer's place, whose loss is 0. Inference only: a forward with the mlp in
+    training mode raises, also with YvSwiGLU, which has gradients by itself.
     """
 
     def __init__(self, cfg: Any, device=None, dtype=None, weight_format: Optional[str] = None,
@@ -88,8 +89,10 @@ class YvHybridBlockMLP(nn.Module):
 
     @torch.no_grad()
     def forward(self, hybrid_out: torch.Tensor, modal_id: Optional[torch.Tensor] = None):
-        x_norm = rms_norm_chain(hybrid_out, self.norm_fusion, self.norm_mlp)
         dense = isinstance(self.mlp, (YvSwiGLU, YvFp8SwiGLU))
+        if dense and self.mlp.training:
+            raise NotImplementedError("YvHybridBlockMLP is an inference forward; call .eval()")
+        x_norm = rms_norm_chain(hybrid_out, self.norm_fusion, self.norm_mlp)
         result = self.mlp(x_norm) if dense else self.mlp(x_norm, modal_id=modal_id)
         mlp_out, aux_loss = result if isinstance(result, (tuple, list)) else (result, None)
         if aux_loss is None:
