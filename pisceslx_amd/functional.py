@@ -661,13 +661,22 @@ def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
+def _no_gradients(what: str, *ts: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError(f"{what} is inference only: an operand requires a gradient (detach it, or use "
+                                          "torch.no_grad)")
+
+
 def quantize_fp8_rows(x: torch.Tensor) -> Fp8Rows:
     """Rows of x [..., features] (bf16 or fp32) in e4m3fn with a scale per 128 values, the left operand of
     fp8_linear: scale = max(max|x| / 448, 1e-12), code = e4m3fn(x / scale), in fp32 divisions and rounded to
     nearest even (quantize_to_fp8, opss/quantize/engine.py:841-883, per 128 values). A group with an infinity or
-    NaN makes every product of its row NaN. Up to 2^24 rows of up to 2^20 features."""
+    NaN makes every product of its row NaN. Up to 2^24 rows of up to 2^20 features; inference only."""
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"x must be [..., features], got {tuple(x.shape)}")
+    _no_gradients("quantize_fp8_rows", x)
     dev, act, K = _same_device(x), _act(x.dtype), x.shape[-1]
     N, groups = x.numel() // K, -(-K // 128)
     rows = Fp8Rows(K, torch.empty(N, groups * 128, dtype=torch.float8_e4m3fn, device=dev),
@@ -677,11 +686,6 @@ def quantize_fp8_rows(x: torch.Tensor) -> Fp8Rows:
     if rc:
         _lib.check(rc, "yvmoe_quantize_fp8_rows")
     return rows
-
-
-def _no_gradients(x: torch.Tensor, what: str) -> None:
-    if x.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError(f"{what} is inference only: x requires a gradient (detach it, or use torch.no_grad)")
 
 
 def _fp8_out(out: Optional[torch.Tensor], shape, dev) -> torch.Tensor:
@@ -704,13 +708,14 @@ def fp8_linear(x, weight: PackedFp8Linear, bias: Optional[torch.Tensor] = None,
     if rows:
         if x.features != K:
             raise ValueError(f"rows have {x.features} features, the weight {K}")
+        _no_gradients("fp8_linear", x.codes, x.scales, weight.scales, bias, out)
         lead, dev = (x.codes.shape[0],), _same_device(x.codes, x.scales, weight.codes, weight.scales, bias, out)
     else:
         if x.dim() == 0 or x.shape[-1] != K:
             raise ValueError(f"x must be [..., {K}], got {tuple(x.shape)}")
         if x.dtype != torch.bfloat16:
             raise ValueError(f"x must be bfloat16 or Fp8Rows, got {x.dtype}")
-        _no_gradients(x, "fp8_linear")
+        _no_gradients("fp8_linear", x, weight.scales, bias, out)
         lead, dev = x.shape[:-1], _same_device(x, weight.codes, weight.scales, bias, out)
     if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != O):
         raise ValueError(f"bias must be bfloat16 [{O}]")
@@ -742,7 +747,7 @@ def fp8_swiglu(x: torch.Tensor, gate: PackedFp8Linear, up: PackedFp8Linear, down
         raise ValueError(f"x must be [..., {H}], got {tuple(x.shape)}")
     if x.dtype != torch.bfloat16:
         raise ValueError(f"x must be bfloat16, got {x.dtype}")
-    _no_gradients(x, "fp8_swiglu")
+    _no_gradients("fp8_swiglu", x, gate.scales, up.scales, down.scales, out)
     dev = _same_device(x, gate.codes, gate.scales, up.codes, up.scales, down.codes, down.scales, out)
     out = _fp8_out(out, x.shape, dev)
     l, N = _lib.lib(), x.numel() // H

@@ -3,7 +3,8 @@ import pytest
 import torch
 
 from pisceslx_amd import YvFp8SwiGLU, YvHybridBlockMLP, YvSwiGLU
-from pisceslx_amd import norms
+from pisceslx_amd import functional as yvf
+from pisceslx_amd import norms, quant
 
 
 class Config:
@@ -25,3 +26,31 @@ def test_half_block_in_training(mlp, monkeypatch):
     # a mlp that is in eval mode, as those that are packed from a block are, serves in a half block as it is made
     served = YvHybridBlockMLP(Config, mlp=mlp().eval())
     assert torch.equal(served(torch.ones(3, 32))[0], y)
+
+
+def operands(N=3, K=72, O=40):
+    """Of 8-bit calls: each a list of its tensors and the call on them."""
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    matrix = lambda o, i: torch.ones(-(-o // 128), -(-i // 128))
+    weight = lambda o, i, s: quant.PackedFp8Linear(i, o, torch.zeros(-(-o // 16), -(-i // 128), 2048, dtype=torch.uint8), s)
+    return {
+        "rows": ([bf(N, K)], yvf.quantize_fp8_rows),
+        "linear": ([bf(N, K), matrix(O, K), bf(O), bf(N, O)],
+                   lambda x, s, b, out: yvf.fp8_linear(x, weight(O, K, s), b, out)),
+        "linear of rows": ([torch.ones(1, N), matrix(O, K), bf(O), bf(N, O)],
+                           lambda xs, s, b, out: yvf.fp8_linear(
+                               quant.Fp8Rows(K, torch.zeros(N, 128, dtype=torch.float8_e4m3fn), xs), weight(O, K, s), b, out)),
+        "block": ([bf(N, K), matrix(O, K), matrix(O, K), matrix(K, O), bf(N, K)],
+                  lambda x, g, u, d, out: yvf.fp8_swiglu(x, weight(O, K, g), weight(O, K, u), weight(K, O, d), out)),
+    }
+
+
+@pytest.mark.parametrize("name,which", [(n, i) for n, (ts, _) in operands().items() for i in range(len(ts))])
+def test_gradients_of_8_bit_operands(name, which):
+    """A gradient of any operand is refused, not only of x; without gradients the next check speaks."""
+    ts, call = operands()[name]
+    ts[which].requires_grad_(True)
+    with pytest.raises(NotImplementedError, match="gradient"):
+        call(*ts)
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU only"):
+        call(*ts)
