@@ -12,6 +12,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .quant import Fp8Rows, PackedExperts, PackedFp8Linear, PackedLinear
@@ -661,12 +662,20 @@ def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
+def _no_tangents(what: str, *ts: Optional[torch.Tensor]) -> None:
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def _no_gradients(what: str, *ts: Optional[torch.Tensor]) -> None:
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
                 raise NotImplementedError(f"{what} is inference only: an operand requires a gradient (detach it, or use "
                                           "torch.no_grad)")
+    _no_tangents(what, *ts)
 
 
 def quantize_fp8_rows(x: torch.Tensor) -> Fp8Rows:
@@ -837,8 +846,9 @@ def swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: to
     x [..., H], w_gate and w_up [F, H], w_down [H, F] (nn.Linear.weight), all bf16 or all fp32, contiguous;
     any sizes up to 2^24 rows and 2^20 features. Sums are fp32; bf16 rounds the activated product and the two
     gradients before it once each, as operands, and the outputs. For the backward pass the call keeps x and the
-    two projections in fp32 (8 bytes a row and feature of F). The gradients are not differentiable again. A backward
-    pass that is being captured is refused while a call's graph of the same leaves on another stream lives.
+    two projections in fp32 (8 bytes a row and feature of F). The gradients are not differentiable again, and there
+    are no forward-mode derivatives. A backward pass that is being captured is refused while a call's graph of the
+    same leaves on another stream lives.
     """
     if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.shape != w_gate.shape[::-1]:
         raise ValueError(f"weights must be [F, H], [F, H], [H, F], got {tuple(w_gate.shape)}, "
@@ -852,6 +862,7 @@ def swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: to
         raise ValueError(f"x and the weights must have one dtype, got {x.dtype}, {w_gate.dtype}, {w_up.dtype}, "
                          f"{w_down.dtype}")
     _act(x.dtype)
+    _no_tangents("swiglu", x, w_gate, w_up, w_down)
     _same_device(x, w_gate, w_up, w_down)
     x2d = _aligned(x if x.dim() == 2 else x.view(-1, H))
     w_gate, w_up, w_down = _aligned(w_gate), _aligned(w_up), _aligned(w_down)

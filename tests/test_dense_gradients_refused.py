@@ -1,6 +1,7 @@
 """What would lose a gradient without a word is refused: on the host, before anything is computed."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from pisceslx_amd import YvFp8SwiGLU, YvHybridBlockMLP, YvSwiGLU
 from pisceslx_amd import functional as yvf
@@ -54,3 +55,30 @@ def test_gradients_of_8_bit_operands(name, which):
         call(*ts)
     with torch.no_grad(), pytest.raises(ValueError, match="GPU only"):
         call(*ts)
+
+
+def block_operands(N=3, H=4, F=8):
+    return [torch.zeros(N, H), torch.zeros(F, H), torch.zeros(F, H), torch.zeros(H, F)]
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("which", range(4))
+def test_forward_derivatives_of_the_block(which, grad):
+    """A tangent of any operand is refused, whether or not one requires a gradient or gradients are on at all."""
+    ts = block_operands()
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(ValueError, match="GPU only"):
+            yvf.swiglu(*ts)
+        ts[which] = forward_ad.make_dual(ts[which], torch.ones_like(ts[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            yvf.swiglu(*ts)
+
+
+@pytest.mark.parametrize("name,which", [("rows", 0), ("linear", 0), ("linear", 1), ("linear", 2), ("linear of rows", 0),
+                                        ("block", 0), ("block", 3)])
+def test_forward_derivatives_of_8_bit_operands(name, which):
+    ts, call = operands()[name]
+    with torch.no_grad(), forward_ad.dual_level():
+        ts[which] = forward_ad.make_dual(ts[which], torch.ones_like(ts[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(*ts)
