@@ -662,6 +662,15 @@ def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
+def _dense_sizes(rows: int, *features: int) -> None:
+    """Refuses what a call does not take; the library's counts have 32 bits."""
+    if rows > 1 << 24:
+        raise ValueError(f"{rows} rows: a call takes up to 2^24")
+    for n in features:
+        if n > 1 << 20:
+            raise ValueError(f"{n} features: a call takes up to 2^20")
+
+
 def _no_tangents(what: str, *ts: Optional[torch.Tensor]) -> None:
     if forward_ad._current_level >= 0:
         for t in ts:
@@ -686,8 +695,10 @@ def quantize_fp8_rows(x: torch.Tensor) -> Fp8Rows:
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"x must be [..., features], got {tuple(x.shape)}")
     _no_gradients("quantize_fp8_rows", x)
-    dev, act, K = _same_device(x), _act(x.dtype), x.shape[-1]
+    K = x.shape[-1]
     N, groups = x.numel() // K, -(-K // 128)
+    _dense_sizes(N, K)
+    dev, act = _same_device(x), _act(x.dtype)
     rows = Fp8Rows(K, torch.empty(N, groups * 128, dtype=torch.float8_e4m3fn, device=dev),
                    torch.empty(groups, N, dtype=torch.float32, device=dev))
     rc = _launch(dev, _lib.lib().yvmoe_quantize_fp8_rows, x.data_ptr(), act, N, K, rows.codes.data_ptr(),
@@ -718,18 +729,22 @@ def fp8_linear(x, weight: PackedFp8Linear, bias: Optional[torch.Tensor] = None,
         if x.features != K:
             raise ValueError(f"rows have {x.features} features, the weight {K}")
         _no_gradients("fp8_linear", x.codes, x.scales, weight.scales, bias, out)
-        lead, dev = (x.codes.shape[0],), _same_device(x.codes, x.scales, weight.codes, weight.scales, bias, out)
+        N = x.codes.shape[0]
+        _dense_sizes(N, K, O)
+        lead, dev = (N,), _same_device(x.codes, x.scales, weight.codes, weight.scales, bias, out)
     else:
         if x.dim() == 0 or x.shape[-1] != K:
             raise ValueError(f"x must be [..., {K}], got {tuple(x.shape)}")
         if x.dtype != torch.bfloat16:
             raise ValueError(f"x must be bfloat16 or Fp8Rows, got {x.dtype}")
         _no_gradients("fp8_linear", x, weight.scales, bias, out)
+        N = x.numel() // K
+        _dense_sizes(N, K, O)
         lead, dev = x.shape[:-1], _same_device(x, weight.codes, weight.scales, bias, out)
     if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != O):
         raise ValueError(f"bias must be bfloat16 [{O}]")
     out = _fp8_out(out, (*lead, O), dev)
-    l, w, N = _lib.lib(), weight.struct(), out.numel() // O
+    l, w = _lib.lib(), weight.struct()
     need = l.yvmoe_fp8_linear_rows_workspace_bytes if rows else l.yvmoe_fp8_linear_workspace_bytes
     nbytes = need(N, K, O)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -757,9 +772,11 @@ def fp8_swiglu(x: torch.Tensor, gate: PackedFp8Linear, up: PackedFp8Linear, down
     if x.dtype != torch.bfloat16:
         raise ValueError(f"x must be bfloat16, got {x.dtype}")
     _no_gradients("fp8_swiglu", x, gate.scales, up.scales, down.scales, out)
+    N = x.numel() // H
+    _dense_sizes(N, H, F)
     dev = _same_device(x, gate.codes, gate.scales, up.codes, up.scales, down.codes, down.scales, out)
     out = _fp8_out(out, x.shape, dev)
-    l, N = _lib.lib(), x.numel() // H
+    l = _lib.lib()
     g, u, d = gate.struct(), up.struct(), down.struct()
     nbytes = l.yvmoe_fp8_swiglu_workspace_bytes(N, H, F)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -862,6 +879,7 @@ def swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: to
         raise ValueError(f"x and the weights must have one dtype, got {x.dtype}, {w_gate.dtype}, {w_up.dtype}, "
                          f"{w_down.dtype}")
     _act(x.dtype)
+    _dense_sizes(x.numel() // H, H, F)
     _no_tangents("swiglu", x, w_gate, w_up, w_down)
     _same_device(x, w_gate, w_up, w_down)
     x2d = _aligned(x if x.dim() == 2 else x.view(-1, H))
