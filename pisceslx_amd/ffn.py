@@ -49,11 +49,19 @@ class YvFp8SwiGLU(nn.Module):
 
     @classmethod
     def from_block(cls, block: nn.Module) -> "YvFp8SwiGLU":
-        """A packed copy of a block with gate_proj, up_proj and down_proj (YvSwiGLU, an expert), on its device."""
+        """A packed copy of a block with gate_proj, up_proj and down_proj, without biases (YvSwiGLU, an expert), on its
+        device."""
         ffn, hidden = block.gate_proj.weight.shape
         m = cls(hidden, ffn, block.gate_proj.weight.device)
         for name in ("gate_proj", "up_proj", "down_proj"):
-            setattr(m, name, YvFp8Linear.from_linear(getattr(block, name)))
+            linear = getattr(block, name)
+            if linear.bias is not None:
+                raise ValueError(f"{name} has a bias: the block has none")
+            p = getattr(m, name)
+            if (linear.in_features, linear.out_features) != (p.in_features, p.out_features):
+                raise ValueError(f"{name} is {linear.out_features} x {linear.in_features}: no gated block of hidden "
+                                 f"{hidden}, ffn {ffn}")
+            setattr(m, name, YvFp8Linear.from_linear(linear))
         return m.eval()
 
     @classmethod
