@@ -15,6 +15,20 @@ from .quant import PackedFp8Linear, PackedLinear, pack_fp8_linear, pack_linear
 _GROUP = 128
 
 
+def _reference_bias(src, key: str, bias: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """A checkpoint's bias for a layer whose own is ``bias``: it has one if and only if the layer does, of its shape."""
+    if bias is not None and key not in src:
+        raise KeyError(f"{key}: not in the checkpoint")
+    if bias is None:
+        if key in src:
+            raise ValueError(f"{key}: the layer has no bias")
+        return None
+    loaded = src.get(key) if isinstance(src, StateSource) else src[key]
+    if loaded.shape != bias.shape:
+        raise ValueError(f"{key} is {list(loaded.shape)}, the layer's bias {list(bias.shape)}")
+    return loaded
+
+
 class YvInt4Linear(nn.Module):
     """y = x Wᵀ + b with W in int4 and a bf16 scale per 128 columns of a row (quant.pack_linear).
 
@@ -65,15 +79,11 @@ class YvInt4Linear(nn.Module):
         """The Linear ``name`` of a reference state dict, full precision or quantized
         (``checkpoint.linear_weight``), packed, and its ``bias``, which the checkpoint has if and only if the
         layer does."""
-        key = f"{name}.bias"
-        if self.bias is not None and key not in src:
-            raise KeyError(f"{key}: not in the checkpoint")
-        if self.bias is None and key in src:
-            raise ValueError(f"{key}: the layer has no bias")
+        bias = _reference_bias(src, f"{name}.bias", self.bias)
         self.set_weight(pack_linear(linear_weight(src, name).to(self.codes.device)))
-        if self.bias is not None:
+        if bias is not None:
             with torch.no_grad():
-                self.bias.copy_(src.get(key) if isinstance(src, StateSource) else src[key])
+                self.bias.copy_(bias)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self.training:
@@ -137,15 +147,11 @@ class YvFp8Linear(nn.Module):
         """The Linear ``name`` of a reference state dict, full precision or quantized
         (``checkpoint.linear_weight``), packed, and its ``bias``, which the checkpoint has if and only if the
         layer does."""
-        key = f"{name}.bias"
-        if self.bias is not None and key not in src:
-            raise KeyError(f"{key}: not in the checkpoint")
-        if self.bias is None and key in src:
-            raise ValueError(f"{key}: the layer has no bias")
+        bias = _reference_bias(src, f"{name}.bias", self.bias)
         self.set_weight(pack_fp8_linear(linear_weight(src, name).to(self.codes.device)))
-        if self.bias is not None:
+        if bias is not None:
             with torch.no_grad():
-                self.bias.copy_(src.get(key) if isinstance(src, StateSource) else src[key])
+                self.bias.copy_(bias)
 
     def forward(self, x) -> torch.Tensor:
         if self.training:
