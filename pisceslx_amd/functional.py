@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import threading
 import weakref
 from dataclasses import dataclass
 from typing import Optional
@@ -812,13 +813,36 @@ def _swiglu_forward(x2d, w_gate, w_up, w_down, keep: bool):
 
 
 _training = weakref.WeakSet()  # contexts of swiglu calls whose graphs live
+_training_lock = threading.Lock()  # one thread's call is added while another's backward pass looks through them
+
+
+def _leaves(ctx) -> set:
+    """ids of the leaves that a backward pass through a call adds gradients to: its own (ctx.leaves), and those behind
+    views, casts, copies and the layers before it. A graph keeps its leaves, so an id stands for one tensor."""
+    found, seen, todo = set(ctx.leaves), set(), [ctx]
+    while todo:
+        for node, _ in getattr(todo.pop(), "next_functions", ()):
+            if node is None or node in seen:
+                continue
+            seen.add(node)
+            if node.name() == "torch::autograd::AccumulateGrad":
+                found.add(id(node.variable))
+            else:
+                todo.append(node)
+    return found
 
 
 def _refuse_other_streams(ctx) -> None:
     """A leaf's gradient is added on the stream of its oldest living graph. Where that is not the stream that is being
-    captured, torch has the two wait for one another, which a capture does not survive."""
-    for other in list(_training):
-        if other.stream != ctx.stream and not other.leaves.isdisjoint(ctx.leaves):
+    captured, torch has the two wait for one another, which a capture does not survive. Only graphs with a swiglu call in
+    them are known here."""
+    with _training_lock:
+        others = [other for other in _training if other.stream != ctx.stream]
+    if not others:
+        return
+    mine = _leaves(ctx)
+    for other in others:
+        if not mine.isdisjoint(_leaves(other)):
             raise RuntimeError("swiglu: this backward pass is being captured while a graph of the same leaves that was "
                                "recorded on another stream lives: drop its outputs first")
 
@@ -831,8 +855,9 @@ class _SwiGLU(torch.autograd.Function):
         ctx.stream = _stream(x2d.device)
         # x2d may be a view of the leaf
         leaves = (t if t.is_leaf else t._base for t in (x2d, w_gate, w_up, w_down))
-        ctx.leaves = {id(t) for t in leaves if t is not None and t.requires_grad}
-        _training.add(ctx)
+        ctx.leaves = {id(t) for t in leaves if t is not None and t.is_leaf and t.requires_grad}
+        with _training_lock:
+            _training.add(ctx)
         return out
 
     @staticmethod
@@ -864,8 +889,9 @@ def swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: to
     any sizes up to 2^24 rows and 2^20 features. Sums are fp32; bf16 rounds the activated product and the two
     gradients before it once each, as operands, and the outputs. For the backward pass the call keeps x and the
     two projections in fp32 (8 bytes a row and feature of F). The gradients are not differentiable again, and there
-    are no forward-mode derivatives. A backward pass that is being captured is refused while a call's graph of the
-    same leaves on another stream lives.
+    are no forward-mode derivatives. A backward pass that is being captured is refused while another
+    call's graph with some of the same leaves (weights or inputs, also behind other operations) that was recorded on
+    another stream lives; leaves that are shared with a graph without such a call are not seen.
     """
     if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.shape != w_gate.shape[::-1]:
         raise ValueError(f"weights must be [F, H], [F, H], [H, F], got {tuple(w_gate.shape)}, "
