@@ -364,8 +364,8 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Args p) {
     }
 }
 
-// s_waitcnt immediate (gfx9 encoding): vmcnt <= n only
-constexpr int vm_only(int n) { return (n & 0xf) | ((n >> 4) << 14) | (0x7 << 4) | (0xf << 8); }
+// s_waitcnt immediate (gfx9 encoding): vmcnt and lgkmcnt 0, loads from memory and reads of LDS
+constexpr int all_done() { return 0x7 << 4; }
 
 // Direct loads to LDS at m0 + 16 (4) x lane, from base + off; an offset of kNone reads zeros (the buffer's bounds are
 // 2^31 bytes, which no other offset reaches, and no lane reads behind a tensor).
@@ -491,8 +491,8 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
     load(0);
     for (int b = 0; b < steps; ++b) {
         const int st = b & 1;
-        // this wavefront's loads of step b have landed, and after the barrier everybody's, and step b - 1 is read
-        __builtin_amdgcn_s_waitcnt(vm_only(0));
+        // this wavefront's loads of step b have landed and its reads of step b - 1 are over, and after the barrier everybody's
+        __builtin_amdgcn_s_waitcnt(all_done());
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");

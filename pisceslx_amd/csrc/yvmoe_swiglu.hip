@@ -67,6 +67,7 @@ struct TileArgs : Finish {
 // s_waitcnt immediates (gfx9 encoding)
 constexpr int vm_only(int n) { return (n & 0xf) | ((n >> 4) << 14) | (0x7 << 4) | (0xf << 8); }
 constexpr int lgkm0() { return 0xf | (0x3 << 14) | (0x7 << 4); }
+constexpr int all_done() { return vm_only(0) & lgkm0(); }  // loads from memory and reads of LDS
 
 // 16 bytes per lane from base + off to LDS at m0 + 16 lane; an offset of kNone reads zeros: the buffer's
 // bounds are 2^31 bytes, which no other offset reaches (the host checks), and no lane reads behind a tensor.
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
         if (chunks > 1) advance();
 #pragma unroll
         for (int j = 0; j < D; ++j) load(1, j);
-        __builtin_amdgcn_s_waitcnt(vm_only(D));
+        __builtin_amdgcn_s_waitcnt(vm_only(D));  // nothing has been read from LDS yet
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -572,8 +573,9 @@ __global__ __launch_bounds__(256) void swiglu_f32_kernel(TileArgs p) {
     if (chunks > 0) load(0);
     for (int c = 0; c < chunks; ++c) {
         const int st = c & 1;
-        // this wavefront's loads of chunk c have landed, and after the barrier everybody's, and chunk c - 1 is read
-        __builtin_amdgcn_s_waitcnt(vm_only(0));
+        // this wavefront's loads of chunk c have landed and its reads of chunk c - 1 are over, and after the barrier
+        // everybody's
+        __builtin_amdgcn_s_waitcnt(all_done());
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
