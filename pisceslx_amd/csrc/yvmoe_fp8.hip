@@ -134,7 +134,8 @@ struct Hidden {
 };
 __device__ __forceinline__ void load8(const Hidden& h, size_t at, int left, float (&v)[8]) {
     if (h.parts == 0) return load8<true, false>(h.p, at, left, v);
-    // columns behind the last one hold sums of zeros (ld is a multiple of 128)
+    // ld is a multiple of 128, so all eight are in the planes; columns behind the last one may never have been written, and
+    // what is read there is dropped (left)
     f32x4 s[2][2];
 #pragma unroll
     for (int m = 0; m < 2; ++m)

@@ -47,8 +47,9 @@ union Frag16 {  // 16 bf16 = two MFMA operands
 __device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
 
 // 1 / (1 + exp(-g)) within six half steps, in half of the instructions that expf and a division take: 2^t with what t = -g
-// log2(e) loses to its rounding multiplied on, and the unit's reciprocal. Below -88.7 it stays at 3e-39; of NaN it is a
-// number, and g times it is NaN.
+// log2(e) loses to its rounding multiplied on, and the unit's reciprocal. Below -87.3, where it is under the smallest normal
+// number, it is 0: the reciprocal gives no subnormal results, and t is held where 2^t is still finite. Of NaN it is a number,
+// and g times it is NaN.
 __device__ __forceinline__ float sigmoid_fast(float g) {
     constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147182f;
     const float y = __builtin_amdgcn_fmed3f(-g, -104.0f, 88.7f), t = y * kLog2e;
