@@ -663,20 +663,19 @@ def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
-def _dense_sizes(rows: int, *features: int) -> None:
-    """Refuses what a call does not take; the library's counts have 32 bits."""
-    if rows > 1 << 24:
+_MAX_ROWS, _MAX_FEATURES = 1 << 24, 1 << 20  # of a call; the library's counts have 32 bits
+
+
+def _too_large(rows: int, *features: int) -> None:
+    if rows > _MAX_ROWS:
         raise ValueError(f"{rows} rows: a call takes up to 2^24")
-    for n in features:
-        if n > 1 << 20:
-            raise ValueError(f"{n} features: a call takes up to 2^20")
+    raise ValueError(f"{max(features)} features: a call takes up to 2^20")
 
 
 def _no_tangents(what: str, *ts: Optional[torch.Tensor]) -> None:
-    if forward_ad._current_level >= 0:
-        for t in ts:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError(f"{what} has no forward-mode derivative")
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def _no_gradients(what: str, *ts: Optional[torch.Tensor]) -> None:
@@ -685,7 +684,8 @@ def _no_gradients(what: str, *ts: Optional[torch.Tensor]) -> None:
             if t is not None and t.requires_grad:
                 raise NotImplementedError(f"{what} is inference only: an operand requires a gradient (detach it, or use "
                                           "torch.no_grad)")
-    _no_tangents(what, *ts)
+    if forward_ad._current_level >= 0:
+        _no_tangents(what, *ts)
 
 
 def quantize_fp8_rows(x: torch.Tensor) -> Fp8Rows:
@@ -695,10 +695,12 @@ def quantize_fp8_rows(x: torch.Tensor) -> Fp8Rows:
     NaN makes every product of its row NaN. Up to 2^24 rows of up to 2^20 features; inference only."""
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"x must be [..., features], got {tuple(x.shape)}")
-    _no_gradients("quantize_fp8_rows", x)
+    if x.requires_grad or forward_ad._current_level >= 0:
+        _no_gradients("quantize_fp8_rows", x)
     K = x.shape[-1]
     N, groups = x.numel() // K, -(-K // 128)
-    _dense_sizes(N, K)
+    if N > _MAX_ROWS or K > _MAX_FEATURES:
+        _too_large(N, K)
     dev, act = _same_device(x), _act(x.dtype)
     rows = Fp8Rows(K, torch.empty(N, groups * 128, dtype=torch.float8_e4m3fn, device=dev),
                    torch.empty(groups, N, dtype=torch.float32, device=dev))
@@ -731,7 +733,8 @@ def fp8_linear(x, weight: PackedFp8Linear, bias: Optional[torch.Tensor] = None,
             raise ValueError(f"rows have {x.features} features, the weight {K}")
         _no_gradients("fp8_linear", x.codes, x.scales, weight.scales, bias, out)
         N = x.codes.shape[0]
-        _dense_sizes(N, K, O)
+        if N > _MAX_ROWS or K > _MAX_FEATURES or O > _MAX_FEATURES:
+            _too_large(N, K, O)
         lead, dev = (N,), _same_device(x.codes, x.scales, weight.codes, weight.scales, bias, out)
     else:
         if x.dim() == 0 or x.shape[-1] != K:
@@ -740,7 +743,8 @@ def fp8_linear(x, weight: PackedFp8Linear, bias: Optional[torch.Tensor] = None,
             raise ValueError(f"x must be bfloat16 or Fp8Rows, got {x.dtype}")
         _no_gradients("fp8_linear", x, weight.scales, bias, out)
         N = x.numel() // K
-        _dense_sizes(N, K, O)
+        if N > _MAX_ROWS or K > _MAX_FEATURES or O > _MAX_FEATURES:
+            _too_large(N, K, O)
         lead, dev = x.shape[:-1], _same_device(x, weight.codes, weight.scales, bias, out)
     if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != O):
         raise ValueError(f"bias must be bfloat16 [{O}]")
@@ -774,7 +778,8 @@ def fp8_swiglu(x: torch.Tensor, gate: PackedFp8Linear, up: PackedFp8Linear, down
         raise ValueError(f"x must be bfloat16, got {x.dtype}")
     _no_gradients("fp8_swiglu", x, gate.scales, up.scales, down.scales, out)
     N = x.numel() // H
-    _dense_sizes(N, H, F)
+    if N > _MAX_ROWS or H > _MAX_FEATURES or F > _MAX_FEATURES:
+        _too_large(N, H, F)
     dev = _same_device(x, gate.codes, gate.scales, up.codes, up.scales, down.codes, down.scales, out)
     out = _fp8_out(out, x.shape, dev)
     l = _lib.lib()
@@ -905,8 +910,11 @@ def swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: to
         raise ValueError(f"x and the weights must have one dtype, got {x.dtype}, {w_gate.dtype}, {w_up.dtype}, "
                          f"{w_down.dtype}")
     _act(x.dtype)
-    _dense_sizes(x.numel() // H, H, F)
-    _no_tangents("swiglu", x, w_gate, w_up, w_down)
+    N = x.numel() // H
+    if N > _MAX_ROWS or H > _MAX_FEATURES or F > _MAX_FEATURES:
+        _too_large(N, H, F)
+    if forward_ad._current_level >= 0:
+        _no_tangents("swiglu", x, w_gate, w_up, w_down)
     _same_device(x, w_gate, w_up, w_down)
     x2d = _aligned(x if x.dim() == 2 else x.view(-1, H))
     w_gate, w_up, w_down = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
