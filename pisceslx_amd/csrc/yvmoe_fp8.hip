@@ -231,7 +231,7 @@ __device__ __forceinline__ uint4 load16(const char* p) { return *(const uint4*)p
 // deal out the blocks of 128 contraction elements and add their sums in LDS, in order. Bound by the stream of the
 // weights, which go to registers in their stored order, kAhead steps ahead. SRC: the rows' codes come from L2, or the
 // work-group makes them in LDS while its first weights are on their way (a launch and a round trip less; each
-// work-group repeats the work, so only for few values).
+// work-group repeats the work, so only for few values). 49 to 64 rows of kSwiGLU take all 256 registers and spill eight.
 template <int EPI, int MR, int SRC>
 __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Args p) {
     constexpr int NM = EPI == kSwiGLU ? 2 : 1;  // matrices
@@ -391,9 +391,10 @@ __device__ __forceinline__ int swizzle(int r) { return (r >> 1 & 3) | ((r ^ r >>
 // Tiles: WR x WC wavefronts of 16 MB rows x 16 NB columns each (kSwiGLU: the wavefront's first NB / 2 blocks are gate
 // columns, the others the up columns of the same h columns). A step is a block of 128 contraction elements: rows
 // (swizzled 128-byte lines), weights (stored order) and both scales go to LDS by direct loads, one step ahead of the
-// products, in two stages with one barrier a step. 256 x 256 tiles: 8192 x 4096 x 8192 in 248 us, 2.2 PFLOP/s, of which
-// 60 are the ends of four rounds of tiles; of the rest the scales are a tenth, the loads another, and the matrix unit by
-// itself, at the card's power, the others. Wavefronts 8 x 1, 4 x 4 or 8 x 2 and fragments read a step ahead are no faster.
+// products, in two stages with one barrier a step. 256 x 256 tiles: 8192 x 4096 x 8192 in 257 us (264 on another card;
+// medians of a long run), 2.1 PFLOP/s, the matrix unit busy half of the time. In copies with a part left out: without the
+// outputs' stores 243, without scales 250, without the loads past a tile's first step 200. In 64 x 128 tiles, several
+// work-groups a CU, 340. Wavefronts 8 x 1, 4 x 4 or 8 x 2 and fragments read a step ahead are no faster.
 template <int EPI, int WR, int WC, int MB, int NB, bool EXACT>
 __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
     constexpr int NW = WR * WC, TM = WR * 16 * MB, TN = WC * 16 * NB;
@@ -548,8 +549,8 @@ __global__ __launch_bounds__(64 * WR * WC) void fp8_tile_kernel(Fp8Args p) {
         return;
     }
     if constexpr (!DUAL) {
-        // The wavefront's outputs through LDS, so that its stores are whole lines (of 8 bytes in 16 rows each: 8192 x
-        // 4096 x 8192 272 us, so 248). Piece c of eight columns of row r lies at c ^ r.
+        // The wavefront's outputs through LDS, so that its stores are whole lines (stores of 8 bytes in 16 rows each took
+        // 24 of 272 us of 8192 x 4096 x 8192 more). Piece c of eight columns of row r lies at c ^ r.
         constexpr int PC = 2 * NB, ROWS = 16 * MB;
         static_assert(NW * ROWS * PC * 16 <= 2 * STAGE, "the tile in LDS");
         unsigned char* mine = &lds[0][0] + wave * (ROWS * PC * 16);

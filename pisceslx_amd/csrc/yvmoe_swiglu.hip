@@ -376,8 +376,9 @@ struct Reader32 {
 // halves with the next half's fragment reads (in the first four fifths of them) and the loads of the chunk after next
 // among them, one barrier between the halves. The columns' operand is the MFMA's first, so that a lane holds four
 // consecutive columns of one row. Bound by the matrix unit, whose operands LDS must bring (1536 of 2048 cycles a chunk):
-// 4096 x 4096 x 11264, bf16: gate and up 645 us (1.17 PFLOP/s), down 290 (1.3, without the loads from memory 1.68), dx
-// 570 (1.33), weights' gradients 1.16; dh 460, 120 of which read g and u and write d and h.
+// 4096 x 4096 x 11264, bf16: gate and up 643 us (1.18 PFLOP/s), down 285 (1.33, without the loads from memory 1.68), dx
+// 566 (1.34), weights' gradients 665 and 332 (1.14); dh 459, 120 of which read g and u and write d and h. The 256 x 256 form
+// of kAlone spills one register.
 template <int EPI, int PL, bool AMC, bool BMC, int MB, int NB>
 __global__ __launch_bounds__(256) void swiglu_tile_kernel(TileArgs p) {
     constexpr int TM = 32 * MB, TN = 32 * NB;

@@ -17,7 +17,7 @@ class YvSwiGLU(nn.Module):
     The parameters have the names and shapes of YvSwiGLUExpert's (``gate_proj.weight``, ``up_proj.weight`` [ffn,
     hidden], ``down_proj.weight`` [hidden, ffn], no biases), so a state dict of an expert loads as it is, and
     quant.pack_experts takes the weights. forward(x [..., hidden]) in the parameters' dtype, bfloat16 or float32, in
-    training and in eval mode.
+    training and in eval mode; torch.autocast casts neither x nor the parameters, and another dtype of x raises.
     """
 
     def __init__(self, hidden_size: int, intermediate_size: int, device=None, dtype=None):
